@@ -1,0 +1,391 @@
+"""Performance cases of the 8-bit serving operators: the paged K/V cache held in int8 with a scale for each
+block of 16 tokens and head (write, read back, attention), and the int8 product with scales for each token and
+output channel.
+
+Each case is one call as a serving step makes it.  Where ``own`` is false ``run`` restates the operator in
+elementary torch operations; ``exact`` restates it in 64 bits.
+"""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+BLOCK = 16  # tokens that share a scale
+# the talker's heads (16 query, 8 kv, 128) and the code predictor's (16, 8, 64); the last two are groups of 8 and 1
+HEADS = {"talker": (16, 8, 128), "predictor": (16, 8, 64), "wide": (16, 2, 128), "full": (8, 8, 128)}
+
+
+def listed():
+    return [
+        # a decode step's new tokens, one a row, most of them into a block that is partly filled
+        {"name": "write-decode-64", "kind": "write", "rows": 64, "new": 1, "high": 2048, "heads": "talker", "page": 16,
+         "batch": 1},
+        # the largest prefill bucket's chunks of 8 prompts, ragged
+        {"name": "write-prefill-8", "kind": "write", "rows": 8, "new": 80, "high": 512, "heads": "talker", "page": 16,
+         "batch": 2},
+        # a long document's prompt, admitted whole
+        {"name": "write-prompt-1", "kind": "write", "rows": 1, "new": 8191, "high": 0, "heads": "talker", "page": 16,
+         "batch": 3},
+        # one listener's stream: one query over a short history, where launches and latency count
+        {"name": "attend-decode-1", "kind": "attend", "rows": 1, "new": 1, "low": 333, "high": 333, "heads": "talker",
+         "page": 16, "batch": 4},
+        # the headline batch: 64 rows of 64 to 2048 tokens
+        {"name": "attend-decode-64", "kind": "attend", "rows": 64, "new": 1, "low": 64, "high": 2048,
+         "heads": "talker", "page": 16, "batch": 5},
+        # a few very long histories, each cut over many workgroups
+        {"name": "attend-decode-long", "kind": "attend", "rows": 3, "new": 1, "low": 40000, "high": 60001,
+         "heads": "talker", "page": 16, "batch": 6},
+        # chunks of 8 prompts over what they have in the cache
+        {"name": "attend-prefill-8", "kind": "attend", "rows": 8, "new": 80, "low": 80, "high": 592, "heads": "talker",
+         "page": 16, "batch": 7},
+        # a chunk of a long prompt: up to 2047 queries over some 6000 keys
+        {"name": "attend-prompt-1", "kind": "attend", "rows": 1, "new": 2047, "low": 6001, "high": 6001,
+         "heads": "talker", "page": 16, "batch": 8},
+        # one stream's qkv projection, rows quantised in the call
+        {"name": "linear-1", "kind": "linear", "rows": 1, "out": 4096, "in": 2048},
+        # the headline batch's down projection
+        {"name": "linear-64", "kind": "linear", "rows": 64, "out": 2048, "in": 6144},
+        # the largest prefill bucket's gate and up projection
+        {"name": "linear-640", "kind": "linear", "rows": 640, "out": 12288, "in": 2048},
+        # a long prompt's chunk through the down projection
+        {"name": "linear-4001", "kind": "linear", "rows": 4001, "out": 2048, "in": 6144},
+    ]
+
+
+def _log(rng, low, high):
+    return max(low, min(high, round(math.exp(rng.uniform(math.log(low), math.log(high + 0.49))))))
+
+
+def draw(rng):
+    kind = rng.choice(("write", "attend", "attend", "linear"))
+    if kind == "linear":
+        out, inner = _log(rng, 16, 6000), 16 * _log(rng, 4, 384)
+        return {"kind": kind, "rows": _log(rng, 1, min(4000, 50_000_000_000 // (out * inner))), "out": out, "in": inner}
+    heads, page, batch = rng.choice(sorted(HEADS)), rng.choice((16, 16, 32, 64)), rng.randrange(100000)
+    if kind == "write":
+        rows = _log(rng, 1, 128)
+        return {"kind": kind, "rows": rows, "new": rng.choice((1, _log(rng, 2, max(2, 8000 // rows)))),
+                "high": _log(rng, 1, 4096), "heads": heads, "page": page, "batch": batch}
+    if rng.random() < 0.6:  # decode
+        rows = _log(rng, 1, 128)
+        high = _log(rng, 2, min(50000, 140000 // rows))
+        return {"kind": kind, "rows": rows, "new": 1, "low": max(1, high // rng.choice((1, 4, 32))), "high": high,
+                "heads": heads, "page": page, "batch": batch}
+    rows = _log(rng, 1, 8)
+    new = _log(rng, 2, 1500 // rows)
+    high = new + rng.choice((0, _log(rng, 1, 4000 // rows)))
+    return {"kind": kind, "rows": rows, "new": new, "low": max(new, high // 2), "high": high, "heads": heads,
+            "page": page, "batch": batch}
+
+
+# -- inputs ------------------------------------------------------------------------------------------
+
+
+def _generator(seed, salt):
+    g = torch.Generator(device="cuda")
+    g.manual_seed((int(seed) * 1_000_003 + salt) % (1 << 62))
+    return g
+
+
+def _shape(case):
+    """Each row's keys in the cache with its new ones, and how many of them are new: the case's own."""
+
+    rng = np.random.default_rng(case["batch"])
+    rows, new = case["rows"], case["new"]
+    if case["kind"] == "write":
+        prior = rng.integers(0, case["high"] + 1, size=rows)
+        news = np.full(rows, 1) if new == 1 else rng.integers(max(1, new - new // 3), new + 1, size=rows)
+        return prior + news, news
+    news = np.full(rows, 1) if new == 1 else rng.integers(max(1, new - new // 3), new + 1, size=rows)
+    return np.maximum(rng.integers(case["low"], case["high"] + 1, size=rows), news), news
+
+
+def _pool(case, seed):
+    """The rows' pages, scattered over a pool with a few pages of nobody's; kv_indptr, indices, last page lengths."""
+
+    lengths, news = _shape(case)
+    page = case["page"]
+    pages = -(-lengths // page)
+    total = int(pages.sum()) + 8
+    indices = np.random.default_rng(seed).permutation(total)[: int(pages.sum())]
+    indptr = np.concatenate(([0], np.cumsum(pages)))
+    return lengths, news, total, indptr, indices
+
+
+def _slots(lengths, starts, indptr, indices, page):
+    """Pages and offsets of each row's positions starts[r] .. lengths[r] - 1, rows in order."""
+
+    counts = lengths - starts
+    row = np.repeat(np.arange(len(lengths)), counts)
+    at = np.arange(counts.sum()) - np.repeat(np.cumsum(counts) - counts, counts) + np.repeat(starts, counts)
+    return torch.from_numpy(indices[indptr[row] + at // page].astype(np.int64)).cuda(), torch.from_numpy(at % page).cuda()
+
+
+def _scale_for(amax):
+    """The least power of two s (at least 2^-126) with amax / s <= 127."""
+
+    mantissa, exponent = torch.frexp(amax)  # amax = mantissa 2^exponent, mantissa in [0.5, 1)
+    s = torch.ldexp(torch.ones_like(amax), exponent - 7 + (mantissa > 127 / 128).to(exponent.dtype))
+    return torch.where(amax > 0, s.clamp(min=2.0**-126), torch.full_like(amax, 2.0**-126))
+
+
+def _filled(total, page, hkv, d, seed):
+    """A pool in use: values of normalised heads (K near N(0, 1), V of another spread per head), quantised."""
+
+    g = _generator(seed, 1)
+    codes = torch.empty(total, 2, page, hkv, d, dtype=torch.int8, device="cuda")
+    scales = torch.empty(total, 2, page // BLOCK, hkv, dtype=torch.float32, device="cuda")
+    spread = torch.empty(2, 1, 1, hkv, 1, device="cuda").uniform_(0.4, 2.5, generator=g)
+    spread[0] = 1.0
+    step = max(1, (1 << 27) // (2 * page * hkv * d))
+    for a in range(0, total, step):
+        x = torch.empty((min(step, total - a), 2, page // BLOCK, BLOCK, hkv, d), device="cuda").normal_(generator=g)
+        x = (x * spread).to(torch.bfloat16).float()
+        s = _scale_for(x.abs().amax(dim=(3, 5)))
+        codes[a:a + step] = (x / s[:, :, :, None, :, None]).round().to(torch.int8).view(-1, 2, page, hkv, d)
+        scales[a:a + step] = s
+    return codes, scales
+
+
+def _write_inputs(case, seed):
+    lengths, news, total, indptr, indices = _pool(case, seed)
+    hq, hkv, d = HEADS[case["heads"]]
+    codes, scales = _filled(total, case["page"], hkv, d, seed)
+    g, tokens = _generator(seed, 2), int(news.sum())
+    # tokens differ in size, as V's do, so that some blocks' scales have to grow
+    size = torch.exp2(torch.empty(2, tokens, 1, 1, device="cuda").normal_(0.0, 0.7, generator=g))
+    kv = (torch.empty(2, tokens, hkv, d, device="cuda").normal_(generator=g) * size).to(torch.bfloat16)
+    pages, offsets = _slots(lengths, lengths - news, indptr, indices, case["page"])
+    first = (lengths - news) // BLOCK * BLOCK  # the whole touched blocks, up to the last new token
+    read_pages, read_offsets = _slots(lengths, first, indptr, indices, case["page"])
+    return {"key": kv[0], "value": kv[1], "cache": codes, "scales": scales, "pages": pages, "offsets": offsets,
+            "read_pages": read_pages, "read_offsets": read_offsets}
+
+
+def _attend_inputs(case, seed):
+    lengths, news, total, indptr, indices = _pool(case, seed)
+    hq, hkv, d = HEADS[case["heads"]]
+    codes, scales = _filled(total, case["page"], hkv, d, seed)
+    q = torch.empty(int(news.sum()), hq, d, device="cuda").normal_(generator=_generator(seed, 3)).to(torch.bfloat16)
+
+    def int32(x):
+        return torch.from_numpy(np.ascontiguousarray(x, dtype=np.int32)).cuda()
+
+    return {"query": q, "cache": codes, "scales": scales, "kv_indptr": int32(indptr), "kv_indices": int32(indices),
+            "last_page_len": int32((lengths - 1) % case["page"] + 1),
+            "qo_indptr": None if case["new"] == 1 else int32(np.concatenate(([0], np.cumsum(news)))),
+            "longest": int(lengths.max()), "most": int(news.max())}
+
+
+def _quantize_rows(x):
+    """Codes rint(127 x / max |x|) and scales max |x| / 127 of each row; 127 x is exact in 32 bits for bf16 x."""
+
+    amax = x.abs().amax(dim=-1, keepdim=True)
+    codes = torch.where(amax > 0, (x * 127.0) / amax, torch.zeros_like(x)).round()
+    return codes, torch.where(amax > 0, amax / 127.0, torch.ones_like(amax)).squeeze(-1)
+
+
+def _linear_inputs(case, seed):
+    g = _generator(seed, 4)
+    x = torch.empty(case["rows"], case["in"], device="cuda").normal_(generator=g)
+    # some channels are larger than the others, as they are after a norm's weight
+    x = (x * torch.exp2(torch.empty(case["in"], device="cuda").normal_(0.0, 0.5, generator=g))).to(torch.bfloat16)
+    w = torch.empty(case["out"], case["in"], device="cuda").normal_(0.0, 0.02, generator=g).to(torch.bfloat16)
+    codes, scales = _quantize_rows(w.float())
+    return {"x": x, "weight": codes.to(torch.int8), "weight_scales": scales}
+
+
+def prepare(case, seed):
+    return {"write": _write_inputs, "attend": _attend_inputs, "linear": _linear_inputs}[case["kind"]](case, seed)
+
+
+# -- one pass ----------------------------------------------------------------------------------------
+
+
+def _write(s):
+    """Plain form: the touched blocks gathered, rescaled where their range grows, and put back."""
+
+    cache, scales = s["cache"], s["scales"]
+    total, _, page, hkv, d = cache.shape
+    per = page // BLOCK
+    blocks, inverse = torch.unique(s["pages"] * per + s["offsets"] // BLOCK, return_inverse=True)
+    n, slot = blocks.shape[0], s["offsets"] % BLOCK
+    kv = torch.stack((s["key"], s["value"]), 1).float()  # [tokens, 2, hkv, d]
+    amax = torch.zeros(n, 2, hkv, device=kv.device)
+    amax.scatter_reduce_(0, inverse[:, None, None].expand(-1, 2, hkv), kv.abs().amax(-1), "amax")
+    first = torch.full((n,), BLOCK, device=kv.device).scatter_reduce_(0, inverse, slot, "amin")
+    at, part = blocks // per, blocks % per
+    old = scales[at, :, part]
+    kept = (first > 0)[:, None, None]
+    new = _scale_for(amax)
+    new = torch.where(kept, torch.maximum(old, new), new)
+    held = cache.view(total, 2, per, BLOCK, hkv, d)[at, :, part]  # [n, 2, 16, hkv, d]
+    earlier = (torch.arange(BLOCK, device=kv.device) < first[:, None])[:, None, :, None, None]
+    scaled = (held.float() * (old / new)[:, :, None, :, None]).round().to(torch.int8)
+    held = torch.where(earlier, scaled, held)
+    held[inverse, :, slot] = (kv / new[inverse][..., None]).round().to(torch.int8)
+    cache.view(total, 2, per, BLOCK, hkv, d)[at, :, part] = held
+    scales[at, :, part] = new
+    out = cache[s["read_pages"], :, s["read_offsets"]].float()
+    out = (out * scales[s["read_pages"], :, s["read_offsets"] // BLOCK][..., None]).to(torch.bfloat16)
+    return out[:, 0], out[:, 1]
+
+
+def _attend(s):
+    """Plain form: the rows' pages gathered into padded K and V, masked scores, softmax, product."""
+
+    q, page = s["query"].float(), s["cache"].shape[2]
+    rows, (_, hq, d), hkv = s["kv_indptr"].shape[0] - 1, q.shape, s["cache"].shape[3]
+    start, count = s["kv_indptr"][:-1].long(), (s["kv_indptr"][1:] - s["kv_indptr"][:-1]).long()
+    length = (count - 1) * page + s["last_page_len"]
+    most = -(-s["longest"] // page)
+    at = torch.arange(most, device=q.device)
+    ids = s["kv_indices"][(start[:, None] + torch.minimum(at, count[:, None] - 1))].long()  # [rows, most]
+    kv = s["cache"][ids].float().unflatten(3, (-1, BLOCK)) * s["scales"][ids][:, :, :, :, None, :, None]
+    kv = kv.permute(2, 0, 5, 1, 3, 4, 6)
+    k, v = kv.reshape(2, rows, hkv, most * page, d).unbind(0)
+    if s["qo_indptr"] is None:
+        first, queries = torch.arange(rows, device=q.device), torch.ones_like(length)
+    else:
+        first, queries = s["qo_indptr"][:-1].long(), (s["qo_indptr"][1:] - s["qo_indptr"][:-1]).long()
+    i = torch.arange(s["most"], device=q.device)
+    real = i < queries[:, None]
+    token = first[:, None] + torch.minimum(i, queries[:, None] - 1)  # [rows, most queries]
+    qs = q[token].view(rows, -1, hkv, hq // hkv, d).transpose(1, 2).reshape(rows, hkv, -1, d)
+    scores = (qs @ k.transpose(2, 3).contiguous()).mul_(1.0 / math.sqrt(d))
+    limit = (length[:, None] - queries[:, None] + i + 1).repeat_interleave(hq // hkv, 1)
+    seen = torch.arange(most * page, device=q.device) < limit[:, :, None]
+    scores.masked_fill_(~seen[:, None], -math.inf)
+    scores = scores.sub_(scores.amax(-1, keepdim=True)).exp_()
+    out = (scores @ v) / scores.sum(-1, keepdim=True)
+    out = out.view(rows, hkv, -1, hq // hkv, d).transpose(1, 2).reshape(rows, -1, hq, d)
+    return out[real].to(torch.bfloat16)  # rows in order, each its own queries: the tokens' order
+
+
+def _linear(s):
+    codes, scales = _quantize_rows(s["x"].float())
+    return ((codes @ s["weight"].float().t()) * scales[:, None] * s["weight_scales"]).to(torch.bfloat16)
+
+
+def _package():
+    from __graft_entry__ import load_package
+
+    load_package()
+    from nari_qwen3_tts_amd import kernels, layers, talker_kv
+
+    return kernels, layers, talker_kv
+
+
+def _run_own(s):
+    kernels, layers, talker_kv = _package()
+    if "key" in s:
+        kernels.paged_cache_write_int8_(s["key"], s["value"], s["cache"], s["scales"], s["pages"], s["offsets"])
+        return kernels.paged_cache_read_int8(s["cache"], s["scales"], s["read_pages"], s["read_offsets"])
+    if "query" in s:
+        metadata = talker_kv.TalkerAttentionMetadata(
+            qo_indptr=s["qo_indptr"], paged_kv_indptr=s["kv_indptr"], paged_kv_indices=s["kv_indices"],
+            paged_kv_last_page_len=s["last_page_len"], position_ids=None, write_pages=None, write_offsets=None,
+            padding_pages=())
+        return kernels.paged_attention_int8(s["query"], s["cache"], s["scales"], metadata)
+    codes, scales = layers.quantize_int8_rows(s["x"])
+    return layers.linear_int8(codes, scales, s["weight"], s["weight_scales"])
+
+
+def run(s):
+    if own:
+        return _run_own(s)
+    return _write(s) if "key" in s else _attend(s) if "query" in s else _linear(s)
+
+
+def work(case):
+    if case["kind"] == "linear":
+        m, n, k = case["rows"], case["out"], case["in"]
+        return {"bytes": 2 * m * k + n * k + 4 * n + 2 * m * n, "flops": 2 * m * n * k}
+    hq, hkv, d = HEADS[case["heads"]]
+    lengths, news = _shape(case)
+    if case["kind"] == "write":
+        # tokens in, codes and scales out; open blocks' earlier codes in; the values read back
+        first = (lengths - news) // BLOCK * BLOCK
+        blocks = int((-(-lengths // BLOCK) - first // BLOCK).sum())
+        tokens, back = int(news.sum()), int((lengths - first).sum())
+        return {"bytes": 2 * hkv * (tokens * (2 * d + d) + 4 * blocks + (back - tokens) * d + back * (d + 2 * d)),
+                "flops": 2 * hkv * d * 3 * back}
+    pairs = int((news * (lengths - news) + news * (news + 1) // 2).sum())
+    keys = int(lengths.sum())
+    return {"bytes": 2 * keys * hkv * d + 8 * keys * hkv // BLOCK + 4 * int(news.sum()) * hq * d,
+            "flops": 4 * hq * d * pairs}
+
+
+# -- the same in 64 bits -------------------------------------------------------------------------------
+
+
+def _exact_write(case, seed):
+    s = _write_inputs(case, seed)
+    lengths, news, total, indptr, indices = _pool(case, seed)
+    values = s["cache"].double().cpu().numpy()  # codes until a block is decoded
+    scales = s["scales"].double().cpu().numpy()
+    fresh = np.stack((s["key"].double().cpu().numpy(), s["value"].double().cpu().numpy()), 1)
+    out, at = [], 0
+    for r in range(len(lengths)):
+        start, end = int(lengths[r] - news[r]), int(lengths[r])
+        while start < end:
+            stop = min(end, (start // BLOCK + 1) * BLOCK)
+            p, o = indices[indptr[r] + start // case["page"]], start % case["page"]
+            b, inside, n = o // BLOCK, o % BLOCK, stop - start
+            x = fresh[at:at + n]  # [n, 2, hkv, d]
+            top = np.abs(x).max(axis=(0, 3))
+            with np.errstate(divide="ignore"):
+                s_new = np.where(top > 0, 2.0 ** np.ceil(np.log2(top / 127.0)), 0.0)
+            s_new = np.where(top > 127.0 * s_new, 2 * s_new, s_new)  # log2's own rounding, either way
+            s_new = np.where(top <= 127.0 * s_new / 2, s_new / 2, s_new)
+            s_new = np.maximum(s_new, 2.0**-126)
+            before = values[p, :, b * BLOCK:b * BLOCK + inside]
+            if inside:
+                s_old = scales[p, :, b]
+                s_new = np.maximum(s_new, s_old)
+                before = np.rint(before * (s_old / s_new)[:, None, :, None])
+            codes = np.rint(x.transpose(1, 0, 2, 3) / s_new[:, None, :, None])
+            out.append((np.concatenate((before, codes), 1) * s_new[:, None, :, None]).transpose(1, 0, 2, 3))
+            at, start = at + n, stop
+    out = torch.from_numpy(np.concatenate(out))
+    return out[:, 0].contiguous(), out[:, 1].contiguous()
+
+
+def _exact_attend(case, seed):
+    s = _attend_inputs(case, seed)
+    lengths, news, total, indptr, indices = _pool(case, seed)
+    hq, hkv, d = HEADS[case["heads"]]
+    out, at = [], 0
+    for r in range(len(lengths)):
+        n, m = int(lengths[r]), int(news[r])
+        ids = torch.from_numpy(indices[indptr[r]:indptr[r + 1]]).cuda()
+        spread = s["scales"][ids].double().repeat_interleave(BLOCK, 2)[..., None]
+        kv = (s["cache"][ids].double() * spread).transpose(0, 1).reshape(2, -1, hkv, d)[:, :n]
+        q = s["query"][at:at + m].double()
+        hidden = torch.arange(n, device="cuda") > torch.arange(n - m, n, device="cuda")[:, None]
+        heads = []
+        for h in range(hq):
+            scores = q[:, h] @ kv[0, :, h // (hq // hkv)].t().contiguous() / math.sqrt(d)
+            p = torch.softmax(scores.masked_fill_(hidden, -math.inf), -1)
+            heads.append(p @ kv[1, :, h // (hq // hkv)].contiguous())
+        out.append(torch.stack(heads, 1))
+        at += m
+    return torch.cat(out)
+
+
+def _exact_linear(case, seed):
+    s = _linear_inputs(case, seed)
+    x = s["x"].double()
+    top = x.abs().amax(1, keepdim=True)
+    codes = torch.round(x * 127 / torch.where(top > 0, top, 1.0))
+    scales = torch.where(top > 0, top / 127, 1.0)
+    return codes * scales @ (s["weight"].double() * s["weight_scales"].double()[:, None]).t()
+
+
+def exact(case, seed):
+    return {"write": _exact_write, "attend": _exact_attend, "linear": _exact_linear}[case["kind"]](case, seed)
