@@ -276,13 +276,13 @@ def _package():
     from __graft_entry__ import load_package
 
     load_package()
-    from nari_qwen3_tts_amd import kernels, layers, talker_kv
+    from nari_qwen3_tts_amd import _lib, kernels, layers, talker_kv
 
-    return kernels, layers, talker_kv
+    return _lib, kernels, layers, talker_kv
 
 
 def _run_own(s):
-    kernels, layers, talker_kv = _package()
+    _lib, kernels, layers, talker_kv = _package()
     if "key" in s:
         kernels.paged_cache_write_int8_(s["key"], s["value"], s["cache"], s["scales"], s["pages"], s["offsets"])
         return kernels.paged_cache_read_int8(s["cache"], s["scales"], s["read_pages"], s["read_offsets"])
@@ -291,7 +291,8 @@ def _run_own(s):
             qo_indptr=s["qo_indptr"], paged_kv_indptr=s["kv_indptr"], paged_kv_indices=s["kv_indices"],
             paged_kv_last_page_len=s["last_page_len"], position_ids=None, write_pages=None, write_offsets=None,
             padding_pages=())
-        return kernels.paged_attention_int8(s["query"], s["cache"], s["scales"], metadata)
+        parts = _lib.NQ_ATTN_DECODE if s["qo_indptr"] is None else _lib.NQ_ATTN_PREFILL
+        return kernels.paged_attention_int8(s["query"], s["cache"], s["scales"], metadata, parts=parts)
     codes, scales = layers.quantize_int8_rows(s["x"])
     return layers.linear_int8(codes, scales, s["weight"], s["weight_scales"])
 
