@@ -207,6 +207,74 @@ int nq_paged_attention_noalloc(const int32_t *qo_indptr, const int32_t *kv_indpt
                                void *stream);
 
 /*
+ * The paged K/V cache in 8 bits.  No counterpart in the reference, whose cache
+ * is bf16 (executor/talker_kv.py:336-340).  codes: int8, element (page, kind,
+ * slot, kv_head, d) at page*c_page + kind*c_kind + slot*c_slot + kv_head*c_head
+ * + d; scales: fp32, one for each block of 16 slots, kind and kv head, at
+ * page*s_page + kind*s_kind + (slot/16)*s_block + kv_head*s_head.  A value is
+ * code * scale.  page_size is a power of two of at least 16, head_dim 64 or
+ * 128; codes and their strides are multiples of 16 bytes (else
+ * NQ_ERR_UNSUPPORTED).
+ *
+ * nq_kv_int8_write quantises bf16 key / value [tokens, num_kv_heads, head_dim]
+ * (token and head strides k_s0, k_s1, v_s0, v_s1, multiples of 8) into the slots (write_pages[t],
+ * write_offsets[t]).  Consecutive tokens in consecutive slots of one block are a run.  With a =
+ * max |x| over a run of one kind and head, whose first slot in the block is o, the block's
+ * scale becomes e(a) if o == 0, else max(scale, e(a)), e(a) = the least power
+ * of two >= 2^-126 with a / e <= 127; the codes of slots below o are rescaled
+ * (rint, ties to even) when the scale grows, slots behind the run keep their
+ * codes and count as empty.  A NaN or infinity in the run, or a scale that is
+ * not finite, makes the block's scale NaN.  A slot outside the pool is skipped
+ * and sets status (device int32, may be NULL) to NQ_ERR_INVALID_ARGUMENT.  The
+ * runs of one call are in different blocks: what a block that two runs share
+ * holds afterwards is not specified.
+ *
+ * nq_kv_int8_read gives the values of slots (pages[t], offsets[t]) back as bf16
+ * (exact for scales that are powers of two; zeros, and status set, outside the pool).
+ */
+int nq_kv_int8_write(const uint16_t *key, int64_t k_s0, int64_t k_s1, const uint16_t *value,
+                     int64_t v_s0, int64_t v_s1, int tokens, int num_kv_heads, int head_dim,
+                     int8_t *codes, int64_t c_page, int64_t c_kind, int64_t c_slot, int64_t c_head,
+                     float *scales, int64_t s_page, int64_t s_kind, int64_t s_block, int64_t s_head,
+                     int num_pages, int page_size, const int64_t *write_pages,
+                     const int64_t *write_offsets, int32_t *status, void *stream);
+int nq_kv_int8_read(const int8_t *codes, int64_t c_page, int64_t c_kind, int64_t c_slot,
+                    int64_t c_head, const float *scales, int64_t s_page, int64_t s_kind,
+                    int64_t s_block, int64_t s_head, int num_pages, int page_size,
+                    const int64_t *pages, const int64_t *offsets, int tokens, int num_kv_heads,
+                    int head_dim, uint16_t *key, int64_t k_s0, int64_t k_s1, uint16_t *value,
+                    int64_t v_s0, int64_t v_s1, int32_t *status, void *stream);
+
+/*
+ * nq_paged_attention over the 8-bit cache, without a plan: the launches read
+ * the ragged metadata themselves.  kv_indptr [n_rows + 1] starts at 0 and does
+ * not decrease; entries are held to [0, num_indices], the length of kv_indices.
+ * parts: NQ_ATTN_DECODE (rows with one query), NQ_ATTN_PREFILL (rows with
+ * several, bottom-right causal), or both; NQ_ATTN_PREFILL alone takes the rows
+ * with one query too, NQ_ATTN_DECODE alone leaves rows with several out.
+ * qo_indptr may be NULL with NQ_ATTN_DECODE alone: row r then owns query r.  A
+ * query that sees no key (a row without pages, or more queries than keys) gets
+ * zeros; query tokens of no row are left as they were.  A page id outside
+ * [0, num_pages) is skipped and sets status (may be NULL) to
+ * NQ_ERR_INVALID_ARGUMENT.  Up to 16 query heads per kv head; q, out and their
+ * strides are multiples of 16 bytes.  workspace holds the partial results of
+ * rows cut over workgroups; calls that overlap in time need one each.  Results do not depend on
+ * the order in which workgroups run.
+ */
+int64_t nq_paged_attention_int8_workspace_bytes(int tokens, int rows, int num_qo_heads,
+                                                int num_kv_heads, int head_dim, int parts);
+int nq_paged_attention_int8(const int32_t *qo_indptr, const int32_t *kv_indptr,
+                            const int32_t *last_page_len, const int32_t *kv_indices, int n_rows,
+                            int num_indices, const uint16_t *q, int64_t q_s0, int64_t q_s1,
+                            int tokens, const int8_t *codes, int64_t c_page, int64_t c_kind,
+                            int64_t c_slot, int64_t c_head, const float *scales, int64_t s_page,
+                            int64_t s_kind, int64_t s_block, int64_t s_head, int num_pages,
+                            int page_size, int num_qo_heads, int num_kv_heads, int head_dim,
+                            float sm_scale, uint16_t *out, int64_t o_s0, int64_t o_s1, int parts,
+                            void *workspace, int64_t workspace_bytes, int32_t *status,
+                            void *stream);
+
+/*
  * Code-predictor short-cache attention: one query per row over the first
  * valid_length positions of a dense per-row cache.
  * Replaces decode_attn_nhd_short_cache (model/kernels.py:408-520).

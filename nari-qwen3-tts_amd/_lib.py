@@ -57,6 +57,13 @@ _SIGNATURES: dict[str, list] = {
                            _I, _I, _I, _P, _L, _P, _P],
     "nq_paged_attention_noalloc": [_P, _P, _P, _P, _I, _P, _L, _L, _P, _L, _L, _L, _L, _I, _I, _I, _I, _I, _F,
                                    _P, _L, _L, _I, _I, _I, _P, _P],
+    "nq_kv_int8_write": [_P, _L, _L, _P, _L, _L, _I, _I, _I, _P, _L, _L, _L, _L, _P, _L, _L, _L, _L, _I, _I, _P, _P, _P,
+                         _P],
+    "nq_kv_int8_read": [_P, _L, _L, _L, _L, _P, _L, _L, _L, _L, _I, _I, _P, _P, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P,
+                        _P],
+    "nq_paged_attention_int8_workspace_bytes": [_I, _I, _I, _I, _I, _I],
+    "nq_paged_attention_int8": [_P, _P, _P, _P, _I, _I, _P, _L, _L, _I, _P, _L, _L, _L, _L, _P, _L, _L, _L, _L, _I, _I,
+                                _I, _I, _I, _F, _P, _L, _L, _I, _P, _L, _P, _P],
     "nq_cp_short_attention": [_P, _L, _L, _P, _L, _L, _L, _L, _I, _I, _I, _I, _I, _F, _P, _L, _L, _P],
     "nq_cp_rope_short_attention": [_P, _I, _I, _P, _P, _P, _L, _F, _F, _I, _P, _L, _L, _P, _L, _L, _L, _L, _I, _I, _I, _I,
                                    _F, _P, _L, _L, _P],
@@ -123,6 +130,7 @@ _SIGNATURES: dict[str, list] = {
 _RESTYPES = {
     "nq_status_string": ctypes.c_char_p,
     "nq_attention_workspace_bytes": ctypes.c_int64,
+    "nq_paged_attention_int8_workspace_bytes": ctypes.c_int64,
     "nq_linear_workspace_bytes": ctypes.c_int64,
     "nq_linear_fp8_workspace_bytes": ctypes.c_int64,
     "nq_tgemm_workspace_bytes": ctypes.c_int64,
@@ -183,6 +191,16 @@ def call(name: str, *args) -> None:
         check(status, name)
 
 
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` with ``device`` current, for tensors on another device than the current one."""
+
+    if device.index is None or device.index == torch.cuda.current_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -200,3 +218,10 @@ def require_device(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and t.device.type != "cuda":
             raise ValueError("HIP kernels need tensors on the GPU (there is no CPU path)")
+
+
+def require_one_device(first: torch.Tensor, *tensors: torch.Tensor | None) -> None:
+    require_device(first, *tensors)
+    for t in tensors:
+        if t is not None and t.device != first.device:
+            raise ValueError("HIP kernels need their tensors on one device")

@@ -1,0 +1,1094 @@
+// The paged K/V cache in 8 bits: int8 codes in the pages' own layout
+// [pages, 2, page_size, Hkv, D] and one fp32 scale for each block of 16 slots,
+// kind (K, V) and kv head; its write, its read back, and the attention over it.
+//
+// Write.  A block's scale is a power of two, the least s with max |x| / s <= 127
+// over the tokens it holds, so x / s and a rescale of the codes by old / new are
+// exact up to the one rounding (ties to even): the codes do not depend on how the
+// arithmetic is carried out, a block is rescaled only when its range grows by a
+// factor of two, and the roundings of all its rescales add up to less than one
+// step (1/2 + 1/4 + ...).  The price is a step of up to twice max |x| / 127.
+//
+// Attention.  S = q . c_K with the codes widened to bf16 (exact), each block's
+// scale applied to its 16 columns of fp32 scores; P times the V scale of its
+// block rounded to bf16, the codes of V widened, fp32 sums.  So the cache moves half
+// the bytes of a bf16 one and is never written out wider.
+#include "nq_common.h"
+#include "nq_internal.h"
+
+namespace nq {
+namespace {
+
+constexpr int kBlk = 16;  // slots that share a scale
+constexpr int kKv8Threads = 256;
+constexpr int kKv8Waves = kKv8Threads / kWave;
+constexpr float kMinScale = 1.1754943508222875e-38f;  // 2^-126
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float floatx4_t __attribute__((ext_vector_type(4)));
+typedef float floatx16_t __attribute__((ext_vector_type(16)));
+
+struct Pool8 {
+    int8_t *codes;
+    int64_t c_page, c_kind, c_slot, c_head;
+    float *scales;
+    int64_t s_page, s_kind, s_block, s_head;
+    int num_pages, page_size;
+};
+
+// Least power of two s >= 2^-126 with amax / s <= 127 (amax finite, >= 0): amax = m 2^E, 1 <= m < 2,
+// gives 2^(E - 6) where m <= 127 / 64, else 2^(E - 5).
+__device__ __forceinline__ float scale_for(float amax) {
+    const uint32_t u = __float_as_uint(amax);
+    const int e = static_cast<int>(u >> 23) - 6 + ((u & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+    return e < 1 ? kMinScale : __uint_as_float(static_cast<uint32_t>(e) << 23);
+}
+
+__device__ __forceinline__ uint32_t pack4_i8(float a, float b, float c, float d) {
+    const int ia = static_cast<int>(rintf(a)), ib = static_cast<int>(rintf(b)), ic = static_cast<int>(rintf(c)),
+              id = static_cast<int>(rintf(d));
+    return (ia & 0xff) | ((ib & 0xff) << 8) | ((ic & 0xff) << 16) | (static_cast<uint32_t>(id) << 24);
+}
+
+template <int B>
+__device__ __forceinline__ float byte_f32(uint32_t w) {
+    return static_cast<float>(static_cast<int8_t>(w >> (8 * B)));
+}
+
+// Eight codes widened to bf16: integers of at most 8 bits, so the upper half of the float is exact.
+__device__ __forceinline__ uint32_t pair_bf16(float lo, float hi) {
+    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+__device__ __forceinline__ bf16x8_t widen8(uint32_t a, uint32_t b) {
+    const uint4 r = make_uint4(pair_bf16(byte_f32<0>(a), byte_f32<1>(a)), pair_bf16(byte_f32<2>(a), byte_f32<3>(a)),
+                               pair_bf16(byte_f32<0>(b), byte_f32<1>(b)), pair_bf16(byte_f32<2>(b), byte_f32<3>(b)));
+    return __builtin_bit_cast(bf16x8_t, r);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Write: a wave takes the leaders among `group` consecutive tokens for one (kind, head).  A leader is a
+// token that does not continue its predecessor's block (same page, next slot, same block of 16); its run
+// are the tokens behind it that do.  So the slot map alone says who owns a block, a run's tokens are
+// quantised with one scale, and a block's earlier slots are read only by the wave that may rescale them.
+// Lane l holds slots l / (D/8) + i * (512/D), values 8 (l % (D/8)) .. + 7.
+template <int D>
+__global__ void __launch_bounds__(kKv8Threads)
+kv8_write_kernel(const uint16_t *__restrict__ key, int64_t k_s0, int64_t k_s1, const uint16_t *__restrict__ value,
+                 int64_t v_s0, int64_t v_s1, const int64_t *__restrict__ pages, const int64_t *__restrict__ offsets,
+                 int tokens, int heads, int group, Pool8 pool, int32_t *__restrict__ status) {
+    constexpr int LPT = D / 8, SPI = kWave / LPT, ITERS = kBlk / SPI;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int which = blockIdx.y * kKv8Waves + threadIdx.x / kWave;
+    if (which >= 2 * heads) return;
+    const int kind = which >= heads ? 1 : 0, head = which - kind * heads;
+    const int base = blockIdx.x * group;
+
+    // lane i: token base - 1 + i and whether it continues token base - 2 + i
+    const int t = base - 1 + lane;
+    const bool in = lane < 33 && t >= 0 && t < tokens;
+    const int64_t page = in ? pages[t] : -1, off = in ? offsets[t] : -1;
+    const bool ok = in && page >= 0 && page < pool.num_pages && off >= 0 && off < pool.page_size;
+    if (in && !ok && lane >= 1 && lane <= group && which == 0 && status) *status = NQ_ERR_INVALID_ARGUMENT;
+    const int ipage = ok ? static_cast<int>(page) : -1, ioff = ok ? static_cast<int>(off) : -1;
+    const int p_page = __shfl_up(ipage, 1, kWave), p_off = __shfl_up(ioff, 1, kWave);
+    const bool cont = ok && lane >= 1 && p_page == ipage && ioff == p_off + 1 && (ioff & (kBlk - 1)) != 0;
+    const uint64_t follows = __ballot(cont), valid = __ballot(ok);
+
+    const uint16_t *src = kind ? value : key;
+    const int64_t s0 = kind ? v_s0 : k_s0, s1 = kind ? v_s1 : k_s1;
+    const int part = lane % LPT, slot0 = lane / LPT;
+    for (int i = 1; i <= group; ++i) {
+        if (!((valid >> i) & 1) || ((follows >> i) & 1)) continue;
+        const uint64_t behind = ~(follows >> (i + 1));
+        const int run = 1 + __builtin_ctzll(behind);  // at most 16: a block's first slot never follows
+        const int pg = __builtin_amdgcn_readlane(ipage, i), of = __builtin_amdgcn_readlane(ioff, i);
+        const int first = of & (kBlk - 1);
+        int8_t *dst = pool.codes + pg * pool.c_page + kind * pool.c_kind + (of - first) * pool.c_slot +
+                      head * pool.c_head + part * 8;
+        float *sp = pool.scales + pg * pool.s_page + kind * pool.s_kind + (of / kBlk) * pool.s_block +
+                    head * pool.s_head;
+        const uint16_t *row = src + (base + i - 1) * s0 + head * s1 + part * 8;
+        const float old = first ? *sp : 0.f;
+        uint4 x[ITERS];
+        uint2 held[ITERS];
+#pragma unroll
+        for (int k = 0; k < ITERS; ++k) {
+            const int slot = slot0 + k * SPI;
+            const bool fresh = slot >= first && slot < first + run;
+            x[k] = fresh ? *reinterpret_cast<const uint4 *>(row + (slot - first) * s0) : make_uint4(0, 0, 0, 0);
+            held[k] = slot < first ? *reinterpret_cast<const uint2 *>(dst + slot * pool.c_slot) : make_uint2(0, 0);
+        }
+        float amax = 0.f;
+        bool odd = false;  // NaN or infinity among the new values
+#pragma unroll
+        for (int k = 0; k < ITERS; ++k) {
+            float f[8];
+            unpack8(x[k], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                amax = fmaxf(amax, fabsf(f[e]));
+                odd |= !(fabsf(f[e]) < __builtin_inff());
+            }
+        }
+        amax = group_max<kWave>(amax);
+        // a scale that is NaN stays: every query that reads the block answers NaN
+        const bool bad = __any(odd) || !(old < __builtin_inff());
+        const float own = scale_for(amax);
+        const float s = bad ? __builtin_nanf("") : (first && old > own ? old : own);
+        const float inv = bad ? 0.f : 1.0f / s;  // exact: s is a power of two, at most 2^122
+        const float shrink = bad ? 1.f : old / s;
+#pragma unroll
+        for (int k = 0; k < ITERS; ++k) {
+            const int slot = slot0 + k * SPI;
+            if (slot >= first && slot < first + run) {
+                float f[8];
+                unpack8(x[k], f);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = bad ? 0.f : f[e] * inv;
+                *reinterpret_cast<uint2 *>(dst + slot * pool.c_slot) =
+                    make_uint2(pack4_i8(f[0], f[1], f[2], f[3]), pack4_i8(f[4], f[5], f[6], f[7]));
+            } else if (slot < first && shrink != 1.f) {
+                const uint32_t a = held[k].x, b = held[k].y;
+                *reinterpret_cast<uint2 *>(dst + slot * pool.c_slot) = make_uint2(
+                    pack4_i8(byte_f32<0>(a) * shrink, byte_f32<1>(a) * shrink, byte_f32<2>(a) * shrink,
+                             byte_f32<3>(a) * shrink),
+                    pack4_i8(byte_f32<0>(b) * shrink, byte_f32<1>(b) * shrink, byte_f32<2>(b) * shrink,
+                             byte_f32<3>(b) * shrink));
+            }
+        }
+        if (lane == 0) *sp = s;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Read back: thread per 16 codes of one (token, kind, head).
+template <int D>
+__global__ void __launch_bounds__(kKv8Threads)
+kv8_read_kernel(Pool8 pool, const int64_t *__restrict__ pages, const int64_t *__restrict__ offsets, int tokens,
+                int heads, uint16_t *__restrict__ key, int64_t k_s0, int64_t k_s1, uint16_t *__restrict__ value,
+                int64_t v_s0, int64_t v_s1, int32_t *__restrict__ status) {
+    constexpr int VEC = D / 16;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kKv8Threads + threadIdx.x;
+    const int per = 2 * heads * VEC;
+    const int64_t t = at / per;
+    if (t >= tokens) return;
+    int rest = static_cast<int>(at - t * per);
+    const int vec = rest % VEC;
+    rest /= VEC;
+    const int head = rest % heads, kind = rest / heads;
+    const int64_t page = pages[t], off = offsets[t];
+    uint16_t *dst = kind ? value + t * v_s0 + head * v_s1 : key + t * k_s0 + head * k_s1;
+    uint4 *o = reinterpret_cast<uint4 *>(dst + vec * 16);
+    if (page < 0 || page >= pool.num_pages || off < 0 || off >= pool.page_size) {
+        if (status) *status = NQ_ERR_INVALID_ARGUMENT;
+        o[0] = o[1] = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    const uint4 c = *reinterpret_cast<const uint4 *>(pool.codes + page * pool.c_page + kind * pool.c_kind +
+                                                     off * pool.c_slot + head * pool.c_head + vec * 16);
+    const float s = pool.scales[page * pool.s_page + kind * pool.s_kind + (off / kBlk) * pool.s_block +
+                                head * pool.s_head];
+    auto four = [&](uint32_t w) {
+        return make_uint2(pack2_bf16(byte_f32<0>(w) * s, byte_f32<1>(w) * s),
+                          pack2_bf16(byte_f32<2>(w) * s, byte_f32<3>(w) * s));
+    };
+    const uint2 a = four(c.x), b = four(c.y), d = four(c.z), e = four(c.w);
+    o[0] = make_uint4(a.x, a.y, b.x, b.y);
+    o[1] = make_uint4(d.x, d.y, e.x, e.y);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Attention.
+constexpr float kLog2e8 = 1.4426950408889634f;
+
+struct Attend8 {
+    const uint16_t *q;
+    int64_t q_s0, q_s1;
+    uint16_t *out;
+    int64_t o_s0, o_s1;
+    const int32_t *qo_indptr, *kv_indptr, *kv_indices, *last_page_len;
+    int rows, tokens, n_indices, group, heads;  // group: query heads per kv head
+    int bpp_log2;                               // blocks of 16 per page
+    float scale;                                // sm_scale log2(e)
+    int32_t *status;
+};
+
+// Largest r in [0, n) with f(r) <= x for a non-decreasing f with f(0) <= x, found by the whole wave: 64
+// probes at once, so one round of loads up to 64 rows and two up to 4096.
+template <typename F>
+__device__ __forceinline__ int wave_find_le(int n, int x, F f) {
+    const int lane = threadIdx.x & (kWave - 1);
+    int lo = 0, count = n;
+    while (count > 1) {
+        const int step = (count + kWave - 1) / kWave;
+        const int at = lane * step;
+        const bool le = at < count && f(lo + at) <= x;
+        const uint64_t m = __ballot(le);
+        const int hit = m ? 63 - __builtin_clzll(m) : 0;
+        lo += hit * step;
+        count = step < count - hit * step ? step : count - hit * step;
+    }
+    return lo;
+}
+
+// What a row asks for.
+struct Row8 {
+    int first_page, n_pages, kv_len, q0, q_len;
+};
+__device__ __forceinline__ Row8 row_of(const Attend8 &a, int r) {
+    Row8 w;
+    int b = a.kv_indptr[r], e = a.kv_indptr[r + 1];
+    b = b < 0 ? 0 : (b > a.n_indices ? a.n_indices : b);
+    e = e < b ? b : (e > a.n_indices ? a.n_indices : e);
+    w.first_page = b;
+    w.n_pages = e - b;
+    const int ps = kBlk << a.bpp_log2;
+    int last = a.last_page_len[r];
+    last = last < 1 ? 1 : (last > ps ? ps : last);
+    w.kv_len = w.n_pages > 0 ? (w.n_pages - 1) * ps + last : 0;
+    w.q0 = a.qo_indptr ? a.qo_indptr[r] : r;
+    w.q_len = a.qo_indptr ? a.qo_indptr[r + 1] - w.q0 : 1;
+    if (w.q0 < 0 || w.q_len < 0 || w.q0 > a.tokens - w.q_len) w.q_len = 0;  // not this call's queries
+    return w;
+}
+
+// Decode rows.  The blocks of all rows, in kv_indices order, are cut into equal spans, one a wave of every
+// kv head; kv_indptr itself is the prefix sum that says whose a block is, so there is no plan launch.
+// A row inside one span is finished by its wave; a row over several leaves (m, l, o) partials, which
+// kv8_merge_kernel joins in order.
+struct Spans {
+    int64_t blocks;
+    int waves;
+};
+__device__ __forceinline__ Spans spans_of(const Attend8 &a, int waves) {
+    int p = a.kv_indptr[a.rows];
+    p = p < 0 ? 0 : (p > a.n_indices ? a.n_indices : p);
+    Spans s;
+    s.blocks = static_cast<int64_t>(p) << a.bpp_log2;
+    const int64_t most = (s.blocks + 1) / 2;  // a wave's step is two blocks
+    s.waves = static_cast<int>(most < waves ? (most < 1 ? 1 : most) : waves);
+    return s;
+}
+__device__ __forceinline__ int64_t span_start(const Spans &s, int64_t i) { return i * s.blocks / s.waves; }
+// the span that holds block b: the largest i with span_start(i) <= b
+__device__ __forceinline__ int span_of(const Spans &s, int64_t b) {
+    return static_cast<int>(((b + 1) * s.waves + s.blocks - 1) / s.blocks) - 1;
+}
+
+// A step: 32 keys (two blocks).  S^T = K Q^T with mfma_16x16x32: lane l loads token l % 16 of each block, values
+// (D/4)(l / 16) .. of K, and holds the scores of query slot l % 16 against tokens 4 (l / 16) + i.  Those are, in
+// that order, the 8 keys of the lane's group in out^T = V^T P^T, so P needs no exchange between lanes; V is loaded
+// as (D/16) values of each of the 8 tokens, and the byte a conversion picks does the transposition.
+template <int D>
+struct Step8 {
+    uint4 k[2][D / 64];
+    uint32_t v[8][D / 64];  // D/16 bytes of a token
+    float ks[2], vs[2];
+    int on[2];  // the block's page is in the pool
+};
+
+template <int D>
+__global__ void __launch_bounds__(kKv8Threads)
+kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml, float *__restrict__ part_o) {
+    constexpr int W = D / 64;  // 16-byte loads of K, dwords of V
+    const int lane = threadIdx.x & (kWave - 1);
+    const int head = blockIdx.x % a.heads;
+    const int wi = (blockIdx.x / a.heads) * kKv8Waves + threadIdx.x / kWave;
+    const Spans sp = spans_of(a, waves);
+    if (wi >= sp.waves) return;
+    const int64_t b0 = span_start(sp, wi), b1 = span_start(sp, wi + 1);
+    if (b0 >= b1) return;
+    const int c = lane & 15, grp = lane >> 4;
+
+    const int8_t *kbase = pool.codes + head * pool.c_head;
+    const int k_lane = static_cast<int>(c * pool.c_slot) + grp * (D / 4);
+    const int64_t v_lane = pool.c_kind + 4 * grp * pool.c_slot + c * (D / 16);
+
+    // a window of 64 blocks' pages and scales, one a lane
+    int64_t wbase = -1;
+    int w_pid = 0;
+    float w_ks = 0.f, w_vs = 0.f;
+    auto open_window = [&](int64_t b) {
+        wbase = b;
+        const int64_t mine = b + lane;
+        w_pid = -1;
+        w_ks = w_vs = 0.f;
+        if (mine < b1) {
+            const int pid = a.kv_indices[mine >> a.bpp_log2];
+            if (pid >= 0 && pid < pool.num_pages) {
+                const int blk = static_cast<int>(mine & ((1 << a.bpp_log2) - 1));
+                const float *s = pool.scales + pid * pool.s_page + blk * pool.s_block + head * pool.s_head;
+                w_pid = pid;
+                w_ks = s[0];
+                w_vs = s[pool.s_kind];
+            } else if (a.status) {
+                *a.status = NQ_ERR_INVALID_ARGUMENT;
+            }
+        }
+    };
+    auto fetch = [&](int64_t b, Step8<D> &st) {
+        if (wbase < 0 || b + 1 >= wbase + kWave) open_window(b);
+        const int i0 = static_cast<int>(b - wbase);
+        const int i1 = b + 1 < b1 ? i0 + 1 : i0;
+        const int8_t *at[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const int i = m ? i1 : i0;
+            const int pid = __builtin_amdgcn_readlane(w_pid, i);
+            st.on[m] = pid >= 0;
+            st.ks[m] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_ks), i));
+            st.vs[m] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_vs), i));
+            const int blk = static_cast<int>((b + i - i0) & ((1 << a.bpp_log2) - 1));
+            at[m] = kbase + (pid < 0 ? 0 : pid) * pool.c_page + blk * (kBlk * pool.c_slot);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+                st.k[m][w] = *reinterpret_cast<const uint4 *>(at[m] + k_lane + 16 * w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int8_t *p = at[e / 4] + v_lane + (e % 4) * pool.c_slot;
+            if constexpr (W == 2) {
+                const uint2 d = *reinterpret_cast<const uint2 *>(p);
+                st.v[e][0] = d.x;
+                st.v[e][1] = d.y;
+            } else {
+                st.v[e][0] = *reinterpret_cast<const uint32_t *>(p);
+            }
+        }
+    };
+
+    Step8<D> next;
+    int64_t held = b0;
+    fetch(b0, next);
+    // the row of the first block, over the block ends of rows in page units
+    int r = wave_find_le(a.rows, static_cast<int>(b0 >> a.bpp_log2), [&](int i) { return a.kv_indptr[i]; });
+
+    int64_t b = b0;
+    while (b < b1 && r < a.rows) {
+        const Row8 row = row_of(a, r);
+        const int64_t rs = static_cast<int64_t>(row.first_page) << a.bpp_log2;
+        const int64_t re = static_cast<int64_t>(row.first_page + row.n_pages) << a.bpp_log2;
+        if (re <= b) {
+            ++r;
+            continue;
+        }
+        if (rs > b) {  // pages of no row
+            b = rs < b1 ? rs : b1;
+            continue;
+        }
+        const int64_t stop = re < b1 ? re : b1;
+        if (row.q_len != 1) {
+            b = stop;
+            ++r;
+            continue;
+        }
+        bf16x8_t qf[D / 32];
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (c < a.group)
+                v = *reinterpret_cast<const uint4 *>(a.q + row.q0 * a.q_s0 + (head * a.group + c) * a.q_s1 +
+                                                     grp * (D / 4) + 8 * s);
+            qf[s] = __builtin_bit_cast(bf16x8_t, v);
+        }
+        floatx4_t acc[D / 16];
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) acc[j] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+        float m_run = -__builtin_inff(), l_run = 0.f;
+        bool any = false;
+        for (; b < stop; b += 2) {
+            if (held != b) fetch(b, next);
+            const Step8<D> cur = next;
+            const int64_t ahead = b + 2 < stop ? b + 2 : stop;
+            if (ahead < b1) {
+                fetch(ahead, next);
+                held = ahead;
+            }
+            int nv[2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                const int64_t left = row.kv_len - (b + m - rs) * kBlk;
+                nv[m] = b + m < stop && cur.on[m] && left > 0 ? static_cast<int>(left < kBlk ? left : kBlk) : 0;
+            }
+            if (nv[0] + nv[1] == 0) continue;
+            any = true;
+            float p[8];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                floatx4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const uint4 k = cur.k[m][w];
+                    s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(k.x, k.y), qf[2 * w], s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(k.z, k.w), qf[2 * w + 1], s, 0, 0, 0);
+                }
+                const float f = cur.ks[m] * a.scale;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[4 * m + i] = 4 * grp + i < nv[m] ? s[i] * f : -__builtin_inff();
+            }
+            float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+            top = fmaxf(top, __shfl_xor(top, 16, kWave));
+            top = fmaxf(top, __shfl_xor(top, 32, kWave));
+            const float m_new = fmaxf(m_run, top);
+            if (__any(m_new != m_run)) {
+                const float alpha = m_run == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+                l_run *= alpha;
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) acc[j] *= alpha;
+                m_run = m_new;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                p[i] = 4 * grp + (i & 3) < nv[i / 4] ? __builtin_amdgcn_exp2f(p[i] - m_run) : 0.f;
+                l_run += p[i];
+                // a block that is masked whole may hold any scale
+                p[i] = p[i] == 0.f ? 0.f : p[i] * cur.vs[i / 4];
+            }
+            const uint4 pw = make_uint4(pack2_bf16(p[0], p[1]), pack2_bf16(p[2], p[3]), pack2_bf16(p[4], p[5]),
+                                        pack2_bf16(p[6], p[7]));
+            const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pw);
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+#define NQ_V_FRAG(J)                                                                                                   \
+    {                                                                                                                  \
+        const uint4 vw = make_uint4(pair_bf16(byte_f32<J>(cur.v[0][w]), byte_f32<J>(cur.v[1][w])),                     \
+                                    pair_bf16(byte_f32<J>(cur.v[2][w]), byte_f32<J>(cur.v[3][w])),                     \
+                                    pair_bf16(byte_f32<J>(cur.v[4][w]), byte_f32<J>(cur.v[5][w])),                     \
+                                    pair_bf16(byte_f32<J>(cur.v[6][w]), byte_f32<J>(cur.v[7][w])));                    \
+        acc[4 * w + J] =                                                                                               \
+            __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vw), pf, acc[4 * w + J], 0, 0, 0);    \
+    }
+                NQ_V_FRAG(0)
+                NQ_V_FRAG(1)
+                NQ_V_FRAG(2)
+                NQ_V_FRAG(3)
+#undef NQ_V_FRAG
+            }
+        }
+        b = stop;
+        l_run += __shfl_xor(l_run, 16, kWave);
+        l_run += __shfl_xor(l_run, 32, kWave);
+        // the lane holds out[slot c][(D/4) grp + (D/16) i + j] in acc[j][i]
+        if (c < a.group) {
+            if (rs >= b0 && re <= b1) {
+                const float inv = any ? 1.0f / l_run : 0.f;
+                uint16_t *o = a.out + row.q0 * a.o_s0 + (head * a.group + c) * a.o_s1 + grp * (D / 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t w[D / 32];
+#pragma unroll
+                    for (int j = 0; j < D / 32; ++j) w[j] = pack2_bf16(acc[2 * j][i] * inv, acc[2 * j + 1][i] * inv);
+                    if constexpr (D == 128)
+                        *reinterpret_cast<uint4 *>(o + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+                    else
+                        *reinterpret_cast<uint2 *>(o + 4 * i) = make_uint2(w[0], w[1]);
+                }
+            } else {
+                const int64_t slot = ((static_cast<int64_t>(head) * waves + wi) * 2 + (rs >= b0 ? 1 : 0)) * a.group + c;
+                if (grp == 0) part_ml[slot] = make_float2(m_run, l_run);
+                float *o = part_o + slot * D + grp * (D / 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < D / 16; j += 4)
+                        *reinterpret_cast<float4 *>(o + (D / 16) * i + j) =
+                            make_float4(acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]);
+            }
+        }
+        if (re <= b1) ++r;
+    }
+}
+
+// Joins a decode row's partials: span i0, where the row begins, left its slot 1, the spans behind it slot 0.
+// Weights 2^(m_i - m), in span order.  A row without pages gets zeros.
+template <int D>
+__global__ void __launch_bounds__(kKv8Threads)
+kv8_merge_kernel(Attend8 a, int waves, const float2 *__restrict__ part_ml, const float *__restrict__ part_o) {
+    __shared__ float s_m[16], s_inv[16];
+    __shared__ float s_o[kKv8Waves][16 * D];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int r = blockIdx.x, head = blockIdx.y;
+    const Row8 row = row_of(a, r);
+    if (row.q_len != 1) return;
+    uint16_t *out = a.out + row.q0 * a.o_s0 + head * a.group * a.o_s1;
+    const int vecs = a.group * (D / 4);
+    if (row.n_pages == 0) {
+        for (int v = threadIdx.x; v < vecs; v += kKv8Threads)
+            *reinterpret_cast<uint2 *>(out + (v / (D / 4)) * a.o_s1 + (v % (D / 4)) * 4) = make_uint2(0, 0);
+        return;
+    }
+    const Spans sp = spans_of(a, waves);
+    const int64_t rs = static_cast<int64_t>(row.first_page) << a.bpp_log2;
+    const int64_t re = static_cast<int64_t>(row.first_page + row.n_pages) << a.bpp_log2;
+    const int i0 = span_of(sp, rs), i1 = span_of(sp, re - 1);
+    if (i0 == i1) return;
+    const int n = i1 - i0 + 1;
+    const int64_t base = static_cast<int64_t>(head) * waves + i0;
+    auto slot = [&](int i, int g) { return ((base + i) * 2 + (i == 0 ? 1 : 0)) * a.group + g; };
+    for (int g = wave; g < a.group; g += kKv8Waves) {
+        float m = -__builtin_inff();
+        for (int i = lane; i < n; i += kWave) m = fmaxf(m, part_ml[slot(i, g)].x);
+        m = group_max<kWave>(m);
+        float l = 0.f;
+        for (int i = lane; i < n; i += kWave) {
+            const float2 ml = part_ml[slot(i, g)];
+            l += ml.y * (ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - m));
+        }
+        l = group_sum<kWave>(l);
+        if (lane == 0) {
+            s_m[g] = m;
+            s_inv[g] = l == 0.f && m == -__builtin_inff() ? 0.f : 1.0f / l;  // no page of the row in the pool
+        }
+    }
+    __syncthreads();
+    for (int v = lane; v < vecs; v += kWave) {
+        const int g = v / (D / 4);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = wave; i < n; i += kKv8Waves) {
+            const int64_t at = slot(i, g);
+            const float2 ml = part_ml[at];
+            const float4 x = *reinterpret_cast<const float4 *>(part_o + at * D + (v % (D / 4)) * 4);
+            const float w = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - s_m[g]);
+            o.x += w * x.x;
+            o.y += w * x.y;
+            o.z += w * x.z;
+            o.w += w * x.w;
+        }
+        *reinterpret_cast<float4 *>(&s_o[wave][4 * v]) = o;
+    }
+    __syncthreads();
+    for (int v = threadIdx.x; v < vecs; v += kKv8Threads) {
+        const int g = v / (D / 4);
+        float4 o = *reinterpret_cast<const float4 *>(&s_o[0][4 * v]);
+#pragma unroll
+        for (int w = 1; w < kKv8Waves; ++w) {
+            const float4 x = *reinterpret_cast<const float4 *>(&s_o[w][4 * v]);
+            o.x += x.x;
+            o.y += x.y;
+            o.z += x.z;
+            o.w += x.w;
+        }
+        const float inv = s_inv[g];
+        *reinterpret_cast<uint2 *>(out + g * a.o_s1 + (v % (D / 4)) * 4) =
+            make_uint2(pack2_bf16(o.x * inv, o.y * inv), pack2_bf16(o.z * inv, o.w * inv));
+    }
+}
+
+// Rows of several queries.  A workgroup takes 128 columns (128 / G queries times the G query heads of one kv
+// head) against 64-key tiles, a wave 32 columns with mfma_32x32x16: S^T = K Q^T, out^T = V^T P^T, so a
+// column's scores, maximum and output stay in two lanes.  K and V are widened to bf16 once a workgroup, on
+// their way to LDS (V transposed, keys in the order in which a lane holds P); a tile's loads are in flight while
+// the one before it is multiplied.  With few tiles the key range is cut into pieces, joined by kv8_join_kernel.
+constexpr int kCols = 128, kKeys = 64;
+
+struct Tile8 {
+    int q0, n_q, limit0;  // first query token, queries, keys the first of them sees
+    int n_keys;           // keys the last of them sees
+};
+__device__ __forceinline__ int tile_queries(const Attend8 &a) { return kCols / a.group; }
+// Slot s of the launch is tile s - (qo_indptr[r] / nq + r) of row r: those bases need no scan, and a row's
+// share is enough for its tiles.  False where the slot is no tile of this launch.
+__device__ __forceinline__ bool tile_of(const Attend8 &a, int slot, int skip_single, Row8 &row, Tile8 &t) {
+    const int nq = tile_queries(a);
+    const int r = wave_find_le(a.rows, slot, [&](int i) { return a.qo_indptr[i] / nq + i; });
+    row = row_of(a, r);
+    const int first = (slot - (row.q0 / nq + r)) * nq;
+    if (first < 0 || first >= row.q_len || (skip_single && row.q_len == 1)) return false;
+    t.q0 = row.q0 + first;
+    t.n_q = row.q_len - first < nq ? row.q_len - first : nq;
+    t.limit0 = row.kv_len - row.q_len + first + 1;
+    const int last = t.limit0 + t.n_q - 1;
+    t.n_keys = last < 0 ? 0 : last;
+    return true;
+}
+__device__ __forceinline__ int pieces_of(const Tile8 &t, int splits) {
+    const int n = (t.n_keys + kKeys - 1) / kKeys / 4;  // at least four key tiles a piece
+    return n < 1 ? 1 : (n < splits ? n : splits);
+}
+
+template <int D>
+struct Smem8 {
+    uint4 k[2][kKeys * (D / 8)];
+    uint4 v[2][D * (kKeys / 8)];
+    float ks[2][kKeys / kBlk], vs[2][kKeys / kBlk];
+};
+// 16-byte chunk positions, exclusive-ored so that eight neighbouring rows, and the writes of a stage, spread over
+// all banks.
+template <int D>
+__device__ __forceinline__ int k_chunk(int key, int chunk) {
+    return key * (D / 8) + (chunk ^ (key & 7));
+}
+__device__ __forceinline__ int v_chunk(int d, int chunk) { return d * (kKeys / 8) + (chunk ^ ((d ^ (d >> 3)) & 7)); }
+
+template <int D>
+__global__ void __launch_bounds__(kKv8Threads, 2)
+kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single, float2 *__restrict__ part_ml,
+                   float *__restrict__ part_o) {
+    constexpr int W = D / 64;
+    __shared__ Smem8<D> sm;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int head = blockIdx.x % a.heads;
+    const int slot = slots - 1 - static_cast<int>(blockIdx.x) / a.heads;  // the longest key ranges first
+    Row8 row;
+    Tile8 t;
+    if (!tile_of(a, slot, skip_single, row, t)) return;
+    const int pieces = pieces_of(t, splits);
+    const int piece = blockIdx.y;
+    if (piece >= pieces) return;
+    const int n_kt = (t.n_keys + kKeys - 1) / kKeys;
+    const int kt0 = static_cast<int>(static_cast<int64_t>(n_kt) * piece / pieces);
+    const int kt1 = static_cast<int>(static_cast<int64_t>(n_kt) * (piece + 1) / pieces);
+
+    const int c = lane & 31, half = lane >> 5;
+    const int col = wave * 32 + c;
+    const int qi = col / a.group, g = col - qi * a.group;
+    const bool live = qi < t.n_q;
+    const int limit = live ? t.limit0 + qi : 0;
+    bf16x8_t qf[D / 16];
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (live)
+            v = *reinterpret_cast<const uint4 *>(a.q + (t.q0 + qi) * a.q_s0 + (head * a.group + g) * a.q_s1 + 16 * s +
+                                                 8 * half);
+        qf[s] = __builtin_bit_cast(bf16x8_t, v);
+    }
+
+    // staging: K thread t holds 16-byte pieces t % 4 (and + 4) of key t / 4; V thread t holds D/16 values of the four keys
+    // 4 (t / 16) ..
+    const int sk_key = threadIdx.x / 4, sk_piece = threadIdx.x & 3;
+    const int sv_quad = threadIdx.x / 16, sv_part = threadIdx.x & 15;
+    uint4 kr[W];
+    uint32_t vr[4][W];
+    float scale_r = 0.f;
+    const int n_blocks = (row.kv_len + kBlk - 1) / kBlk;
+    auto page_of = [&](int blk, bool &on) {  // blk: block of the row; beyond its keys, the last
+        const int b = blk < n_blocks ? blk : n_blocks - 1;
+        const int pid = a.kv_indices[row.first_page + (b >> a.bpp_log2)];
+        on = pid >= 0 && pid < pool.num_pages;
+        return on ? pid : 0;
+    };
+    auto load = [&](int kt) {
+        bool on;
+        {
+            const int blk = kt * (kKeys / kBlk) + sk_key / kBlk;
+            const int pid = page_of(blk, on);
+            const int b = blk < n_blocks ? blk : n_blocks - 1;
+            const int in_page = b & ((1 << a.bpp_log2) - 1);
+            const int8_t *p = pool.codes + pid * pool.c_page + (in_page * kBlk + sk_key % kBlk) * pool.c_slot +
+                              head * pool.c_head + 16 * sk_piece;
+#pragma unroll
+            for (int w = 0; w < W; ++w) kr[w] = *reinterpret_cast<const uint4 *>(p + 64 * w);
+        }
+        {
+            const int blk = kt * (kKeys / kBlk) + sv_quad / 4;
+            const int pid = page_of(blk, on);
+            const int b = blk < n_blocks ? blk : n_blocks - 1;
+            const int in_page = b & ((1 << a.bpp_log2) - 1);
+            const int8_t *p = pool.codes + pid * pool.c_page + pool.c_kind +
+                              (in_page * kBlk + 4 * (sv_quad % 4)) * pool.c_slot + head * pool.c_head +
+                              sv_part * (D / 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (W == 2) {
+                    const uint2 d = *reinterpret_cast<const uint2 *>(p + e * pool.c_slot);
+                    vr[e][0] = d.x;
+                    vr[e][1] = d.y;
+                } else {
+                    vr[e][0] = *reinterpret_cast<const uint32_t *>(p + e * pool.c_slot);
+                }
+            }
+        }
+        if (threadIdx.x < 2 * (kKeys / kBlk)) {  // the tile's scales; a block that is not there weighs nothing
+            const int kind = threadIdx.x / (kKeys / kBlk);
+            const int blk = kt * (kKeys / kBlk) + threadIdx.x % (kKeys / kBlk);
+            scale_r = 0.f;
+            if (blk < n_blocks) {
+                const int pid = page_of(blk, on);
+                scale_r = pool.scales[pid * pool.s_page + kind * pool.s_kind +
+                                      (blk & ((1 << a.bpp_log2) - 1)) * pool.s_block + head * pool.s_head];
+                if (!on) {
+                    scale_r = kind ? 0.f : -__builtin_inff();  // K: marks the block as absent
+                    if (a.status) *a.status = NQ_ERR_INVALID_ARGUMENT;
+                }
+            }
+        }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const int chunk = 8 * w + 2 * sk_piece;
+            sm.k[buf][k_chunk<D>(sk_key, chunk)] = __builtin_bit_cast(uint4, widen8(kr[w].x, kr[w].y));
+            sm.k[buf][k_chunk<D>(sk_key, chunk + 1)] = __builtin_bit_cast(uint4, widen8(kr[w].z, kr[w].w));
+        }
+        // key 8 a + 4 b + i of a block sits at position 8 b + 4 a + i
+        const int quad = sv_quad & 3, chunk = 2 * (sv_quad / 4) + (quad & 1), upper = quad >> 1;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+#define NQ_V_PUT(J)                                                                                        \
+    reinterpret_cast<uint2 *>(&sm.v[buf][v_chunk(sv_part * (D / 16) + 4 * w + J, chunk)])[upper] =         \
+        make_uint2(pair_bf16(byte_f32<J>(vr[0][w]), byte_f32<J>(vr[1][w])),                                \
+                   pair_bf16(byte_f32<J>(vr[2][w]), byte_f32<J>(vr[3][w])));
+            NQ_V_PUT(0)
+            NQ_V_PUT(1)
+            NQ_V_PUT(2)
+            NQ_V_PUT(3)
+#undef NQ_V_PUT
+        }
+        if (threadIdx.x < kKeys / kBlk) sm.ks[buf][threadIdx.x] = scale_r;
+        else if (threadIdx.x < 2 * (kKeys / kBlk)) sm.vs[buf][threadIdx.x - kKeys / kBlk] = scale_r;
+    };
+
+    floatx16_t acc[D / 32];
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[j][i] = 0.f;
+    float m_run = -__builtin_inff(), l_run = 0.f;
+    bool any = false;  // whether the column has seen a key
+    if (kt0 < kt1) {
+        load(kt0);
+        store(0);
+    }
+    for (int kt = kt0; kt < kt1; ++kt) {
+        const int buf = (kt - kt0) & 1;
+        __syncthreads();
+        if (kt + 1 < kt1) load(kt + 1);
+        float p[32];
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+            floatx16_t s;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                    __builtin_bit_cast(bf16x8_t, sm.k[buf][k_chunk<D>(32 * sub + c, 2 * k + half)]), qf[k], s, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[16 * sub + i] = s[i];
+        }
+        const int key0 = kt * kKeys;
+        float ks[4], vs[4];
+        bool whole = key0 + kKeys <= t.limit0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            ks[k] = sm.ks[buf][k];
+            vs[k] = sm.vs[buf][k];
+            whole = whole && ks[k] != -__builtin_inff();
+        }
+        float top = -__builtin_inff();
+        if (whole) {
+            any = true;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                p[i] *= ks[i / 8] * a.scale;
+                top = fmaxf(top, p[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                // lane's i: key 32 (i / 16) + 8 (i / 4 % 4) + 4 half + i % 4
+                const int key = key0 + 32 * (i / 16) + 8 * (i / 4 % 4) + 4 * half + (i & 3);
+                const bool see = key < limit && ks[i / 8] != -__builtin_inff();
+                any |= see;
+                p[i] = see ? p[i] * (ks[i / 8] * a.scale) : -__builtin_inff();
+                top = fmaxf(top, p[i]);
+            }
+        }
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        const float m_new = fmaxf(m_run, top);
+        if (__any(m_new != m_run)) {
+            const float alpha = m_run == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+            l_run *= alpha;
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) acc[j] *= alpha;
+            m_run = m_new;
+        }
+        const float m_use = any || m_run != -__builtin_inff() ? m_run : 0.f;
+        uint32_t pw[16];
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+                const float x = __builtin_amdgcn_exp2f(p[i] - m_use), y = __builtin_amdgcn_exp2f(p[i + 1] - m_use);
+                l_run += x + y;
+                pw[i / 2] = pack2_bf16(x * vs[i / 8], y * vs[i / 8]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+                float z[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int key = key0 + 32 * (i / 16) + 8 * (i / 4 % 4) + 4 * half + ((i + e) & 3);
+                    const bool see = key < limit && ks[i / 8] != -__builtin_inff();
+                    z[e] = see ? __builtin_amdgcn_exp2f(p[i + e] - m_use) : 0.f;
+                    l_run += z[e];
+                    z[e] = see ? z[e] * vs[i / 8] : 0.f;  // masked blocks may hold any scale
+                }
+                pw[i / 2] = pack2_bf16(z[0], z[1]);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const bf16x8_t pf =
+                __builtin_bit_cast(bf16x8_t, make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]));
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j)
+                acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                    __builtin_bit_cast(bf16x8_t, sm.v[buf][v_chunk(32 * j + c, 2 * k + half)]), pf, acc[j], 0, 0, 0);
+        }
+        if (kt + 1 < kt1) store(buf ^ 1);
+    }
+    l_run += __shfl_xor(l_run, 32, kWave);
+    any = any | static_cast<bool>(__shfl_xor(static_cast<int>(any), 32, kWave));
+    if (!live) return;
+    // the lane holds out[col][32 j + 8 (i / 4) + 4 half + i % 4] in acc[j][i]
+    if (pieces == 1) {
+        const float inv = any ? 1.0f / l_run : 0.f;
+        uint16_t *o = a.out + (t.q0 + qi) * a.o_s0 + (head * a.group + g) * a.o_s1 + 4 * half;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<uint2 *>(o + 32 * j + 2 * i) =
+                    make_uint2(pack2_bf16(acc[j][i] * inv, acc[j][i + 1] * inv),
+                               pack2_bf16(acc[j][i + 2] * inv, acc[j][i + 3] * inv));
+    } else {
+        const int64_t at = ((static_cast<int64_t>(slot) * a.heads + head) * splits + piece) * kCols + col;
+        if (half == 0) part_ml[at] = make_float2(any ? m_run : -__builtin_inff(), l_run);
+        float *o = part_o + at * D + 4 * half;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<float4 *>(o + 32 * j + 2 * i) =
+                    make_float4(acc[j][i], acc[j][i + 1], acc[j][i + 2], acc[j][i + 3]);
+    }
+}
+
+// Joins the pieces of a tile, in order: a wave a column at a time.
+template <int D>
+__global__ void __launch_bounds__(kKv8Threads)
+kv8_join_kernel(Attend8 a, int slots, int splits, int skip_single, const float2 *__restrict__ part_ml,
+                const float *__restrict__ part_o) {
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int head = blockIdx.x % a.heads, slot = static_cast<int>(blockIdx.x) / a.heads;
+    Row8 row;
+    Tile8 t;
+    if (!tile_of(a, slot, skip_single, row, t)) return;
+    const int pieces = pieces_of(t, splits);
+    if (pieces == 1) return;
+    const int64_t base = (static_cast<int64_t>(slot) * a.heads + head) * splits * kCols;
+    constexpr int PER = D / kWave;  // values a lane
+    for (int col = blockIdx.y * kKv8Waves + wave; col < t.n_q * a.group; col += gridDim.y * kKv8Waves) {
+        float m = -__builtin_inff();
+        for (int i = 0; i < pieces; ++i) m = fmaxf(m, part_ml[base + i * kCols + col].x);
+        float l = 0.f, o[PER];
+#pragma unroll
+        for (int e = 0; e < PER; ++e) o[e] = 0.f;
+        for (int i = 0; i < pieces; ++i) {
+            const float2 ml = part_ml[base + i * kCols + col];
+            const float w = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);
+            l += w * ml.y;
+            const float *x = part_o + (base + i * kCols + col) * D + PER * lane;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) o[e] += w * x[e];
+        }
+        const bool none = l == 0.f && m == -__builtin_inff();
+        const float inv = none ? 0.f : 1.0f / l;
+        const int qi = col / a.group, g = col - qi * a.group;
+        uint16_t *out = a.out + (t.q0 + qi) * a.o_s0 + (head * a.group + g) * a.o_s1 + PER * lane;
+        if constexpr (PER == 2) *reinterpret_cast<uint32_t *>(out) = pack2_bf16(o[0] * inv, o[1] * inv);
+        else out[0] = f32_to_bf16(o[0] * inv);
+    }
+}
+
+// Waves of the decode launch per kv head: eight a CU.
+int decode_waves(int heads) {
+    const int groups = 512 / heads;  // workgroups of four waves
+    return (groups < 1 ? 1 : groups) * kKv8Waves;
+}
+struct Prefill8 {
+    int slots, splits;
+};
+// Pieces so that about 512 workgroups (two a CU) have work.
+Prefill8 prefill_plan(int tokens, int rows, int group, int heads) {
+    const int nq = kCols / group;
+    const int slots = tokens / nq + rows;
+    const int wgs = slots * heads;
+    int s = (512 + wgs - 1) / wgs;
+    s = s < 1 ? 1 : (s > 8 ? 8 : s);
+    return {slots, s};
+}
+struct Layout8 {
+    int64_t d_ml, d_o, p_ml, p_o, total;
+};
+int64_t up256(int64_t x) { return (x + 255) & ~int64_t(255); }
+Layout8 layout8(int tokens, int rows, int qo_heads, int heads, int D, int parts) {
+    const int group = qo_heads / heads;
+    Layout8 L = {0, 0, 0, 0, 0};
+    int64_t off = 0;
+    if (parts & NQ_ATTN_DECODE) {
+        const int64_t n = 2ll * decode_waves(heads) * qo_heads;
+        L.d_ml = off;
+        off = up256(off + n * 8);
+        L.d_o = off;
+        off = up256(off + n * D * 4);
+    }
+    if (parts & NQ_ATTN_PREFILL) {
+        const Prefill8 p = prefill_plan(tokens, rows, group, heads);
+        const int64_t n = p.splits > 1 ? static_cast<int64_t>(p.slots) * heads * p.splits * kCols : 0;
+        L.p_ml = off;
+        off = up256(off + n * 8);
+        L.p_o = off;
+        off = up256(off + n * D * 4);
+    }
+    L.total = off;
+    return L;
+}
+
+bool al(const void *p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int check_pool(const Pool8 &p, int heads, int head_dim) {
+    NQ_CHECK_ARG(p.codes && p.scales && p.num_pages >= 1 && heads >= 1);
+    NQ_CHECK_ARG(p.page_size >= 1 && (p.page_size & (p.page_size - 1)) == 0);
+    NQ_CHECK_ARG(p.c_page >= 0 && p.c_kind >= 0 && p.c_slot >= 0 && p.c_head >= 0);
+    NQ_CHECK_ARG(p.s_page >= 0 && p.s_kind >= 0 && p.s_block >= 0 && p.s_head >= 0);
+    if ((head_dim != 64 && head_dim != 128) || p.page_size < kBlk) return NQ_ERR_UNSUPPORTED;
+    if (!al(p.codes, 16) || p.c_page % 16 || p.c_kind % 16 || p.c_slot % 16 || p.c_head % 16 || !al(p.scales, 4))
+        return NQ_ERR_UNSUPPORTED;
+    if (p.c_slot > (1 << 26)) return NQ_ERR_UNSUPPORTED;  // 16 slots of a block stay within 32-bit offsets
+    return NQ_OK;
+}
+
+}  // namespace
+}  // namespace nq
+
+using namespace nq;
+
+extern "C" int nq_kv_int8_write(const uint16_t *key, int64_t k_s0, int64_t k_s1, const uint16_t *value, int64_t v_s0,
+                                int64_t v_s1, int tokens, int num_kv_heads, int head_dim, int8_t *codes,
+                                int64_t c_page, int64_t c_kind, int64_t c_slot, int64_t c_head, float *scales,
+                                int64_t s_page, int64_t s_kind, int64_t s_block, int64_t s_head, int num_pages,
+                                int page_size, const int64_t *write_pages, const int64_t *write_offsets,
+                                int32_t *status, void *stream) {
+    NQ_CHECK_ARG(tokens >= 0);
+    const Pool8 pool = {codes, c_page, c_kind, c_slot, c_head, scales, s_page, s_kind, s_block, s_head, num_pages,
+                        page_size};
+    const int rc = check_pool(pool, num_kv_heads, head_dim);
+    if (rc != NQ_OK) return rc;
+    if (tokens == 0) return NQ_OK;
+    NQ_CHECK_ARG(key && value && write_pages && write_offsets);
+    if (!al(key, 16) || !al(value, 16) || k_s0 % 8 || k_s1 % 8 || v_s0 % 8 || v_s1 % 8) return NQ_ERR_UNSUPPORTED;
+    // one token a wave while that leaves at most eight waves a SIMD of work, else 16
+    const int group = static_cast<int64_t>(tokens) * num_kv_heads * 2 <= 8192 ? 1 : 16;
+    const dim3 grid((tokens + group - 1) / group, (2 * num_kv_heads + kKv8Waves - 1) / kKv8Waves);
+    const auto kernel = head_dim == 128 ? kv8_write_kernel<128> : kv8_write_kernel<64>;
+    hipLaunchKernelGGL(kernel, grid, dim3(kKv8Threads), 0, static_cast<hipStream_t>(stream), key, k_s0, k_s1, value,
+                       v_s0, v_s1, write_pages, write_offsets, tokens, num_kv_heads, group, pool, status);
+    return NQ_LAUNCH_STATUS();
+}
+
+extern "C" int nq_kv_int8_read(const int8_t *codes, int64_t c_page, int64_t c_kind, int64_t c_slot, int64_t c_head,
+                               const float *scales, int64_t s_page, int64_t s_kind, int64_t s_block, int64_t s_head,
+                               int num_pages, int page_size, const int64_t *pages, const int64_t *offsets, int tokens,
+                               int num_kv_heads, int head_dim, uint16_t *key, int64_t k_s0, int64_t k_s1,
+                               uint16_t *value, int64_t v_s0, int64_t v_s1, int32_t *status, void *stream) {
+    NQ_CHECK_ARG(tokens >= 0);
+    const Pool8 pool = {const_cast<int8_t *>(codes), c_page, c_kind, c_slot, c_head, const_cast<float *>(scales),
+                        s_page, s_kind, s_block, s_head, num_pages, page_size};
+    const int rc = check_pool(pool, num_kv_heads, head_dim);
+    if (rc != NQ_OK) return rc;
+    if (tokens == 0) return NQ_OK;
+    NQ_CHECK_ARG(key && value && pages && offsets);
+    if (!al(key, 16) || !al(value, 16) || k_s0 % 8 || k_s1 % 8 || v_s0 % 8 || v_s1 % 8) return NQ_ERR_UNSUPPORTED;
+    const int64_t threads = static_cast<int64_t>(tokens) * 2 * num_kv_heads * (head_dim / 16);
+    const int64_t groups = (threads + kKv8Threads - 1) / kKv8Threads;
+    if (groups > 0x7fffffffll) return NQ_ERR_UNSUPPORTED;
+    const auto kernel = head_dim == 128 ? kv8_read_kernel<128> : kv8_read_kernel<64>;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(kKv8Threads), 0,
+                       static_cast<hipStream_t>(stream), pool, pages, offsets, tokens, num_kv_heads, key, k_s0, k_s1,
+                       value, v_s0, v_s1, status);
+    return NQ_LAUNCH_STATUS();
+}
+
+extern "C" int64_t nq_paged_attention_int8_workspace_bytes(int tokens, int rows, int num_qo_heads, int num_kv_heads,
+                                                           int head_dim, int parts) {
+    if (tokens < 1 || rows < 1 || num_kv_heads < 1 || num_kv_heads > 512 || num_qo_heads < num_kv_heads ||
+        num_qo_heads % num_kv_heads || num_qo_heads / num_kv_heads > 16 || (head_dim != 64 && head_dim != 128) ||
+        parts < 1 || parts > (NQ_ATTN_DECODE | NQ_ATTN_PREFILL))
+        return -1;
+    return layout8(tokens, rows, num_qo_heads, num_kv_heads, head_dim, parts).total;
+}
+
+namespace {
+
+template <int D>
+int launch_attention8(const Attend8 &a, const Pool8 &pool, int parts, char *ws, const Layout8 &L, hipStream_t st) {
+    if (parts & NQ_ATTN_DECODE) {
+        const int waves = decode_waves(a.heads);
+        float2 *ml = reinterpret_cast<float2 *>(ws + L.d_ml);
+        float *o = reinterpret_cast<float *>(ws + L.d_o);
+        hipLaunchKernelGGL((kv8_decode_kernel<D>), dim3(waves / kKv8Waves * a.heads), dim3(kKv8Threads), 0, st, a, pool,
+                           waves, ml, o);
+        hipLaunchKernelGGL((kv8_merge_kernel<D>), dim3(a.rows, a.heads), dim3(kKv8Threads), 0, st, a, waves, ml, o);
+    }
+    if (parts & NQ_ATTN_PREFILL) {
+        const Prefill8 p = prefill_plan(a.tokens, a.rows, a.group, a.heads);
+        const int skip = (parts & NQ_ATTN_DECODE) ? 1 : 0;
+        float2 *ml = reinterpret_cast<float2 *>(ws + L.p_ml);
+        float *o = reinterpret_cast<float *>(ws + L.p_o);
+        hipLaunchKernelGGL((kv8_prefill_kernel<D>), dim3(p.slots * a.heads, p.splits), dim3(kKv8Threads), 0, st, a,
+                           pool, p.slots, p.splits, skip, ml, o);
+        if (p.splits > 1)
+            hipLaunchKernelGGL((kv8_join_kernel<D>), dim3(p.slots * a.heads, 8), dim3(kKv8Threads), 0, st, a, p.slots,
+                               p.splits, skip, ml, o);
+    }
+    return NQ_LAUNCH_STATUS();
+}
+
+}  // namespace
+
+extern "C" int nq_paged_attention_int8(const int32_t *qo_indptr, const int32_t *kv_indptr,
+                                       const int32_t *last_page_len, const int32_t *kv_indices, int n_rows,
+                                       int num_indices, const uint16_t *q, int64_t q_s0, int64_t q_s1, int tokens,
+                                       const int8_t *codes, int64_t c_page, int64_t c_kind, int64_t c_slot,
+                                       int64_t c_head, const float *scales, int64_t s_page, int64_t s_kind,
+                                       int64_t s_block, int64_t s_head, int num_pages, int page_size,
+                                       int num_qo_heads, int num_kv_heads, int head_dim, float sm_scale,
+                                       uint16_t *out, int64_t o_s0, int64_t o_s1, int parts, void *workspace,
+                                       int64_t workspace_bytes, int32_t *status, void *stream) {
+    NQ_CHECK_ARG(n_rows >= 0 && tokens >= 0 && num_indices >= 0 && num_kv_heads >= 1);
+    NQ_CHECK_ARG(num_qo_heads >= num_kv_heads && num_qo_heads % num_kv_heads == 0);
+    NQ_CHECK_ARG(parts >= 1 && parts <= (NQ_ATTN_DECODE | NQ_ATTN_PREFILL));
+    NQ_CHECK_ARG(qo_indptr || parts == NQ_ATTN_DECODE);
+    const Pool8 pool = {const_cast<int8_t *>(codes), c_page, c_kind, c_slot, c_head, const_cast<float *>(scales),
+                        s_page, s_kind, s_block, s_head, num_pages, page_size};
+    const int rc = check_pool(pool, num_kv_heads, head_dim);
+    if (rc != NQ_OK) return rc;
+    if (n_rows == 0 || tokens == 0) return NQ_OK;
+    const int64_t need =
+        nq_paged_attention_int8_workspace_bytes(tokens, n_rows, num_qo_heads, num_kv_heads, head_dim, parts);
+    if (need < 0) return NQ_ERR_UNSUPPORTED;
+    NQ_CHECK_ARG(q && out && kv_indptr && last_page_len && (kv_indices || num_indices == 0));
+    NQ_CHECK_ARG(qo_indptr || n_rows <= tokens);
+    NQ_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && al(workspace, 16)));
+    if (!al(q, 16) || q_s0 % 8 || q_s1 % 8 || !al(out, 16) || o_s0 % 8 || o_s1 % 8) return NQ_ERR_UNSUPPORTED;
+    int bpp = 0;
+    while ((kBlk << bpp) < page_size) ++bpp;
+    const Prefill8 p = prefill_plan(tokens, n_rows, num_qo_heads / num_kv_heads, num_kv_heads);
+    if (static_cast<int64_t>(p.slots) * num_kv_heads > 0x3fffffff || num_kv_heads > 65535 ||
+        (static_cast<int64_t>(num_indices) * page_size) > 0x7fffffffll)
+        return NQ_ERR_UNSUPPORTED;
+    const Attend8 a = {q,     q_s0,        q_s1,   out,         o_s0,
+                       o_s1,  qo_indptr,   kv_indptr, kv_indices,  last_page_len,
+                       n_rows, tokens,     num_indices, num_qo_heads / num_kv_heads, num_kv_heads,
+                       bpp,   sm_scale * kLog2e8, status};
+    char *ws = static_cast<char *>(workspace);
+    const Layout8 L = layout8(tokens, n_rows, num_qo_heads, num_kv_heads, head_dim, parts);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return head_dim == 128 ? launch_attention8<128>(a, pool, parts, ws, L, st)
+                           : launch_attention8<64>(a, pool, parts, ws, L, st);
+}

@@ -340,7 +340,170 @@ def paged_attention_noalloc(query: torch.Tensor, layer_cache: torch.Tensor, meta
     return out
 
 
+INT8_BLOCK = 16  # cache slots that share a scale
+
+
+def _int8_cache(layer_cache: torch.Tensor, layer_scales: torch.Tensor) -> tuple:
+    """The C ABI's cache arguments after checks: codes and strides, scales and strides, pages, page size."""
+
+    if layer_cache.dtype != torch.int8 or layer_scales.dtype != torch.float32:
+        raise TypeError("the 8-bit cache is int8 codes with float32 scales")
+    if layer_cache.ndim != 5 or layer_cache.shape[1] != 2 or layer_cache.shape[0] < 1 or layer_cache.stride(4) != 1:
+        raise ValueError("the 8-bit cache must be [pages, 2, page_size, Hkv, D], contiguous per head")
+    pages, _, page_size, heads, _ = layer_cache.shape
+    if page_size < INT8_BLOCK or page_size & (page_size - 1):
+        raise TypeError(f"the 8-bit cache needs a page size that is a power of two of at least {INT8_BLOCK}")
+    if layer_scales.shape != (pages, 2, page_size // INT8_BLOCK, heads):
+        raise ValueError("the scales must be [pages, 2, page_size // 16, Hkv]")
+    return (layer_cache.data_ptr(), *layer_cache.stride()[:4], layer_scales.data_ptr(), *layer_scales.stride(),
+            pages, page_size)
+
+
+def _int8_slots(pages: torch.Tensor, offsets: torch.Tensor) -> int:
+    if pages.dtype != torch.long or offsets.dtype != torch.long:
+        raise TypeError("cache slots must be int64")
+    if pages.ndim != 1 or pages.shape != offsets.shape or not pages.is_contiguous() or not offsets.is_contiguous():
+        raise ValueError("cache slots must be contiguous vectors with one entry per token")
+    return pages.shape[0]
+
+
+def _int8_heads(key: torch.Tensor, value: torch.Tensor, tokens: int, layer_cache: torch.Tensor) -> None:
+    _require_bf16(key, value)
+    if key.shape != (tokens, *layer_cache.shape[3:]) or value.shape != key.shape:
+        raise ValueError("key and value must be [tokens, Hkv, D] with the cache's heads")
+    if key.stride(2) != 1 or value.stride(2) != 1:
+        raise ValueError("key and value must be contiguous per head")
+
+
+def _int8_status(status: torch.Tensor | None) -> int | None:
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+        raise TypeError("status must be an int32 tensor")
+    return _lib.ptr(status)
+
+
+def paged_cache_write_int8_(key: torch.Tensor, value: torch.Tensor, layer_cache: torch.Tensor,
+                            layer_scales: torch.Tensor, write_pages: torch.Tensor, write_offsets: torch.Tensor,
+                            status: torch.Tensor | None = None) -> None:
+    """Quantize ``key`` and ``value`` [tokens, Hkv, D] (bf16, rotated) into one layer of the 8-bit cache:
+    codes int8 [pages, 2, page_size, Hkv, D], scales float32 [pages, 2, page_size // 16, Hkv], a value
+    being code * scale.
+
+    Tokens go to the slots (``write_pages[t]``, ``write_offsets[t]``).  A block of 16 slots has one scale per
+    kind and head, the least power of two s (at least 2^-126) with max |x| / s <= 127 over the tokens in it; when
+    a later token makes it grow, the codes of the block's earlier slots are rescaled (rounded to the nearest,
+    ties to even), which adds less than one step to any value.  A write at a block's first slot starts the block anew; a write further
+    on takes the slots before it as held and those behind the written ones as empty.  Tokens that
+    share a block stand next to each other in slot order (as a request's do); two separate runs into one block in
+    one call leave that block unspecified.  A NaN or infinity makes its block's scale NaN.  A slot outside the pool is skipped and
+    ``status`` (int32, optional) set to NQ_ERR_INVALID_ARGUMENT.  No counterpart in the reference."""
+
+    cache = _int8_cache(layer_cache, layer_scales)
+    tokens = _int8_slots(write_pages, write_offsets)
+    _int8_heads(key, value, tokens, layer_cache)
+    _lib.require_one_device(key, value, layer_cache, layer_scales, write_pages, write_offsets, status)
+    _lib.call_on(
+        key.device, "nq_kv_int8_write", key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(),
+        value.stride(0), value.stride(1), tokens, layer_cache.shape[3], layer_cache.shape[4], *cache,
+        write_pages.data_ptr(), write_offsets.data_ptr(), _int8_status(status), _lib.stream(key.device),
+    )
+
+
+def paged_cache_read_int8(layer_cache: torch.Tensor, layer_scales: torch.Tensor, pages: torch.Tensor,
+                          offsets: torch.Tensor, key: torch.Tensor | None = None, value: torch.Tensor | None = None,
+                          status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """K and V [tokens, Hkv, D] of the slots (``pages[t]``, ``offsets[t]``) of the 8-bit cache as bf16 (to move a
+    request to a bf16 pool, or off the device): code * scale, which bf16 holds exactly for the scales that
+    ``paged_cache_write_int8_`` makes.  A slot outside the pool gives zeros and sets ``status``."""
+
+    cache = _int8_cache(layer_cache, layer_scales)
+    tokens = _int8_slots(pages, offsets)
+    shape = (tokens, *layer_cache.shape[3:])
+    key = torch.empty(shape, dtype=torch.bfloat16, device=layer_cache.device) if key is None else key
+    value = torch.empty(shape, dtype=torch.bfloat16, device=layer_cache.device) if value is None else value
+    _int8_heads(key, value, tokens, layer_cache)
+    _lib.require_one_device(layer_cache, layer_scales, pages, offsets, key, value, status)
+    _lib.call_on(
+        key.device, "nq_kv_int8_read", *cache, pages.data_ptr(), offsets.data_ptr(), tokens, layer_cache.shape[3],
+        layer_cache.shape[4], key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
+        value.stride(1), _int8_status(status), _lib.stream(key.device),
+    )
+    return key, value
+
+
+def paged_attention_int8_workspace_bytes(tokens: int, rows: int, qo_heads: int, kv_heads: int, head_dim: int,
+                                         parts: int = _lib.NQ_ATTN_DECODE | _lib.NQ_ATTN_PREFILL) -> int:
+    """The workspace ``paged_attention_int8`` needs; raises for shapes it does not cover."""
+
+    n = int(_lib.load().nq_paged_attention_int8_workspace_bytes(tokens, rows, qo_heads, kv_heads, head_dim, parts))
+    if n < 0:
+        raise TypeError(f"no 8-bit paged attention for {tokens} tokens, {rows} rows, {qo_heads} / {kv_heads} heads of "
+                        f"{head_dim}")
+    return n
+
+
+def paged_attention_int8(query: torch.Tensor, layer_cache: torch.Tensor, layer_scales: torch.Tensor, metadata, *,
+                         sm_scale: float | None = None, parts: int | None = None,
+                         status: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+    """Paged attention of ``query`` [tokens, Hq, D] (bf16) over one layer of the 8-bit cache (see
+    ``paged_cache_write_int8_``) with ``metadata`` (a TalkerAttentionMetadata; its qo_indptr, paged_kv_indptr,
+    paged_kv_indices and paged_kv_last_page_len are read), without a plan.
+
+    ``parts`` as ``paged_attention_noalloc`` takes them: NQ_ATTN_DECODE for the rows with one query,
+    NQ_ATTN_PREFILL for those with several (alone: for all of them); both by default, NQ_ATTN_DECODE where the
+    metadata has no qo_indptr.  A query that sees no key gets zeros; tokens of no row keep what ``out`` held.
+    ``workspace`` (``paged_attention_int8_workspace_bytes``; allocated if None) belongs to one call at a
+    time.  The same inputs give the same bits.  No counterpart in the reference."""
+
+    cache = _int8_cache(layer_cache, layer_scales)
+    if query.ndim != 3 or query.stride(2) != 1:
+        raise ValueError("query must be [tokens, Hq, D], contiguous per head")
+    tokens, hq, d = query.shape
+    hkv = layer_cache.shape[3]
+    if layer_cache.shape[4] != d or hq < hkv or hq % hkv:
+        raise ValueError("query and cache disagree on the heads")
+    out = torch.empty_like(query, memory_format=torch.contiguous_format) if out is None else out
+    _require_bf16(query, out)
+    if out.shape != query.shape or out.stride(2) != 1:
+        raise ValueError("out must be [tokens, Hq, D] like the query")
+    qo, kv, ids, last = (metadata.qo_indptr, metadata.paged_kv_indptr, metadata.paged_kv_indices,
+                         metadata.paged_kv_last_page_len)
+    for t in (qo, kv, ids, last):
+        if t is not None and t.dtype != torch.int32:
+            raise TypeError("paged metadata must be int32")
+        if t is not None and (t.ndim != 1 or not t.is_contiguous()):
+            raise ValueError("paged metadata must be contiguous vectors")
+    rows = kv.shape[0] - 1
+    if rows < 0 or last.shape[0] < rows or (qo is not None and qo.shape[0] != rows + 1):
+        raise ValueError("paged metadata must describe one set of rows")
+    if parts is None:
+        parts = _lib.NQ_ATTN_DECODE if qo is None else _lib.NQ_ATTN_DECODE | _lib.NQ_ATTN_PREFILL
+    if qo is None and (parts != _lib.NQ_ATTN_DECODE or rows > tokens):
+        raise ValueError("without qo_indptr every row has one query and only NQ_ATTN_DECODE runs")
+    _lib.require_one_device(query, layer_cache, layer_scales, out, qo, kv, ids, last, status, workspace)
+    if tokens == 0 or rows == 0:
+        return out
+    need = paged_attention_int8_workspace_bytes(tokens, rows, hq, hkv, d, parts)
+    if workspace is None:
+        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=query.device)
+    elif workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
+        raise ValueError(f"8-bit paged attention needs a contiguous workspace of {need} bytes")
+    _lib.call_on(
+        query.device, "nq_paged_attention_int8", _lib.ptr(qo), kv.data_ptr(), last.data_ptr(), ids.data_ptr(), rows,
+        ids.shape[0], query.data_ptr(), query.stride(0), query.stride(1), tokens, *cache, hq, hkv, d,
+        float(d) ** -0.5 if sm_scale is None else float(sm_scale), out.data_ptr(), out.stride(0), out.stride(1),
+        int(parts), workspace.data_ptr(), workspace.numel() * workspace.element_size(), _int8_status(status),
+        _lib.stream(query.device),
+    )
+    return out
+
+
 __all__ = [
+    "INT8_BLOCK",
+    "paged_attention_int8",
+    "paged_attention_int8_workspace_bytes",
+    "paged_cache_read_int8",
+    "paged_cache_write_int8_",
     "paged_attention_noalloc",
     "decode_attn_nhd_short_cache",
     "paired_qk_norm_rope_",
