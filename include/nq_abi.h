@@ -860,6 +860,24 @@ int nq_codec_transconv_overlap(const int32_t *offsets, int B, int u_in, int stri
                                const int32_t *slots, float *overlap, const float *new_overlap, int Cout,
                                float *out, int64_t ldo, void *stream);
 
+/*
+ * Products of 8-bit integers with one scale per token and per output channel (no
+ * counterpart in the reference, whose 8-bit product is FP8 with block scales,
+ * model/layers.py:195-262).
+ * nq_quantize_int8_rows: row r of bf16 x [M, K] gives codes rint(127 x / max
+ * |x|) (ties to even) and the scale max |x| / 127: activations per token, or
+ * weights [N, K] per output channel.  A row of zeros has scale 1, a row that holds a NaN
+ * or an infinity codes of 0 and a NaN scale.
+ * nq_linear_int8: out[m, n] = bf16(sum_k xq[m, k] wq[n, k] * sx[m] * sw[n]),
+ * the sum in int32.  K is a multiple of 16 up to 2^17 for the product; codes and their row
+ * strides are multiples of 16 bytes (x of the quantisation and its codes' rows: of 8
+ * elements).  M, N: any.
+ */
+int nq_quantize_int8_rows(const uint16_t *x, int64_t x_s0, int M, int K, int8_t *q, int64_t q_s0,
+                          float *scales, void *stream);
+int nq_linear_int8(const int8_t *xq, int64_t x_s0, const float *sx, const int8_t *wq, int64_t w_s0,
+                   const float *sw, int M, int N, int K, uint16_t *out, int64_t o_s0, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -951,13 +951,17 @@ Layout8 layout8(int tokens, int rows, int qo_heads, int heads, int D, int parts)
 
 bool al(const void *p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+// A stride that breaks the alignment of what lies behind it (that of a dimension of one is never used).
+bool odd_stride(int n, int64_t stride, int multiple) { return n > 1 && stride % multiple; }
+
 int check_pool(const Pool8 &p, int heads, int head_dim) {
     NQ_CHECK_ARG(p.codes && p.scales && p.num_pages >= 1 && heads >= 1);
     NQ_CHECK_ARG(p.page_size >= 1 && (p.page_size & (p.page_size - 1)) == 0);
     NQ_CHECK_ARG(p.c_page >= 0 && p.c_kind >= 0 && p.c_slot >= 0 && p.c_head >= 0);
     NQ_CHECK_ARG(p.s_page >= 0 && p.s_kind >= 0 && p.s_block >= 0 && p.s_head >= 0);
     if ((head_dim != 64 && head_dim != 128) || p.page_size < kBlk) return NQ_ERR_UNSUPPORTED;
-    if (!al(p.codes, 16) || p.c_page % 16 || p.c_kind % 16 || p.c_slot % 16 || p.c_head % 16 || !al(p.scales, 4))
+    if (!al(p.codes, 16) || odd_stride(p.num_pages, p.c_page, 16) || p.c_kind % 16 || p.c_slot % 16 ||
+        odd_stride(heads, p.c_head, 16) || !al(p.scales, 4))
         return NQ_ERR_UNSUPPORTED;
     if (p.c_slot > (1 << 26)) return NQ_ERR_UNSUPPORTED;  // 16 slots of a block stay within 32-bit offsets
     return NQ_OK;
@@ -981,7 +985,9 @@ extern "C" int nq_kv_int8_write(const uint16_t *key, int64_t k_s0, int64_t k_s1,
     if (rc != NQ_OK) return rc;
     if (tokens == 0) return NQ_OK;
     NQ_CHECK_ARG(key && value && write_pages && write_offsets);
-    if (!al(key, 16) || !al(value, 16) || k_s0 % 8 || k_s1 % 8 || v_s0 % 8 || v_s1 % 8) return NQ_ERR_UNSUPPORTED;
+    if (!al(key, 16) || !al(value, 16) || odd_stride(tokens, k_s0, 8) || odd_stride(num_kv_heads, k_s1, 8) ||
+        odd_stride(tokens, v_s0, 8) || odd_stride(num_kv_heads, v_s1, 8))
+        return NQ_ERR_UNSUPPORTED;
     // one token a wave while that leaves at most eight waves a SIMD of work, else 16
     const int group = static_cast<int64_t>(tokens) * num_kv_heads * 2 <= 8192 ? 1 : 16;
     const dim3 grid((tokens + group - 1) / group, (2 * num_kv_heads + kKv8Waves - 1) / kKv8Waves);
@@ -1003,7 +1009,9 @@ extern "C" int nq_kv_int8_read(const int8_t *codes, int64_t c_page, int64_t c_ki
     if (rc != NQ_OK) return rc;
     if (tokens == 0) return NQ_OK;
     NQ_CHECK_ARG(key && value && pages && offsets);
-    if (!al(key, 16) || !al(value, 16) || k_s0 % 8 || k_s1 % 8 || v_s0 % 8 || v_s1 % 8) return NQ_ERR_UNSUPPORTED;
+    if (!al(key, 16) || !al(value, 16) || odd_stride(tokens, k_s0, 8) || odd_stride(num_kv_heads, k_s1, 8) ||
+        odd_stride(tokens, v_s0, 8) || odd_stride(num_kv_heads, v_s1, 8))
+        return NQ_ERR_UNSUPPORTED;
     const int64_t threads = static_cast<int64_t>(tokens) * 2 * num_kv_heads * (head_dim / 16);
     const int64_t groups = (threads + kKv8Threads - 1) / kKv8Threads;
     if (groups > 0x7fffffffll) return NQ_ERR_UNSUPPORTED;
@@ -1075,7 +1083,9 @@ extern "C" int nq_paged_attention_int8(const int32_t *qo_indptr, const int32_t *
     NQ_CHECK_ARG(q && out && kv_indptr && last_page_len && (kv_indices || num_indices == 0));
     NQ_CHECK_ARG(qo_indptr || n_rows <= tokens);
     NQ_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && al(workspace, 16)));
-    if (!al(q, 16) || q_s0 % 8 || q_s1 % 8 || !al(out, 16) || o_s0 % 8 || o_s1 % 8) return NQ_ERR_UNSUPPORTED;
+    if (!al(q, 16) || odd_stride(tokens, q_s0, 8) || odd_stride(num_qo_heads, q_s1, 8) || !al(out, 16) ||
+        odd_stride(tokens, o_s0, 8) || odd_stride(num_qo_heads, o_s1, 8))
+        return NQ_ERR_UNSUPPORTED;
     int bpp = 0;
     while ((kBlk << bpp) < page_size) ++bpp;
     const Prefill8 p = prefill_plan(tokens, n_rows, num_qo_heads / num_kv_heads, num_kv_heads);

@@ -15,6 +15,10 @@ keeps the reference's name, block layout and errors; the activations are
 quantized per row and 128 columns by the add-RMSNorm that produces them
 (``add_rmsnorm_fp8`` / ``linear_add_rmsnorm_fp8``) or by
 ``quantize_fp8_rows``, and ``linear_fp8`` runs the block-scaled product.
+
+8-bit integers (no reference counterpart): ``quantize_int8_rows`` gives codes with
+one scale per row, of activations (per token) as of weights (per output
+channel), and ``linear_int8`` runs their product for any number of rows.
 """
 
 from __future__ import annotations
@@ -743,7 +747,62 @@ def linear_fp8_swiglu(q: torch.Tensor, scales: torch.Tensor, packed: torch.Tenso
     return out
 
 
+def quantize_int8_rows(x: torch.Tensor, q: torch.Tensor | None = None,
+                       scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """bf16 [rows, K] -> (int8 codes rint(127 x / max|x|), float32 scales max|x| / 127 [rows]): activations per
+    token, or a weight [out, in] per output channel.  K a multiple of 16; a row of zeros has scale 1, one with a
+    NaN or an infinity a NaN scale (its products are NaN)."""
+
+    if x.dtype != torch.bfloat16:
+        raise TypeError("row quantization needs bf16 [rows, K]")
+    if x.dim() != 2 or x.stride(1) != 1:
+        raise ValueError("row quantization needs [rows, K] with unit inner stride")
+    rows, k = x.shape
+    if k < 16 or k % 16:
+        raise ValueError("int8 row quantization needs a multiple of 16 columns")
+    q = torch.empty((rows, k), dtype=torch.int8, device=x.device) if q is None else q
+    scales = torch.empty(rows, dtype=torch.float32, device=x.device) if scales is None else scales
+    if q.dtype != torch.int8 or scales.dtype != torch.float32:
+        raise TypeError("int8 codes and float32 scales expected")
+    if q.shape != x.shape or q.stride(1) != 1 or scales.shape != (rows,) or not scales.is_contiguous():
+        raise ValueError(f"codes must be [{rows}, {k}] with unit inner stride and scales [{rows}], contiguous")
+    _lib.require_one_device(x, q, scales)
+    _lib.call_on(x.device, "nq_quantize_int8_rows", x.data_ptr(), x.stride(0), rows, k, q.data_ptr(), q.stride(0),
+                 scales.data_ptr(), _lib.stream(x.device))
+    return q, scales
+
+
+def linear_int8(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, weight_scales: torch.Tensor,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """out[m, n] = bf16(sum_k q[m, k] weight_q[n, k] * scales[m] * weight_scales[n]) for int8 codes [rows, in] and
+    [out, in] with the scales of ``quantize_int8_rows``; the sum is exact (int32), so the same codes give the
+    same bits at any number of rows.  ``in`` a multiple of 16 up to 131072, any rows and out."""
+
+    if q.dtype != torch.int8 or weight_q.dtype != torch.int8:
+        raise TypeError("the int8 projection needs int8 codes")
+    if scales.dtype != torch.float32 or weight_scales.dtype != torch.float32:
+        raise TypeError("int8 scales must be float32")
+    if q.dim() != 2 or weight_q.dim() != 2 or q.stride(1) != 1 or weight_q.stride(1) != 1:
+        raise ValueError("int8 codes must be matrices with unit inner stride")
+    (rows, k), n = q.shape, weight_q.shape[0]
+    if weight_q.shape[1] != k or k < 16 or k % 16:
+        raise ValueError("int8 codes must share an inner size that is a multiple of 16")
+    if scales.shape != (rows,) or weight_scales.shape != (n,) or not (
+            scales.is_contiguous() and weight_scales.is_contiguous()):
+        raise ValueError("int8 scales must be contiguous, one per row and one per output")
+    out = torch.empty((rows, n), dtype=torch.bfloat16, device=q.device) if out is None else out
+    if out.dtype != torch.bfloat16 or out.shape != (rows, n) or out.stride(1) != 1:
+        raise ValueError(f"out must be bf16 [{rows}, {n}] with unit inner stride")
+    _lib.require_one_device(q, scales, weight_q, weight_scales, out)
+    _lib.call_on(q.device, "nq_linear_int8", q.data_ptr(), q.stride(0), scales.data_ptr(), weight_q.data_ptr(),
+                 weight_q.stride(0), weight_scales.data_ptr(), rows, n, k, out.data_ptr(), out.stride(0),
+                 _lib.stream(q.device))
+    return out
+
+
 __all__ = [
+    "linear_int8",
+    "quantize_int8_rows",
     "NormRows",
     "decode_linear",
     "decode_linear_splits",

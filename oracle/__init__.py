@@ -14,6 +14,7 @@ Modules and what they restate (reference paths are relative to
 - ``attention`` -- paged GQA decode / causal prefill and the short-cache
                    attention (executor/talker_kv.py:140-306,
                    model/kernels.py:408-463, model/components.py:235-252)
+- ``int8``      -- int8 row quantisation and product (no reference counterpart)
 - ``kv_int8``   -- the K/V cache in 8 bits, its write and attention (no reference counterpart)
 - ``qk_rope``   -- paired q/k RMSNorm + RoPE + cache write
                    (model/kernels.py:15-91, 163-248)

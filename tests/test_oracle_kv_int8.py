@@ -147,7 +147,7 @@ def test_host_checks_of_the_c_entries(nq):
 
     lib = _lib.load()
 
-    def write(key=16, k_s0=128, tokens=1, heads=2, d=64, codes=16, c_slot=128, pages=4, ps=16):
+    def write(key=16, k_s0=128, tokens=2, heads=2, d=64, codes=16, c_slot=128, pages=4, ps=16):
         return lib.nq_kv_int8_write(key, k_s0, 64, 16, 128, 64, tokens, heads, d, codes, 4096, 2048, c_slot, 64, 16, 4,
                                     2, 2, 1, pages, ps, 16, 16, None, None)
 
