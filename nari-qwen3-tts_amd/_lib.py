@@ -193,14 +193,20 @@ def call(name: str, *args) -> None:
         check(status, name)
 
 
-def call_on(device: torch.device, name: str, *args) -> None:
-    """``call`` with ``device`` current, for tensors on another device than the current one."""
+def launch(index: int, name: str, *args) -> None:
+    """``call`` on torch's current stream of device ``index`` (appended to ``args``), with that device current:
+    the short way for entry points whose checks already know their device."""
 
-    if device.index is None or device.index == torch.cuda.current_device():
-        call(name, *args)
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(load(), name)
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            call(name, *args)
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status != NQ_OK:
+        check(status, name)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
@@ -222,8 +228,13 @@ def require_device(*tensors: torch.Tensor) -> None:
             raise ValueError("HIP kernels need tensors on the GPU (there is no CPU path)")
 
 
-def require_one_device(first: torch.Tensor, *tensors: torch.Tensor | None) -> None:
-    require_device(first, *tensors)
+def one_device(first: torch.Tensor, *tensors: torch.Tensor | None) -> int:
+    """The index of the GPU that holds every one of ``tensors`` (None aside)."""
+
+    index = first.get_device()
+    if index < 0:
+        raise ValueError("HIP kernels need tensors on the GPU (there is no CPU path)")
     for t in tensors:
-        if t is not None and t.device != first.device:
-            raise ValueError("HIP kernels need their tensors on one device")
+        if t is not None and t.get_device() != index:
+            raise ValueError("HIP kernels need their tensors on one GPU")
+    return index

@@ -19,6 +19,9 @@
 namespace nq {
 namespace {
 
+#ifndef NQ_DEC_OCC
+#define NQ_DEC_OCC 4
+#endif
 constexpr int kBlk = 16;  // slots that share a scale
 constexpr int kKv8Threads = 256;
 constexpr int kKv8Waves = kKv8Threads / kWave;
@@ -27,6 +30,8 @@ constexpr float kMinScale = 1.1754943508222875e-38f;  // 2^-126
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float floatx4_t __attribute__((ext_vector_type(4)));
 typedef float floatx16_t __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));  // plain vectors stay in registers
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 struct Pool8 {
     int8_t *codes;
@@ -60,9 +65,14 @@ __device__ __forceinline__ uint32_t pair_bf16(float lo, float hi) {
     return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
 __device__ __forceinline__ bf16x8_t widen8(uint32_t a, uint32_t b) {
-    const uint4 r = make_uint4(pair_bf16(byte_f32<0>(a), byte_f32<1>(a)), pair_bf16(byte_f32<2>(a), byte_f32<3>(a)),
-                               pair_bf16(byte_f32<0>(b), byte_f32<1>(b)), pair_bf16(byte_f32<2>(b), byte_f32<3>(b)));
+    const u32x4 r = {pair_bf16(byte_f32<0>(a), byte_f32<1>(a)), pair_bf16(byte_f32<2>(a), byte_f32<3>(a)),
+                     pair_bf16(byte_f32<0>(b), byte_f32<1>(b)), pair_bf16(byte_f32<2>(b), byte_f32<3>(b))};
     return __builtin_bit_cast(bf16x8_t, r);
+}
+// The same times a scale: exact for a power of two.
+__device__ __forceinline__ u32x4 scale8(uint32_t a, uint32_t b, float s) {
+    return u32x4{pack2_bf16(byte_f32<0>(a) * s, byte_f32<1>(a) * s), pack2_bf16(byte_f32<2>(a) * s, byte_f32<3>(a) * s),
+                 pack2_bf16(byte_f32<0>(b) * s, byte_f32<1>(b) * s), pack2_bf16(byte_f32<2>(b) * s, byte_f32<3>(b) * s)};
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -209,7 +219,8 @@ struct Attend8 {
     const int32_t *qo_indptr, *kv_indptr, *kv_indices, *last_page_len;
     int rows, tokens, n_indices, group, heads;  // group: query heads per kv head
     int bpp_log2;                               // blocks of 16 per page
-    float scale;                                // sm_scale log2(e)
+    float scale;                                // |sm_scale| log2(e)
+    uint32_t flip;                              // sign bits of a bf16 pair where sm_scale is negative
     int32_t *status;
 };
 
@@ -228,28 +239,69 @@ __device__ __forceinline__ int wave_find_le(int n, int x, F f) {
         lo += hit * step;
         count = step < count - hit * step ? step : count - hit * step;
     }
-    return lo;
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// The ragged metadata, copied to LDS at entry (one round trip, then searches and row changes cost LDS reads);
+// read in place beyond kMetaRows rows.
+constexpr int kMetaRows = 1024;
+struct Meta8 {
+    int32_t kv[kMetaRows + 1], qo[kMetaRows + 1], last[kMetaRows];
+};
+struct Rows8 {
+    const Attend8 &a;
+    const Meta8 &m;
+    __device__ __forceinline__ bool held() const { return a.rows <= kMetaRows; }
+    __device__ __forceinline__ int kv(int i) const { return held() ? m.kv[i] : a.kv_indptr[i]; }
+    __device__ __forceinline__ int qo(int i) const {
+        if (!a.qo_indptr) return i;
+        return held() ? m.qo[i] : a.qo_indptr[i];
+    }
+    __device__ __forceinline__ int last(int i) const { return held() ? m.last[i] : a.last_page_len[i]; }
+};
+struct InPlace8 {  // the same without the copy, for kernels that look at one row
+    const Attend8 &a;
+    __device__ __forceinline__ int kv(int i) const { return a.kv_indptr[i]; }
+    __device__ __forceinline__ int qo(int i) const { return a.qo_indptr ? a.qo_indptr[i] : i; }
+    __device__ __forceinline__ int last(int i) const { return a.last_page_len[i]; }
+};
+__device__ __forceinline__ void load_meta(const Attend8 &a, Meta8 &m) {
+    if (a.rows <= kMetaRows) {
+        for (int i = threadIdx.x; i <= a.rows; i += blockDim.x) {
+            m.kv[i] = a.kv_indptr[i];
+            if (a.qo_indptr) m.qo[i] = a.qo_indptr[i];
+            if (i < a.rows) m.last[i] = a.last_page_len[i];
+        }
+    }
+    __syncthreads();
 }
 
 // What a row asks for.
 struct Row8 {
     int first_page, n_pages, kv_len, q0, q_len;
 };
-__device__ __forceinline__ Row8 row_of(const Attend8 &a, int r) {
+template <typename R>
+__device__ __forceinline__ Row8 row_of(const Attend8 &a, const R &rows, int r) {
     Row8 w;
-    int b = a.kv_indptr[r], e = a.kv_indptr[r + 1];
+    int b = __builtin_amdgcn_readfirstlane(rows.kv(r)), e = __builtin_amdgcn_readfirstlane(rows.kv(r + 1));
     b = b < 0 ? 0 : (b > a.n_indices ? a.n_indices : b);
     e = e < b ? b : (e > a.n_indices ? a.n_indices : e);
     w.first_page = b;
     w.n_pages = e - b;
     const int ps = kBlk << a.bpp_log2;
-    int last = a.last_page_len[r];
+    int last = __builtin_amdgcn_readfirstlane(rows.last(r));
     last = last < 1 ? 1 : (last > ps ? ps : last);
     w.kv_len = w.n_pages > 0 ? (w.n_pages - 1) * ps + last : 0;
-    w.q0 = a.qo_indptr ? a.qo_indptr[r] : r;
-    w.q_len = a.qo_indptr ? a.qo_indptr[r + 1] - w.q0 : 1;
+    w.q0 = __builtin_amdgcn_readfirstlane(rows.qo(r));
+    w.q_len = __builtin_amdgcn_readfirstlane(rows.qo(r + 1)) - w.q0;
     if (w.q0 < 0 || w.q_len < 0 || w.q0 > a.tokens - w.q_len) w.q_len = 0;  // not this call's queries
     return w;
+}
+
+__device__ __forceinline__ bf16x8_t load_q(const uint16_t *p, bool on, uint32_t flip) {
+    u32x4 v = {0, 0, 0, 0};
+    if (on) v = *reinterpret_cast<const u32x4 *>(p) ^ flip;
+    return __builtin_bit_cast(bf16x8_t, v);
 }
 
 // Decode rows.  The blocks of all rows, in kv_indices order, are cut into equal spans, one a wave of every
@@ -260,8 +312,9 @@ struct Spans {
     int64_t blocks;
     int waves;
 };
-__device__ __forceinline__ Spans spans_of(const Attend8 &a, int waves) {
-    int p = a.kv_indptr[a.rows];
+template <typename R>
+__device__ __forceinline__ Spans spans_of(const Attend8 &a, const R &rows, int waves) {
+    int p = __builtin_amdgcn_readfirstlane(rows.kv(a.rows));
     p = p < 0 ? 0 : (p > a.n_indices ? a.n_indices : p);
     Spans s;
     s.blocks = static_cast<int64_t>(p) << a.bpp_log2;
@@ -279,45 +332,47 @@ __device__ __forceinline__ int span_of(const Spans &s, int64_t b) {
 // (D/4)(l / 16) .. of K, and holds the scores of query slot l % 16 against tokens 4 (l / 16) + i.  Those are, in
 // that order, the 8 keys of the lane's group in out^T = V^T P^T, so P needs no exchange between lanes; V is loaded
 // as (D/16) values of each of the 8 tokens, and the byte a conversion picks does the transposition.
+// K of the next step is asked for as soon as this one's is multiplied, V likewise: one set of registers, so that
+// four waves a SIMD are resident, and loads always in flight.
 template <int D>
-struct Step8 {
-    uint4 k[2][D / 64];
-    uint32_t v[8][D / 64];  // D/16 bytes of a token
-    float ks[2], vs[2];
-    int on[2];  // the block's page is in the pool
-};
-
-template <int D>
-__global__ void __launch_bounds__(kKv8Threads)
+__global__ void __launch_bounds__(kKv8Threads, NQ_DEC_OCC)
 kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml, float *__restrict__ part_o) {
     constexpr int W = D / 64;  // 16-byte loads of K, dwords of V
+    __shared__ Meta8 meta;
+    load_meta(a, meta);
+    const Rows8 rows{a, meta};
     const int lane = threadIdx.x & (kWave - 1);
-    const int head = blockIdx.x % a.heads;
-    const int wi = (blockIdx.x / a.heads) * kKv8Waves + threadIdx.x / kWave;
-    const Spans sp = spans_of(a, waves);
+    // XCD x (workgroups x, x + 8, ..) takes spans x, x + 8, .. of every head: the heads of a span read the same
+    // token rows at about the same time, from one L2
+    const int unit = __builtin_amdgcn_readfirstlane((blockIdx.x / 8) * kKv8Waves + threadIdx.x / kWave);
+    const int head = unit % a.heads;
+    const int wi = unit / a.heads * 8 + static_cast<int>(blockIdx.x % 8);
+    const Spans sp = spans_of(a, rows, waves);
     if (wi >= sp.waves) return;
-    const int64_t b0 = span_start(sp, wi), b1 = span_start(sp, wi + 1);
+    const int b0 = static_cast<int>(span_start(sp, wi)), b1 = static_cast<int>(span_start(sp, wi + 1));
     if (b0 >= b1) return;
     const int c = lane & 15, grp = lane >> 4;
 
     const int8_t *kbase = pool.codes + head * pool.c_head;
-    const int k_lane = static_cast<int>(c * pool.c_slot) + grp * (D / 4);
-    const int64_t v_lane = pool.c_kind + 4 * grp * pool.c_slot + c * (D / 16);
+    const int8_t *vbase = kbase + pool.c_kind;
+    const int c_slot = static_cast<int>(pool.c_slot);
+    const int k_lane = c * c_slot + grp * (D / 4);
+    const int v_lane = 4 * grp * c_slot + c * (D / 16);
+    const int in_page = (1 << a.bpp_log2) - 1;
 
     // a window of 64 blocks' pages and scales, one a lane
-    int64_t wbase = -1;
+    int wbase = b0;
     int w_pid = 0;
     float w_ks = 0.f, w_vs = 0.f;
-    auto open_window = [&](int64_t b) {
+    auto open_window = [&](int b) __attribute__((always_inline)) {
         wbase = b;
-        const int64_t mine = b + lane;
+        const int mine = b + lane;
         w_pid = -1;
         w_ks = w_vs = 0.f;
         if (mine < b1) {
             const int pid = a.kv_indices[mine >> a.bpp_log2];
             if (pid >= 0 && pid < pool.num_pages) {
-                const int blk = static_cast<int>(mine & ((1 << a.bpp_log2) - 1));
-                const float *s = pool.scales + pid * pool.s_page + blk * pool.s_block + head * pool.s_head;
+                const float *s = pool.scales + pid * pool.s_page + (mine & in_page) * pool.s_block + head * pool.s_head;
                 w_pid = pid;
                 w_ks = s[0];
                 w_vs = s[pool.s_kind];
@@ -326,50 +381,55 @@ kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml
             }
         }
     };
-    auto fetch = [&](int64_t b, Step8<D> &st) {
-        if (wbase < 0 || b + 1 >= wbase + kWave) open_window(b);
-        const int i0 = static_cast<int>(b - wbase);
-        const int i1 = b + 1 < b1 ? i0 + 1 : i0;
-        const int8_t *at[2];
+    struct Blocks {  // the two blocks of a step (the second repeats the first at the span's end)
+        int at;
+        int64_t off[2];
+        float ks[2], vs[2];
+        bool on[2];
+    };
+    auto look = [&](int b) __attribute__((always_inline)) {
+        if (b + 1 >= wbase + kWave) open_window(b);
+        Blocks n;
+        n.at = b;
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            const int i = m ? i1 : i0;
-            const int pid = __builtin_amdgcn_readlane(w_pid, i);
-            st.on[m] = pid >= 0;
-            st.ks[m] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_ks), i));
-            st.vs[m] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_vs), i));
-            const int blk = static_cast<int>((b + i - i0) & ((1 << a.bpp_log2) - 1));
-            at[m] = kbase + (pid < 0 ? 0 : pid) * pool.c_page + blk * (kBlk * pool.c_slot);
+            const int blk = m && b + 1 < b1 ? b + 1 : b;
+            const int pid = __builtin_amdgcn_readlane(w_pid, blk - wbase);
+            n.on[m] = pid >= 0;
+            n.ks[m] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_ks), blk - wbase));
+            n.vs[m] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_vs), blk - wbase));
+            n.off[m] = (pid < 0 ? 0 : pid) * pool.c_page + (blk & in_page) * (kBlk * pool.c_slot);
         }
+        return n;
+    };
+    u32x4 k[2][W];
+    u32x2 v[8];
+    auto load_k = [&](const Blocks &n) __attribute__((always_inline)) {
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int w = 0; w < W; ++w)
-                st.k[m][w] = *reinterpret_cast<const uint4 *>(at[m] + k_lane + 16 * w);
+                k[m][w] = *reinterpret_cast<const u32x4 *>(kbase + n.off[m] + (k_lane + 16 * w));
+    };
+    auto load_v = [&](const Blocks &n) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int8_t *p = at[e / 4] + v_lane + (e % 4) * pool.c_slot;
-            if constexpr (W == 2) {
-                const uint2 d = *reinterpret_cast<const uint2 *>(p);
-                st.v[e][0] = d.x;
-                st.v[e][1] = d.y;
-            } else {
-                st.v[e][0] = *reinterpret_cast<const uint32_t *>(p);
-            }
+            const int8_t *p = vbase + n.off[e / 4] + (v_lane + (e % 4) * c_slot);
+            if constexpr (W == 2) v[e] = *reinterpret_cast<const u32x2 *>(p);
+            else v[e].x = *reinterpret_cast<const uint32_t *>(p);
         }
     };
 
-    Step8<D> next;
-    int64_t held = b0;
-    fetch(b0, next);
-    // the row of the first block, over the block ends of rows in page units
-    int r = wave_find_le(a.rows, static_cast<int>(b0 >> a.bpp_log2), [&](int i) { return a.kv_indptr[i]; });
-
-    int64_t b = b0;
+    open_window(b0);
+    Blocks cur = look(b0);
+    load_k(cur);
+    load_v(cur);
+    // the row of the first block
+    int r = wave_find_le(a.rows, b0 >> a.bpp_log2, [&](int i) { return rows.kv(i); });
+    int b = b0;
     while (b < b1 && r < a.rows) {
-        const Row8 row = row_of(a, r);
-        const int64_t rs = static_cast<int64_t>(row.first_page) << a.bpp_log2;
-        const int64_t re = static_cast<int64_t>(row.first_page + row.n_pages) << a.bpp_log2;
+        const Row8 row = row_of(a, rows, r);
+        const int rs = row.first_page << a.bpp_log2, re = (row.first_page + row.n_pages) << a.bpp_log2;
         if (re <= b) {
             ++r;
             continue;
@@ -378,7 +438,7 @@ kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml
             b = rs < b1 ? rs : b1;
             continue;
         }
-        const int64_t stop = re < b1 ? re : b1;
+        const int stop = re < b1 ? re : b1;
         if (row.q_len != 1) {
             b = stop;
             ++r;
@@ -386,12 +446,13 @@ kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml
         }
         bf16x8_t qf[D / 32];
 #pragma unroll
-        for (int s = 0; s < D / 32; ++s) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (c < a.group)
-                v = *reinterpret_cast<const uint4 *>(a.q + row.q0 * a.q_s0 + (head * a.group + c) * a.q_s1 +
-                                                     grp * (D / 4) + 8 * s);
-            qf[s] = __builtin_bit_cast(bf16x8_t, v);
+        for (int s = 0; s < D / 32; ++s)
+            qf[s] = load_q(a.q + row.q0 * a.q_s0 + (head * a.group + c) * a.q_s1 + grp * (D / 4) + 8 * s, c < a.group,
+                           a.flip);
+        if (cur.at != b) {  // behind pages that are not this launch's
+            cur = look(b);
+            load_k(cur);
+            load_v(cur);
         }
         floatx4_t acc[D / 16];
 #pragma unroll
@@ -399,35 +460,35 @@ kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml
         float m_run = -__builtin_inff(), l_run = 0.f;
         bool any = false;
         for (; b < stop; b += 2) {
-            if (held != b) fetch(b, next);
-            const Step8<D> cur = next;
-            const int64_t ahead = b + 2 < stop ? b + 2 : stop;
-            if (ahead < b1) {
-                fetch(ahead, next);
-                held = ahead;
-            }
             int nv[2];
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                const int64_t left = row.kv_len - (b + m - rs) * kBlk;
-                nv[m] = b + m < stop && cur.on[m] && left > 0 ? static_cast<int>(left < kBlk ? left : kBlk) : 0;
+                const int left = row.kv_len - (b + m - rs) * kBlk;
+                nv[m] = b + m < stop && cur.on[m] && left > 0 ? (left < kBlk ? left : kBlk) : 0;
             }
-            if (nv[0] + nv[1] == 0) continue;
-            any = true;
+            any |= nv[0] + nv[1] > 0;
             float p[8];
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 floatx4_t s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
-                    const uint4 k = cur.k[m][w];
-                    s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(k.x, k.y), qf[2 * w], s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(k.z, k.w), qf[2 * w + 1], s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(k[m][w].x, k[m][w].y), qf[2 * w], s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(k[m][w].z, k[m][w].w), qf[2 * w + 1], s, 0, 0, 0);
                 }
-                const float f = cur.ks[m] * a.scale;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) p[4 * m + i] = 4 * grp + i < nv[m] ? s[i] * f : -__builtin_inff();
+                for (int i = 0; i < 4; ++i) p[4 * m + i] = s[i];
+                __builtin_amdgcn_sched_barrier(0);
             }
+            const float f[2] = {cur.ks[0] * a.scale, cur.ks[1] * a.scale}, vs[2] = {cur.vs[0], cur.vs[1]};
+            const int ahead = b + 2 < stop ? b + 2 : stop;
+            if (ahead < b1) {
+                cur = look(ahead);
+                load_k(cur);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                p[i] = 4 * grp + (i & 3) < nv[i / 4] ? p[i] * f[i / 4] : -__builtin_inff();
             float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
             top = fmaxf(top, __shfl_xor(top, 16, kWave));
             top = fmaxf(top, __shfl_xor(top, 32, kWave));
@@ -444,28 +505,30 @@ kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml
                 p[i] = 4 * grp + (i & 3) < nv[i / 4] ? __builtin_amdgcn_exp2f(p[i] - m_run) : 0.f;
                 l_run += p[i];
                 // a block that is masked whole may hold any scale
-                p[i] = p[i] == 0.f ? 0.f : p[i] * cur.vs[i / 4];
+                p[i] = p[i] == 0.f ? 0.f : p[i] * vs[i / 4];
             }
-            const uint4 pw = make_uint4(pack2_bf16(p[0], p[1]), pack2_bf16(p[2], p[3]), pack2_bf16(p[4], p[5]),
-                                        pack2_bf16(p[6], p[7]));
+            const u32x4 pw = {pack2_bf16(p[0], p[1]), pack2_bf16(p[2], p[3]), pack2_bf16(p[4], p[5]),
+                              pack2_bf16(p[6], p[7])};
             const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pw);
 #pragma unroll
             for (int w = 0; w < W; ++w) {
 #define NQ_V_FRAG(J)                                                                                                   \
     {                                                                                                                  \
-        const uint4 vw = make_uint4(pair_bf16(byte_f32<J>(cur.v[0][w]), byte_f32<J>(cur.v[1][w])),                     \
-                                    pair_bf16(byte_f32<J>(cur.v[2][w]), byte_f32<J>(cur.v[3][w])),                     \
-                                    pair_bf16(byte_f32<J>(cur.v[4][w]), byte_f32<J>(cur.v[5][w])),                     \
-                                    pair_bf16(byte_f32<J>(cur.v[6][w]), byte_f32<J>(cur.v[7][w])));                    \
+        const u32x4 vw = {                                                                                             \
+            pair_bf16(byte_f32<J>(v[0][w]), byte_f32<J>(v[1][w])), pair_bf16(byte_f32<J>(v[2][w]), byte_f32<J>(v[3][w])), \
+            pair_bf16(byte_f32<J>(v[4][w]), byte_f32<J>(v[5][w])), pair_bf16(byte_f32<J>(v[6][w]), byte_f32<J>(v[7][w]))}; \
         acc[4 * w + J] =                                                                                               \
             __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vw), pf, acc[4 * w + J], 0, 0, 0);    \
     }
                 NQ_V_FRAG(0)
                 NQ_V_FRAG(1)
+                __builtin_amdgcn_sched_barrier(0);
                 NQ_V_FRAG(2)
                 NQ_V_FRAG(3)
+                __builtin_amdgcn_sched_barrier(0);
 #undef NQ_V_FRAG
             }
+            if (ahead < b1) load_v(cur);
         }
         b = stop;
         l_run += __shfl_xor(l_run, 16, kWave);
@@ -481,9 +544,9 @@ kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml
 #pragma unroll
                     for (int j = 0; j < D / 32; ++j) w[j] = pack2_bf16(acc[2 * j][i] * inv, acc[2 * j + 1][i] * inv);
                     if constexpr (D == 128)
-                        *reinterpret_cast<uint4 *>(o + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+                        *reinterpret_cast<u32x4 *>(o + 8 * i) = u32x4{w[0], w[1], w[2], w[3]};
                     else
-                        *reinterpret_cast<uint2 *>(o + 4 * i) = make_uint2(w[0], w[1]);
+                        *reinterpret_cast<u32x2 *>(o + 4 * i) = u32x2{w[0], w[1]};
                 }
             } else {
                 const int64_t slot = ((static_cast<int64_t>(head) * waves + wi) * 2 + (rs >= b0 ? 1 : 0)) * a.group + c;
@@ -502,98 +565,103 @@ kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml
 }
 
 // Joins a decode row's partials: span i0, where the row begins, left its slot 1, the spans behind it slot 0.
-// Weights 2^(m_i - m), in span order.  A row without pages gets zeros.
+// Weights 2^(m_i - m), in span order.  A row without pages gets zeros.  A workgroup takes one query head:
+// D/4 threads a partial, 1024 / D partials at a time, four rounds of loads in flight.
 template <int D>
 __global__ void __launch_bounds__(kKv8Threads)
 kv8_merge_kernel(Attend8 a, int waves, const float2 *__restrict__ part_ml, const float *__restrict__ part_o) {
-    __shared__ float s_m[16], s_inv[16];
-    __shared__ float s_o[kKv8Waves][16 * D];
+    constexpr int TP = D / 4, AT = kKv8Threads / TP;  // threads a partial, partials at a time
+    __shared__ float s_red[2][kKv8Waves];
+    __shared__ float4 s_o[AT][TP];
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int r = blockIdx.x, head = blockIdx.y;
-    const Row8 row = row_of(a, r);
+    const int r = blockIdx.x, head = blockIdx.y / a.group, g = blockIdx.y % a.group;
+    const InPlace8 rows{a};
+    const Spans sp = spans_of(a, rows, waves);
+    const Row8 row = row_of(a, rows, r);
     if (row.q_len != 1) return;
-    uint16_t *out = a.out + row.q0 * a.o_s0 + head * a.group * a.o_s1;
-    const int vecs = a.group * (D / 4);
+    uint16_t *out = a.out + row.q0 * a.o_s0 + (head * a.group + g) * a.o_s1;
     if (row.n_pages == 0) {
-        for (int v = threadIdx.x; v < vecs; v += kKv8Threads)
-            *reinterpret_cast<uint2 *>(out + (v / (D / 4)) * a.o_s1 + (v % (D / 4)) * 4) = make_uint2(0, 0);
+        if (threadIdx.x < TP) *reinterpret_cast<u32x2 *>(out + 4 * threadIdx.x) = u32x2{0, 0};
         return;
     }
-    const Spans sp = spans_of(a, waves);
     const int64_t rs = static_cast<int64_t>(row.first_page) << a.bpp_log2;
     const int64_t re = static_cast<int64_t>(row.first_page + row.n_pages) << a.bpp_log2;
-    const int i0 = span_of(sp, rs), i1 = span_of(sp, re - 1);
-    if (i0 == i1) return;
-    const int n = i1 - i0 + 1;
+    const int i0 = span_of(sp, rs), n = span_of(sp, re - 1) - i0 + 1;
+    if (n == 1) return;
     const int64_t base = static_cast<int64_t>(head) * waves + i0;
-    auto slot = [&](int i, int g) { return ((base + i) * 2 + (i == 0 ? 1 : 0)) * a.group + g; };
-    for (int g = wave; g < a.group; g += kKv8Waves) {
-        float m = -__builtin_inff();
-        for (int i = lane; i < n; i += kWave) m = fmaxf(m, part_ml[slot(i, g)].x);
-        m = group_max<kWave>(m);
-        float l = 0.f;
-        for (int i = lane; i < n; i += kWave) {
-            const float2 ml = part_ml[slot(i, g)];
-            l += ml.y * (ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - m));
-        }
-        l = group_sum<kWave>(l);
-        if (lane == 0) {
-            s_m[g] = m;
-            s_inv[g] = l == 0.f && m == -__builtin_inff() ? 0.f : 1.0f / l;  // no page of the row in the pool
-        }
-    }
+    auto slot = [&](int i) __attribute__((always_inline)) { return ((base + i) * 2 + (i == 0 ? 1 : 0)) * a.group + g; };
+    float m = -__builtin_inff();
+    for (int i = threadIdx.x; i < n; i += kKv8Threads) m = fmaxf(m, part_ml[slot(i)].x);
+    m = group_max<kWave>(m);
+    if (lane == 0) s_red[0][wave] = m;
     __syncthreads();
-    for (int v = lane; v < vecs; v += kWave) {
-        const int g = v / (D / 4);
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = wave; i < n; i += kKv8Waves) {
-            const int64_t at = slot(i, g);
-            const float2 ml = part_ml[at];
-            const float4 x = *reinterpret_cast<const float4 *>(part_o + at * D + (v % (D / 4)) * 4);
-            const float w = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - s_m[g]);
-            o.x += w * x.x;
-            o.y += w * x.y;
-            o.z += w * x.z;
-            o.w += w * x.w;
-        }
-        *reinterpret_cast<float4 *>(&s_o[wave][4 * v]) = o;
-    }
-    __syncthreads();
-    for (int v = threadIdx.x; v < vecs; v += kKv8Threads) {
-        const int g = v / (D / 4);
-        float4 o = *reinterpret_cast<const float4 *>(&s_o[0][4 * v]);
 #pragma unroll
-        for (int w = 1; w < kKv8Waves; ++w) {
-            const float4 x = *reinterpret_cast<const float4 *>(&s_o[w][4 * v]);
-            o.x += x.x;
-            o.y += x.y;
-            o.z += x.z;
-            o.w += x.w;
+    for (int w = 0; w < kKv8Waves; ++w) m = fmaxf(m, s_red[0][w]);
+
+    const int at = threadIdx.x / TP, v = threadIdx.x % TP;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+    for (int i = at; i < n; i += 4 * AT) {
+        float2 ml[4];
+        float4 x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t p = slot(i + k * AT < n ? i + k * AT : i);
+            ml[k] = part_ml[p];
+            x[k] = *reinterpret_cast<const float4 *>(part_o + p * D + 4 * v);
         }
-        const float inv = s_inv[g];
-        *reinterpret_cast<uint2 *>(out + g * a.o_s1 + (v % (D / 4)) * 4) =
-            make_uint2(pack2_bf16(o.x * inv, o.y * inv), pack2_bf16(o.z * inv, o.w * inv));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (i + k * AT >= n) continue;
+            const float w = ml[k].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[k].x - m);
+            l += w * ml[k].y;
+            o.x += w * x[k].x;
+            o.y += w * x[k].y;
+            o.z += w * x[k].z;
+            o.w += w * x[k].w;
+        }
     }
+    s_o[at][v] = o;
+    __shared__ float s_l[AT];
+    if (v == 0) s_l[at] = l;
+    __syncthreads();
+    if (threadIdx.x >= TP) return;
+    l = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < AT; ++k) {
+        const float4 x = s_o[k][v];
+        l += s_l[k];
+        o.x += x.x;
+        o.y += x.y;
+        o.z += x.z;
+        o.w += x.w;
+    }
+    const float inv = l == 0.f && m == -__builtin_inff() ? 0.f : 1.0f / l;  // 0: no page of the row is in the pool
+    *reinterpret_cast<u32x2 *>(out + 4 * v) = u32x2{pack2_bf16(o.x * inv, o.y * inv), pack2_bf16(o.z * inv, o.w * inv)};
 }
 
-// Rows of several queries.  A workgroup takes 128 columns (128 / G queries times the G query heads of one kv
-// head) against 64-key tiles, a wave 32 columns with mfma_32x32x16: S^T = K Q^T, out^T = V^T P^T, so a
-// column's scores, maximum and output stay in two lanes.  K and V are widened to bf16 once a workgroup, on
-// their way to LDS (V transposed, keys in the order in which a lane holds P); a tile's loads are in flight while
-// the one before it is multiplied.  With few tiles the key range is cut into pieces, joined by kv8_join_kernel.
-constexpr int kCols = 128, kKeys = 64;
+// Rows of several queries.  A workgroup of NW waves takes 32 NW columns (queries times the G query heads of one kv
+// head) against 64-key tiles, a wave 32 columns with mfma_32x32x16: S^T = K Q^T, out^T = V^T P^T, so a column's
+// scores, maximum and output stay in two lanes and P needs no exchange.  K and V are widened to bf16, times their
+// scales, once a workgroup on their way to LDS (V transposed, keys in the order in which a lane holds P); a
+// tile's loads are in flight while the one before it is multiplied.  Sums are rescaled only when a maximum has grown
+// by more than 2^8 (P stays below that, and bf16 and fp32 lose nothing by it).  With few tiles the key range is
+// cut into pieces, joined by kv8_join_kernel.
+constexpr int kKeys = 64;
+constexpr float kLag = 8.0f;
 
 struct Tile8 {
     int q0, n_q, limit0;  // first query token, queries, keys the first of them sees
     int n_keys;           // keys the last of them sees
 };
-__device__ __forceinline__ int tile_queries(const Attend8 &a) { return kCols / a.group; }
 // Slot s of the launch is tile s - (qo_indptr[r] / nq + r) of row r: those bases need no scan, and a row's
 // share is enough for its tiles.  False where the slot is no tile of this launch.
-__device__ __forceinline__ bool tile_of(const Attend8 &a, int slot, int skip_single, Row8 &row, Tile8 &t) {
-    const int nq = tile_queries(a);
-    const int r = wave_find_le(a.rows, slot, [&](int i) { return a.qo_indptr[i] / nq + i; });
-    row = row_of(a, r);
+template <typename R>
+__device__ __forceinline__ bool tile_of(const Attend8 &a, const R &rows, int nq, int slot, int skip_single, Row8 &row,
+                                        Tile8 &t) {
+    const int r = wave_find_le(a.rows, slot, [&](int i) { return rows.qo(i) / nq + i; });
+    row = row_of(a, rows, r);
     const int first = (slot - (row.q0 / nq + r)) * nq;
     if (first < 0 || first >= row.q_len || (skip_single && row.q_len == 1)) return false;
     t.q0 = row.q0 + first;
@@ -604,15 +672,16 @@ __device__ __forceinline__ bool tile_of(const Attend8 &a, int slot, int skip_sin
     return true;
 }
 __device__ __forceinline__ int pieces_of(const Tile8 &t, int splits) {
-    const int n = (t.n_keys + kKeys - 1) / kKeys / 4;  // at least four key tiles a piece
+    const int n = (t.n_keys + kKeys - 1) / kKeys / 2;  // at least two key tiles a piece
     return n < 1 ? 1 : (n < splits ? n : splits);
 }
 
 template <int D>
 struct Smem8 {
-    uint4 k[2][kKeys * (D / 8)];
-    uint4 v[2][D * (kKeys / 8)];
-    float ks[2][kKeys / kBlk], vs[2][kKeys / kBlk];
+    u32x4 k[2][kKeys * (D / 8)];
+    u32x4 v[2][D * (kKeys / 8)];
+    int absent[2][kKeys / kBlk];  // the block's page is not in the pool
+    Meta8 meta;
 };
 // 16-byte chunk positions, exclusive-ored so that eight neighbouring rows, and the writes of a stage, spread over
 // all banks.
@@ -622,24 +691,121 @@ __device__ __forceinline__ int k_chunk(int key, int chunk) {
 }
 __device__ __forceinline__ int v_chunk(int d, int chunk) { return d * (kKeys / 8) + (chunk ^ ((d ^ (d >> 3)) & 7)); }
 
-template <int D>
-__global__ void __launch_bounds__(kKv8Threads, 2)
+template <int D, int NW>
+__global__ void __launch_bounds__(NW * kWave, 2)
 kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single, float2 *__restrict__ part_ml,
                    float *__restrict__ part_o) {
-    constexpr int W = D / 64;
+    constexpr int T = NW * kWave, COLS = 32 * NW;
+    // K: a thread stages KL 16-byte pieces of one key; V: VB values of each of four keys
+    constexpr int KL = kKeys * D / 16 / T, KT = T / kKeys;  // KT threads a key
+    constexpr int VB = kKeys * D / 4 / T;                   // 4, 8 (or 2) bytes
+    static_assert(KL * T * 16 == kKeys * D || KL == 0, "K stages evenly");
     __shared__ Smem8<D> sm;
+    load_meta(a, sm.meta);
+    const Rows8 rows{a, sm.meta};
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int head = blockIdx.x % a.heads;
     const int slot = slots - 1 - static_cast<int>(blockIdx.x) / a.heads;  // the longest key ranges first
     Row8 row;
     Tile8 t;
-    if (!tile_of(a, slot, skip_single, row, t)) return;
+    if (!tile_of(a, rows, COLS / a.group, slot, skip_single, row, t)) return;
     const int pieces = pieces_of(t, splits);
     const int piece = blockIdx.y;
     if (piece >= pieces) return;
     const int n_kt = (t.n_keys + kKeys - 1) / kKeys;
-    const int kt0 = static_cast<int>(static_cast<int64_t>(n_kt) * piece / pieces);
-    const int kt1 = static_cast<int>(static_cast<int64_t>(n_kt) * (piece + 1) / pieces);
+    const int kt0 = n_kt * piece / pieces, kt1 = n_kt * (piece + 1) / pieces;
+
+    // staging: a wave holds 64 / NW keys of one block, so its page, its scales and their addresses are uniform
+    constexpr int KB = KL > 0 ? 16 : 8;  // bytes of a K load
+    const int sk_key = threadIdx.x / KT, sk_piece = threadIdx.x % KT;
+    constexpr int VT = T / (kKeys / 4);  // threads of a quad of keys
+    const int sv_quad = threadIdx.x / VT, sv_part = threadIdx.x % VT;
+    const int uwave = __builtin_amdgcn_readfirstlane(wave);
+    const int c_slot = static_cast<int>(pool.c_slot);
+    const int k_off = sk_key % kBlk * c_slot + KB * sk_piece;
+    const int v_off = 4 * (sv_quad % 4) * c_slot + VB * sv_part;
+    const int8_t *base = pool.codes + head * pool.c_head;
+    const float *s_base = pool.scales + head * pool.s_head;
+    u32x4 kr[KL > 0 ? KL : 1];
+    u32x2 vr[4];
+    float r_ks = 0.f, r_vs = 0.f;
+    bool r_on = true;
+    const int n_blocks = (row.kv_len + kBlk - 1) / kBlk;
+    const int in_page = (1 << a.bpp_log2) - 1;
+    auto block_of = [&](int kt) __attribute__((always_inline)) {  // beyond the row's keys, which are masked: the last
+        const int blk = kt * (kKeys / kBlk) + uwave * (kKeys / kBlk) / NW;
+        return blk < n_blocks ? blk : n_blocks - 1;
+    };
+    auto page_of = [&](int kt) __attribute__((always_inline)) {
+        return a.kv_indices[row.first_page + (block_of(kt) >> a.bpp_log2)];
+    };
+    int page = 0;  // of the next load
+    auto load = [&](int kt) __attribute__((always_inline)) {
+        r_on = page >= 0 && page < pool.num_pages;
+        if (!r_on && a.status) *a.status = NQ_ERR_INVALID_ARGUMENT;
+        const int64_t pid = r_on ? page : 0;
+        const int blk = block_of(kt) & in_page;
+        const int8_t *kp = base + pid * pool.c_page + blk * (kBlk * pool.c_slot);
+        const int8_t *vp = kp + pool.c_kind;
+        if constexpr (KL > 0) {
+#pragma unroll
+            for (int w = 0; w < KL; ++w) kr[w] = *reinterpret_cast<const u32x4 *>(kp + (k_off + 16 * KT * w));
+        } else {
+            const u32x2 half = *reinterpret_cast<const u32x2 *>(kp + k_off);
+            kr[0] = u32x4{half.x, half.y, 0, 0};
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int8_t *p = vp + (v_off + e * c_slot);
+            if constexpr (VB == 8) vr[e] = *reinterpret_cast<const u32x2 *>(p);
+            else if constexpr (VB == 4) vr[e].x = *reinterpret_cast<const uint32_t *>(p);
+            else vr[e].x = *reinterpret_cast<const uint16_t *>(p);
+        }
+        const float *sc = s_base + pid * pool.s_page + blk * pool.s_block;
+        r_ks = sc[0];
+        r_vs = sc[pool.s_kind];
+        if (kt + 1 < kt1) page = page_of(kt + 1);
+    };
+    auto store = [&](int buf) __attribute__((always_inline)) {
+        // A V scale that is not finite answers through the scores of the queries that see the block, not through
+        // 0 * NaN in those that do not.
+        const bool fine = fabsf(r_vs) < __builtin_inff();
+        const float ks = fine ? r_ks : __builtin_nanf(""), vs = fine ? r_vs : 0.f;
+        if constexpr (KL > 0) {
+#pragma unroll
+            for (int w = 0; w < KL; ++w) {
+                const int chunk = 2 * (KT * w + sk_piece);
+                sm.k[buf][k_chunk<D>(sk_key, chunk)] = scale8(kr[w].x, kr[w].y, ks);
+                sm.k[buf][k_chunk<D>(sk_key, chunk + 1)] = scale8(kr[w].z, kr[w].w, ks);
+            }
+        } else {
+            sm.k[buf][k_chunk<D>(sk_key, sk_piece)] = scale8(kr[0].x, kr[0].y, ks);
+        }
+        // key 8 a + 4 b + i of a block sits at position 8 b + 4 a + i
+        const int quad = sv_quad & 3, chunk = 2 * (sv_quad / 4) + (quad & 1), upper = quad >> 1;
+#define NQ_V_PUT(W, J)                                                                                     \
+    reinterpret_cast<u32x2 *>(&sm.v[buf][v_chunk(sv_part * VB + 4 * W + J, chunk)])[upper] =               \
+        u32x2{pack2_bf16(byte_f32<J>(vr[0][W]) * vs, byte_f32<J>(vr[1][W]) * vs),                          \
+              pack2_bf16(byte_f32<J>(vr[2][W]) * vs, byte_f32<J>(vr[3][W]) * vs)};
+        NQ_V_PUT(0, 0)
+        NQ_V_PUT(0, 1)
+        if constexpr (VB >= 4) {
+            NQ_V_PUT(0, 2)
+            NQ_V_PUT(0, 3)
+        }
+        if constexpr (VB == 8) {
+            NQ_V_PUT(1, 0)
+            NQ_V_PUT(1, 1)
+            NQ_V_PUT(1, 2)
+            NQ_V_PUT(1, 3)
+        }
+#undef NQ_V_PUT
+        if (threadIdx.x % (KT * kBlk) == 0) sm.absent[buf][sk_key / kBlk] = !r_on;
+    };
+    if (kt0 < kt1) {
+        page = page_of(kt0);
+        load(kt0);
+    }
 
     const int c = lane & 31, half = lane >> 5;
     const int col = wave * 32 + c;
@@ -648,99 +814,17 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
     const int limit = live ? t.limit0 + qi : 0;
     bf16x8_t qf[D / 16];
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (live)
-            v = *reinterpret_cast<const uint4 *>(a.q + (t.q0 + qi) * a.q_s0 + (head * a.group + g) * a.q_s1 + 16 * s +
-                                                 8 * half);
-        qf[s] = __builtin_bit_cast(bf16x8_t, v);
+    for (int s = 0; s < D / 16; ++s)
+        qf[s] = load_q(a.q + (t.q0 + qi) * a.q_s0 + (head * a.group + g) * a.q_s1 + 16 * s + 8 * half, live, a.flip);
+
+    // Where the lane reads: chunks 2 k + half of key row c, and of V row c.  The exclusive-or moves the low three
+    // bits only, so the other chunks, rows and buffers are these places plus constants: chunk + 8 for K; V row + 32 flips bit 2.
+    int at_k[4], at_v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        at_k[k] = k_chunk<D>(c, 2 * k + half);
+        at_v[k] = v_chunk(c, 2 * k + half);
     }
-
-    // staging: K thread t holds 16-byte pieces t % 4 (and + 4) of key t / 4; V thread t holds D/16 values of the four keys
-    // 4 (t / 16) ..
-    const int sk_key = threadIdx.x / 4, sk_piece = threadIdx.x & 3;
-    const int sv_quad = threadIdx.x / 16, sv_part = threadIdx.x & 15;
-    uint4 kr[W];
-    uint32_t vr[4][W];
-    float scale_r = 0.f;
-    const int n_blocks = (row.kv_len + kBlk - 1) / kBlk;
-    auto page_of = [&](int blk, bool &on) {  // blk: block of the row; beyond its keys, the last
-        const int b = blk < n_blocks ? blk : n_blocks - 1;
-        const int pid = a.kv_indices[row.first_page + (b >> a.bpp_log2)];
-        on = pid >= 0 && pid < pool.num_pages;
-        return on ? pid : 0;
-    };
-    auto load = [&](int kt) {
-        bool on;
-        {
-            const int blk = kt * (kKeys / kBlk) + sk_key / kBlk;
-            const int pid = page_of(blk, on);
-            const int b = blk < n_blocks ? blk : n_blocks - 1;
-            const int in_page = b & ((1 << a.bpp_log2) - 1);
-            const int8_t *p = pool.codes + pid * pool.c_page + (in_page * kBlk + sk_key % kBlk) * pool.c_slot +
-                              head * pool.c_head + 16 * sk_piece;
-#pragma unroll
-            for (int w = 0; w < W; ++w) kr[w] = *reinterpret_cast<const uint4 *>(p + 64 * w);
-        }
-        {
-            const int blk = kt * (kKeys / kBlk) + sv_quad / 4;
-            const int pid = page_of(blk, on);
-            const int b = blk < n_blocks ? blk : n_blocks - 1;
-            const int in_page = b & ((1 << a.bpp_log2) - 1);
-            const int8_t *p = pool.codes + pid * pool.c_page + pool.c_kind +
-                              (in_page * kBlk + 4 * (sv_quad % 4)) * pool.c_slot + head * pool.c_head +
-                              sv_part * (D / 16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if constexpr (W == 2) {
-                    const uint2 d = *reinterpret_cast<const uint2 *>(p + e * pool.c_slot);
-                    vr[e][0] = d.x;
-                    vr[e][1] = d.y;
-                } else {
-                    vr[e][0] = *reinterpret_cast<const uint32_t *>(p + e * pool.c_slot);
-                }
-            }
-        }
-        if (threadIdx.x < 2 * (kKeys / kBlk)) {  // the tile's scales; a block that is not there weighs nothing
-            const int kind = threadIdx.x / (kKeys / kBlk);
-            const int blk = kt * (kKeys / kBlk) + threadIdx.x % (kKeys / kBlk);
-            scale_r = 0.f;
-            if (blk < n_blocks) {
-                const int pid = page_of(blk, on);
-                scale_r = pool.scales[pid * pool.s_page + kind * pool.s_kind +
-                                      (blk & ((1 << a.bpp_log2) - 1)) * pool.s_block + head * pool.s_head];
-                if (!on) {
-                    scale_r = kind ? 0.f : -__builtin_inff();  // K: marks the block as absent
-                    if (a.status) *a.status = NQ_ERR_INVALID_ARGUMENT;
-                }
-            }
-        }
-    };
-    auto store = [&](int buf) {
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const int chunk = 8 * w + 2 * sk_piece;
-            sm.k[buf][k_chunk<D>(sk_key, chunk)] = __builtin_bit_cast(uint4, widen8(kr[w].x, kr[w].y));
-            sm.k[buf][k_chunk<D>(sk_key, chunk + 1)] = __builtin_bit_cast(uint4, widen8(kr[w].z, kr[w].w));
-        }
-        // key 8 a + 4 b + i of a block sits at position 8 b + 4 a + i
-        const int quad = sv_quad & 3, chunk = 2 * (sv_quad / 4) + (quad & 1), upper = quad >> 1;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-#define NQ_V_PUT(J)                                                                                        \
-    reinterpret_cast<uint2 *>(&sm.v[buf][v_chunk(sv_part * (D / 16) + 4 * w + J, chunk)])[upper] =         \
-        make_uint2(pair_bf16(byte_f32<J>(vr[0][w]), byte_f32<J>(vr[1][w])),                                \
-                   pair_bf16(byte_f32<J>(vr[2][w]), byte_f32<J>(vr[3][w])));
-            NQ_V_PUT(0)
-            NQ_V_PUT(1)
-            NQ_V_PUT(2)
-            NQ_V_PUT(3)
-#undef NQ_V_PUT
-        }
-        if (threadIdx.x < kKeys / kBlk) sm.ks[buf][threadIdx.x] = scale_r;
-        else if (threadIdx.x < 2 * (kKeys / kBlk)) sm.vs[buf][threadIdx.x - kKeys / kBlk] = scale_r;
-    };
-
     floatx16_t acc[D / 32];
 #pragma unroll
     for (int j = 0; j < D / 32; ++j)
@@ -748,72 +832,65 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
         for (int i = 0; i < 16; ++i) acc[j][i] = 0.f;
     float m_run = -__builtin_inff(), l_run = 0.f;
     bool any = false;  // whether the column has seen a key
-    if (kt0 < kt1) {
-        load(kt0);
-        store(0);
-    }
+    if (kt0 < kt1) store(0);
     for (int kt = kt0; kt < kt1; ++kt) {
         const int buf = (kt - kt0) & 1;
         __syncthreads();
         if (kt + 1 < kt1) load(kt + 1);
-        float p[32];
+        floatx16_t s[2];
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) {
-            floatx16_t s;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = 0.f;
+            for (int i = 0; i < 16; ++i) s[sub][i] = 0.f;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                    __builtin_bit_cast(bf16x8_t, sm.k[buf][k_chunk<D>(32 * sub + c, 2 * k + half)]), qf[k], s, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) p[16 * sub + i] = s[i];
+                s[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                    __builtin_bit_cast(bf16x8_t, sm.k[buf][at_k[k % 4] + 32 * (D / 8) * sub + 8 * (k / 4)]), qf[k],
+                    s[sub], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);  // one half's operands in registers at a time
         }
         const int key0 = kt * kKeys;
-        float ks[4], vs[4];
-        bool whole = key0 + kKeys <= t.limit0;
+        int gone[kKeys / kBlk], none = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            ks[k] = sm.ks[buf][k];
-            vs[k] = sm.vs[buf][k];
-            whole = whole && ks[k] != -__builtin_inff();
-        }
+        for (int k = 0; k < kKeys / kBlk; ++k) none |= gone[k] = sm.absent[buf][k];
+        const bool whole = key0 + kKeys <= t.limit0 && !__builtin_amdgcn_readfirstlane(none);
+        // lane's element i: key 32 (i / 16) + 8 (i / 4 % 4) + 4 half + i % 4
+        auto sees = [&](int i) __attribute__((always_inline)) {
+            return key0 + 32 * (i / 16) + 8 * (i / 4 % 4) + 4 * half + (i & 3) < limit && !gone[i / 8];
+        };
         float top = -__builtin_inff();
         if (whole) {
             any = true;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                p[i] *= ks[i / 8] * a.scale;
-                top = fmaxf(top, p[i]);
-            }
+            for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i / 16][i % 16]);
         } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-                // lane's i: key 32 (i / 16) + 8 (i / 4 % 4) + 4 half + i % 4
-                const int key = key0 + 32 * (i / 16) + 8 * (i / 4 % 4) + 4 * half + (i & 3);
-                const bool see = key < limit && ks[i / 8] != -__builtin_inff();
+                const bool see = sees(i);
                 any |= see;
-                p[i] = see ? p[i] * (ks[i / 8] * a.scale) : -__builtin_inff();
-                top = fmaxf(top, p[i]);
+                top = fmaxf(top, see ? s[i / 16][i % 16] : -__builtin_inff());
             }
         }
         top = fmaxf(top, __shfl_xor(top, 32, kWave));
-        const float m_new = fmaxf(m_run, top);
-        if (__any(m_new != m_run)) {
+        top = top == -__builtin_inff() ? top : top * a.scale;
+        if (__any(top > m_run + kLag)) {
+            const float m_new = fmaxf(m_run, top);
             const float alpha = m_run == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
             l_run *= alpha;
 #pragma unroll
             for (int j = 0; j < D / 32; ++j) acc[j] *= alpha;
             m_run = m_new;
         }
-        const float m_use = any || m_run != -__builtin_inff() ? m_run : 0.f;
         uint32_t pw[16];
+        float sum[2] = {0.f, 0.f};
         if (whole) {
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-                const float x = __builtin_amdgcn_exp2f(p[i] - m_use), y = __builtin_amdgcn_exp2f(p[i + 1] - m_use);
-                l_run += x + y;
-                pw[i / 2] = pack2_bf16(x * vs[i / 8], y * vs[i / 8]);
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16], a.scale, -m_run));
+                const float y = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16 + 1], a.scale, -m_run));
+                sum[0] += x;
+                sum[1] += y;
+                pw[i / 2] = pack2_bf16(x, y);
             }
         } else {
 #pragma unroll
@@ -821,23 +898,24 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
                 float z[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int key = key0 + 32 * (i / 16) + 8 * (i / 4 % 4) + 4 * half + ((i + e) & 3);
-                    const bool see = key < limit && ks[i / 8] != -__builtin_inff();
-                    z[e] = see ? __builtin_amdgcn_exp2f(p[i + e] - m_use) : 0.f;
-                    l_run += z[e];
-                    z[e] = see ? z[e] * vs[i / 8] : 0.f;  // masked blocks may hold any scale
+                    z[e] = sees(i + e) ? __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16 + e], a.scale, -m_run)) : 0.f;
+                    sum[e] += z[e];
                 }
                 pw[i / 2] = pack2_bf16(z[0], z[1]);
             }
         }
+        l_run += sum[0] + sum[1];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const bf16x8_t pf =
-                __builtin_bit_cast(bf16x8_t, make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]));
+                __builtin_bit_cast(bf16x8_t, u32x4{pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]});
 #pragma unroll
             for (int j = 0; j < D / 32; ++j)
                 acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                    __builtin_bit_cast(bf16x8_t, sm.v[buf][v_chunk(32 * j + c, 2 * k + half)]), pf, acc[j], 0, 0, 0);
+                    __builtin_bit_cast(bf16x8_t, sm.v[buf][at_v[k ^ (2 * (j & 1))] + 32 * (kKeys / 8) * j]), pf, acc[j],
+                    0, 0, 0);
+            if (k & 1) __builtin_amdgcn_sched_barrier(0);
         }
         if (kt + 1 < kt1) store(buf ^ 1);
     }
@@ -852,11 +930,11 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
         for (int j = 0; j < D / 32; ++j)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<uint2 *>(o + 32 * j + 2 * i) =
-                    make_uint2(pack2_bf16(acc[j][i] * inv, acc[j][i + 1] * inv),
-                               pack2_bf16(acc[j][i + 2] * inv, acc[j][i + 3] * inv));
+                *reinterpret_cast<u32x2 *>(o + 32 * j + 2 * i) =
+                    u32x2{pack2_bf16(acc[j][i] * inv, acc[j][i + 1] * inv),
+                          pack2_bf16(acc[j][i + 2] * inv, acc[j][i + 3] * inv)};
     } else {
-        const int64_t at = ((static_cast<int64_t>(slot) * a.heads + head) * splits + piece) * kCols + col;
+        const int64_t at = ((static_cast<int64_t>(slot) * a.heads + head) * splits + piece) * COLS + col;
         if (half == 0) part_ml[at] = make_float2(any ? m_run : -__builtin_inff(), l_run);
         float *o = part_o + at * D + 4 * half;
 #pragma unroll
@@ -868,41 +946,57 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
     }
 }
 
-// Joins the pieces of a tile, in order: a wave a column at a time.
+// Joins the pieces of a tile, in order: D/8 threads a column, every piece's values in flight at once.
+constexpr int kMaxPieces = 8;
 template <int D>
 __global__ void __launch_bounds__(kKv8Threads)
-kv8_join_kernel(Attend8 a, int slots, int splits, int skip_single, const float2 *__restrict__ part_ml,
+kv8_join_kernel(Attend8 a, int cols, int slots, int splits, int skip_single, const float2 *__restrict__ part_ml,
                 const float *__restrict__ part_o) {
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    constexpr int TP = D / 8;
+    __shared__ Meta8 meta;
+    load_meta(a, meta);
     const int head = blockIdx.x % a.heads, slot = static_cast<int>(blockIdx.x) / a.heads;
     Row8 row;
     Tile8 t;
-    if (!tile_of(a, slot, skip_single, row, t)) return;
+    if (!tile_of(a, Rows8{a, meta}, cols / a.group, slot, skip_single, row, t)) return;
     const int pieces = pieces_of(t, splits);
-    if (pieces == 1) return;
-    const int64_t base = (static_cast<int64_t>(slot) * a.heads + head) * splits * kCols;
-    constexpr int PER = D / kWave;  // values a lane
-    for (int col = blockIdx.y * kKv8Waves + wave; col < t.n_q * a.group; col += gridDim.y * kKv8Waves) {
-        float m = -__builtin_inff();
-        for (int i = 0; i < pieces; ++i) m = fmaxf(m, part_ml[base + i * kCols + col].x);
-        float l = 0.f, o[PER];
+    const int col = blockIdx.y * (kKv8Threads / TP) + threadIdx.x / TP, v = threadIdx.x % TP;
+    if (pieces == 1 || col >= t.n_q * a.group) return;
+    const int64_t base = (static_cast<int64_t>(slot) * a.heads + head) * splits * cols + col;
+    float2 ml[kMaxPieces];
+    float4 x[kMaxPieces][2];
 #pragma unroll
-        for (int e = 0; e < PER; ++e) o[e] = 0.f;
-        for (int i = 0; i < pieces; ++i) {
-            const float2 ml = part_ml[base + i * kCols + col];
-            const float w = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);
-            l += w * ml.y;
-            const float *x = part_o + (base + i * kCols + col) * D + PER * lane;
-#pragma unroll
-            for (int e = 0; e < PER; ++e) o[e] += w * x[e];
+    for (int i = 0; i < kMaxPieces; ++i) {
+        if (i < pieces) {
+            ml[i] = part_ml[base + static_cast<int64_t>(i) * cols];
+            const float4 *p = reinterpret_cast<const float4 *>(part_o + (base + static_cast<int64_t>(i) * cols) * D + 8 * v);
+            x[i][0] = p[0];
+            x[i][1] = p[1];
         }
-        const bool none = l == 0.f && m == -__builtin_inff();
-        const float inv = none ? 0.f : 1.0f / l;
-        const int qi = col / a.group, g = col - qi * a.group;
-        uint16_t *out = a.out + (t.q0 + qi) * a.o_s0 + (head * a.group + g) * a.o_s1 + PER * lane;
-        if constexpr (PER == 2) *reinterpret_cast<uint32_t *>(out) = pack2_bf16(o[0] * inv, o[1] * inv);
-        else out[0] = f32_to_bf16(o[0] * inv);
     }
+    float m = -__builtin_inff(), l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kMaxPieces; ++i)
+        if (i < pieces) m = fmaxf(m, ml[i].x);
+#pragma unroll
+    for (int i = 0; i < kMaxPieces; ++i) {
+        if (i < pieces) {
+            const float w = ml[i].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[i].x - m);
+            l += w * ml[i].y;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                o[4 * h] += w * x[i][h].x;
+                o[4 * h + 1] += w * x[i][h].y;
+                o[4 * h + 2] += w * x[i][h].z;
+                o[4 * h + 3] += w * x[i][h].w;
+            }
+        }
+    }
+    const float inv = l == 0.f && m == -__builtin_inff() ? 0.f : 1.0f / l;
+    const int qi = col / a.group, g = col - qi * a.group;
+    *reinterpret_cast<u32x4 *>(a.out + (t.q0 + qi) * a.o_s0 + (head * a.group + g) * a.o_s1 + 8 * v) =
+        u32x4{pack2_bf16(o[0] * inv, o[1] * inv), pack2_bf16(o[2] * inv, o[3] * inv), pack2_bf16(o[4] * inv, o[5] * inv),
+              pack2_bf16(o[6] * inv, o[7] * inv)};
 }
 
 // Waves of the decode launch per kv head: eight a CU.
@@ -911,16 +1005,26 @@ int decode_waves(int heads) {
     return (groups < 1 ? 1 : groups) * kKv8Waves;
 }
 struct Prefill8 {
-    int slots, splits;
+    int waves, cols, slots, splits;
 };
-// Pieces so that about 512 workgroups (two a CU) have work.
+// Eight waves (a CU holds one such workgroup) where the rows fill their 256 columns on average, else four (two a CU).
+// Pieces: the fewest that keep 85 % of the CUs in work, or come nearest to it.
 Prefill8 prefill_plan(int tokens, int rows, int group, int heads) {
-    const int nq = kCols / group;
-    const int slots = tokens / nq + rows;
-    const int wgs = slots * heads;
-    int s = (512 + wgs - 1) / wgs;
-    s = s < 1 ? 1 : (s > 8 ? 8 : s);
-    return {slots, s};
+    Prefill8 p;
+    p.waves = static_cast<int64_t>(tokens) * group >= 256ll * rows ? 8 : 4;
+    p.cols = 32 * p.waves;
+    p.slots = tokens / (p.cols / group) + rows;
+    const int64_t wgs = static_cast<int64_t>(p.slots) * heads, room = p.waves == 8 ? 256 : 512;
+    double best = 0.0;
+    p.splits = 1;
+    for (int s = 1; s <= kMaxPieces && best < 0.85; ++s) {
+        const double use = static_cast<double>(wgs * s) / static_cast<double>((wgs * s + room - 1) / room * room);
+        if (use > best * 1.05) {
+            best = use;
+            p.splits = s;
+        }
+    }
+    return p;
 }
 struct Layout8 {
     int64_t d_ml, d_o, p_ml, p_o, total;
@@ -939,7 +1043,7 @@ Layout8 layout8(int tokens, int rows, int qo_heads, int heads, int D, int parts)
     }
     if (parts & NQ_ATTN_PREFILL) {
         const Prefill8 p = prefill_plan(tokens, rows, group, heads);
-        const int64_t n = p.splits > 1 ? static_cast<int64_t>(p.slots) * heads * p.splits * kCols : 0;
+        const int64_t n = p.splits > 1 ? static_cast<int64_t>(p.slots) * heads * p.splits * p.cols : 0;
         L.p_ml = off;
         off = up256(off + n * 8);
         L.p_o = off;
@@ -963,7 +1067,7 @@ int check_pool(const Pool8 &p, int heads, int head_dim) {
     if (!al(p.codes, 16) || odd_stride(p.num_pages, p.c_page, 16) || p.c_kind % 16 || p.c_slot % 16 ||
         odd_stride(heads, p.c_head, 16) || !al(p.scales, 4))
         return NQ_ERR_UNSUPPORTED;
-    if (p.c_slot > (1 << 26)) return NQ_ERR_UNSUPPORTED;  // 16 slots of a block stay within 32-bit offsets
+    if (p.c_slot >= (1 << 26)) return NQ_ERR_UNSUPPORTED;  // 16 slots of a block stay within 32-bit offsets
     return NQ_OK;
 }
 
@@ -1039,20 +1143,26 @@ int launch_attention8(const Attend8 &a, const Pool8 &pool, int parts, char *ws, 
         const int waves = decode_waves(a.heads);
         float2 *ml = reinterpret_cast<float2 *>(ws + L.d_ml);
         float *o = reinterpret_cast<float *>(ws + L.d_o);
-        hipLaunchKernelGGL((kv8_decode_kernel<D>), dim3(waves / kKv8Waves * a.heads), dim3(kKv8Threads), 0, st, a, pool,
-                           waves, ml, o);
-        hipLaunchKernelGGL((kv8_merge_kernel<D>), dim3(a.rows, a.heads), dim3(kKv8Threads), 0, st, a, waves, ml, o);
+        hipLaunchKernelGGL((kv8_decode_kernel<D>), dim3(((waves + 7) / 8 * a.heads + kKv8Waves - 1) / kKv8Waves * 8),
+                           dim3(kKv8Threads), 0, st, a, pool, waves, ml, o);
+        hipLaunchKernelGGL((kv8_merge_kernel<D>), dim3(a.rows, a.heads * a.group), dim3(kKv8Threads), 0, st, a, waves, ml, o);
     }
     if (parts & NQ_ATTN_PREFILL) {
         const Prefill8 p = prefill_plan(a.tokens, a.rows, a.group, a.heads);
         const int skip = (parts & NQ_ATTN_DECODE) ? 1 : 0;
         float2 *ml = reinterpret_cast<float2 *>(ws + L.p_ml);
         float *o = reinterpret_cast<float *>(ws + L.p_o);
-        hipLaunchKernelGGL((kv8_prefill_kernel<D>), dim3(p.slots * a.heads, p.splits), dim3(kKv8Threads), 0, st, a,
-                           pool, p.slots, p.splits, skip, ml, o);
+        const dim3 grid(p.slots * a.heads, p.splits);
+        if (p.waves == 8)
+            hipLaunchKernelGGL((kv8_prefill_kernel<D, 8>), grid, dim3(8 * kWave), 0, st, a, pool, p.slots, p.splits, skip,
+                               ml, o);
+        else
+            hipLaunchKernelGGL((kv8_prefill_kernel<D, 4>), grid, dim3(4 * kWave), 0, st, a, pool, p.slots, p.splits, skip,
+                               ml, o);
         if (p.splits > 1)
-            hipLaunchKernelGGL((kv8_join_kernel<D>), dim3(p.slots * a.heads, 8), dim3(kKv8Threads), 0, st, a, p.slots,
-                               p.splits, skip, ml, o);
+            hipLaunchKernelGGL((kv8_join_kernel<D>), dim3(p.slots * a.heads, p.cols * (D / 8) / kKv8Threads),
+                               dim3(kKv8Threads), 0, st, a, p.cols,
+                               p.slots, p.splits, skip, ml, o);
     }
     return NQ_LAUNCH_STATUS();
 }
@@ -1095,7 +1205,7 @@ extern "C" int nq_paged_attention_int8(const int32_t *qo_indptr, const int32_t *
     const Attend8 a = {q,     q_s0,        q_s1,   out,         o_s0,
                        o_s1,  qo_indptr,   kv_indptr, kv_indices,  last_page_len,
                        n_rows, tokens,     num_indices, num_qo_heads / num_kv_heads, num_kv_heads,
-                       bpp,   sm_scale * kLog2e8, status};
+                       bpp,   fabsf(sm_scale) * kLog2e8, sm_scale < 0.f ? 0x80008000u : 0u, status};
     char *ws = static_cast<char *>(workspace);
     const Layout8 L = layout8(tokens, n_rows, num_qo_heads, num_kv_heads, head_dim, parts);
     hipStream_t st = static_cast<hipStream_t>(stream);

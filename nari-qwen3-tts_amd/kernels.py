@@ -344,41 +344,49 @@ INT8_BLOCK = 16  # cache slots that share a scale
 
 
 def _int8_cache(layer_cache: torch.Tensor, layer_scales: torch.Tensor) -> tuple:
-    """The C ABI's cache arguments after checks: codes and strides, scales and strides, pages, page size."""
+    """Heads, head size and the C ABI's cache arguments after checks: codes and strides, scales and strides, pages,
+    page size."""
 
-    if layer_cache.dtype != torch.int8 or layer_scales.dtype != torch.float32:
+    if layer_cache.dtype is not torch.int8 or layer_scales.dtype is not torch.float32:
         raise TypeError("the 8-bit cache is int8 codes with float32 scales")
-    if layer_cache.ndim != 5 or layer_cache.shape[1] != 2 or layer_cache.shape[0] < 1 or layer_cache.stride(4) != 1:
+    shape, strides = layer_cache.shape, layer_cache.stride()
+    if len(shape) != 5 or shape[1] != 2 or shape[0] < 1 or strides[4] != 1:
         raise ValueError("the 8-bit cache must be [pages, 2, page_size, Hkv, D], contiguous per head")
-    pages, _, page_size, heads, _ = layer_cache.shape
+    pages, _, page_size, heads, d = shape
     if page_size < INT8_BLOCK or page_size & (page_size - 1):
         raise TypeError(f"the 8-bit cache needs a page size that is a power of two of at least {INT8_BLOCK}")
     if layer_scales.shape != (pages, 2, page_size // INT8_BLOCK, heads):
         raise ValueError("the scales must be [pages, 2, page_size // 16, Hkv]")
-    return (layer_cache.data_ptr(), *layer_cache.stride()[:4], layer_scales.data_ptr(), *layer_scales.stride(),
-            pages, page_size)
+    return heads, d, (layer_cache.data_ptr(), *strides[:4], layer_scales.data_ptr(), *layer_scales.stride(), pages,
+                      page_size)
 
 
 def _int8_slots(pages: torch.Tensor, offsets: torch.Tensor) -> int:
-    if pages.dtype != torch.long or offsets.dtype != torch.long:
+    if pages.dtype is not torch.long or offsets.dtype is not torch.long:
         raise TypeError("cache slots must be int64")
-    if pages.ndim != 1 or pages.shape != offsets.shape or not pages.is_contiguous() or not offsets.is_contiguous():
+    shape = pages.shape
+    if len(shape) != 1 or offsets.shape != shape or not pages.is_contiguous() or not offsets.is_contiguous():
         raise ValueError("cache slots must be contiguous vectors with one entry per token")
-    return pages.shape[0]
+    return shape[0]
 
 
-def _int8_heads(key: torch.Tensor, value: torch.Tensor, tokens: int, layer_cache: torch.Tensor) -> None:
-    _require_bf16(key, value)
-    if key.shape != (tokens, *layer_cache.shape[3:]) or value.shape != key.shape:
-        raise ValueError("key and value must be [tokens, Hkv, D] with the cache's heads")
-    if key.stride(2) != 1 or value.stride(2) != 1:
-        raise ValueError("key and value must be contiguous per head")
+def _int8_heads(t: torch.Tensor, shape: tuple) -> tuple:
+    """Pointer, token and head stride of key or value."""
+
+    if t.dtype is not torch.bfloat16:
+        raise TypeError("HIP attention kernels take bf16 tensors")
+    strides = t.stride()
+    if t.shape != shape or strides[2] != 1:
+        raise ValueError("key and value must be [tokens, Hkv, D] with the cache's heads, contiguous per head")
+    return t.data_ptr(), strides[0], strides[1]
 
 
 def _int8_status(status: torch.Tensor | None) -> int | None:
-    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+    if status is None:
+        return None
+    if status.dtype is not torch.int32 or status.numel() < 1:
         raise TypeError("status must be an int32 tensor")
-    return _lib.ptr(status)
+    return status.data_ptr()
 
 
 def paged_cache_write_int8_(key: torch.Tensor, value: torch.Tensor, layer_cache: torch.Tensor,
@@ -397,14 +405,13 @@ def paged_cache_write_int8_(key: torch.Tensor, value: torch.Tensor, layer_cache:
     one call leave that block unspecified.  A NaN or infinity makes its block's scale NaN.  A slot outside the pool is skipped and
     ``status`` (int32, optional) set to NQ_ERR_INVALID_ARGUMENT.  No counterpart in the reference."""
 
-    cache = _int8_cache(layer_cache, layer_scales)
+    heads, d, cache = _int8_cache(layer_cache, layer_scales)
     tokens = _int8_slots(write_pages, write_offsets)
-    _int8_heads(key, value, tokens, layer_cache)
-    _lib.require_one_device(key, value, layer_cache, layer_scales, write_pages, write_offsets, status)
-    _lib.call_on(
-        key.device, "nq_kv_int8_write", key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(),
-        value.stride(0), value.stride(1), tokens, layer_cache.shape[3], layer_cache.shape[4], *cache,
-        write_pages.data_ptr(), write_offsets.data_ptr(), _int8_status(status), _lib.stream(key.device),
+    shape = (tokens, heads, d)
+    source = _int8_heads(key, shape) + _int8_heads(value, shape)
+    _lib.launch(
+        _lib.one_device(key, value, layer_cache, layer_scales, write_pages, write_offsets, status), "nq_kv_int8_write",
+        *source, tokens, heads, d, *cache, write_pages.data_ptr(), write_offsets.data_ptr(), _int8_status(status),
     )
 
 
@@ -415,17 +422,15 @@ def paged_cache_read_int8(layer_cache: torch.Tensor, layer_scales: torch.Tensor,
     request to a bf16 pool, or off the device): code * scale, which bf16 holds exactly for the scales that
     ``paged_cache_write_int8_`` makes.  A slot outside the pool gives zeros and sets ``status``."""
 
-    cache = _int8_cache(layer_cache, layer_scales)
+    heads, d, cache = _int8_cache(layer_cache, layer_scales)
     tokens = _int8_slots(pages, offsets)
-    shape = (tokens, *layer_cache.shape[3:])
+    shape = (tokens, heads, d)
     key = torch.empty(shape, dtype=torch.bfloat16, device=layer_cache.device) if key is None else key
     value = torch.empty(shape, dtype=torch.bfloat16, device=layer_cache.device) if value is None else value
-    _int8_heads(key, value, tokens, layer_cache)
-    _lib.require_one_device(layer_cache, layer_scales, pages, offsets, key, value, status)
-    _lib.call_on(
-        key.device, "nq_kv_int8_read", *cache, pages.data_ptr(), offsets.data_ptr(), tokens, layer_cache.shape[3],
-        layer_cache.shape[4], key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
-        value.stride(1), _int8_status(status), _lib.stream(key.device),
+    target = _int8_heads(key, shape) + _int8_heads(value, shape)
+    _lib.launch(
+        _lib.one_device(layer_cache, layer_scales, pages, offsets, key, value, status), "nq_kv_int8_read", *cache,
+        pages.data_ptr(), offsets.data_ptr(), tokens, heads, d, *target, _int8_status(status),
     )
     return key, value
 
@@ -455,24 +460,27 @@ def paged_attention_int8(query: torch.Tensor, layer_cache: torch.Tensor, layer_s
     ``workspace`` (``paged_attention_int8_workspace_bytes``; allocated if None) belongs to one call at a
     time.  The same inputs give the same bits.  No counterpart in the reference."""
 
-    cache = _int8_cache(layer_cache, layer_scales)
-    if query.ndim != 3 or query.stride(2) != 1:
+    hkv, d, cache = _int8_cache(layer_cache, layer_scales)
+    shape, strides = query.shape, query.stride()
+    if len(shape) != 3 or strides[2] != 1:
         raise ValueError("query must be [tokens, Hq, D], contiguous per head")
-    tokens, hq, d = query.shape
-    hkv = layer_cache.shape[3]
-    if layer_cache.shape[4] != d or hq < hkv or hq % hkv:
+    tokens, hq, q_dim = shape
+    if q_dim != d or hq < hkv or hq % hkv:
         raise ValueError("query and cache disagree on the heads")
     out = torch.empty_like(query, memory_format=torch.contiguous_format) if out is None else out
-    _require_bf16(query, out)
-    if out.shape != query.shape or out.stride(2) != 1:
+    if query.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16:
+        raise TypeError("HIP attention kernels take bf16 tensors")
+    o_strides = out.stride()
+    if out.shape != shape or o_strides[2] != 1:
         raise ValueError("out must be [tokens, Hq, D] like the query")
     qo, kv, ids, last = (metadata.qo_indptr, metadata.paged_kv_indptr, metadata.paged_kv_indices,
                          metadata.paged_kv_last_page_len)
     for t in (qo, kv, ids, last):
-        if t is not None and t.dtype != torch.int32:
-            raise TypeError("paged metadata must be int32")
-        if t is not None and (t.ndim != 1 or not t.is_contiguous()):
-            raise ValueError("paged metadata must be contiguous vectors")
+        if t is not None:
+            if t.dtype is not torch.int32:
+                raise TypeError("paged metadata must be int32")
+            if t.ndim != 1 or not t.is_contiguous():
+                raise ValueError("paged metadata must be contiguous vectors")
     rows = kv.shape[0] - 1
     if rows < 0 or last.shape[0] < rows or (qo is not None and qo.shape[0] != rows + 1):
         raise ValueError("paged metadata must describe one set of rows")
@@ -480,20 +488,21 @@ def paged_attention_int8(query: torch.Tensor, layer_cache: torch.Tensor, layer_s
         parts = _lib.NQ_ATTN_DECODE if qo is None else _lib.NQ_ATTN_DECODE | _lib.NQ_ATTN_PREFILL
     if qo is None and (parts != _lib.NQ_ATTN_DECODE or rows > tokens):
         raise ValueError("without qo_indptr every row has one query and only NQ_ATTN_DECODE runs")
-    _lib.require_one_device(query, layer_cache, layer_scales, out, qo, kv, ids, last, status, workspace)
+    index = _lib.one_device(query, layer_cache, layer_scales, out, qo, kv, ids, last, status, workspace)
     if tokens == 0 or rows == 0:
         return out
     need = paged_attention_int8_workspace_bytes(tokens, rows, hq, hkv, d, parts)
     if workspace is None:
-        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=query.device)
-    elif workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
-        raise ValueError(f"8-bit paged attention needs a contiguous workspace of {need} bytes")
-    _lib.call_on(
-        query.device, "nq_paged_attention_int8", _lib.ptr(qo), kv.data_ptr(), last.data_ptr(), ids.data_ptr(), rows,
-        ids.shape[0], query.data_ptr(), query.stride(0), query.stride(1), tokens, *cache, hq, hkv, d,
-        float(d) ** -0.5 if sm_scale is None else float(sm_scale), out.data_ptr(), out.stride(0), out.stride(1),
-        int(parts), workspace.data_ptr(), workspace.numel() * workspace.element_size(), _int8_status(status),
-        _lib.stream(query.device),
+        workspace, size = torch.empty(need, dtype=torch.uint8, device=query.device), need
+    else:
+        size = workspace.numel() * workspace.element_size()
+        if size < need or not workspace.is_contiguous():
+            raise ValueError(f"8-bit paged attention needs a contiguous workspace of {need} bytes")
+    _lib.launch(
+        index, "nq_paged_attention_int8", None if qo is None else qo.data_ptr(), kv.data_ptr(), last.data_ptr(),
+        ids.data_ptr(), rows, ids.shape[0], query.data_ptr(), strides[0], strides[1], tokens, *cache, hq, hkv, d,
+        float(d) ** -0.5 if sm_scale is None else float(sm_scale), out.data_ptr(), o_strides[0], o_strides[1],
+        int(parts), workspace.data_ptr(), size, _int8_status(status),
     )
     return out
 

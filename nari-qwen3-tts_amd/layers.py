@@ -753,22 +753,23 @@ def quantize_int8_rows(x: torch.Tensor, q: torch.Tensor | None = None,
     token, or a weight [out, in] per output channel.  K a multiple of 16; a row of zeros has scale 1, one with a
     NaN or an infinity a NaN scale (its products are NaN)."""
 
-    if x.dtype != torch.bfloat16:
+    if x.dtype is not torch.bfloat16:
         raise TypeError("row quantization needs bf16 [rows, K]")
-    if x.dim() != 2 or x.stride(1) != 1:
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 2 or strides[1] != 1:
         raise ValueError("row quantization needs [rows, K] with unit inner stride")
-    rows, k = x.shape
+    rows, k = shape
     if k < 16 or k % 16:
         raise ValueError("int8 row quantization needs a multiple of 16 columns")
-    q = torch.empty((rows, k), dtype=torch.int8, device=x.device) if q is None else q
+    q = torch.empty(shape, dtype=torch.int8, device=x.device) if q is None else q
     scales = torch.empty(rows, dtype=torch.float32, device=x.device) if scales is None else scales
-    if q.dtype != torch.int8 or scales.dtype != torch.float32:
+    if q.dtype is not torch.int8 or scales.dtype is not torch.float32:
         raise TypeError("int8 codes and float32 scales expected")
-    if q.shape != x.shape or q.stride(1) != 1 or scales.shape != (rows,) or not scales.is_contiguous():
+    q_strides = q.stride()
+    if q.shape != shape or q_strides[1] != 1 or scales.shape != (rows,) or not scales.is_contiguous():
         raise ValueError(f"codes must be [{rows}, {k}] with unit inner stride and scales [{rows}], contiguous")
-    _lib.require_one_device(x, q, scales)
-    _lib.call_on(x.device, "nq_quantize_int8_rows", x.data_ptr(), x.stride(0), rows, k, q.data_ptr(), q.stride(0),
-                 scales.data_ptr(), _lib.stream(x.device))
+    _lib.launch(_lib.one_device(x, q, scales), "nq_quantize_int8_rows", x.data_ptr(), strides[0], rows, k,
+                q.data_ptr(), q_strides[0], scales.data_ptr())
     return q, scales
 
 
@@ -778,25 +779,26 @@ def linear_int8(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, w
     [out, in] with the scales of ``quantize_int8_rows``; the sum is exact (int32), so the same codes give the
     same bits at any number of rows.  ``in`` a multiple of 16 up to 131072, any rows and out."""
 
-    if q.dtype != torch.int8 or weight_q.dtype != torch.int8:
+    if q.dtype is not torch.int8 or weight_q.dtype is not torch.int8:
         raise TypeError("the int8 projection needs int8 codes")
-    if scales.dtype != torch.float32 or weight_scales.dtype != torch.float32:
+    if scales.dtype is not torch.float32 or weight_scales.dtype is not torch.float32:
         raise TypeError("int8 scales must be float32")
-    if q.dim() != 2 or weight_q.dim() != 2 or q.stride(1) != 1 or weight_q.stride(1) != 1:
+    q_strides, w_strides, w_shape = q.stride(), weight_q.stride(), weight_q.shape
+    if len(q_strides) != 2 or len(w_shape) != 2 or q_strides[1] != 1 or w_strides[1] != 1:
         raise ValueError("int8 codes must be matrices with unit inner stride")
-    (rows, k), n = q.shape, weight_q.shape[0]
-    if weight_q.shape[1] != k or k < 16 or k % 16:
+    (rows, k), n = q.shape, w_shape[0]
+    if w_shape[1] != k or k < 16 or k % 16:
         raise ValueError("int8 codes must share an inner size that is a multiple of 16")
     if scales.shape != (rows,) or weight_scales.shape != (n,) or not (
             scales.is_contiguous() and weight_scales.is_contiguous()):
         raise ValueError("int8 scales must be contiguous, one per row and one per output")
     out = torch.empty((rows, n), dtype=torch.bfloat16, device=q.device) if out is None else out
-    if out.dtype != torch.bfloat16 or out.shape != (rows, n) or out.stride(1) != 1:
+    o_strides = out.stride()
+    if out.dtype is not torch.bfloat16 or out.shape != (rows, n) or o_strides[1] != 1:
         raise ValueError(f"out must be bf16 [{rows}, {n}] with unit inner stride")
-    _lib.require_one_device(q, scales, weight_q, weight_scales, out)
-    _lib.call_on(q.device, "nq_linear_int8", q.data_ptr(), q.stride(0), scales.data_ptr(), weight_q.data_ptr(),
-                 weight_q.stride(0), weight_scales.data_ptr(), rows, n, k, out.data_ptr(), out.stride(0),
-                 _lib.stream(q.device))
+    _lib.launch(_lib.one_device(q, scales, weight_q, weight_scales, out), "nq_linear_int8", q.data_ptr(),
+                q_strides[0], scales.data_ptr(), weight_q.data_ptr(), w_strides[0], weight_scales.data_ptr(), rows, n,
+                k, out.data_ptr(), o_strides[0])
     return out
 
 
