@@ -13,25 +13,28 @@
 // scale applied to its 16 columns of fp32 scores; P times the V scale of its
 // block rounded to bf16, the codes of V widened, fp32 sums.  So the cache moves half
 // the bytes of a bf16 one and is never written out wider.
+#include <stddef.h>
+
+#include <type_traits>
+
 #include "nq_common.h"
 #include "nq_internal.h"
 
 namespace nq {
 namespace {
 
-#ifndef NQ_DEC_OCC
-#define NQ_DEC_OCC 4
-#endif
 constexpr int kBlk = 16;  // slots that share a scale
 constexpr int kKv8Threads = 256;
 constexpr int kKv8Waves = kKv8Threads / kWave;
 constexpr float kMinScale = 1.1754943508222875e-38f;  // 2^-126
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef float floatx4_t __attribute__((ext_vector_type(4)));
 typedef float floatx16_t __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));  // plain vectors stay in registers
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 struct Pool8 {
     int8_t *codes;
@@ -60,6 +63,8 @@ __device__ __forceinline__ float byte_f32(uint32_t w) {
     return static_cast<float>(static_cast<int8_t>(w >> (8 * B)));
 }
 
+__device__ __forceinline__ float byte_of(uint32_t w, int j) { return static_cast<float>(static_cast<int8_t>(w >> (8 * j))); }
+
 // Eight codes widened to bf16: integers of at most 8 bits, so the upper half of the float is exact.
 __device__ __forceinline__ uint32_t pair_bf16(float lo, float hi) {
     return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
@@ -69,12 +74,6 @@ __device__ __forceinline__ bf16x8_t widen8(uint32_t a, uint32_t b) {
                      pair_bf16(byte_f32<0>(b), byte_f32<1>(b)), pair_bf16(byte_f32<2>(b), byte_f32<3>(b))};
     return __builtin_bit_cast(bf16x8_t, r);
 }
-// The same times a scale: exact for a power of two.
-__device__ __forceinline__ u32x4 scale8(uint32_t a, uint32_t b, float s) {
-    return u32x4{pack2_bf16(byte_f32<0>(a) * s, byte_f32<1>(a) * s), pack2_bf16(byte_f32<2>(a) * s, byte_f32<3>(a) * s),
-                 pack2_bf16(byte_f32<0>(b) * s, byte_f32<1>(b) * s), pack2_bf16(byte_f32<2>(b) * s, byte_f32<3>(b) * s)};
-}
-
 // ---------------------------------------------------------------------------------------------
 // Write: a wave takes the leaders among `group` consecutive tokens for one (kind, head).  A leader is a
 // token that does not continue its predecessor's block (same page, next slot, same block of 16); its run
@@ -219,10 +218,25 @@ struct Attend8 {
     const int32_t *qo_indptr, *kv_indptr, *kv_indices, *last_page_len;
     int rows, tokens, n_indices, group, heads;  // group: query heads per kv head
     int bpp_log2;                               // blocks of 16 per page
-    float scale;                                // |sm_scale| log2(e)
+    float scale;                                // |sm_scale| log2(e), above 0
     uint32_t flip;                              // sign bits of a bf16 pair where sm_scale is negative
     int32_t *status;
 };
+
+// The larger (the sum) of a lane's value and that of the lane 32 on or back.
+__device__ __forceinline__ float halves_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// The same over lanes 16, 32 and 48 on.
+__device__ __forceinline__ float quarters_max(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return halves_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
 
 // Largest r in [0, n) with f(r) <= x for a non-decreasing f with f(0) <= x, found by the whole wave: 64
 // probes at once, so one round of loads up to 64 rows and two up to 4096.
@@ -244,7 +258,7 @@ __device__ __forceinline__ int wave_find_le(int n, int x, F f) {
 
 // The ragged metadata, copied to LDS at entry (one round trip, then searches and row changes cost LDS reads);
 // read in place beyond kMetaRows rows.
-constexpr int kMetaRows = 1024;
+constexpr int kMetaRows = 512;
 struct Meta8 {
     int32_t kv[kMetaRows + 1], qo[kMetaRows + 1], last[kMetaRows];
 };
@@ -332,10 +346,10 @@ __device__ __forceinline__ int span_of(const Spans &s, int64_t b) {
 // (D/4)(l / 16) .. of K, and holds the scores of query slot l % 16 against tokens 4 (l / 16) + i.  Those are, in
 // that order, the 8 keys of the lane's group in out^T = V^T P^T, so P needs no exchange between lanes; V is loaded
 // as (D/16) values of each of the 8 tokens, and the byte a conversion picks does the transposition.
-// K of the next step is asked for as soon as this one's is multiplied, V likewise: one set of registers, so that
-// four waves a SIMD are resident, and loads always in flight.
+// K of the next step is asked for as soon as this one's is multiplied, V likewise: one set of registers, and loads always
+// in flight.
 template <int D>
-__global__ void __launch_bounds__(kKv8Threads, NQ_DEC_OCC)
+__global__ void __launch_bounds__(kKv8Threads, 2)
 kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml, float *__restrict__ part_o) {
     constexpr int W = D / 64;  // 16-byte loads of K, dwords of V
     __shared__ Meta8 meta;
@@ -490,8 +504,7 @@ kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml
             for (int i = 0; i < 8; ++i)
                 p[i] = 4 * grp + (i & 3) < nv[i / 4] ? p[i] * f[i / 4] : -__builtin_inff();
             float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
-            top = fmaxf(top, __shfl_xor(top, 16, kWave));
-            top = fmaxf(top, __shfl_xor(top, 32, kWave));
+            top = quarters_max(top);
             const float m_new = fmaxf(m_run, top);
             if (__any(m_new != m_run)) {
                 const float alpha = m_run == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
@@ -678,16 +691,19 @@ __device__ __forceinline__ int pieces_of(const Tile8 &t, int splits) {
 
 template <int D>
 struct Smem8 {
-    u32x4 k[2][kKeys * (D / 8)];
+    u32x4 k[2][kKeys * (D / 8 + 1)];
     u32x4 v[2][D * (kKeys / 8)];
-    int absent[2][kKeys / kBlk];  // the block's page is not in the pool
+    floatx4_t ks[2];               // K scales of the tile's blocks, 1 where one is not finite
+    i32x4_t odd[2];                // kAbsent: the block's page is not in the pool; kPoison: a scale is not finite
     Meta8 meta;
 };
-// 16-byte chunk positions, exclusive-ored so that eight neighbouring rows, and the writes of a stage, spread over
-// all banks.
+constexpr int kAbsent = 1, kPoison = 2;
+// Places of 16-byte chunks: rows of K one chunk longer than their values, V's chunks exclusive-ored with their row.
+// Measured free of conflicts for the operand reads (32 rows, two chunks each) and K's writes; V's 8-byte writes take half as
+// long again as without any.
 template <int D>
 __device__ __forceinline__ int k_chunk(int key, int chunk) {
-    return key * (D / 8) + (chunk ^ (key & 7));
+    return key * (D / 8 + 1) + chunk;
 }
 __device__ __forceinline__ int v_chunk(int d, int chunk) { return d * (kKeys / 8) + (chunk ^ ((d ^ (d >> 3)) & 7)); }
 
@@ -696,10 +712,10 @@ __global__ void __launch_bounds__(NW * kWave, 2)
 kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single, float2 *__restrict__ part_ml,
                    float *__restrict__ part_o) {
     constexpr int T = NW * kWave, COLS = 32 * NW;
-    // K: a thread stages KL 16-byte pieces of one key; V: VB values of each of four keys
-    constexpr int KL = kKeys * D / 16 / T, KT = T / kKeys;  // KT threads a key
-    constexpr int VB = kKeys * D / 4 / T;                   // 4, 8 (or 2) bytes
-    static_assert(KL * T * 16 == kKeys * D || KL == 0, "K stages evenly");
+    // K: a thread stages KP pieces of eight values of one key; V: VB values of each of four keys
+    constexpr int KT = T / kKeys, KP = D / 8 / KT;  // KT threads a key
+    constexpr int VB = kKeys * D / 4 / T;           // 2, 4 or 8
+    static_assert(KP >= 1 && KP * KT * 8 == D && VB >= 2 && VB <= 8, "a tile stages evenly");
     __shared__ Smem8<D> sm;
     load_meta(a, sm.meta);
     const Rows8 rows{a, sm.meta};
@@ -715,96 +731,96 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
     const int n_kt = (t.n_keys + kKeys - 1) / kKeys;
     const int kt0 = n_kt * piece / pieces, kt1 = n_kt * (piece + 1) / pieces;
 
+    constexpr int kBufK = 16 * kKeys * (D / 8 + 1), kBufV = 16 * D * (kKeys / 8);
     // staging: a wave holds 64 / NW keys of one block, so its page, its scales and their addresses are uniform
-    constexpr int KB = KL > 0 ? 16 : 8;  // bytes of a K load
     const int sk_key = threadIdx.x / KT, sk_piece = threadIdx.x % KT;
     constexpr int VT = T / (kKeys / 4);  // threads of a quad of keys
     const int sv_quad = threadIdx.x / VT, sv_part = threadIdx.x % VT;
     const int uwave = __builtin_amdgcn_readfirstlane(wave);
     const int c_slot = static_cast<int>(pool.c_slot);
-    const int k_off = sk_key % kBlk * c_slot + KB * sk_piece;
-    const int v_off = 4 * (sv_quad % 4) * c_slot + VB * sv_part;
+    const int k_off = sk_key % kBlk * c_slot + 8 * sk_piece;
+    const int quad = sv_quad & 3;
+    const int v_off = 4 * quad * c_slot + VB * sv_part;
     const int8_t *base = pool.codes + head * pool.c_head;
     const float *s_base = pool.scales + head * pool.s_head;
-    u32x4 kr[KL > 0 ? KL : 1];
-    u32x2 vr[4];
-    float r_ks = 0.f, r_vs = 0.f;
-    bool r_on = true;
     const int n_blocks = (row.kv_len + kBlk - 1) / kBlk;
     const int in_page = (1 << a.bpp_log2) - 1;
-    auto block_of = [&](int kt) __attribute__((always_inline)) {  // beyond the row's keys, which are masked: the last
+    // Pages and scales are uniform, but fetched as vectors: a scalar load outstanding would make every wait for an LDS
+    // read in the loop a wait for that load too.
+    int zero = 0;
+    asm volatile("" : "+v"(zero));
+    // the wave's block of tile kt, held to the row's: what lies beyond its keys is masked, a tile beyond the last never used
+    auto block_of = [&](int kt) __attribute__((always_inline)) {
         const int blk = kt * (kKeys / kBlk) + uwave * (kKeys / kBlk) / NW;
         return blk < n_blocks ? blk : n_blocks - 1;
     };
     auto page_of = [&](int kt) __attribute__((always_inline)) {
-        return a.kv_indices[row.first_page + (block_of(kt) >> a.bpp_log2)];
+        return a.kv_indices[row.first_page + (block_of(kt) >> a.bpp_log2) + zero];
     };
-    int page = 0;  // of the next load
-    auto load = [&](int kt) __attribute__((always_inline)) {
-        r_on = page >= 0 && page < pool.num_pages;
-        if (!r_on && a.status) *a.status = NQ_ERR_INVALID_ARGUMENT;
-        const int64_t pid = r_on ? page : 0;
+    // The staging registers: K of one tile and V of the tile before it, with what their block needs.
+    struct Stage {
+        u32x2 k[KP], v[4];
+        float ks, vs, v_vs;  // scales of K's block, V scale of V's
+        bool on;             // K's page is in the pool
+    };
+    const int8_t *v_from = base;  // V of the tile whose K was asked for last
+    auto load = [&](int kt, int found, bool with_v, float v_vs, Stage &r) __attribute__((always_inline)) {
+        if (with_v) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int8_t *p = v_from + (v_off + e * c_slot);
+                if constexpr (VB == 8) r.v[e] = *reinterpret_cast<const u32x2 *>(p);
+                else if constexpr (VB == 4) r.v[e].x = *reinterpret_cast<const uint32_t *>(p);
+                else r.v[e].x = *reinterpret_cast<const uint16_t *>(p);
+            }
+            r.v_vs = v_vs;
+        }
+        const int page = __builtin_amdgcn_readfirstlane(found);
+        r.on = page >= 0 && page < pool.num_pages;
+        const int64_t pid = r.on ? page : 0;
         const int blk = block_of(kt) & in_page;
         const int8_t *kp = base + pid * pool.c_page + blk * (kBlk * pool.c_slot);
-        const int8_t *vp = kp + pool.c_kind;
-        if constexpr (KL > 0) {
 #pragma unroll
-            for (int w = 0; w < KL; ++w) kr[w] = *reinterpret_cast<const u32x4 *>(kp + (k_off + 16 * KT * w));
-        } else {
-            const u32x2 half = *reinterpret_cast<const u32x2 *>(kp + k_off);
-            kr[0] = u32x4{half.x, half.y, 0, 0};
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int8_t *p = vp + (v_off + e * c_slot);
-            if constexpr (VB == 8) vr[e] = *reinterpret_cast<const u32x2 *>(p);
-            else if constexpr (VB == 4) vr[e].x = *reinterpret_cast<const uint32_t *>(p);
-            else vr[e].x = *reinterpret_cast<const uint16_t *>(p);
-        }
+        for (int e = 0; e < KP; ++e) r.k[e] = *reinterpret_cast<const u32x2 *>(kp + (k_off + 8 * KT * e));
         const float *sc = s_base + pid * pool.s_page + blk * pool.s_block;
-        r_ks = sc[0];
-        r_vs = sc[pool.s_kind];
-        if (kt + 1 < kt1) page = page_of(kt + 1);
+        r.ks = sc[zero];
+        r.vs = (sc + pool.s_kind)[zero];
+        v_from = kp + pool.c_kind;
     };
-    auto store = [&](int buf) __attribute__((always_inline)) {
-        // A V scale that is not finite answers through the scores of the queries that see the block, not through
-        // 0 * NaN in those that do not.
-        const bool fine = fabsf(r_vs) < __builtin_inff();
-        const float ks = fine ? r_ks : __builtin_nanf(""), vs = fine ? r_vs : 0.f;
-        if constexpr (KL > 0) {
+    // First places of what a thread stages.  Key 8 a + 4 b + i of a block sits at position 8 b + 4 a + i of V's rows.
+    char *stage = reinterpret_cast<char *>(&sm);
+    const int put_k0 = static_cast<int>(offsetof(Smem8<D>, k)) + 16 * k_chunk<D>(sk_key, sk_piece);
+    const int put_v0 = static_cast<int>(offsetof(Smem8<D>, v)) +
+                       16 * v_chunk(sv_part * VB, 2 * (sv_quad / 4) + (quad & 1)) + 8 * (quad >> 1);
+    auto wide_k = [&](const Stage &r, int piece) __attribute__((always_inline)) {
+        return widen8(r.k[piece].x, r.k[piece].y);
+    };
+    auto wide_v = [&](const Stage &r, int col) __attribute__((always_inline)) {
+        const float vs = fabsf(r.v_vs) < __builtin_inff() ? r.v_vs : 0.f;
+        const int w = col / 4, j = col % 4;
+        return u32x2{pack2_bf16(byte_of(r.v[0][w], j) * vs, byte_of(r.v[1][w], j) * vs),
+                     pack2_bf16(byte_of(r.v[2][w], j) * vs, byte_of(r.v[3][w], j) * vs)};
+    };
+    auto put_k = [&](const Stage &r, const bf16x8_t (&x)[KP], int buf) __attribute__((always_inline)) {
 #pragma unroll
-            for (int w = 0; w < KL; ++w) {
-                const int chunk = 2 * (KT * w + sk_piece);
-                sm.k[buf][k_chunk<D>(sk_key, chunk)] = scale8(kr[w].x, kr[w].y, ks);
-                sm.k[buf][k_chunk<D>(sk_key, chunk + 1)] = scale8(kr[w].z, kr[w].w, ks);
-            }
-        } else {
-            sm.k[buf][k_chunk<D>(sk_key, sk_piece)] = scale8(kr[0].x, kr[0].y, ks);
-        }
-        // key 8 a + 4 b + i of a block sits at position 8 b + 4 a + i
-        const int quad = sv_quad & 3, chunk = 2 * (sv_quad / 4) + (quad & 1), upper = quad >> 1;
-#define NQ_V_PUT(W, J)                                                                                     \
-    reinterpret_cast<u32x2 *>(&sm.v[buf][v_chunk(sv_part * VB + 4 * W + J, chunk)])[upper] =               \
-        u32x2{pack2_bf16(byte_f32<J>(vr[0][W]) * vs, byte_f32<J>(vr[1][W]) * vs),                          \
-              pack2_bf16(byte_f32<J>(vr[2][W]) * vs, byte_f32<J>(vr[3][W]) * vs)};
-        NQ_V_PUT(0, 0)
-        NQ_V_PUT(0, 1)
-        if constexpr (VB >= 4) {
-            NQ_V_PUT(0, 2)
-            NQ_V_PUT(0, 3)
-        }
-        if constexpr (VB == 8) {
-            NQ_V_PUT(1, 0)
-            NQ_V_PUT(1, 1)
-            NQ_V_PUT(1, 2)
-            NQ_V_PUT(1, 3)
-        }
-#undef NQ_V_PUT
-        if (threadIdx.x % (KT * kBlk) == 0) sm.absent[buf][sk_key / kBlk] = !r_on;
+        for (int e = 0; e < KP; ++e) *reinterpret_cast<bf16x8_t *>(stage + put_k0 + 16 * KT * e + buf * kBufK) = x[e];
+        // A scale that is not finite, K's or V's, answers through the scores of the queries that see the block, not
+        // through 0 * NaN in those that do not.
+        const bool fine = fabsf(r.ks) < __builtin_inff() && fabsf(r.vs) < __builtin_inff();
+        const int blk = uwave * (kKeys / kBlk) / NW;
+        sm.ks[buf][blk] = fine ? r.ks : 1.0f;
+        sm.odd[buf][blk] = !r.on ? kAbsent : fine ? 0 : kPoison;
     };
+    auto put_v = [&](const u32x2 (&x)[VB], int buf) __attribute__((always_inline)) {
+        // value VB part + col, col < VB, a power of two up to 8: its row's exclusive-or is the first's xor col
+#pragma unroll
+        for (int col = 0; col < VB; ++col)
+            *reinterpret_cast<u32x2 *>(stage + ((put_v0 + buf * kBufV) ^ (16 * col)) + 16 * (kKeys / 8) * col) = x[col];
+    };
+    int found0 = 0, found1 = 0;
     if (kt0 < kt1) {
-        page = page_of(kt0);
-        load(kt0);
+        found0 = page_of(kt0);
+        found1 = page_of(kt0 + 1);
     }
 
     const int c = lane & 31, half = lane >> 5;
@@ -817,62 +833,76 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
     for (int s = 0; s < D / 16; ++s)
         qf[s] = load_q(a.q + (t.q0 + qi) * a.q_s0 + (head * a.group + g) * a.q_s1 + 16 * s + 8 * half, live, a.flip);
 
-    // Where the lane reads: chunks 2 k + half of key row c, and of V row c.  The exclusive-or moves the low three
-    // bits only, so the other chunks, rows and buffers are these places plus constants: chunk + 8 for K; V row + 32 flips bit 2.
-    int at_k[4], at_v[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        at_k[k] = k_chunk<D>(c, 2 * k + half);
-        at_v[k] = v_chunk(c, 2 * k + half);
-    }
+    // Where the lane reads, in bytes: chunk half of K row c and of V row c.  The other operands are constants away, V's
+    // after an exclusive-or of the chunk (row c + 32 j flips its bit 2 where j is odd).
+    const char *lds = reinterpret_cast<const char *>(&sm);
+    const int at_k = static_cast<int>(offsetof(Smem8<D>, k)) + 16 * k_chunk<D>(c, half);
+    const int at_v = static_cast<int>(offsetof(Smem8<D>, v)) + 16 * v_chunk(c, half);
+    auto operand = [&](int at) __attribute__((always_inline)) {
+        return __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const u32x4 *>(lds + at));
+    };
+    auto k_at = [&](int base, int k, int sub) __attribute__((always_inline)) {
+        return base + 32 * k + 16 * k_chunk<D>(32 * sub, 0);
+    };
+    auto v_at = [&](int base, int k, int j) __attribute__((always_inline)) {
+        return (base ^ (32 * (k ^ (2 * (j & 1))))) + 16 * (kKeys / 8) * 32 * j;
+    };
     floatx16_t acc[D / 32];
 #pragma unroll
     for (int j = 0; j < D / 32; ++j)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[j][i] = 0.f;
-    float m_run = -__builtin_inff(), l_run = 0.f;
+    float m_run = -__builtin_inff(), l_run = 0.f, top = -__builtin_inff();
     bool any = false;  // whether the column has seen a key
-    if (kt0 < kt1) store(0);
-    for (int kt = kt0; kt < kt1; ++kt) {
-        const int buf = (kt - kt0) & 1;
-        __syncthreads();
-        if (kt + 1 < kt1) load(kt + 1);
-        floatx16_t s[2];
+    floatx4_t f_k = {0.f, 0.f, 0.f, 0.f};
+    Stage st;
+
+    auto scores = [&](int kt, floatx16_t (&s)[2]) __attribute__((always_inline)) {
+        const int base = at_k + (kt & 1) * kBufK;
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
+        for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[sub][i] = 0.f;
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-                s[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                    __builtin_bit_cast(bf16x8_t, sm.k[buf][at_k[k % 4] + 32 * (D / 8) * sub + 8 * (k / 4)]), qf[k],
-                    s[sub], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);  // one half's operands in registers at a time
-        }
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub)
+                s[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(k_at(base, k, sub)), qf[k], s[sub], 0, 0, 0);
+    };
+    // Keys that a column does not see, in tiles that hold any such key.
+    auto mask = [&](int kt, i32x4_t odd, floatx16_t (&s)[2]) __attribute__((always_inline)) {
         const int key0 = kt * kKeys;
-        int gone[kKeys / kBlk], none = 0;
-#pragma unroll
-        for (int k = 0; k < kKeys / kBlk; ++k) none |= gone[k] = sm.absent[buf][k];
-        const bool whole = key0 + kKeys <= t.limit0 && !__builtin_amdgcn_readfirstlane(none);
-        // lane's element i: key 32 (i / 16) + 8 (i / 4 % 4) + 4 half + i % 4
-        auto sees = [&](int i) __attribute__((always_inline)) {
-            return key0 + 32 * (i / 16) + 8 * (i / 4 % 4) + 4 * half + (i & 3) < limit && !gone[i / 8];
-        };
-        float top = -__builtin_inff();
-        if (whole) {
+        const int some = __builtin_amdgcn_readfirstlane(odd[0] | odd[1] | odd[2] | odd[3]);
+        if (key0 + kKeys <= t.limit0 && !some) {
             any = true;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i / 16][i % 16]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const bool see = sees(i);
-                any |= see;
-                top = fmaxf(top, see ? s[i / 16][i % 16] : -__builtin_inff());
-            }
+            return;
         }
-        top = fmaxf(top, __shfl_xor(top, 32, kWave));
-        top = top == -__builtin_inff() ? top : top * a.scale;
+        if ((some & kAbsent) && a.status) *a.status = NQ_ERR_INVALID_ARGUMENT;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            // the lane's element i: key 32 (i / 16) + 8 (i / 4 % 4) + 4 half + i % 4
+            const bool see = key0 + 32 * (i / 16) + 8 * (i / 4 % 4) + 4 * half + (i & 3) < limit && odd[i / 8] != kAbsent;
+            any |= see;
+            const float v = odd[i / 8] == kPoison ? __builtin_nanf("") : s[i / 16][i % 16];
+            s[i / 16][i % 16] = see ? v : -__builtin_inff();
+        }
+    };
+    // A tile's factors, scale of the block times sm_scale log2(e), and the maximum of its scores times them
+    // (scales are positive).
+    auto factors = [&](int kt) __attribute__((always_inline)) { return sm.ks[kt & 1] * a.scale; };
+    auto block_top = [&](const floatx16_t (&s)[2], int k) __attribute__((always_inline)) {
+        float m = s[k / 2][8 * (k % 2)];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = fmaxf(m, s[k / 2][8 * (k % 2) + i]);
+        return m;
+    };
+    // Tile kt: its scores are in `s` and their maximum in `top`; the next tile's go to `next`.  Two blocks of
+    // independent work each, interleaved two MFMAs at a time (the fences hold the order): the next scores beside
+    // this tile's exponentials, then P V beside the next maximum and the staging of the tiles behind, V one
+    // ahead and K two.
+    constexpr int CH = D / 16, PER = 32 / CH;  // chunks of two MFMAs, score elements beside each
+    auto step = [&](auto last, int kt, floatx16_t (&s)[2], floatx16_t (&next)[2]) __attribute__((always_inline)) {
+        __syncthreads();
         if (__any(top > m_run + kLag)) {
             const float m_new = fmaxf(m_run, top);
             const float alpha = m_run == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
@@ -881,45 +911,137 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
             for (int j = 0; j < D / 32; ++j) acc[j] *= alpha;
             m_run = m_new;
         }
+        const float m_use = m_run == -__builtin_inff() ? 0.f : m_run;  // no key yet: 2^(-inf) for all
+        i32x4_t n_odd = {0, 0, 0, 0};
+        floatx4_t n_f = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (!last) {
+            n_odd = sm.odd[(kt + 1) & 1];
+            n_f = factors(kt + 1);
+        }
+        constexpr int JP = D / 64;  // pairs of 32-value rows of V
+        int v_base = at_v + (kt & 1) * kBufV;
+        asm volatile("" : "+v"(v_base));  // places are made from it where they are used, not kept
+        bf16x8_t vf[2][2];
+        auto read_v = [&](int ch) __attribute__((always_inline)) {
+            vf[ch & 1][0] = operand(v_at(v_base, ch / JP, 2 * (ch % JP)));
+            vf[ch & 1][1] = operand(v_at(v_base, ch / JP, 2 * (ch % JP) + 1));
+        };
         uint32_t pw[16];
         float sum[2] = {0.f, 0.f};
-        if (whole) {
+        {
+            const int base = at_k + ((kt + 1) & 1) * kBufK;
+            bf16x8_t f[2][2];
+            auto read = [&](int k) __attribute__((always_inline)) {
+                f[k & 1][0] = operand(k_at(base, k, 0));
+                f[k & 1][1] = operand(k_at(base, k, 1));
+            };
+            if constexpr (!last) {
+                read(0);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16], a.scale, -m_run));
-                const float y = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16 + 1], a.scale, -m_run));
-                sum[0] += x;
-                sum[1] += y;
-                pw[i / 2] = pack2_bf16(x, y);
+                for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) next[sub][i] = 0.f;
             }
-        } else {
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-                float z[2];
+            for (int k = 0; k < CH; ++k) {
+                if constexpr (!last) {
+                    if (k + 1 < CH) read(k + 1);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    z[e] = sees(i + e) ? __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16 + e], a.scale, -m_run)) : 0.f;
-                    sum[e] += z[e];
+                    for (int sub = 0; sub < 2; ++sub)
+                        next[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[k & 1][sub], qf[k], next[sub], 0, 0, 0);
                 }
-                pw[i / 2] = pack2_bf16(z[0], z[1]);
+#pragma unroll
+                for (int i = PER * k; i < PER * (k + 1); i += 2) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16], f_k[i / 8], -m_use));
+                    const float y = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16 + 1], f_k[i / 8], -m_use));
+                    pw[i / 2] = pack2_bf16(x, y);
+                    float &l = sum[i / 2 % 2];  // of the rounded values, those that meet V
+                    l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pw[i / 2]),
+                                                        __builtin_bit_cast(bf16x2_t, 0x3f803f80u), l, false);
+                    asm volatile("" : "+v"(pw[i / 2]), "+v"(l));  // made here, not where they are used
+                }
+                if (k == CH - 1) read_v(0);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         l_run += sum[0] + sum[1];
-        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!last) {
+            mask(kt + 1, n_odd, next);
+            f_k = n_f;
+        }
+        float high = -__builtin_inff();
+        u32x2 xv[VB];
+        bf16x8_t xk[KP];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int ch = 0; ch < CH; ++ch) {
+            const int k = ch / JP, j = 2 * (ch % JP);
+            if (ch + 1 < CH) read_v(ch + 1);
             const bf16x8_t pf =
                 __builtin_bit_cast(bf16x8_t, u32x4{pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]});
 #pragma unroll
-            for (int j = 0; j < D / 32; ++j)
-                acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                    __builtin_bit_cast(bf16x8_t, sm.v[buf][at_v[k ^ (2 * (j & 1))] + 32 * (kKeys / 8) * j]), pf, acc[j],
-                    0, 0, 0);
-            if (k & 1) __builtin_amdgcn_sched_barrier(0);
+            for (int h = 0; h < 2; ++h)
+                acc[j + h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ch & 1][h], pf, acc[j + h], 0, 0, 0);
+            if constexpr (!last) {
+                if (ch % (CH / 4) == 0) high = fmaxf(high, block_top(next, ch / (CH / 4)) * f_k[ch / (CH / 4)]);
+                constexpr int HALF = CH / 2;  // V of tile kt + 1 first, then K of kt + 2 (or of a tile that is never used)
+                if (ch < HALF) {
+#pragma unroll
+                    for (int e = VB * ch / HALF; e < VB * (ch + 1) / HALF; ++e) xv[e] = wide_v(st, e);
+                } else {
+#pragma unroll
+                    for (int e = KP * (ch - HALF) / HALF; e < KP * (ch - HALF + 1) / HALF; ++e) xk[e] = wide_k(st, e);
+                }
+                if (ch == CH - 1) {  // writes behind the last reads; then the registers are free for the tiles behind
+                    put_v(xv, (kt + 1) & 1);
+                    put_k(st, xk, kt & 1);
+                    load(kt + 3, found0, true, st.vs, st);
+                    found0 = page_of(kt + 4);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (kt + 1 < kt1) store(buf ^ 1);
+        if constexpr (!last) top = halves_max(high);
+    };
+    floatx16_t s0[2], s1[2];
+    if (kt0 < kt1) {
+        Stage first;
+        load(kt0, found0, false, 0.f, first);
+        load(kt0 + 1, found1, true, first.vs, st);
+        found1 = page_of(kt0 + 2);
+        found0 = page_of(kt0 + 3);
+        bf16x8_t xk[KP];
+#pragma unroll
+        for (int e = 0; e < KP; ++e) xk[e] = wide_k(first, e);
+        put_k(first, xk, kt0 & 1);
+#pragma unroll
+        for (int e = 0; e < KP; ++e) xk[e] = wide_k(st, e);
+        put_k(st, xk, (kt0 + 1) & 1);
+        u32x2 xv[VB];
+#pragma unroll
+        for (int e = 0; e < VB; ++e) xv[e] = wide_v(st, e);
+        put_v(xv, kt0 & 1);
+        load(kt0 + 2, found1, true, st.vs, st);
+        __syncthreads();
+        scores(kt0, s0);
+        mask(kt0, sm.odd[kt0 & 1], s0);
+        f_k = factors(kt0);
+        top = -__builtin_inff();
+#pragma unroll
+        for (int k = 0; k < kKeys / kBlk; ++k) top = fmaxf(top, block_top(s0, k) * f_k[k]);
+        top = halves_max(top);
+        int kt = kt0;
+        for (; kt + 2 < kt1; kt += 2) {
+            step(std::false_type{}, kt, s0, s1);
+            step(std::false_type{}, kt + 1, s1, s0);
+        }
+        if (kt + 1 < kt1) {
+            step(std::false_type{}, kt, s0, s1);
+            step(std::true_type{}, kt + 1, s1, s0);
+        } else {
+            step(std::true_type{}, kt, s0, s1);
+        }
     }
-    l_run += __shfl_xor(l_run, 32, kWave);
+    l_run = halves_sum(l_run);
     any = any | static_cast<bool>(__shfl_xor(static_cast<int>(any), 32, kWave));
     if (!live) return;
     // the lane holds out[col][32 j + 8 (i / 4) + 4 half + i % 4] in acc[j][i]
@@ -1008,22 +1130,14 @@ struct Prefill8 {
     int waves, cols, slots, splits;
 };
 // Eight waves (a CU holds one such workgroup) where the rows fill their 256 columns on average, else four (two a CU).
-// Pieces: the fewest that keep 85 % of the CUs in work, or come nearest to it.
+// Pieces: as many as fit the CUs at once, up to kMaxPieces.
 Prefill8 prefill_plan(int tokens, int rows, int group, int heads) {
     Prefill8 p;
     p.waves = static_cast<int64_t>(tokens) * group >= 256ll * rows ? 8 : 4;
     p.cols = 32 * p.waves;
     p.slots = tokens / (p.cols / group) + rows;
     const int64_t wgs = static_cast<int64_t>(p.slots) * heads, room = p.waves == 8 ? 256 : 512;
-    double best = 0.0;
-    p.splits = 1;
-    for (int s = 1; s <= kMaxPieces && best < 0.85; ++s) {
-        const double use = static_cast<double>(wgs * s) / static_cast<double>((wgs * s + room - 1) / room * room);
-        if (use > best * 1.05) {
-            best = use;
-            p.splits = s;
-        }
-    }
+    p.splits = wgs >= room ? 1 : static_cast<int>(room / wgs < kMaxPieces ? room / wgs : kMaxPieces);
     return p;
 }
 struct Layout8 {
@@ -1205,7 +1319,7 @@ extern "C" int nq_paged_attention_int8(const int32_t *qo_indptr, const int32_t *
     const Attend8 a = {q,     q_s0,        q_s1,   out,         o_s0,
                        o_s1,  qo_indptr,   kv_indptr, kv_indices,  last_page_len,
                        n_rows, tokens,     num_indices, num_qo_heads / num_kv_heads, num_kv_heads,
-                       bpp,   fabsf(sm_scale) * kLog2e8, sm_scale < 0.f ? 0x80008000u : 0u, status};
+                       bpp,   fmaxf(fabsf(sm_scale) * kLog2e8, kMinScale), sm_scale < 0.f ? 0x80008000u : 0u, status};
     char *ws = static_cast<char *>(workspace);
     const Layout8 L = layout8(tokens, n_rows, num_qo_heads, num_kv_heads, head_dim, parts);
     hipStream_t st = static_cast<hipStream_t>(stream);
