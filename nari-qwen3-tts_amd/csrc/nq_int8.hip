@@ -5,12 +5,11 @@
 // in fp32 for a bf16 x and the quotient correctly rounded, and a quotient that is
 // no tie lies at least 1 / 512 from one, so the codes are those of exact arithmetic.
 //
-// Few rows: a workgroup owns 16 output channels and all of K, its waves
-// interleave K in pieces of 128 and add their int32 sums through LDS; weights and
-// rows go straight from memory into mfma_i32_16x16x64_i8 operands.  Integer sums are exact in
-// any order, so cutting K costs no determinism.
+// Few rows: a workgroup owns 16 output channels and all of K, its waves interleave K in
+// pieces of 128 bytes, each through LDS of its own, and add their int32 sums at the end.
+// Integer sums are exact in any order, so cutting K costs no determinism.
 // Many rows: (32 TM WM) x (32 TN WN) tiles of mfma_i32_32x32x32_i8, K staged 128 bytes at a
-// time through LDS, double buffered, the next stages' loads in flight.
+// time through three LDS buffers, the next two stages' loads in flight.
 #include "nq_common.h"
 #include "nq_internal.h"
 
@@ -23,9 +22,18 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 constexpr int kQThreads = 256;
 constexpr int kQVec = 4;  // 8-value vectors a thread keeps; longer rows are read twice
 
-// 127 x / amax; above 2^64 both are scaled down first (by a power of two), so that 127 x stays finite.
-__device__ __forceinline__ int code_of(float x, float amax, float down) {
-    return static_cast<int>(rintf((x * down * 127.0f) / amax));
+// rint(127 x / top) as the low byte of a float: t = 127 x is exact, q = t / top follows from t * (1 / top) by one
+// correction, which gives the quotient itself where that is a float (every tie is) and within its last place elsewhere,
+// far from any tie; adding 1.5 * 2^23 rounds it to an integer, ties to even.  A fifth of the instructions of a
+// division and a conversion.
+__device__ __forceinline__ uint32_t code_bits(float x, float top, float inv) {
+    const float t = x * 127.0f;
+    const float q = t * inv;
+    return __float_as_uint(fmaf(fmaf(-q, top, t), inv, q) + 12582912.0f);
+}
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u),
+                                 0x05040100u);
 }
 
 __global__ void __launch_bounds__(kQThreads)
@@ -71,17 +79,20 @@ quantize_int8_rows_kernel(const uint16_t *__restrict__ x, int64_t x_s0, int K, i
         amax = fmaxf(amax, s_max[w]);
         bad |= s_odd[w];
     }
-    const float down = amax > 1.8446744073709552e19f ? 5.421010862427522e-20f : 1.0f;
-    const float top = amax * down;
+    // very large and very small rows are scaled by a power of two first: 127 x and 1 / top stay normal
+    const float scale = amax > 1.8446744073709552e19f ? 5.421010862427522e-20f
+                        : amax < 5.421010862427522e-20f ? 1.8446744073709552e19f : 1.0f;
     const bool zero = bad || amax == 0.f;
-    auto put = [&](int vi, const uint4 &v) {
+    const float top = zero ? 1.0f : amax * scale;
+    const float inv = 1.0f / top;
+    auto put = [&](int vi, const uint4 &v) __attribute__((always_inline)) {
         float f[8];
         unpack8(v, f);
-        uint32_t w[2] = {0u, 0u};
+        uint32_t c[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            w[e / 4] |= static_cast<uint32_t>((zero ? 0 : code_of(f[e], top, down)) & 0xff) << (8 * (e % 4));
-        *reinterpret_cast<uint2 *>(q + row * q_s0 + vi * 8) = make_uint2(w[0], w[1]);
+        for (int e = 0; e < 8; ++e) c[e] = code_bits(zero ? 0.f : f[e] * scale, top, inv);
+        *reinterpret_cast<uint2 *>(q + row * q_s0 + vi * 8) =
+            make_uint2(low_bytes(c[0], c[1], c[2], c[3]), low_bytes(c[4], c[5], c[6], c[7]));
     };
 #pragma unroll
     for (int i = 0; i < kQVec; ++i) {
@@ -104,103 +115,158 @@ struct Int8Args {
     int M, N, K;
     uint16_t *out;
     int64_t o_s0;
-    int wide;  // out rows take 8-byte stores
+    int wide;  // out rows take 16-byte stores
 };
 
 __device__ __forceinline__ float scaled(int sum, float sx, float sw) { return static_cast<float>(sum) * sx * sw; }
 
-// MT 16-row tiles of x against 16 weight rows.  Lane l holds row l % 16 of either operand, bytes
-// 32 (l / 16) .. + 31 of a 128-byte piece of K, the same order in both; it ends with weight rows 4 (l / 16) .. + 3
-// of x row l % 16.
-template <int MT, int NW>
-__global__ void __launch_bounds__(NW * kWave)
+constexpr int kStage = 128;         // bytes of K a stage
+constexpr int kChunks = kStage / 16;
+
+// LDS place of 16-byte chunk c of row r: measured free of conflicts for the operand reads (32 rows and two chunks, 16
+// rows and four) and for the writes (eight rows).
+__device__ __forceinline__ int chunk_at(int r, int c) { return r * kChunks + (c ^ ((r >> 1) & 7)); }
+
+__device__ const i32x4 kZero16 = {0, 0, 0, 0};  // what a chunk behind K is read from
+
+// Waits until at most N of the wave's loads are under way (and all its LDS reads are back), then the barrier: what those
+// loads wrote to LDS is there for every wave, and what they read there may be overwritten.
+template <int N>
+__device__ __forceinline__ void arrive() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// 16 MT rows of x against 16 weight rows, the waves splitting K: wave w takes the 128-byte pieces w, w + kRowWaves, ..,
+// each into one of its own two LDS buffers, and the eight sums meet in LDS at the end; nobody waits for another wave
+// before that.  The loads write LDS themselves, eight lanes a row, so that each covers whole lines: operands loaded straight
+// into registers have neighbouring lanes in different rows, four times the line look-ups, and took 16.1 us instead of
+// 6.5 at 64 x 2048 (K 6144).  Two buffers of eight waves against one of sixteen and three of eight: 5.9, 6.6 and 6.4 us
+// at 32 rows of that product.
+constexpr int kRowWaves = 8;
+
+template <int MT>
+__global__ void __launch_bounds__(kRowWaves * kWave)
 int8_rows_kernel(Int8Args a) {
-    __shared__ __attribute__((aligned(16))) int part[NW][MT][kWave * 4];
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int r16 = lane & 15, kq = lane >> 4;
+    constexpr int NW = kRowWaves, V = 2 * (MT + 1);  // loads of 1 KB (eight rows) a piece: the weights', then x's
+    constexpr int kBuf = 1024 * V;
+    constexpr int kPart = MT * 256;  // sums of a wave
+    static_assert(kPart * 4 <= 2 * kBuf, "the sums fit where the operands were");
+    __shared__ __attribute__((aligned(16))) char lds[NW * 2 * kBuf];
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
-    const int wn = n0 + r16 < a.N ? n0 + r16 : a.N - 1;
-    const int8_t *wp = a.w + wn * a.w_s0 + 32 * kq;
-    const int8_t *xp[MT];
+    // load v writes rows 8 v .. + 7 of a piece, lane l place l % 8 of row l / 8
+    const int8_t *from[V];
+    int col[V];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int r = m0 + 16 * m + r16;
-        xp[m] = a.x + (r < a.M ? r : a.M - 1) * a.x_s0 + 32 * kq;
+    for (int v = 0; v < V; ++v) {
+        const bool x = v >= 2;
+        const int rr = 8 * (x ? v - 2 : v) + lane / 8, g = (x ? m0 : n0) + rr, n = x ? a.M : a.N;
+        col[v] = wave * kStage + 16 * ((lane & 7) ^ ((rr >> 1) & 7));
+        from[v] = (x ? a.x : a.w) + (g < n ? g : n - 1) * (x ? a.x_s0 : a.w_s0) + col[v];
     }
+    char *mine = lds + wave * 2 * kBuf;
+    auto load = [&](int piece, int buf) __attribute__((always_inline)) {
+        const int at = piece * NW * kStage;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int8_t *p = at + col[v] < a.K ? from[v] + at : reinterpret_cast<const int8_t *>(&kZero16);
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void *)p,
+                (__attribute__((address_space(3))) void *)(mine + buf * kBuf + 1024 * v), 16, 0, 0);
+        }
+    };
+    // operand h: lane l holds row l % 16, bytes 64 h + 16 (l / 16) .. + 15 of the piece, the same order in both
+    int get[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) get[h] = 16 * chunk_at(lane & 15, 4 * h + (lane >> 4));
     i32x4 acc[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[m] = i32x4{0, 0, 0, 0};
-    const i32x4 none = {0, 0, 0, 0};
-#pragma unroll 2
-    for (int k = wave * 128; k < a.K; k += NW * 128) {
-        const int at = k + 32 * kq;
-        i32x4 wv[2], xv[MT][2];
+    const int pieces = (a.K + NW * kStage - 1) / (NW * kStage);
+    load(0, 0);
+    load(1, 1);
+    for (int p = 0; p < pieces; p += 2) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const bool in = at + 16 * h < a.K;  // K is a multiple of 16
-            wv[h] = in ? *reinterpret_cast<const i32x4 *>(wp + k + 16 * h) : none;
+        for (int d = 0; d < 2; ++d) {  // pieces behind the last read zeros, so that the waits can count
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(V) : "memory");
+            i32x4 w[2], x[2][MT];
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-                xv[m][h] = in ? *reinterpret_cast<const i32x4 *>(xp[m] + k + 16 * h) : none;
+            for (int h = 0; h < 2; ++h) {
+                const char *src = mine + d * kBuf + get[h];
+                w[h] = *reinterpret_cast<const i32x4 *>(src);
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    x[h][m] = *reinterpret_cast<const i32x4 *>(src + 2048 * (m + 1));
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the buffer is written again
+            load(p + d + 2, d);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    acc[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[h], x[h][m], acc[m], 0, 0, 0);
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-                acc[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[h], xv[m][h], acc[m], 0, 0, 0);
     }
+    arrive<0>();  // every wave's loads and reads are done
+    int *part = reinterpret_cast<int *>(lds);
 #pragma unroll
-    for (int m = 0; m < MT; ++m) *reinterpret_cast<i32x4 *>(&part[wave][m][lane * 4]) = acc[m];
+    for (int m = 0; m < MT; ++m) *reinterpret_cast<i32x4 *>(part + wave * kPart + m * 256 + lane * 4) = acc[m];
     __syncthreads();
     // element e of tile m: lane e / 4, weight row 4 (lane / 16) + e % 4, x row lane % 16; threads along weight rows
-    for (int i = threadIdx.x; i < MT * 256; i += NW * kWave) {
+    for (int i = threadIdx.x; i < kPart; i += NW * kWave) {
         const int m = i / 256, row = (i & 255) >> 4, n = i & 15;
-        const int e = ((n >> 2) * 16 + row) * 4 + (n & 3);
+        const int e = m * 256 + ((n >> 2) * 16 + row) * 4 + (n & 3);
         int sum = 0;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) sum += part[w][m][e];
+        for (int w = 0; w < NW; ++w) sum += part[w * kPart + e];
         const int r = m0 + 16 * m + row;
         if (r < a.M && n0 + n < a.N)
             a.out[r * a.o_s0 + n0 + n] = f32_to_bf16(scaled(sum, a.sx[r], a.sw[n0 + n]));
     }
 }
 
-constexpr int kStage = 128;         // bytes of K a stage
-constexpr int kChunks = kStage / 16;
-
-// LDS place of 16-byte chunk c of row r: eight neighbouring rows read at one c, and a row's eight chunks written
-// together, touch all banks.
-__device__ __forceinline__ int chunk_at(int r, int c) { return r * kChunks + (c ^ (r & 7)); }
-
+// WM x WN waves, each TM x TN parts of 32 x 32.  K goes through three LDS buffers, 128 bytes a stage, written by the
+// loads themselves (a register on the way would cost its write to LDS: 0.14 us a stage of 128 x 256).  Step k: stage k
+// has arrived, the loads of stage k + 2 are issued; the operands of each 32 bytes are read while the MFMAs of the 32
+// before run, also across the barrier.  The results cross LDS once more, so that they leave in whole lines.
 template <int WM, int WN, int TM, int TN>
 __global__ void __launch_bounds__(WM * WN * kWave)
 int8_tile_kernel(Int8Args a, int tiles_m, int tiles) {
-    constexpr int T = WM * WN * kWave, BM = 32 * TM * WM, BN = 32 * TN * WN;
-    constexpr int XV = BM * kChunks / T, WV = BN * kChunks / T;
-    static_assert(XV * T == BM * kChunks && WV * T == BN * kChunks, "stage splits evenly over the threads");
-    __shared__ i32x4 xs[2][BM * kChunks];
-    __shared__ i32x4 ws[2][BN * kChunks];
+    constexpr int NW = WM * WN, T = NW * kWave, BM = 32 * TM * WM, BN = 32 * TN * WN;
+    constexpr int V = (BM + BN) / 8 / NW;  // loads of 1 KB (eight rows) a wave and stage
+    constexpr int STEPS = kStage / 32;
+    static_assert(V * NW * 8 == BM + BN && STEPS == 4, "a stage splits evenly over the waves");
+    constexpr int kBuf = (BM + BN) * kStage;     // bytes of a stage: weights, then x
+    constexpr int kOutPitch = BN * 2 + 16;       // bytes of a result row
+    constexpr int kOut = BM * kOutPitch;
+    __shared__ __attribute__((aligned(16))) char lds[3 * kBuf > kOut ? 3 * kBuf : kOut];
     // XCD b % 8 takes tiles (b % 8) per ..: neighbours in m share their weights in one L2
     const int per = (tiles + 7) / 8;
     const int t = static_cast<int>(blockIdx.x % 8) * per + static_cast<int>(blockIdx.x / 8);
     if (t >= tiles) return;
     const int m0 = t % tiles_m * BM, n0 = t / tiles_m * BN;
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int r32 = lane & 31, half = lane >> 5;
     const int wm = wave / WN, wn = wave % WN;
 
-    const int chunk = threadIdx.x % kChunks;
-    const int8_t *xp[XV], *wp[WV];
+    // load v writes rows 8 (wave V + v) .. + 7 of a stage, lane l place l % 8 of row l / 8
+    const int8_t *from[V];
+    int col[V];
 #pragma unroll
-    for (int v = 0; v < XV; ++v) {
-        const int r = m0 + (threadIdx.x + v * T) / kChunks;
-        xp[v] = a.x + (r < a.M ? r : a.M - 1) * a.x_s0 + 16 * chunk;
+    for (int v = 0; v < V; ++v) {
+        const int r = 8 * (wave * V + v) + lane / 8;
+        const bool x = r >= BN;
+        const int rr = x ? r - BN : r, g = (x ? m0 : n0) + rr, n = x ? a.M : a.N;
+        col[v] = 16 * ((lane & 7) ^ ((rr >> 1) & 7));
+        from[v] = (x ? a.x : a.w) + (g < n ? g : n - 1) * (x ? a.x_s0 : a.w_s0) + col[v];
     }
+    int get[STEPS];  // chunk 2 j + half of row r32: the parts are constants away (32 rows keep the exclusive-or)
 #pragma unroll
-    for (int v = 0; v < WV; ++v) {
-        const int r = n0 + (threadIdx.x + v * T) / kChunks;
-        wp[v] = a.w + (r < a.N ? r : a.N - 1) * a.w_s0 + 16 * chunk;
-    }
+    for (int j = 0; j < STEPS; ++j) get[j] = 16 * chunk_at(r32, 2 * j + half);
+    const int w_part = wn * TN * 32 * kStage, x_part = BN * kStage + wm * TM * 32 * kStage;
+
     i32x16 acc[TM][TN];
 #pragma unroll
     for (int m = 0; m < TM; ++m)
@@ -209,77 +275,98 @@ int8_tile_kernel(Int8Args a, int tiles_m, int tiles) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[m][n][i] = 0;
 
-    i32x4 xr[XV], wr[WV];
-    const i32x4 none = {0, 0, 0, 0};
-    auto load = [&](int k) {
-        const bool in = k + 16 * chunk < a.K;
-#pragma unroll
-        for (int v = 0; v < WV; ++v) wr[v] = in ? *reinterpret_cast<const i32x4 *>(wp[v] + k) : none;
-#pragma unroll
-        for (int v = 0; v < XV; ++v) xr[v] = in ? *reinterpret_cast<const i32x4 *>(xp[v] + k) : none;
+    const int stages = (a.K + kStage - 1) / kStage;
+    auto load = [&](int k, int buf, int v) __attribute__((always_inline)) {
+        const int8_t *p = k * kStage + col[v] < a.K ? from[v] + k * kStage : reinterpret_cast<const int8_t *>(&kZero16);
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void *)p,
+            (__attribute__((address_space(3))) void *)(lds + buf + 1024 * (wave * V + v)), 16, 0, 0);
     };
-    auto store = [&](int buf) {
+    i32x4 wf[2][TN], xf[2][TM];
+    auto read = [&](int buf, int j) __attribute__((always_inline)) {
 #pragma unroll
-        for (int v = 0; v < XV; ++v) xs[buf][chunk_at((threadIdx.x + v * T) / kChunks, chunk)] = xr[v];
+        for (int n = 0; n < TN; ++n)
+            wf[j & 1][n] = *reinterpret_cast<const i32x4 *>(lds + buf + w_part + get[j] + n * 32 * kStage);
 #pragma unroll
-        for (int v = 0; v < WV; ++v) ws[buf][chunk_at((threadIdx.x + v * T) / kChunks, chunk)] = wr[v];
+        for (int m = 0; m < TM; ++m)
+            xf[j & 1][m] = *reinterpret_cast<const i32x4 *>(lds + buf + x_part + get[j] + m * 32 * kStage);
     };
-    load(0);
-    store(0);
-    if (kStage < a.K) load(kStage);
-    int buf = 0;
-    for (int k = 0; k < a.K; k += kStage, buf ^= 1) {
-        __syncthreads();
-        if (k + kStage < a.K) {
-            store(buf ^ 1);
-            if (k + 2 * kStage < a.K) load(k + 2 * kStage);
+    auto multiply = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+        for (int m = 0; m < TM; ++m)
+#pragma unroll
+            for (int n = 0; n < TN; ++n)
+                acc[m][n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[j & 1][n], xf[j & 1][m], acc[m][n], 0, 0, 0);
+    };
+    int b0 = 0, b1 = kBuf, b2 = 2 * kBuf;  // buffers of stages k, k + 1, k + 2
+#pragma unroll
+    for (int v = 0; v < V; ++v) load(0, b0, v);
+#pragma unroll
+    for (int v = 0; v < V; ++v) load(1, b1, v);
+    for (int k = 0; k < stages; ++k) {
+        arrive<V>();  // stage k is there; stage k + 1 may be under way
+        read(b0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (k > 0) multiply(STEPS - 1);  // the last operands of stage k - 1
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) {
+            // into the buffer that the barrier freed; stages behind the last read zeros, so that the waits can count
+#pragma unroll
+            for (int v = V * j / STEPS; v < V * (j + 1) / STEPS; ++v) load(k + 2, b2, v);
+            __builtin_amdgcn_sched_barrier(0);
+            if (j + 1 < STEPS) {
+                read(b0, j + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(j);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-#pragma unroll
-        for (int s = 0; s < kStage / 32; ++s) {
-            i32x4 wf[TN], xf[TM];
-#pragma unroll
-            for (int n = 0; n < TN; ++n) wf[n] = ws[buf][chunk_at((wn * TN + n) * 32 + r32, 2 * s + half)];
-#pragma unroll
-            for (int m = 0; m < TM; ++m) xf[m] = xs[buf][chunk_at((wm * TM + m) * 32 + r32, 2 * s + half)];
-#pragma unroll
-            for (int m = 0; m < TM; ++m)
-#pragma unroll
-                for (int n = 0; n < TN; ++n)
-                    acc[m][n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[n], xf[m], acc[m][n], 0, 0, 0);
-        }
+        const int b = b0;
+        b0 = b1;
+        b1 = b2;
+        b2 = b;
     }
-    // the lane holds x row r32, weight rows 8 (i / 4) + 4 half + i % 4 of a 32 x 32 part
+    multiply(STEPS - 1);
+    arrive<0>();  // no load is left that would write over the results
+
+    // the lane holds x row r32, weight rows 8 (i / 4) + 4 half + i % 4 of each part
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
-        const int row = m0 + (wm * TM + m) * 32 + r32;
-        if (row >= a.M) continue;
-        const float sx = a.sx[row];
-        uint16_t *orow = a.out + row * a.o_s0;
+        const int r = (wm * TM + m) * 32 + r32;
+        const float sx = m0 + r < a.M ? a.sx[m0 + r] : 0.f;
 #pragma unroll
         for (int n = 0; n < TN; ++n)
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
-                const int col = n0 + (wn * TN + n) * 32 + 2 * i + 4 * half;
-                if (a.wide && col + 3 < a.N) {
-                    const float4 sw = *reinterpret_cast<const float4 *>(a.sw + col);
-                    *reinterpret_cast<uint2 *>(orow + col) =
-                        make_uint2(pack2_bf16(scaled(acc[m][n][i], sx, sw.x), scaled(acc[m][n][i + 1], sx, sw.y)),
-                                   pack2_bf16(scaled(acc[m][n][i + 2], sx, sw.z), scaled(acc[m][n][i + 3], sx, sw.w)));
-                } else {
+                const int c = (wn * TN + n) * 32 + 2 * i + 4 * half;
+                float sw[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (col + e < a.N) orow[col + e] = f32_to_bf16(scaled(acc[m][n][i + e], sx, a.sw[col + e]));
-                }
+                for (int e = 0; e < 4; ++e) sw[e] = n0 + c + e < a.N ? a.sw[n0 + c + e] : 0.f;
+                *reinterpret_cast<uint2 *>(lds + r * kOutPitch + 2 * c) =
+                    make_uint2(pack2_bf16(scaled(acc[m][n][i], sx, sw[0]), scaled(acc[m][n][i + 1], sx, sw[1])),
+                               pack2_bf16(scaled(acc[m][n][i + 2], sx, sw[2]), scaled(acc[m][n][i + 3], sx, sw[3])));
             }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < BM * BN / 8; i += T) {
+        const int r = i / (BN / 8), c = i % (BN / 8) * 8;
+        if (m0 + r >= a.M || n0 + c >= a.N) continue;
+        const char *src = lds + r * kOutPitch + 2 * c;
+        uint16_t *dst = a.out + (m0 + r) * a.o_s0 + n0 + c;
+        if (a.wide && n0 + c + 8 <= a.N) {
+            *reinterpret_cast<i32x4 *>(dst) = *reinterpret_cast<const i32x4 *>(src);
+        } else {
+            for (int e = 0; e < 8 && n0 + c + e < a.N; ++e) dst[e] = reinterpret_cast<const uint16_t *>(src)[e];
+        }
     }
 }
 
 bool al(const void *p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-template <int MT, int NW>
+template <int MT>
 void launch_rows(const Int8Args &a, hipStream_t st) {
-    hipLaunchKernelGGL((int8_rows_kernel<MT, NW>), dim3((a.N + 15) / 16, (a.M + 16 * MT - 1) / (16 * MT)),
-                       dim3(NW * kWave), 0, st, a);
+    hipLaunchKernelGGL(int8_rows_kernel<MT>, dim3((a.N + 15) / 16, (a.M + 16 * MT - 1) / (16 * MT)),
+                       dim3(kRowWaves * kWave), 0, st, a);
 }
 
 template <int WM, int WN, int TM, int TN>
@@ -311,17 +398,27 @@ extern "C" int nq_linear_int8(const int8_t *xq, int64_t x_s0, const float *sx, c
     NQ_CHECK_ARG(M >= 0 && N >= 0 && K >= 0);
     if (M == 0 || N == 0) return NQ_OK;
     NQ_CHECK_ARG(xq && sx && wq && sw && out && K >= 16 && x_s0 >= 0 && w_s0 >= 0 && (M == 1 || o_s0 >= N));
-    if (K % 16 || K > (1 << 17) || (M > 1 && x_s0 % 16) || (N > 1 && w_s0 % 16) || !al(xq, 16) || !al(wq, 16) || !al(sx, 4) || !al(sw, 4))
+    if (K % 16 || K > (1 << 17) || (M > 1 && x_s0 % 16) || (N > 1 && w_s0 % 16) || !al(xq, 16) || !al(wq, 16) ||
+        !al(sx, 4) || !al(sw, 4))
         return NQ_ERR_UNSUPPORTED;
     if (static_cast<int64_t>((M + 31) / 32) * ((N + 31) / 32) > 0x3fffffff || N > 0x7fffff00 || M > 0x7fffff00)
         return NQ_ERR_UNSUPPORTED;
     const Int8Args a = {xq,  x_s0, sx,   wq, w_s0, sw, M, N, K, out, o_s0,
-                        (M == 1 || o_s0 % 4 == 0) && al(out, 8) && al(sw, 16)};
+                        (M == 1 || o_s0 % 8 == 0) && al(out, 16)};
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (M <= 16) launch_rows<1, 16>(a, st);
-    else if (M <= 32) launch_rows<2, 16>(a, st);
-    else if (M <= 64) launch_rows<4, 16>(a, st);
-    else if (static_cast<int64_t>((M + 127) / 128) * ((N + 127) / 128) >= 256) launch_tiles<2, 2, 2, 2>(a, st);
-    else launch_tiles<2, 2, 1, 1>(a, st);
+    // Few tiles: the waves split K.  Otherwise the largest tile that still gives every CU one: a stage of 128 bytes takes
+    // 0.29, 0.38 and 1.0 us at 64 x 64, 64 x 128 and 128 x 256.  Measured, K 2048, us:
+    //   M 64  N 4096:  64-row pieces 5.5, 32-row pieces 6.6, 64 x 64 tiles 8.4;   N 6144: 9.8, 9.4, 8.4
+    //   M 32  N 6144:  32-row pieces 6.8, 64 x 64 tiles 8.2;                      N 12288: 10.0, 8.4
+    //   M 256 N 4096:  64 x 64 tiles 9.1, 64 x 128 9.6, 128 x 256 19;             N 6144: 11.0, 10.1, 20
+    //   M 640 N 6144:  64 x 128 tiles 15.8, 128 x 256 21.0;                       N 12288: 28.0, 24.4
+    auto count = [&](int bm, int bn) { return static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+    auto rounds = [](int64_t tiles) { return (tiles + 255) / 256; };
+    if (M <= 16) launch_rows<1>(a, st);
+    else if (count(32, 16) <= (M <= 32 ? 512 : 256)) launch_rows<2>(a, st);
+    else if (count(64, 16) <= 256) launch_rows<4>(a, st);
+    else if (count(64, 64) <= 256) launch_tiles<2, 2, 1, 1>(a, st);
+    else if (3 * rounds(count(128, 256)) > rounds(count(64, 128))) launch_tiles<2, 4, 1, 1>(a, st);
+    else launch_tiles<2, 4, 2, 2>(a, st);
     return NQ_LAUNCH_STATUS();
 }
