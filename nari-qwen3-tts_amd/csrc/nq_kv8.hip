@@ -347,7 +347,9 @@ __device__ __forceinline__ int span_of(const Spans &s, int64_t b) {
 // that order, the 8 keys of the lane's group in out^T = V^T P^T, so P needs no exchange between lanes; V is loaded
 // as (D/16) values of each of the 8 tokens, and the byte a conversion picks does the transposition.
 // K of the next step is asked for as soon as this one's is multiplied, V likewise: one set of registers, and loads always
-// in flight.
+// in flight.  Each byte is read once, so the loads are non-temporal: 64 rows of 64 to 2048 keys (135 MB) take 31.8 us
+// instead of 34.4, 3 rows of 40000 to 60001 (308 MB) 56.3 instead of 60.0, 5.5 TB/s.  Two waves a SIMD: three take as
+// long, four 49.6 and 81.7 us.
 template <int D>
 __global__ void __launch_bounds__(kKv8Threads, 2)
 kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml, float *__restrict__ part_o) {
@@ -423,14 +425,15 @@ kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml
         for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int w = 0; w < W; ++w)
-                k[m][w] = *reinterpret_cast<const u32x4 *>(kbase + n.off[m] + (k_lane + 16 * w));
+                k[m][w] =
+                    __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kbase + n.off[m] + (k_lane + 16 * w)));
     };
     auto load_v = [&](const Blocks &n) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int8_t *p = vbase + n.off[e / 4] + (v_lane + (e % 4) * c_slot);
-            if constexpr (W == 2) v[e] = *reinterpret_cast<const u32x2 *>(p);
-            else v[e].x = *reinterpret_cast<const uint32_t *>(p);
+            if constexpr (W == 2) v[e] = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(p));
+            else v[e].x = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(p));
         }
     };
 
@@ -1206,8 +1209,11 @@ extern "C" int nq_kv_int8_write(const uint16_t *key, int64_t k_s0, int64_t k_s1,
     if (!al(key, 16) || !al(value, 16) || odd_stride(tokens, k_s0, 8) || odd_stride(num_kv_heads, k_s1, 8) ||
         odd_stride(tokens, v_s0, 8) || odd_stride(num_kv_heads, v_s1, 8))
         return NQ_ERR_UNSUPPORTED;
-    // one token a wave while that leaves at most eight waves a SIMD of work, else 16
-    const int group = static_cast<int64_t>(tokens) * num_kv_heads * 2 <= 8192 ? 1 : 16;
+    // A wave takes its leaders one after another, about 2 us each, so many short runs want small groups and a long prompt
+    // large ones.  Measured with groups of 1, 4, 8, 16, us, 8 heads: 64 runs of 1 token 5.0, 11.4, 19.6, 35.9; 1024 of 1
+    // 18.0, 15.4, 22.2, 36.8; 8 of 80 13.2, 7.5, 6.6, 8.8; 8 of 300 23.9, 10.4, 9.6, 12.3; 1 of 8191 63, 41.5, 25.5, 18.9.
+    const int64_t units = 2ll * tokens * num_kv_heads;
+    const int group = units <= 4096 ? 1 : units <= 24576 ? 4 : units <= 65536 ? 8 : 16;
     const dim3 grid((tokens + group - 1) / group, (2 * num_kv_heads + kKv8Waves - 1) / kKv8Waves);
     const auto kernel = head_dim == 128 ? kv8_write_kernel<128> : kv8_write_kernel<64>;
     hipLaunchKernelGGL(kernel, grid, dim3(kKv8Threads), 0, static_cast<hipStream_t>(stream), key, k_s0, k_s1, value,
