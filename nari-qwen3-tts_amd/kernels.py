@@ -425,8 +425,9 @@ def paged_cache_read_int8(layer_cache: torch.Tensor, layer_scales: torch.Tensor,
     heads, d, cache = _int8_cache(layer_cache, layer_scales)
     tokens = _int8_slots(pages, offsets)
     shape = (tokens, heads, d)
-    key = torch.empty(shape, dtype=torch.bfloat16, device=layer_cache.device) if key is None else key
-    value = torch.empty(shape, dtype=torch.bfloat16, device=layer_cache.device) if value is None else value
+    # sizes as numbers parse faster than as a tuple
+    key = torch.empty(tokens, heads, d, dtype=torch.bfloat16, device=layer_cache.device) if key is None else key
+    value = torch.empty(tokens, heads, d, dtype=torch.bfloat16, device=layer_cache.device) if value is None else value
     target = _int8_heads(key, shape) + _int8_heads(value, shape)
     _lib.launch(
         _lib.one_device(layer_cache, layer_scales, pages, offsets, key, value, status), "nq_kv_int8_read", *cache,
@@ -467,7 +468,7 @@ def paged_attention_int8(query: torch.Tensor, layer_cache: torch.Tensor, layer_s
     tokens, hq, q_dim = shape
     if q_dim != d or hq < hkv or hq % hkv:
         raise ValueError("query and cache disagree on the heads")
-    out = torch.empty_like(query, memory_format=torch.contiguous_format) if out is None else out
+    out = torch.empty(tokens, hq, d, dtype=query.dtype, device=query.device) if out is None else out
     if query.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16:
         raise TypeError("HIP attention kernels take bf16 tensors")
     o_strides = out.stride()

@@ -761,7 +761,7 @@ def quantize_int8_rows(x: torch.Tensor, q: torch.Tensor | None = None,
     rows, k = shape
     if k < 16 or k % 16:
         raise ValueError("int8 row quantization needs a multiple of 16 columns")
-    q = torch.empty(shape, dtype=torch.int8, device=x.device) if q is None else q
+    q = torch.empty(rows, k, dtype=torch.int8, device=x.device) if q is None else q  # sizes as numbers parse faster
     scales = torch.empty(rows, dtype=torch.float32, device=x.device) if scales is None else scales
     if q.dtype is not torch.int8 or scales.dtype is not torch.float32:
         raise TypeError("int8 codes and float32 scales expected")
@@ -792,7 +792,7 @@ def linear_int8(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, w
     if scales.shape != (rows,) or weight_scales.shape != (n,) or not (
             scales.is_contiguous() and weight_scales.is_contiguous()):
         raise ValueError("int8 scales must be contiguous, one per row and one per output")
-    out = torch.empty((rows, n), dtype=torch.bfloat16, device=q.device) if out is None else out
+    out = torch.empty(rows, n, dtype=torch.bfloat16, device=q.device) if out is None else out
     o_strides = out.stride()
     if out.dtype is not torch.bfloat16 or out.shape != (rows, n) or o_strides[1] != 1:
         raise ValueError(f"out must be bf16 [{rows}, {n}] with unit inner stride")
