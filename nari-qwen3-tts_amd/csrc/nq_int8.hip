@@ -10,6 +10,8 @@
 // Integer sums are exact in any order, so cutting K costs no determinism.
 // Many rows: (32 TM WM) x (32 TN WN) tiles of mfma_i32_32x32x32_i8, K staged 128 bytes at a
 // time through three LDS buffers, the next two stages' loads in flight.
+#include <type_traits>
+
 #include "nq_common.h"
 #include "nq_internal.h"
 
@@ -231,6 +233,10 @@ int8_rows_kernel(Int8Args a) {
 // loads themselves (a register on the way would cost its write to LDS: 0.14 us a stage of 128 x 256).  Step k: stage k
 // has arrived, the loads of stage k + 2 are issued; the operands of each 32 bytes are read while the MFMAs of the 32
 // before run, also across the barrier.  The results cross LDS once more, so that they leave in whole lines.
+// Bound by LDS: 128 x 256 reads 128 KB and writes 48 KB a stage, 0.65 us at 128 bytes a clock, beside 0.51 us of MFMAs;
+// the stage takes 1.0 us, and launch, first loads and results 10 us.  640 x 12288 (K 2048) 24.4 us = 1320 TOP/s, 4001 x
+// 2048 (K 6144) 57.4 us = 1750 TOP/s (2496 is what a library's 8192^3 reaches).  Other waves for that tile at the same
+// sizes: 2 x 2 of 64 x 128 33 and 69 us, 1 x 4 of 128 x 64 32 and 68, 4 x 2 of 32 x 64 (128 x 128) 30 and 70.
 template <int WM, int WN, int TM, int TN>
 __global__ void __launch_bounds__(WM * WN * kWave)
 int8_tile_kernel(Int8Args a, int tiles_m, int tiles) {
@@ -276,8 +282,10 @@ int8_tile_kernel(Int8Args a, int tiles_m, int tiles) {
             for (int i = 0; i < 16; ++i) acc[m][n][i] = 0;
 
     const int stages = (a.K + kStage - 1) / kStage;
-    auto load = [&](int k, int buf, int v) __attribute__((always_inline)) {
-        const int8_t *p = k * kStage + col[v] < a.K ? from[v] + k * kStage : reinterpret_cast<const int8_t *>(&kZero16);
+    auto load = [&](auto whole, int k, int buf, int v) __attribute__((always_inline)) {
+        const int8_t *p = from[v];
+        if constexpr (!whole) p = k * kStage + col[v] < a.K ? p : reinterpret_cast<const int8_t *>(&kZero16);
+        from[v] += kStage;
         __builtin_amdgcn_global_load_lds(
             (const __attribute__((address_space(1))) void *)p,
             (__attribute__((address_space(3))) void *)(lds + buf + 1024 * (wave * V + v)), 16, 0, 0);
@@ -299,11 +307,13 @@ int8_tile_kernel(Int8Args a, int tiles_m, int tiles) {
                 acc[m][n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[j & 1][n], xf[j & 1][m], acc[m][n], 0, 0, 0);
     };
     int b0 = 0, b1 = kBuf, b2 = 2 * kBuf;  // buffers of stages k, k + 1, k + 2
+    constexpr std::true_type whole{};      // stages inside K: no look at the chunks, 14 vector instructions instead of 40
+    constexpr std::false_type part{};
 #pragma unroll
-    for (int v = 0; v < V; ++v) load(0, b0, v);
+    for (int v = 0; v < V; ++v) load(part, 0, b0, v);
 #pragma unroll
-    for (int v = 0; v < V; ++v) load(1, b1, v);
-    for (int k = 0; k < stages; ++k) {
+    for (int v = 0; v < V; ++v) load(part, 1, b1, v);
+    auto step = [&](auto next, int k) __attribute__((always_inline)) {
         arrive<V>();  // stage k is there; stage k + 1 may be under way
         read(b0, 0);
         __builtin_amdgcn_sched_barrier(0);
@@ -312,7 +322,7 @@ int8_tile_kernel(Int8Args a, int tiles_m, int tiles) {
         for (int j = 0; j < STEPS; ++j) {
             // into the buffer that the barrier freed; stages behind the last read zeros, so that the waits can count
 #pragma unroll
-            for (int v = V * j / STEPS; v < V * (j + 1) / STEPS; ++v) load(k + 2, b2, v);
+            for (int v = V * j / STEPS; v < V * (j + 1) / STEPS; ++v) load(next, k + 2, b2, v);
             __builtin_amdgcn_sched_barrier(0);
             if (j + 1 < STEPS) {
                 read(b0, j + 1);
@@ -325,7 +335,10 @@ int8_tile_kernel(Int8Args a, int tiles_m, int tiles) {
         b0 = b1;
         b1 = b2;
         b2 = b;
-    }
+    };
+    int k = 0;
+    for (; (k + 3) * kStage <= a.K; ++k) step(whole, k);
+    for (; k < stages; ++k) step(part, k);
     multiply(STEPS - 1);
     arrive<0>();  // no load is left that would write over the results
 
