@@ -4,9 +4,9 @@ Import this package after ``torch``.  Submodules:
 
 - ``talker_kv``  -- PagedTalkerKV + HIP attention bindings (GPU planner, attention plan)
 - ``cache``      -- host page ownership with pending/publish/discard publications
-- ``kernels``    -- qk-norm/RoPE/KV-write and short-cache attention entry points
+- ``kernels``    -- qk-norm/RoPE/KV-write, short-cache attention, 8-bit cache and attention entry points
 - ``sampling``   -- fused uniform-driven sampler and Philox uniforms
-- ``layers``     -- fused add-RMSNorm, RMSNorm, SwiGLU
+- ``layers``     -- fused add-RMSNorm, RMSNorm, SwiGLU, projections (bf16, FP8, int8)
 - ``talker``     -- one random-init talker decode step (the metric's unit)
 - ``graphs``     -- hipGraph capture driver and bucket lowering
 - ``build``      -- hipcc recipe for ``libnq_hip.so``

@@ -80,6 +80,9 @@ __device__ __forceinline__ bf16x8_t widen8(uint32_t a, uint32_t b) {
 // are the tokens behind it that do.  So the slot map alone says who owns a block, a run's tokens are
 // quantised with one scale, and a block's earlier slots are read only by the wave that may rescale them.
 // Lane l holds slots l / (D/8) + i * (512/D), values 8 (l % (D/8)) .. + 7.
+// Bound by its chain of loads (slots, then the block's scale and tokens) where tokens are few: 64 single tokens 4.5 us,
+// 4 of them the launch and the chain; by HBM where they are many: 7677 tokens of 8 heads of 128 (47 MB) 14.8 us, 3.2 TB/s,
+// one round of waves that all load first and store last.
 template <int D>
 __global__ void __launch_bounds__(kKv8Threads)
 kv8_write_kernel(const uint16_t *__restrict__ key, int64_t k_s0, int64_t k_s1, const uint16_t *__restrict__ value,
@@ -170,7 +173,8 @@ kv8_write_kernel(const uint16_t *__restrict__ key, int64_t k_s0, int64_t k_s1, c
 }
 
 // ---------------------------------------------------------------------------------------------
-// Read back: thread per 16 codes of one (token, kind, head).
+// Read back: thread per 16 codes of one (token, kind, head).  Bound by HBM: 7677 tokens of 8 heads of 128 (47 MB) 11.3 us,
+// 4.2 TB/s.
 template <int D>
 __global__ void __launch_bounds__(kKv8Threads)
 kv8_read_kernel(Pool8 pool, const int64_t *__restrict__ pages, const int64_t *__restrict__ offsets, int tokens,
@@ -347,9 +351,9 @@ __device__ __forceinline__ int span_of(const Spans &s, int64_t b) {
 // that order, the 8 keys of the lane's group in out^T = V^T P^T, so P needs no exchange between lanes; V is loaded
 // as (D/16) values of each of the 8 tokens, and the byte a conversion picks does the transposition.
 // K of the next step is asked for as soon as this one's is multiplied, V likewise: one set of registers, and loads always
-// in flight.  Each byte is read once, so the loads are non-temporal: 64 rows of 64 to 2048 keys (135 MB) take 31.8 us
-// instead of 34.4, 3 rows of 40000 to 60001 (308 MB) 56.3 instead of 60.0, 5.5 TB/s.  Two waves a SIMD: three take as
-// long, four 49.6 and 81.7 us.
+// in flight.  Each byte is read once, so the loads are non-temporal: 64 rows of 66 to 2047 keys (135 MB) take 31.8 us
+// instead of 34.4, 3 rows of about 50000 (308 MB) 56.3 instead of 60.0, 5.5 TB/s.  Two waves a SIMD: with plain
+// loads three took as long and four (registers spilled) 49.6 and 81.7 us.
 template <int D>
 __global__ void __launch_bounds__(kKv8Threads, 2)
 kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml, float *__restrict__ part_o) {
@@ -582,7 +586,8 @@ kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml
 
 // Joins a decode row's partials: span i0, where the row begins, left its slot 1, the spans behind it slot 0.
 // Weights 2^(m_i - m), in span order.  A row without pages gets zeros.  A workgroup takes one query head:
-// D/4 threads a partial, 1024 / D partials at a time, four rounds of loads in flight.
+// D/4 threads a partial, 1024 / D partials at a time, four rounds of loads in flight.  Bound by its launch and two
+// dependent loads: 4.2 us for 64 rows of 16 heads, 5.6 us where 3 rows left 2048 partials.
 template <int D>
 __global__ void __launch_bounds__(kKv8Threads)
 kv8_merge_kernel(Attend8 a, int waves, const float2 *__restrict__ part_ml, const float *__restrict__ part_o) {
@@ -664,6 +669,13 @@ kv8_merge_kernel(Attend8 a, int waves, const float2 *__restrict__ part_ml, const
 // tile's loads are in flight while the one before it is multiplied.  Sums are rescaled only when a maximum has grown
 // by more than 2^8 (P stays below that, and bf16 and fp32 lose nothing by it).  With few tiles the key range is
 // cut into pieces, joined by kv8_join_kernel.
+// 1856 queries of 16 heads over 6001 keys (77 GFLOP): 118.8 us and 9.2 for the join, 600 TFLOP/s.  A tile takes 2.3 us: 0.97
+// us of MFMAs (two waves a SIMD), 1.2 of vector instructions (32 exponentials, 64 for the staging and 160 others a
+// wave), 1.2 of LDS (278 KB read, 34 KB written a workgroup) and the barrier, which overlap in part only; without
+// the staging 101 us, without the operand reads 106, without the exponentials 112, without all three 85.  With
+// uniform pieces the longest one takes 47 tiles where 39 is the mean.  Tried and no faster: operands read three MFMAs
+// ahead with the barrier inside the step (spills, +-3 %), 64 columns a wave at one wave a SIMD (201 us, moves between the
+// register files), spans that cross tiles for even work (126 us and 17 for the join).
 constexpr int kKeys = 64;
 constexpr float kLag = 8.0f;
 
@@ -1071,7 +1083,8 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
     }
 }
 
-// Joins the pieces of a tile, in order: D/8 threads a column, every piece's values in flight at once.
+// Joins the pieces of a tile, in order: D/8 threads a column, every piece's values in flight at once.  Bound by its reads:
+// 66 MB of partials 9.2 us.
 constexpr int kMaxPieces = 8;
 template <int D>
 __global__ void __launch_bounds__(kKv8Threads)
