@@ -708,7 +708,7 @@ template <int D>
 struct Smem8 {
     u32x4 k[2][kKeys * (D / 8 + 1)];
     u32x4 v[2][D * (kKeys / 8)];
-    floatx4_t ks[2];               // K scales of the tile's blocks, 1 where one is not finite
+    floatx4_t ks[2];               // K scales of the tile's blocks times sm_scale log2(e), 1 where one is not finite
     i32x4_t odd[2];                // kAbsent: the block's page is not in the pool; kPoison: a scale is not finite
     Meta8 meta;
 };
@@ -823,7 +823,8 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
         // through 0 * NaN in those that do not.
         const bool fine = fabsf(r.ks) < __builtin_inff() && fabsf(r.vs) < __builtin_inff();
         const int blk = uwave * (kKeys / kBlk) / NW;
-        sm.ks[buf][blk] = fine ? r.ks : 1.0f;
+        // above zero, also for a block that was never written: a masked score, minus infinity, stays that
+        sm.ks[buf][blk] = r.on && fine ? fmaxf(r.ks * a.scale, kMinScale) : 1.0f;
         sm.odd[buf][blk] = !r.on ? kAbsent : fine ? 0 : kPoison;
     };
     auto put_v = [&](const u32x2 (&x)[VB], int buf) __attribute__((always_inline)) {
@@ -902,9 +903,8 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
             s[i / 16][i % 16] = see ? v : -__builtin_inff();
         }
     };
-    // A tile's factors, scale of the block times sm_scale log2(e), and the maximum of its scores times them
-    // (scales are positive).
-    auto factors = [&](int kt) __attribute__((always_inline)) { return sm.ks[kt & 1] * a.scale; };
+    // A tile's factors, and the maximum of its scores times them (factors are positive).
+    auto factors = [&](int kt) __attribute__((always_inline)) { return sm.ks[kt & 1]; };
     auto block_top = [&](const floatx16_t (&s)[2], int k) __attribute__((always_inline)) {
         float m = s[k / 2][8 * (k % 2)];
 #pragma unroll

@@ -424,3 +424,56 @@ def test_rows_that_share_pages(nq, device):
     q, codes, scales, meta = _batch(device, 320, [64, 64, 50], None, hq=4, hkv=2, d=64, ps=16)
     meta.paged_kv_indices[4:8] = meta.paged_kv_indices[:4]
     _check(q, codes, scales, meta)
+
+
+def test_blocks_that_were_never_written(nq, device):
+    """A pool of zeros, scales too: every value is zero, and so is every output, masked keys or not."""
+
+    for queries in (None, [5, 70, 2], [1, 33, 2]):
+        q, codes, scales, meta = _batch(device, 330, [20, 70, 2], queries, hq=4, hkv=2, d=64, ps=64)
+        codes.zero_()
+        scales.zero_()
+        assert not _check(q, codes, scales, meta).any()
+
+
+@pytest.mark.parametrize("sm_scale", [0.0, 1e-38, -1e-30])
+def test_scores_that_vanish(nq, device, sm_scale):
+    """Factors of the scores down to zero, with blocks of zeros (scale 2^-126) among the keys: plain means."""
+
+    for queries in (None, [40, 9]):
+        q, codes, scales, meta = _batch(device, 331, [90, 40], queries, hq=4, hkv=2, d=128, ps=16)
+        codes[meta.paged_kv_indices[1], 0] = 0
+        scales[meta.paged_kv_indices[1], 0] = 2.0**-126
+        _check(q, codes, scales, meta, sm_scale=sm_scale)
+
+
+def test_page_outside_the_pool_beside_odd_scales(nq, device):
+    """A skipped page takes nothing from the pool, whatever its first page holds."""
+
+    from nari_qwen3_tts_amd.kernels import paged_attention_int8
+
+    for queries in (None, [30, 1]):
+        q, codes, scales, meta = _batch(device, 332, [100, 40], queries, hq=4, hkv=2, d=64, ps=16)
+        ids = meta.paged_kv_indices.cpu().numpy()
+        ids = np.where(ids == 0, next(p for p in range(codes.shape[0]) if p not in ids), ids)
+        ids[2] = codes.shape[0]
+        meta.paged_kv_indices.copy_(torch.tensor(ids, dtype=torch.int32))
+        outs = []
+        for value in (1.0, -1.0, 0.0, float("nan"), float("-inf")):
+            scales[0] = value
+            status = torch.zeros(1, dtype=torch.int32, device=device)
+            outs.append(paged_attention_int8(q, codes, scales, meta, status=status))
+            assert int(status) == -1
+        assert outs[0].isfinite().all()
+        for out in outs[1:]:
+            assert torch.equal(out.view(torch.int16), outs[0].view(torch.int16))
+
+
+def test_many_rows(nq, device):
+    """More rows than the kernels copy to LDS."""
+
+    rng = np.random.default_rng(333)
+    lens = rng.integers(0, 60, 700).tolist()
+    _check(*_batch(device, 333, lens, None, hq=2, hkv=1, d=64, ps=16))
+    queries = rng.integers(0, 4, 700).tolist()
+    _check(*_batch(device, 334, lens, queries, hq=2, hkv=1, d=64, ps=16))
