@@ -236,7 +236,7 @@ int8_rows_kernel(Int8Args a) {
 // has arrived, the loads of stage k + 2 are issued; the operands of each 32 bytes are read while the MFMAs of the 32
 // before run, also across the barrier.  The results cross LDS once more, so that they leave in whole lines.
 // Bound by LDS: 128 x 256 reads 128 KB and writes 48 KB a stage, 0.65 us at 128 bytes a clock, beside 0.51 us of MFMAs;
-// the stage takes 1.0 us, and launch, first loads and results 10 us.  640 x 12288 (K 2048) 24.4 us = 1320 TOP/s, 4001 x
+// the stage takes 1.0 us, and launch, first loads and results 9 us.  640 x 12288 (K 2048) 22.9 us = 1410 TOP/s, 4001 x
 // 2048 (K 6144) 57.4 us = 1750 TOP/s (2496 is what a library's 8192^3 reaches).  Other waves for that tile at the same
 // sizes: 2 x 2 of 64 x 128 33 and 69 us, 1 x 4 of 128 x 64 32 and 68, 4 x 2 of 32 x 64 (128 x 128) 30 and 70.
 template <int WM, int WN, int TM, int TN>
@@ -249,7 +249,10 @@ int8_tile_kernel(Int8Args a, int tiles_m, int tiles) {
     constexpr int kBuf = (BM + BN) * kStage;     // bytes of a stage: weights, then x
     constexpr int kOutPitch = BN * 2 + 16;       // bytes of a result row
     constexpr int kOut = BM * kOutPitch;
-    __shared__ __attribute__((aligned(16))) char lds[3 * kBuf > kOut ? 3 * kBuf : kOut];
+    constexpr int kScales = 3 * kBuf > kOut ? 3 * kBuf : kOut;  // behind the buffers: the tile's scales, there when the sums are
+    // one array: with a second one the compiler waits for every load in flight before it reads LDS (57 us become 87)
+    __shared__ __attribute__((aligned(16))) char lds[kScales + 4 * (BM + BN)];
+    float *const s_w = reinterpret_cast<float *>(lds + kScales), *const s_x = s_w + BN;
     // XCD b % 8 takes tiles (b % 8) per ..: neighbours in m share their weights in one L2
     const int per = (tiles + 7) / 8;
     const int t = static_cast<int>(blockIdx.x % 8) * per + static_cast<int>(blockIdx.x / 8);
@@ -258,6 +261,8 @@ int8_tile_kernel(Int8Args a, int tiles_m, int tiles) {
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int r32 = lane & 31, half = lane >> 5;
     const int wm = wave / WN, wn = wave % WN;
+    for (int i = threadIdx.x; i < BN; i += T) s_w[i] = n0 + i < a.N ? a.sw[n0 + i] : 0.f;
+    for (int i = threadIdx.x; i < BM; i += T) s_x[i] = m0 + i < a.M ? a.sx[m0 + i] : 0.f;
 
     // load v writes rows 8 (wave V + v) .. + 7 of a stage, lane l place l % 8 of row l / 8
     const int8_t *from[V];
@@ -348,18 +353,16 @@ int8_tile_kernel(Int8Args a, int tiles_m, int tiles) {
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
         const int r = (wm * TM + m) * 32 + r32;
-        const float sx = m0 + r < a.M ? a.sx[m0 + r] : 0.f;
+        const float sx = s_x[r];
 #pragma unroll
         for (int n = 0; n < TN; ++n)
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const int c = (wn * TN + n) * 32 + 2 * i + 4 * half;
-                float sw[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sw[e] = n0 + c + e < a.N ? a.sw[n0 + c + e] : 0.f;
+                const float4 sw = *reinterpret_cast<const float4 *>(s_w + c);
                 *reinterpret_cast<uint2 *>(lds + r * kOutPitch + 2 * c) =
-                    make_uint2(pack2_bf16(scaled(acc[m][n][i], sx, sw[0]), scaled(acc[m][n][i + 1], sx, sw[1])),
-                               pack2_bf16(scaled(acc[m][n][i + 2], sx, sw[2]), scaled(acc[m][n][i + 3], sx, sw[3])));
+                    make_uint2(pack2_bf16(scaled(acc[m][n][i], sx, sw.x), scaled(acc[m][n][i + 1], sx, sw.y)),
+                               pack2_bf16(scaled(acc[m][n][i + 2], sx, sw.z), scaled(acc[m][n][i + 3], sx, sw.w)));
             }
     }
     __syncthreads();
@@ -426,7 +429,7 @@ extern "C" int nq_linear_int8(const int8_t *xq, int64_t x_s0, const float *sx, c
     //   M 64  N 4096:  64-row pieces 5.5, 32-row pieces 6.6, 64 x 64 tiles 8.4;   N 6144: 9.8, 9.4, 8.4
     //   M 32  N 6144:  32-row pieces 6.8, 64 x 64 tiles 8.2;                      N 12288: 10.0, 8.4
     //   M 256 N 4096:  64 x 64 tiles 9.1, 64 x 128 9.6, 128 x 256 19;             N 6144: 11.0, 10.1, 20
-    //   M 640 N 6144:  64 x 128 tiles 15.8, 128 x 256 21.0;                       N 12288: 28.0, 24.4
+    //   M 640 N 6144:  64 x 128 tiles 15.8, 128 x 256 21.0;                       N 12288: 28.0, 24.4 (22.9 since)
     auto count = [&](int bm, int bn) { return static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
     auto rounds = [](int64_t tiles) { return (tiles + 255) / 256; };
     if (M <= 16) launch_rows<1>(a, st);

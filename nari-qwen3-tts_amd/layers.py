@@ -777,7 +777,7 @@ def linear_int8(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, w
                 out: torch.Tensor | None = None) -> torch.Tensor:
     """out[m, n] = bf16(sum_k q[m, k] weight_q[n, k] * scales[m] * weight_scales[n]) for int8 codes [rows, in] and
     [out, in] with the scales of ``quantize_int8_rows``; the sum is exact (int32), so the same codes give the
-    same bits at any number of rows.  ``in`` a multiple of 16 up to 131072, any rows and out."""
+    same bits at any number of rows.  ``in`` a multiple of 16 up to 131072 (codes within +-127), any rows and out."""
 
     if q.dtype is not torch.int8 or weight_q.dtype is not torch.int8:
         raise TypeError("the int8 projection needs int8 codes")
