@@ -425,13 +425,17 @@ def paged_cache_read_int8(layer_cache: torch.Tensor, layer_scales: torch.Tensor,
     heads, d, cache = _int8_cache(layer_cache, layer_scales)
     tokens = _int8_slots(pages, offsets)
     shape = (tokens, heads, d)
-    # sizes as numbers parse faster than as a tuple
-    key = torch.empty(tokens, heads, d, dtype=torch.bfloat16, device=layer_cache.device) if key is None else key
-    value = torch.empty(tokens, heads, d, dtype=torch.bfloat16, device=layer_cache.device) if value is None else value
-    target = _int8_heads(key, shape) + _int8_heads(value, shape)
+    target = []
+    for given in (key, value):
+        if given is None:  # sizes as numbers parse faster than as a tuple
+            t = torch.empty(tokens, heads, d, dtype=torch.bfloat16, device=layer_cache.device)
+            target.append((t, (t.data_ptr(), heads * d, d)))
+        else:
+            target.append((given, _int8_heads(given, shape)))
+    (key, key_args), (value, value_args) = target
     _lib.launch(
         _lib.one_device(layer_cache, layer_scales, pages, offsets, key, value, status), "nq_kv_int8_read", *cache,
-        pages.data_ptr(), offsets.data_ptr(), tokens, heads, d, *target, _int8_status(status),
+        pages.data_ptr(), offsets.data_ptr(), tokens, heads, d, *key_args, *value_args, _int8_status(status),
     )
     return key, value
 
@@ -468,11 +472,9 @@ def paged_attention_int8(query: torch.Tensor, layer_cache: torch.Tensor, layer_s
     tokens, hq, q_dim = shape
     if q_dim != d or hq < hkv or hq % hkv:
         raise ValueError("query and cache disagree on the heads")
-    out = torch.empty(tokens, hq, d, dtype=query.dtype, device=query.device) if out is None else out
-    if query.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16:
+    if query.dtype is not torch.bfloat16 or (out is not None and out.dtype is not torch.bfloat16):
         raise TypeError("HIP attention kernels take bf16 tensors")
-    o_strides = out.stride()
-    if out.shape != shape or o_strides[2] != 1:
+    if out is not None and (out.shape != shape or out.stride(2) != 1):
         raise ValueError("out must be [tokens, Hq, D] like the query")
     qo, kv, ids, last = (metadata.qo_indptr, metadata.paged_kv_indptr, metadata.paged_kv_indices,
                          metadata.paged_kv_last_page_len)
@@ -490,6 +492,8 @@ def paged_attention_int8(query: torch.Tensor, layer_cache: torch.Tensor, layer_s
     if qo is None and (parts != _lib.NQ_ATTN_DECODE or rows > tokens):
         raise ValueError("without qo_indptr every row has one query and only NQ_ATTN_DECODE runs")
     index = _lib.one_device(query, layer_cache, layer_scales, out, qo, kv, ids, last, status, workspace)
+    o_strides = (hq * d, d) if out is None else out.stride()
+    out = torch.empty(tokens, hq, d, dtype=torch.bfloat16, device=query.device) if out is None else out
     if tokens == 0 or rows == 0:
         return out
     need = paged_attention_int8_workspace_bytes(tokens, rows, hq, hkv, d, parts)

@@ -761,15 +761,23 @@ def quantize_int8_rows(x: torch.Tensor, q: torch.Tensor | None = None,
     rows, k = shape
     if k < 16 or k % 16:
         raise ValueError("int8 row quantization needs a multiple of 16 columns")
-    q = torch.empty(rows, k, dtype=torch.int8, device=x.device) if q is None else q  # sizes as numbers parse faster
-    scales = torch.empty(rows, dtype=torch.float32, device=x.device) if scales is None else scales
-    if q.dtype is not torch.int8 or scales.dtype is not torch.float32:
-        raise TypeError("int8 codes and float32 scales expected")
-    q_strides = q.stride()
-    if q.shape != shape or q_strides[1] != 1 or scales.shape != (rows,) or not scales.is_contiguous():
-        raise ValueError(f"codes must be [{rows}, {k}] with unit inner stride and scales [{rows}], contiguous")
+    q_row = k
+    if q is None:
+        q = torch.empty(rows, k, dtype=torch.int8, device=x.device)  # sizes as numbers parse faster than as a tuple
+    elif q.dtype is not torch.int8:
+        raise TypeError("int8 codes expected")
+    elif q.shape != shape or q.stride(1) != 1:
+        raise ValueError(f"codes must be [{rows}, {k}] with unit inner stride")
+    else:
+        q_row = q.stride(0)
+    if scales is None:
+        scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+    elif scales.dtype is not torch.float32:
+        raise TypeError("float32 scales expected")
+    elif scales.shape != (rows,) or not scales.is_contiguous():
+        raise ValueError(f"scales must be [{rows}], contiguous")
     _lib.launch(_lib.one_device(x, q, scales), "nq_quantize_int8_rows", x.data_ptr(), strides[0], rows, k,
-                q.data_ptr(), q_strides[0], scales.data_ptr())
+                q.data_ptr(), q_row, scales.data_ptr())
     return q, scales
 
 
@@ -792,13 +800,16 @@ def linear_int8(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, w
     if scales.shape != (rows,) or weight_scales.shape != (n,) or not (
             scales.is_contiguous() and weight_scales.is_contiguous()):
         raise ValueError("int8 scales must be contiguous, one per row and one per output")
-    out = torch.empty(rows, n, dtype=torch.bfloat16, device=q.device) if out is None else out
-    o_strides = out.stride()
-    if out.dtype is not torch.bfloat16 or out.shape != (rows, n) or o_strides[1] != 1:
+    o_row = n
+    if out is None:
+        out = torch.empty(rows, n, dtype=torch.bfloat16, device=q.device)
+    elif out.dtype is not torch.bfloat16 or out.shape != (rows, n) or out.stride(1) != 1:
         raise ValueError(f"out must be bf16 [{rows}, {n}] with unit inner stride")
+    else:
+        o_row = out.stride(0)
     _lib.launch(_lib.one_device(q, scales, weight_q, weight_scales, out), "nq_linear_int8", q.data_ptr(),
                 q_strides[0], scales.data_ptr(), weight_q.data_ptr(), w_strides[0], weight_scales.data_ptr(), rows, n,
-                k, out.data_ptr(), o_strides[0])
+                k, out.data_ptr(), o_row)
     return out
 
 
