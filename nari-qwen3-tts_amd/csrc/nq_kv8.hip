@@ -663,44 +663,57 @@ kv8_merge_kernel(Attend8 a, int waves, const float2 *__restrict__ part_ml, const
 }
 
 // Rows of several queries.  A workgroup of NW waves takes 32 NW columns (queries times the G query heads of one kv
-// head) against 64-key tiles, a wave 32 columns with mfma_32x32x16: S^T = K Q^T, out^T = V^T P^T, so a column's
-// scores, maximum and output stay in two lanes and P needs no exchange.  K and V are widened to bf16, times their
-// scales, once a workgroup on their way to LDS (V transposed, keys in the order in which a lane holds P); a
+// head) against 32-key tiles, a wave 32 columns with mfma_32x32x16: S^T = K Q^T, out^T = V^T P^T, so a column's
+// scores, maximum and output stay in two lanes and P needs no exchange.  K and V are widened to bf16, V times its
+// scale, once a workgroup on their way to LDS (V transposed, keys in the order in which a lane holds P); a
 // tile's loads are in flight while the one before it is multiplied.  Sums are rescaled only when a maximum has grown
 // by more than 2^8 (P stays below that, and bf16 and fp32 lose nothing by it).  With few tiles the key range is
 // cut into pieces, joined by kv8_join_kernel.
-// 1856 queries of 16 heads over 6001 keys (77 GFLOP): 118.8 us and 9.2 for the join, 600 TFLOP/s.  A tile takes 2.3 us: 0.97
-// us of MFMAs (two waves a SIMD), 1.2 of vector instructions (32 exponentials, 64 for the staging and 160 others a
-// wave), 1.2 of LDS (278 KB read, 34 KB written a workgroup) and the barrier, which overlap in part only; without
-// the staging 101 us, without the operand reads 106, without the exponentials 112, without all three 85.  With
-// uniform pieces the longest one takes 47 tiles where 39 is the mean.  Tried and no faster: operands read three MFMAs
-// ahead with the barrier inside the step (spills, +-3 %), 64 columns a wave at one wave a SIMD (201 us, moves between the
-// register files), spans that cross tiles for even work (126 us and 17 for the join).
-constexpr int kKeys = 64;
+constexpr int kKeys = 32;
 constexpr float kLag = 8.0f;
 
 struct Tile8 {
     int q0, n_q, limit0;  // first query token, queries, keys the first of them sees
     int n_keys;           // keys the last of them sees
 };
-// Slot s of the launch is tile s - (qo_indptr[r] / nq + r) of row r: those bases need no scan, and a row's
-// share is enough for its tiles.  False where the slot is no tile of this launch.
+// The launch's tiles, counted from the last one of the last row (a row's last tile sees the most keys) down to the first of
+// row 0; found by the whole wave, which sums the rows' tiles 64 at a time.  So workgroups without a tile come
+// last: between the others they would hold back the ones behind them, 51 us instead of 35 for 16 rows of 256 queries.
 template <typename R>
-__device__ __forceinline__ bool tile_of(const Attend8 &a, const R &rows, int nq, int slot, int skip_single, Row8 &row,
+__device__ __forceinline__ bool tile_of(const Attend8 &a, const R &rows, int nq, int index, int skip_single, Row8 &row,
                                         Tile8 &t) {
-    const int r = wave_find_le(a.rows, slot, [&](int i) { return rows.qo(i) / nq + i; });
-    row = row_of(a, rows, r);
-    const int first = (slot - (row.q0 / nq + r)) * nq;
-    if (first < 0 || first >= row.q_len || (skip_single && row.q_len == 1)) return false;
-    t.q0 = row.q0 + first;
-    t.n_q = row.q_len - first < nq ? row.q_len - first : nq;
-    t.limit0 = row.kv_len - row.q_len + first + 1;
-    const int last = t.limit0 + t.n_q - 1;
-    t.n_keys = last < 0 ? 0 : last;
-    return true;
+    const int lane = threadIdx.x & (kWave - 1);
+    int before = 0;
+    for (int top = a.rows - 1; top >= 0; top -= kWave) {
+        const int r = top - lane;
+        int n = 0;
+        if (r >= 0) {
+            const int q0 = rows.qo(r), len = rows.qo(r + 1) - q0;
+            const bool mine = q0 >= 0 && len > 0 && q0 <= a.tokens - len && !(skip_single && len == 1);
+            n = mine ? (len + nq - 1) / nq : 0;
+        }
+        for (int d = 1; d < kWave && d < a.rows; d *= 2) {  // lanes behind row 0 hold none
+            const int x = __shfl_up(n, d, kWave);
+            if (lane >= d) n += x;
+        }
+        const uint64_t past = __ballot(before + n > index);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            row = row_of(a, rows, top - at);
+            const int first = (before + __builtin_amdgcn_readlane(n, at) - 1 - index) * nq;
+            t.q0 = row.q0 + first;
+            t.n_q = row.q_len - first < nq ? row.q_len - first : nq;
+            t.limit0 = row.kv_len - row.q_len + first + 1;
+            const int last = t.limit0 + t.n_q - 1;
+            t.n_keys = last < 0 ? 0 : last;
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(n, kWave - 1);
+    }
+    return false;
 }
 __device__ __forceinline__ int pieces_of(const Tile8 &t, int splits) {
-    const int n = (t.n_keys + kKeys - 1) / kKeys / 2;  // at least two key tiles a piece
+    const int n = (t.n_keys + kKeys - 1) / kKeys / 4;  // at least four key tiles a piece
     return n < 1 ? 1 : (n < splits ? n : splits);
 }
 
@@ -708,35 +721,34 @@ template <int D>
 struct Smem8 {
     u32x4 k[2][kKeys * (D / 8 + 1)];
     u32x4 v[2][D * (kKeys / 8)];
-    floatx4_t ks[2];               // K scales of the tile's blocks times sm_scale log2(e), 1 where one is not finite
-    i32x4_t odd[2];                // kAbsent: the block's page is not in the pool; kPoison: a scale is not finite
+    float ks[2][kKeys / kBlk];     // K scales of the tile's blocks times sm_scale log2(e), 1 where one is not finite
+    int odd[2][kKeys / kBlk];      // kAbsent: the block's page is not in the pool; kPoison: a scale is not finite
     Meta8 meta;
 };
 constexpr int kAbsent = 1, kPoison = 2;
-// Places of 16-byte chunks: rows of K one chunk longer than their values, V's chunks exclusive-ored with their row.
-// Measured free of conflicts for the operand reads (32 rows, two chunks each) and K's writes; V's 8-byte writes take half as
-// long again as without any.
+// Places of 16-byte chunks, free of conflicts for the operand reads (32 rows, two chunks each): rows of K one chunk longer
+// than their values, V's chunks exclusive-ored with bits of their row.
 template <int D>
 __device__ __forceinline__ int k_chunk(int key, int chunk) {
     return key * (D / 8 + 1) + chunk;
 }
-__device__ __forceinline__ int v_chunk(int d, int chunk) { return d * (kKeys / 8) + (chunk ^ ((d ^ (d >> 3)) & 7)); }
+__device__ __forceinline__ int v_chunk(int d, int chunk) { return d * (kKeys / 8) + (chunk ^ ((d >> 2) & 3)); }
 
 template <int D, int NW>
 __global__ void __launch_bounds__(NW * kWave, 2)
-kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single, float2 *__restrict__ part_ml,
+kv8_prefill_kernel(Attend8 a, Pool8 pool, int splits, int skip_single, float2 *__restrict__ part_ml,
                    float *__restrict__ part_o) {
-    constexpr int T = NW * kWave, COLS = 32 * NW;
+    constexpr int T = NW * kWave, COLS = 32 * NW, NB = kKeys / kBlk;
     // K: a thread stages KP pieces of eight values of one key; V: VB values of each of four keys
     constexpr int KT = T / kKeys, KP = D / 8 / KT;  // KT threads a key
-    constexpr int VB = kKeys * D / 4 / T;           // 2, 4 or 8
-    static_assert(KP >= 1 && KP * KT * 8 == D && VB >= 2 && VB <= 8, "a tile stages evenly");
-    __shared__ Smem8<D> sm;
+    constexpr int VB = kKeys * D / 4 / T;           // 2 or 4
+    static_assert(KP >= 1 && KP * KT * 8 == D && (VB == 2 || VB == 4), "a tile stages evenly");
+    using Smem = Smem8<D>;
+    __shared__ Smem sm;
     load_meta(a, sm.meta);
     const Rows8 rows{a, sm.meta};
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int head = blockIdx.x % a.heads;
-    const int slot = slots - 1 - static_cast<int>(blockIdx.x) / a.heads;  // the longest key ranges first
+    const int head = blockIdx.x % a.heads, slot = static_cast<int>(blockIdx.x) / a.heads;
     Row8 row;
     Tile8 t;
     if (!tile_of(a, rows, COLS / a.group, slot, skip_single, row, t)) return;
@@ -744,10 +756,11 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
     const int piece = blockIdx.y;
     if (piece >= pieces) return;
     const int n_kt = (t.n_keys + kKeys - 1) / kKeys;
-    const int kt0 = n_kt * piece / pieces, kt1 = n_kt * (piece + 1) / pieces;
+    const int kt0 = static_cast<int>(static_cast<int64_t>(n_kt) * piece / pieces),
+              kt1 = static_cast<int>(static_cast<int64_t>(n_kt) * (piece + 1) / pieces);
 
     constexpr int kBufK = 16 * kKeys * (D / 8 + 1), kBufV = 16 * D * (kKeys / 8);
-    // staging: a wave holds 64 / NW keys of one block, so its page, its scales and their addresses are uniform
+    // staging: a wave holds 32 / NW keys of one block, so its page, its scales and their addresses are uniform
     const int sk_key = threadIdx.x / KT, sk_piece = threadIdx.x % KT;
     constexpr int VT = T / (kKeys / 4);  // threads of a quad of keys
     const int sv_quad = threadIdx.x / VT, sv_part = threadIdx.x % VT;
@@ -762,41 +775,44 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
     const int in_page = (1 << a.bpp_log2) - 1;
     // Pages and scales are uniform, but fetched as vectors: a scalar load outstanding would make every wait for an LDS
     // read in the loop a wait for that load too.
-    int zero = 0;
+    uint32_t zero = 0;
     asm volatile("" : "+v"(zero));
     // the wave's block of tile kt, held to the row's: what lies beyond its keys is masked, a tile beyond the last never used
     auto block_of = [&](int kt) __attribute__((always_inline)) {
-        const int blk = kt * (kKeys / kBlk) + uwave * (kKeys / kBlk) / NW;
+        const int blk = kt * NB + uwave * NB / NW;
         return blk < n_blocks ? blk : n_blocks - 1;
     };
     auto page_of = [&](int kt) __attribute__((always_inline)) {
-        return a.kv_indices[row.first_page + (block_of(kt) >> a.bpp_log2) + zero];
+        return (a.kv_indices + row.first_page + (block_of(kt) >> a.bpp_log2))[zero];
     };
     // The staging registers: K of one tile and V of the tile before it, with what their block needs.
     struct Stage {
-        u32x2 k[KP], v[4];
-        float ks, vs, v_vs;  // scales of K's block, V scale of V's
-        bool on;             // K's page is in the pool
+        u32x2 k[KP];
+        uint32_t v[4];
+        float ks, vs, next_vs, v_vs;  // scales of K's block, V scales of the block before it and of V's
+        bool on;                      // K's page is in the pool
     };
-    const int8_t *v_from = base;  // V of the tile whose K was asked for last
-    auto load = [&](int kt, int found, bool with_v, float v_vs, Stage &r) __attribute__((always_inline)) {
-        if (with_v) {
+    const int8_t *v_from = base, *v_next = base;  // V of the tile whose K was asked for last, and of the one before
+    auto load_v = [&](Stage &r) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int8_t *p = v_from + (v_off + e * c_slot);
-                if constexpr (VB == 8) r.v[e] = *reinterpret_cast<const u32x2 *>(p);
-                else if constexpr (VB == 4) r.v[e].x = *reinterpret_cast<const uint32_t *>(p);
-                else r.v[e].x = *reinterpret_cast<const uint16_t *>(p);
-            }
-            r.v_vs = v_vs;
+        for (int e = 0; e < 4; ++e) {
+            const int8_t *p = v_next + static_cast<uint32_t>(v_off + e * c_slot);
+            if constexpr (VB == 4) r.v[e] = *reinterpret_cast<const uint32_t *>(p);
+            else r.v[e] = *reinterpret_cast<const uint16_t *>(p);
         }
+        r.v_vs = r.next_vs;
+    };
+    auto load_k = [&](int kt, int found, Stage &r) __attribute__((always_inline)) {
+        v_next = v_from;
+        r.next_vs = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(r.vs)));
         const int page = __builtin_amdgcn_readfirstlane(found);
         r.on = page >= 0 && page < pool.num_pages;
         const int64_t pid = r.on ? page : 0;
         const int blk = block_of(kt) & in_page;
         const int8_t *kp = base + pid * pool.c_page + blk * (kBlk * pool.c_slot);
 #pragma unroll
-        for (int e = 0; e < KP; ++e) r.k[e] = *reinterpret_cast<const u32x2 *>(kp + (k_off + 8 * KT * e));
+        for (int e = 0; e < KP; ++e)
+            r.k[e] = *reinterpret_cast<const u32x2 *>(kp + static_cast<uint32_t>(k_off) + 8 * KT * e);
         const float *sc = s_base + pid * pool.s_page + blk * pool.s_block;
         r.ks = sc[zero];
         r.vs = (sc + pool.s_kind)[zero];
@@ -804,34 +820,27 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
     };
     // First places of what a thread stages.  Key 8 a + 4 b + i of a block sits at position 8 b + 4 a + i of V's rows.
     char *stage = reinterpret_cast<char *>(&sm);
-    const int put_k0 = static_cast<int>(offsetof(Smem8<D>, k)) + 16 * k_chunk<D>(sk_key, sk_piece);
-    const int put_v0 = static_cast<int>(offsetof(Smem8<D>, v)) +
+    const int put_k0 = static_cast<int>(offsetof(Smem, k)) + 16 * k_chunk<D>(sk_key, sk_piece);
+    const int put_v0 = static_cast<int>(offsetof(Smem, v)) +
                        16 * v_chunk(sv_part * VB, 2 * (sv_quad / 4) + (quad & 1)) + 8 * (quad >> 1);
-    auto wide_k = [&](const Stage &r, int piece) __attribute__((always_inline)) {
-        return widen8(r.k[piece].x, r.k[piece].y);
+    auto put_k = [&](const Stage &r, int e, int buf) __attribute__((always_inline)) {
+        *reinterpret_cast<bf16x8_t *>(stage + put_k0 + 16 * KT * e + buf * kBufK) = widen8(r.k[e].x, r.k[e].y);
     };
-    auto wide_v = [&](const Stage &r, int col) __attribute__((always_inline)) {
-        const float vs = fabsf(r.v_vs) < __builtin_inff() ? r.v_vs : 0.f;
-        const int w = col / 4, j = col % 4;
-        return u32x2{pack2_bf16(byte_of(r.v[0][w], j) * vs, byte_of(r.v[1][w], j) * vs),
-                     pack2_bf16(byte_of(r.v[2][w], j) * vs, byte_of(r.v[3][w], j) * vs)};
-    };
-    auto put_k = [&](const Stage &r, const bf16x8_t (&x)[KP], int buf) __attribute__((always_inline)) {
-#pragma unroll
-        for (int e = 0; e < KP; ++e) *reinterpret_cast<bf16x8_t *>(stage + put_k0 + 16 * KT * e + buf * kBufK) = x[e];
+    auto put_scales = [&](const Stage &r, int buf) __attribute__((always_inline)) {
         // A scale that is not finite, K's or V's, answers through the scores of the queries that see the block, not
         // through 0 * NaN in those that do not.
         const bool fine = fabsf(r.ks) < __builtin_inff() && fabsf(r.vs) < __builtin_inff();
-        const int blk = uwave * (kKeys / kBlk) / NW;
+        const int blk = uwave * NB / NW;
         // above zero, also for a block that was never written: a masked score, minus infinity, stays that
         sm.ks[buf][blk] = r.on && fine ? fmaxf(r.ks * a.scale, kMinScale) : 1.0f;
         sm.odd[buf][blk] = !r.on ? kAbsent : fine ? 0 : kPoison;
     };
-    auto put_v = [&](const u32x2 (&x)[VB], int buf) __attribute__((always_inline)) {
-        // value VB part + col, col < VB, a power of two up to 8: its row's exclusive-or is the first's xor col
-#pragma unroll
-        for (int col = 0; col < VB; ++col)
-            *reinterpret_cast<u32x2 *>(stage + ((put_v0 + buf * kBufV) ^ (16 * col)) + 16 * (kKeys / 8) * col) = x[col];
+    auto put_v = [&](const Stage &r, int col, int buf) __attribute__((always_inline)) {
+        const float vs = fabsf(r.v_vs) < __builtin_inff() ? r.v_vs : 0.f;
+        // value VB part + col: the same bits 2 and 3 of the row as part's first
+        *reinterpret_cast<u32x2 *>(stage + put_v0 + buf * kBufV + 16 * (kKeys / 8) * col) =
+            u32x2{pack2_bf16(byte_of(r.v[0], col) * vs, byte_of(r.v[1], col) * vs),
+                  pack2_bf16(byte_of(r.v[2], col) * vs, byte_of(r.v[3], col) * vs)};
     };
     int found0 = 0, found1 = 0;
     if (kt0 < kt1) {
@@ -850,18 +859,12 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
         qf[s] = load_q(a.q + (t.q0 + qi) * a.q_s0 + (head * a.group + g) * a.q_s1 + 16 * s + 8 * half, live, a.flip);
 
     // Where the lane reads, in bytes: chunk half of K row c and of V row c.  The other operands are constants away, V's
-    // after an exclusive-or of the chunk (row c + 32 j flips its bit 2 where j is odd).
+    // after an exclusive-or of the chunk (rows 32 j on keep it).
     const char *lds = reinterpret_cast<const char *>(&sm);
-    const int at_k = static_cast<int>(offsetof(Smem8<D>, k)) + 16 * k_chunk<D>(c, half);
-    const int at_v = static_cast<int>(offsetof(Smem8<D>, v)) + 16 * v_chunk(c, half);
+    const int at_k = static_cast<int>(offsetof(Smem, k)) + 16 * k_chunk<D>(c, half);
+    const int at_v = static_cast<int>(offsetof(Smem, v)) + 16 * v_chunk(c, half);
     auto operand = [&](int at) __attribute__((always_inline)) {
         return __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const u32x4 *>(lds + at));
-    };
-    auto k_at = [&](int base, int k, int sub) __attribute__((always_inline)) {
-        return base + 32 * k + 16 * k_chunk<D>(32 * sub, 0);
-    };
-    auto v_at = [&](int base, int k, int j) __attribute__((always_inline)) {
-        return (base ^ (32 * (k ^ (2 * (j & 1))))) + 16 * (kKeys / 8) * 32 * j;
     };
     floatx16_t acc[D / 32];
 #pragma unroll
@@ -870,54 +873,53 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
         for (int i = 0; i < 16; ++i) acc[j][i] = 0.f;
     float m_run = -__builtin_inff(), l_run = 0.f, top = -__builtin_inff();
     bool any = false;  // whether the column has seen a key
-    floatx4_t f_k = {0.f, 0.f, 0.f, 0.f};
+    float f_k[NB] = {};
     Stage st;
 
-    auto scores = [&](int kt, floatx16_t (&s)[2]) __attribute__((always_inline)) {
-        const int base = at_k + (kt & 1) * kBufK;
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[sub][i] = 0.f;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-            for (int sub = 0; sub < 2; ++sub)
-                s[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(k_at(base, k, sub)), qf[k], s[sub], 0, 0, 0);
-    };
     // Keys that a column does not see, in tiles that hold any such key.
-    auto mask = [&](int kt, i32x4_t odd, floatx16_t (&s)[2]) __attribute__((always_inline)) {
+    auto mask = [&](int kt, const int (&odd)[NB], floatx16_t &s) __attribute__((always_inline)) {
         const int key0 = kt * kKeys;
-        const int some = __builtin_amdgcn_readfirstlane(odd[0] | odd[1] | odd[2] | odd[3]);
+        const int some = __builtin_amdgcn_readfirstlane(odd[0] | odd[1]);
         if (key0 + kKeys <= t.limit0 && !some) {
             any = true;
             return;
         }
         if ((some & kAbsent) && a.status) *a.status = NQ_ERR_INVALID_ARGUMENT;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            // the lane's element i: key 32 (i / 16) + 8 (i / 4 % 4) + 4 half + i % 4
-            const bool see = key0 + 32 * (i / 16) + 8 * (i / 4 % 4) + 4 * half + (i & 3) < limit && odd[i / 8] != kAbsent;
+        for (int i = 0; i < 16; ++i) {
+            // the lane's element i: key 8 (i / 4) + 4 half + i % 4
+            const bool see = key0 + 8 * (i / 4) + 4 * half + (i & 3) < limit && odd[i / 8] != kAbsent;
             any |= see;
-            const float v = odd[i / 8] == kPoison ? __builtin_nanf("") : s[i / 16][i % 16];
-            s[i / 16][i % 16] = see ? v : -__builtin_inff();
+            const float v = odd[i / 8] == kPoison ? __builtin_nanf("") : s[i];
+            s[i] = see ? v : -__builtin_inff();
         }
     };
-    // A tile's factors, and the maximum of its scores times them (factors are positive).
-    auto factors = [&](int kt) __attribute__((always_inline)) { return sm.ks[kt & 1]; };
-    auto block_top = [&](const floatx16_t (&s)[2], int k) __attribute__((always_inline)) {
-        float m = s[k / 2][8 * (k % 2)];
+    // A block's largest score; times its factor (positive) it counts for the maximum.
+    auto block_top = [&](const floatx16_t &s, int k) __attribute__((always_inline)) {
+        float m = s[8 * k];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) m = fmaxf(m, s[k / 2][8 * (k % 2) + i]);
+        for (int i = 1; i < 8; ++i) m = fmaxf(m, s[8 * k + i]);
         return m;
     };
     // Tile kt: its scores are in `s` and their maximum in `top`; the next tile's go to `next`.  Two blocks of
-    // independent work each, interleaved two MFMAs at a time (the fences hold the order): the next scores beside
-    // this tile's exponentials, then P V beside the next maximum and the staging of the tiles behind, V one
-    // ahead and K two.
-    constexpr int CH = D / 16, PER = 32 / CH;  // chunks of two MFMAs, score elements beside each
-    auto step = [&](auto last, int kt, floatx16_t (&s)[2], floatx16_t (&next)[2]) __attribute__((always_inline)) {
-        __syncthreads();
+    // independent work each, interleaved chunk by chunk (the fences hold the order): the next scores beside this
+    // tile's exponentials and the staging of K two tiles ahead, then P V beside the next maximum and the staging of V
+    // one tile ahead.  Operands are read AHEAD MFMAs before their own, the next tile's first ones too.  The one barrier
+    // stands between the last read of K of tile kt + 1 and the first of V of tile kt: K of kt + 2 is staged before
+    // it, where K of kt was, last read before the barrier of kt - 1; V of kt + 1 behind it, where V of kt - 1 was.
+    constexpr int NK = D / 16, NV = NB * (D / 32);  // operands of a tile's scores and of its P V
+    constexpr int PER = 16 / NK, STEPS = NK / 2;    // score elements beside each of the first; chunks that stage K
+    constexpr int AHEAD = D == 128 ? 3 : 2;
+    static_assert(NK % 4 == 0 && NV % 4 == 0 && NK - AHEAD >= STEPS, "the ring's places and the barrier's");
+    bf16x8_t ring[4];
+    auto read_k = [&](int n, int buf) __attribute__((always_inline)) {
+        ring[n & 3] = operand(at_k + buf * kBufK + 32 * n);
+    };
+    auto read_v = [&](int n, int base) __attribute__((always_inline)) {
+        ring[n & 3] = operand((base ^ (32 * (n / (D / 32)))) + 16 * (kKeys / 8) * 32 * (n % (D / 32)));
+    };
+    auto step = [&](auto last, auto buf, int kt, floatx16_t &s, floatx16_t &next) __attribute__((always_inline)) {
+        constexpr int B = buf, N = 1 - B;  // tile kt's buffer, the next one's
         if (__any(top > m_run + kLag)) {
             const float m_new = fmaxf(m_run, top);
             const float alpha = m_run == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
@@ -927,133 +929,131 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
             m_run = m_new;
         }
         const float m_use = m_run == -__builtin_inff() ? 0.f : m_run;  // no key yet: 2^(-inf) for all
-        i32x4_t n_odd = {0, 0, 0, 0};
-        floatx4_t n_f = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (!last) {
-            n_odd = sm.odd[(kt + 1) & 1];
-            n_f = factors(kt + 1);
-        }
-        constexpr int JP = D / 64;  // pairs of 32-value rows of V
-        int v_base = at_v + (kt & 1) * kBufV;
+        int v_base = at_v + B * kBufV;
         asm volatile("" : "+v"(v_base));  // places are made from it where they are used, not kept
-        bf16x8_t vf[2][2];
-        auto read_v = [&](int ch) __attribute__((always_inline)) {
-            vf[ch & 1][0] = operand(v_at(v_base, ch / JP, 2 * (ch % JP)));
-            vf[ch & 1][1] = operand(v_at(v_base, ch / JP, 2 * (ch % JP) + 1));
-        };
-        uint32_t pw[16];
+        int n_odd[NB] = {};
+        float n_f[NB] = {};
+        uint32_t pw[8];
         float sum[2] = {0.f, 0.f};
-        {
-            const int base = at_k + ((kt + 1) & 1) * kBufK;
-            bf16x8_t f[2][2];
-            auto read = [&](int k) __attribute__((always_inline)) {
-                f[k & 1][0] = operand(k_at(base, k, 0));
-                f[k & 1][1] = operand(k_at(base, k, 1));
-            };
-            if constexpr (!last) {
-                read(0);
-#pragma unroll
-                for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) next[sub][i] = 0.f;
-            }
-#pragma unroll
-            for (int k = 0; k < CH; ++k) {
-                if constexpr (!last) {
-                    if (k + 1 < CH) read(k + 1);
-#pragma unroll
-                    for (int sub = 0; sub < 2; ++sub)
-                        next[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[k & 1][sub], qf[k], next[sub], 0, 0, 0);
-                }
-#pragma unroll
-                for (int i = PER * k; i < PER * (k + 1); i += 2) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16], f_k[i / 8], -m_use));
-                    const float y = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16 + 1], f_k[i / 8], -m_use));
-                    pw[i / 2] = pack2_bf16(x, y);
-                    float &l = sum[i / 2 % 2];  // of the rounded values, those that meet V
-                    l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pw[i / 2]),
-                                                        __builtin_bit_cast(bf16x2_t, 0x3f803f80u), l, false);
-                    asm volatile("" : "+v"(pw[i / 2]), "+v"(l));  // made here, not where they are used
-                }
-                if (k == CH - 1) read_v(0);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        l_run += sum[0] + sum[1];
         if constexpr (!last) {
-            mask(kt + 1, n_odd, next);
-            f_k = n_f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) next[i] = 0.f;
         }
-        float high = -__builtin_inff();
-        u32x2 xv[VB];
-        bf16x8_t xk[KP];
 #pragma unroll
-        for (int ch = 0; ch < CH; ++ch) {
-            const int k = ch / JP, j = 2 * (ch % JP);
-            if (ch + 1 < CH) read_v(ch + 1);
-            const bf16x8_t pf =
-                __builtin_bit_cast(bf16x8_t, u32x4{pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]});
+        for (int n = 0; n < NK; ++n) {
+            if constexpr (!last)
+                if (n == STEPS - 1) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                acc[j + h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ch & 1][h], pf, acc[j + h], 0, 0, 0);
-            if constexpr (!last) {
-                if (ch % (CH / 4) == 0) high = fmaxf(high, block_top(next, ch / (CH / 4)) * f_k[ch / (CH / 4)]);
-                constexpr int HALF = CH / 2;  // V of tile kt + 1 first, then K of kt + 2 (or of a tile that is never used)
-                if (ch < HALF) {
-#pragma unroll
-                    for (int e = VB * ch / HALF; e < VB * (ch + 1) / HALF; ++e) xv[e] = wide_v(st, e);
-                } else {
-#pragma unroll
-                    for (int e = KP * (ch - HALF) / HALF; e < KP * (ch - HALF + 1) / HALF; ++e) xk[e] = wide_k(st, e);
+                    for (int b = 0; b < NB; ++b) {
+                        n_odd[b] = sm.odd[N][b];
+                        n_f[b] = sm.ks[N][b];
+                    }
                 }
-                if (ch == CH - 1) {  // writes behind the last reads; then the registers are free for the tiles behind
-                    put_v(xv, (kt + 1) & 1);
-                    put_k(st, xk, kt & 1);
-                    load(kt + 3, found0, true, st.vs, st);
+            if (n + AHEAD == NK) __syncthreads();
+            if (n + AHEAD >= NK) read_v(n + AHEAD - NK, v_base);
+            else if constexpr (!last) read_k(n + AHEAD, N);
+            if constexpr (!last) next = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[n & 3], qf[n], next, 0, 0, 0);
+#pragma unroll
+            for (int i = PER * n; i < PER * (n + 1); i += 2) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[i], f_k[i / 8], -m_use));
+                const float y = __builtin_amdgcn_exp2f(fmaf(s[i + 1], f_k[i / 8], -m_use));
+                pw[i / 2] = pack2_bf16(x, y);
+                float &l = sum[i / 2 % 2];
+                l += x + y;
+                asm volatile("" : "+v"(pw[i / 2]), "+v"(l));  // made here, not where they are used
+            }
+            if constexpr (!last) {  // K of tile kt + 2, or of one that is never used
+                if (n < STEPS) {
+#pragma unroll
+                    for (int e = KP * n / STEPS; e < KP * (n + 1) / STEPS; ++e) put_k(st, e, B);
+                }
+                if (n == STEPS - 1) {  // then its registers are free for the tile behind
+                    put_scales(st, B);
+                    load_k(kt + 3, found0, st);
                     found0 = page_of(kt + 4);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        l_run += sum[0] + sum[1];
+        if constexpr (!last) {
+            mask(kt + 1, n_odd, next);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) f_k[b] = n_f[b];
+        }
+        float high = -__builtin_inff();
+#pragma unroll
+        for (int ch = 0; ch < NV / 2; ++ch) {
+#pragma unroll
+            for (int n = 2 * ch; n < 2 * ch + 2; ++n) {
+                if (n + AHEAD < NV) read_v(n + AHEAD, v_base);
+                else if constexpr (!last) read_k(n + AHEAD - NV, B);  // of tile kt + 2
+                const int k = n / (D / 32), j = n % (D / 32);
+                const bf16x8_t pf =
+                    __builtin_bit_cast(bf16x8_t, u32x4{pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]});
+                acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[n & 3], pf, acc[j], 0, 0, 0);
+            }
+            if constexpr (!last) {
+                constexpr int PCH = NV / 2;
+                if (ch % (PCH / NB) == 0) high = fmaxf(high, block_top(next, ch * NB / PCH) * f_k[ch * NB / PCH]);
+#pragma unroll
+                for (int e = VB * ch / PCH; e < VB * (ch + 1) / PCH; ++e) put_v(st, e, N);
+                if (ch == PCH - 1) load_v(st);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if constexpr (!last) top = halves_max(high);
     };
-    floatx16_t s0[2], s1[2];
     if (kt0 < kt1) {
         Stage first;
-        load(kt0, found0, false, 0.f, first);
-        load(kt0 + 1, found1, true, first.vs, st);
+        first.vs = 0.f;
+        load_k(kt0, found0, first);
+        st.vs = first.vs;
+        load_k(kt0 + 1, found1, st);
+        load_v(st);
         found1 = page_of(kt0 + 2);
         found0 = page_of(kt0 + 3);
-        bf16x8_t xk[KP];
 #pragma unroll
-        for (int e = 0; e < KP; ++e) xk[e] = wide_k(first, e);
-        put_k(first, xk, kt0 & 1);
+        for (int e = 0; e < KP; ++e) {
+            put_k(first, e, 0);
+            put_k(st, e, 1);
+        }
+        put_scales(first, 0);
+        put_scales(st, 1);
 #pragma unroll
-        for (int e = 0; e < KP; ++e) xk[e] = wide_k(st, e);
-        put_k(st, xk, (kt0 + 1) & 1);
-        u32x2 xv[VB];
-#pragma unroll
-        for (int e = 0; e < VB; ++e) xv[e] = wide_v(st, e);
-        put_v(xv, kt0 & 1);
-        load(kt0 + 2, found1, true, st.vs, st);
+        for (int e = 0; e < VB; ++e) put_v(st, e, 0);
+        load_k(kt0 + 2, found1, st);
+        load_v(st);
         __syncthreads();
-        scores(kt0, s0);
-        mask(kt0, sm.odd[kt0 & 1], s0);
-        f_k = factors(kt0);
-        top = -__builtin_inff();
+        floatx16_t s0, s1;
 #pragma unroll
-        for (int k = 0; k < kKeys / kBlk; ++k) top = fmaxf(top, block_top(s0, k) * f_k[k]);
+        for (int i = 0; i < 16; ++i) s0[i] = 0.f;
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+            s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(at_k + 32 * n), qf[n], s0, 0, 0, 0);
+        mask(kt0, sm.odd[0], s0);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) f_k[b] = sm.ks[0][b];
+#pragma unroll
+        for (int k = 0; k < NB; ++k) top = fmaxf(top, block_top(s0, k) * f_k[k]);
         top = halves_max(top);
+        __syncthreads();  // the first step stages over the first tile's K
+        if (kt0 + 1 < kt1) {
+#pragma unroll
+            for (int n = 0; n < AHEAD; ++n) read_k(n, 1);
+        }
+        constexpr std::integral_constant<int, 0> b0{};
+        constexpr std::integral_constant<int, 1> b1{};
         int kt = kt0;
         for (; kt + 2 < kt1; kt += 2) {
-            step(std::false_type{}, kt, s0, s1);
-            step(std::false_type{}, kt + 1, s1, s0);
+            step(std::false_type{}, b0, kt, s0, s1);
+            step(std::false_type{}, b1, kt + 1, s1, s0);
         }
         if (kt + 1 < kt1) {
-            step(std::false_type{}, kt, s0, s1);
-            step(std::true_type{}, kt + 1, s1, s0);
+            step(std::false_type{}, b0, kt, s0, s1);
+            step(std::true_type{}, b1, kt + 1, s1, s0);
         } else {
-            step(std::true_type{}, kt, s0, s1);
+            step(std::true_type{}, b0, kt, s0, s1);
         }
     }
     l_run = halves_sum(l_run);
@@ -1088,7 +1088,7 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int slots, int splits, int skip_single
 constexpr int kMaxPieces = 8;
 template <int D>
 __global__ void __launch_bounds__(kKv8Threads)
-kv8_join_kernel(Attend8 a, int cols, int slots, int splits, int skip_single, const float2 *__restrict__ part_ml,
+kv8_join_kernel(Attend8 a, int cols, int splits, int skip_single, const float2 *__restrict__ part_ml,
                 const float *__restrict__ part_o) {
     constexpr int TP = D / 8;
     __shared__ Meta8 meta;
@@ -1145,15 +1145,21 @@ int decode_waves(int heads) {
 struct Prefill8 {
     int waves, cols, slots, splits;
 };
-// Eight waves (a CU holds one such workgroup) where the rows fill their 256 columns on average, else four (two a CU).
+// Four waves, two workgroups a CU: their starts, barriers and ends overlap.  Eight (one a CU) stage each tile half as often
+// per column, which counts where few tiles have long key ranges, of heads of 128: rows of 2000 columns and more that still
+// leave two pieces a workgroup.  Measured with four and eight waves, us, 16 query heads of 128 on 8:
+//   1 row of 1800 queries over 6001 keys 145, 137;  1 of 2000 over 2000 60, 57;  1 of 1000 over 12000 139, 131
+//   1 of 4000 over 4000 128, 148;  4 of 2000 over 2000 116, 137;  64 of 128 over 512 67, 78;  1 of 300 over 300 17.4, 20.3
 // Pieces: as many as fit the CUs at once, up to kMaxPieces.
-Prefill8 prefill_plan(int tokens, int rows, int group, int heads) {
-    Prefill8 p;
-    p.waves = static_cast<int64_t>(tokens) * group >= 256ll * rows ? 8 : 4;
-    p.cols = 32 * p.waves;
-    p.slots = tokens / (p.cols / group) + rows;
-    const int64_t wgs = static_cast<int64_t>(p.slots) * heads, room = p.waves == 8 ? 256 : 512;
-    p.splits = wgs >= room ? 1 : static_cast<int>(room / wgs < kMaxPieces ? room / wgs : kMaxPieces);
+Prefill8 prefill_plan(int tokens, int rows, int group, int heads, int D) {
+    const int64_t columns = static_cast<int64_t>(tokens) * group;
+    auto pieces = [&](int cols, int room) {
+        const int64_t wgs = (columns / cols + (rows + 1) / 2) * heads, n = room / wgs;  // rows' last tiles: half a tile each
+        return static_cast<int>(n < 1 ? 1 : n < kMaxPieces ? n : kMaxPieces);
+    };
+    Prefill8 p = {4, 128, 0, pieces(128, 512)};
+    if (D == 128 && columns >= 2000ll * rows && pieces(256, 256) > 1) p = {8, 256, 0, pieces(256, 256)};
+    p.slots = tokens / (p.cols / group) + rows;  // no batch has more tiles
     return p;
 }
 struct Layout8 {
@@ -1172,7 +1178,7 @@ Layout8 layout8(int tokens, int rows, int qo_heads, int heads, int D, int parts)
         off = up256(off + n * D * 4);
     }
     if (parts & NQ_ATTN_PREFILL) {
-        const Prefill8 p = prefill_plan(tokens, rows, group, heads);
+        const Prefill8 p = prefill_plan(tokens, rows, group, heads, D);
         const int64_t n = p.splits > 1 ? static_cast<int64_t>(p.slots) * heads * p.splits * p.cols : 0;
         L.p_ml = off;
         off = up256(off + n * 8);
@@ -1281,21 +1287,16 @@ int launch_attention8(const Attend8 &a, const Pool8 &pool, int parts, char *ws, 
         hipLaunchKernelGGL((kv8_merge_kernel<D>), dim3(a.rows, a.heads * a.group), dim3(kKv8Threads), 0, st, a, waves, ml, o);
     }
     if (parts & NQ_ATTN_PREFILL) {
-        const Prefill8 p = prefill_plan(a.tokens, a.rows, a.group, a.heads);
+        const Prefill8 p = prefill_plan(a.tokens, a.rows, a.group, a.heads, D);
         const int skip = (parts & NQ_ATTN_DECODE) ? 1 : 0;
         float2 *ml = reinterpret_cast<float2 *>(ws + L.p_ml);
         float *o = reinterpret_cast<float *>(ws + L.p_o);
         const dim3 grid(p.slots * a.heads, p.splits);
-        if (p.waves == 8)
-            hipLaunchKernelGGL((kv8_prefill_kernel<D, 8>), grid, dim3(8 * kWave), 0, st, a, pool, p.slots, p.splits, skip,
-                               ml, o);
-        else
-            hipLaunchKernelGGL((kv8_prefill_kernel<D, 4>), grid, dim3(4 * kWave), 0, st, a, pool, p.slots, p.splits, skip,
-                               ml, o);
+        const auto kernel = p.waves == 4 ? kv8_prefill_kernel<D, 4> : kv8_prefill_kernel<128, 8>;  // eight: D is 128
+        hipLaunchKernelGGL(kernel, grid, dim3(p.waves * kWave), 0, st, a, pool, p.splits, skip, ml, o);
         if (p.splits > 1)
             hipLaunchKernelGGL((kv8_join_kernel<D>), dim3(p.slots * a.heads, p.cols * (D / 8) / kKv8Threads),
-                               dim3(kKv8Threads), 0, st, a, p.cols,
-                               p.slots, p.splits, skip, ml, o);
+                               dim3(kKv8Threads), 0, st, a, p.cols, p.splits, skip, ml, o);
     }
     return NQ_LAUNCH_STATUS();
 }
@@ -1331,7 +1332,7 @@ extern "C" int nq_paged_attention_int8(const int32_t *qo_indptr, const int32_t *
         return NQ_ERR_UNSUPPORTED;
     int bpp = 0;
     while ((kBlk << bpp) < page_size) ++bpp;
-    const Prefill8 p = prefill_plan(tokens, n_rows, num_qo_heads / num_kv_heads, num_kv_heads);
+    const Prefill8 p = prefill_plan(tokens, n_rows, num_qo_heads / num_kv_heads, num_kv_heads, head_dim);
     if (static_cast<int64_t>(p.slots) * num_kv_heads > 0x3fffffff || num_kv_heads > 65535 ||
         (static_cast<int64_t>(num_indices) * page_size) > 0x7fffffffll)
         return NQ_ERR_UNSUPPORTED;
