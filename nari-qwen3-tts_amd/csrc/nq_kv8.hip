@@ -669,6 +669,13 @@ kv8_merge_kernel(Attend8 a, int waves, const float2 *__restrict__ part_ml, const
 // tile's loads are in flight while the one before it is multiplied.  Sums are rescaled only when a maximum has grown
 // by more than 2^8 (P stays below that, and bf16 and fp32 lose nothing by it).  With few tiles the key range is
 // cut into pieces, joined by kv8_join_kernel.
+// 1856 queries of 16 heads over 6001 keys (77 GFLOP): 127 us and 10 for the join, 610 TFLOP/s; 64 rows of 128 queries over
+// 512 keys 67 us.  A step of eight waves takes 1.25 us: 0.49 us of MFMAs (two waves a SIMD), 0.8 of vector instructions,
+// 0.6 of LDS (139 KB read, 17 KB written a workgroup), the loads' issue, and the barrier, which overlap in part only;
+// without the loads it takes 0.17 us less.  With uniform pieces the longest one takes 94 tiles where 79 is the mean.
+// 64-key tiles take 1 to 10 % less where one long prompt fills the card and up to 1.6 times as long for batches
+// (registers spill, one workgroup a CU).  Tried and no faster: 64 columns a wave at one wave a SIMD (156 us), spans that
+// cross tiles for even work (143 us), staging two steps ahead.
 constexpr int kKeys = 32;
 constexpr float kLag = 8.0f;
 
@@ -760,14 +767,13 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int splits, int skip_single, float2 *_
               kt1 = static_cast<int>(static_cast<int64_t>(n_kt) * (piece + 1) / pieces);
 
     constexpr int kBufK = 16 * kKeys * (D / 8 + 1), kBufV = 16 * D * (kKeys / 8);
-    // staging: a wave holds 32 / NW keys of one block, so its page, its scales and their addresses are uniform
-    const int sk_key = threadIdx.x / KT, sk_piece = threadIdx.x % KT;
-    constexpr int VT = T / (kKeys / 4);  // threads of a quad of keys
-    const int sv_quad = threadIdx.x / VT, sv_part = threadIdx.x % VT;
+    // Staging: a wave holds keys of one block, so its page, its scales and their addresses are uniform: 32 / NW keys of K;
+    // of V the four quads of keys and 16 VB values, so that its writes (eight bytes a row of V and quad) spread over the banks.
     const int uwave = __builtin_amdgcn_readfirstlane(wave);
+    const int sk_key = threadIdx.x / KT, sk_piece = threadIdx.x % KT;
+    const int quad = lane >> 4, sv_part = uwave % (NW / NB) * 16 + (lane & 15);
     const int c_slot = static_cast<int>(pool.c_slot);
     const int k_off = sk_key % kBlk * c_slot + 8 * sk_piece;
-    const int quad = sv_quad & 3;
     const int v_off = 4 * quad * c_slot + VB * sv_part;
     const int8_t *base = pool.codes + head * pool.c_head;
     const float *s_base = pool.scales + head * pool.s_head;
@@ -822,7 +828,7 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int splits, int skip_single, float2 *_
     char *stage = reinterpret_cast<char *>(&sm);
     const int put_k0 = static_cast<int>(offsetof(Smem, k)) + 16 * k_chunk<D>(sk_key, sk_piece);
     const int put_v0 = static_cast<int>(offsetof(Smem, v)) +
-                       16 * v_chunk(sv_part * VB, 2 * (sv_quad / 4) + (quad & 1)) + 8 * (quad >> 1);
+                       16 * v_chunk(sv_part * VB, 2 * (uwave * NB / NW) + (quad & 1)) + 8 * (quad >> 1);
     auto put_k = [&](const Stage &r, int e, int buf) __attribute__((always_inline)) {
         *reinterpret_cast<bf16x8_t *>(stage + put_k0 + 16 * KT * e + buf * kBufK) = widen8(r.k[e].x, r.k[e].y);
     };
@@ -837,10 +843,16 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int splits, int skip_single, float2 *_
     };
     auto put_v = [&](const Stage &r, int col, int buf) __attribute__((always_inline)) {
         const float vs = fabsf(r.v_vs) < __builtin_inff() ? r.v_vs : 0.f;
+        uint32_t x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[e] = r.v[e];
+            asm("" : "+v"(x[e]));  // any 32 bits: one conversion picks a byte, where 16 known ones are shifted first
+        }
         // value VB part + col: the same bits 2 and 3 of the row as part's first
         *reinterpret_cast<u32x2 *>(stage + put_v0 + buf * kBufV + 16 * (kKeys / 8) * col) =
-            u32x2{pack2_bf16(byte_of(r.v[0], col) * vs, byte_of(r.v[1], col) * vs),
-                  pack2_bf16(byte_of(r.v[2], col) * vs, byte_of(r.v[3], col) * vs)};
+            u32x2{pack2_bf16(byte_of(x[0], col) * vs, byte_of(x[1], col) * vs),
+                  pack2_bf16(byte_of(x[2], col) * vs, byte_of(x[3], col) * vs)};
     };
     int found0 = 0, found1 = 0;
     if (kt0 < kt1) {
