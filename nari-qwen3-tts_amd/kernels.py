@@ -341,6 +341,7 @@ def paged_attention_noalloc(query: torch.Tensor, layer_cache: torch.Tensor, meta
 
 
 INT8_BLOCK = 16  # cache slots that share a scale
+_INT8_SLOTS = 0x7FFF0000  # slots that a call's page list may name
 
 
 def _int8_cache(layer_cache: torch.Tensor, layer_scales: torch.Tensor) -> tuple:
@@ -457,7 +458,8 @@ def paged_attention_int8(query: torch.Tensor, layer_cache: torch.Tensor, layer_s
                          out: torch.Tensor | None = None) -> torch.Tensor:
     """Paged attention of ``query`` [tokens, Hq, D] (bf16) over one layer of the 8-bit cache (see
     ``paged_cache_write_int8_``) with ``metadata`` (a TalkerAttentionMetadata; its qo_indptr, paged_kv_indptr,
-    paged_kv_indices and paged_kv_last_page_len are read), without a plan.
+    paged_kv_indices and paged_kv_last_page_len are read), without a plan.  A captured call may be replayed with whatever
+    the planner has written since: a paged_kv_indices that is the first part of a buffer stands for the whole buffer.
 
     ``parts`` as ``paged_attention_noalloc`` takes them: NQ_ATTN_DECODE for the rows with one query,
     NQ_ATTN_PREFILL for those with several (alone: for all of them); both by default, NQ_ATTN_DECODE where the
@@ -492,6 +494,12 @@ def paged_attention_int8(query: torch.Tensor, layer_cache: torch.Tensor, layer_s
     if qo is None and (parts != _lib.NQ_ATTN_DECODE or rows > tokens):
         raise ValueError("without qo_indptr every row has one query and only NQ_ATTN_DECODE runs")
     index = _lib.one_device(query, layer_cache, layer_scales, out, qo, kv, ids, last, status, workspace)
+    # paged_kv_indptr says which entries count.  A planner's paged_kv_indices is the part of its buffer that one step fills:
+    # a captured call reads the lists of later steps from the same buffer, so the bound is what the buffer holds.
+    entries = ids.shape[0]
+    room = ids.untyped_storage().nbytes() // 4 - ids.storage_offset()
+    if room > entries:
+        entries = max(entries, min(room, _INT8_SLOTS // cache[-1]))
     o_strides = (hq * d, d) if out is None else out.stride()
     out = torch.empty(tokens, hq, d, dtype=torch.bfloat16, device=query.device) if out is None else out
     if tokens == 0 or rows == 0:
@@ -505,7 +513,7 @@ def paged_attention_int8(query: torch.Tensor, layer_cache: torch.Tensor, layer_s
             raise ValueError(f"8-bit paged attention needs a contiguous workspace of {need} bytes")
     _lib.launch(
         index, "nq_paged_attention_int8", None if qo is None else qo.data_ptr(), kv.data_ptr(), last.data_ptr(),
-        ids.data_ptr(), rows, ids.shape[0], query.data_ptr(), strides[0], strides[1], tokens, *cache, hq, hkv, d,
+        ids.data_ptr(), rows, entries, query.data_ptr(), strides[0], strides[1], tokens, *cache, hq, hkv, d,
         float(d) ** -0.5 if sm_scale is None else float(sm_scale), out.data_ptr(), o_strides[0], o_strides[1],
         int(parts), workspace.data_ptr(), size, _int8_status(status),
     )

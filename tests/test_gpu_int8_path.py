@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from helpers import to_np
+from helpers import DecodeKey, PrefillKey, adopt_random, make_kv, to_np
 from oracle import int8 as o_int8
 from oracle import kv_int8 as o_kv
 
@@ -224,3 +224,66 @@ def test_two_graphs_with_one_workspace(nq, device):
         torch.cuda.synchronize()
         for i in set(turn):
             assert torch.equal(outs[i].view(torch.int16), want[i].view(torch.int16))
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+def test_captured_steps_with_the_planner(nq, device, prefill):
+    """Write and attention on the metadata of the framework's own planner, captured with requests of one token (as a capture
+    slot is warmed) and replayed with others: longer histories, more pages, padding rows and padding tokens."""
+
+    from nari_qwen3_tts_amd import _lib, kernels
+
+    rng = np.random.default_rng(403 + prefill)
+    kv = make_kv(nq, device, hq=HQ, hkv=HKV, d=D, pages=96, ps=PS, scratch=5)
+    key = PrefillKey(5, 60) if prefill else DecodeKey(5)
+    ctx = kv.create_prefill(key, slot=0) if prefill else kv.create_decode(key, slot=0)
+    pubs = kv.prepare_capture(ctx, key)
+    meta, tokens = ctx.metadata, ctx.token_capacity
+    parts = _lib.NQ_ATTN_PREFILL if prefill else _lib.NQ_ATTN_DECODE
+    codes = torch.tensor(rng.integers(-127, 128, (96, 2, PS, HKV, D)), dtype=torch.int8, device=device)
+    scales = torch.tensor(2.0 ** rng.integers(-9, -4, (96, 2, PS // 16, HKV)), dtype=torch.float32, device=device)
+    x = torch.zeros(tokens, HQ + 2 * HKV, D, dtype=torch.bfloat16, device=device)
+    out = torch.zeros(tokens, HQ, D, dtype=torch.bfloat16, device=device)
+    status = torch.zeros(1, dtype=torch.int32, device=device)
+
+    def step():
+        kernels.paged_cache_write_int8_(x[:, HQ:HQ + HKV], x[:, HQ + HKV:], codes, scales, meta.write_pages,
+                                        meta.write_offsets, status)
+        kernels.paged_attention_int8(x[:, :HQ], codes, scales, meta, parts=parts, status=status, out=out)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    kv.finish_capture(ctx, pubs)
+
+    rids = tuple(adopt_random(kv, rng, [300, 3, 120]))
+    for turn in range(4):
+        news = [int(n) for n in rng.integers(1, 20, 3)]
+        pubs = kv.prepare_prefill(ctx, key, rids, news) if prefill else kv.prepare_decode(ctx, key, rids)
+        x.copy_(torch.tensor(rng.standard_normal(x.shape), dtype=torch.bfloat16, device=device))
+        want_c, want_s = codes.cpu().numpy(), scales.cpu().numpy()
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(status) == 0
+        now = ctx.metadata
+        live = sum(news) if prefill else 3
+        pages, offsets = now.write_pages.cpu().numpy(), now.write_offsets.cpu().numpy()
+        heads = to_np(x)
+        o_kv.write(want_c, want_s, heads[:, HQ:HQ + HKV], heads[:, HQ + HKV:], pages, offsets)
+        got_c, got_s = codes.cpu().numpy(), scales.cpu().numpy()
+        held = [p for p in range(96) if p not in kv._scratch_pages]
+        assert np.array_equal(got_c[held], want_c[held]) and np.array_equal(got_s[held], want_s[held])
+        want, bound = o_kv.attention(heads[:, :HQ], got_c, got_s, *(
+            None if t is None else t.cpu().numpy() for t in (
+                now.paged_kv_indptr, now.paged_kv_indices, now.paged_kv_last_page_len, now.qo_indptr)))
+        assert np.all(np.abs(to_np(out)[:live] - want[:live]) <= bound[:live]), turn
+        if prefill:
+            assert (out[live:] == 7.0).all()
+        for p in pubs:
+            p.publish()
