@@ -393,9 +393,12 @@ kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml
             const int pid = a.kv_indices[mine >> a.bpp_log2];
             if (pid >= 0 && pid < pool.num_pages) {
                 const float *s = pool.scales + pid * pool.s_page + (mine & in_page) * pool.s_block + head * pool.s_head;
+                // A scale that is not finite, K's or V's, answers through the scores of the rows that see the block: its
+                // V factor alone would be lost where a probability vanishes, and infinite ones can cancel.
+                const bool fine = fabsf(s[0]) < __builtin_inff() && fabsf(s[pool.s_kind]) < __builtin_inff();
                 w_pid = pid;
-                w_ks = s[0];
-                w_vs = s[pool.s_kind];
+                w_ks = fine ? s[0] : __builtin_nanf("");
+                w_vs = fine ? s[pool.s_kind] : 0.f;
             } else if (a.status) {
                 *a.status = NQ_ERR_INVALID_ARGUMENT;
             }
@@ -524,8 +527,7 @@ kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml
             for (int i = 0; i < 8; ++i) {
                 p[i] = 4 * grp + (i & 3) < nv[i / 4] ? __builtin_amdgcn_exp2f(p[i] - m_run) : 0.f;
                 l_run += p[i];
-                // a block that is masked whole may hold any scale
-                p[i] = p[i] == 0.f ? 0.f : p[i] * vs[i / 4];
+                p[i] *= vs[i / 4];
             }
             const u32x4 pw = {pack2_bf16(p[0], p[1]), pack2_bf16(p[2], p[3]), pack2_bf16(p[4], p[5]),
                               pack2_bf16(p[6], p[7])};

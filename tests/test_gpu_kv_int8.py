@@ -477,3 +477,32 @@ def test_many_rows(nq, device):
     _check(*_batch(device, 333, lens, None, hq=2, hkv=1, d=64, ps=16))
     queries = rng.integers(0, 4, 700).tolist()
     _check(*_batch(device, 334, lens, queries, hq=2, hkv=1, d=64, ps=16))
+
+
+# -- scales that no value has ---------------------------------------------------------------------------
+
+
+def _check_poisoned(device, queries, kind, value):
+    """A visible block of vanishing probability whose scale of one kind and kv head is ``value``: the query heads of that kv
+    head answer NaN, the others as before.  Row 0 (32 keys) lies in one decode span, row 1 (500) crosses several."""
+
+    from nari_qwen3_tts_amd.kernels import paged_attention_int8
+
+    q, codes, scales, meta = _batch(device, 340, [32, 500], queries, hq=4, hkv=2, d=64, ps=16)
+    q.fill_(1.0)
+    first = [meta.paged_kv_indices[0], meta.paged_kv_indices[2]]  # the rows' first blocks: scores of -508
+    for page in first:
+        codes[page, 0], scales[page, 0] = -127, 2.0**-4
+    want, bound = _want(q, codes, scales, meta, 1.0)
+    for page in first:
+        scales[page, kind, :, 0] = value
+    out = paged_attention_int8(q, codes, scales, meta, sm_scale=1.0)
+    assert out[:, :2].isnan().all()
+    _compare(out[:, 2:], want[:, 2:], bound[:, 2:])
+
+
+@pytest.mark.parametrize("queries", [None, [1, 1], [3, 40], [1, 40]])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_visible_scales_that_are_not_finite_answer_nan(nq, device, queries, kind, value):
+    _check_poisoned(device, queries, kind, value)
