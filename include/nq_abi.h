@@ -212,7 +212,9 @@ int nq_paged_attention_noalloc(const int32_t *qo_indptr, const int32_t *kv_indpt
  * slot, kv_head, d) at page*c_page + kind*c_kind + slot*c_slot + kv_head*c_head
  * + d; scales: fp32, one for each block of 16 slots, kind and kv head, at
  * page*s_page + kind*s_kind + (slot/16)*s_block + kv_head*s_head.  A value is
- * code * scale.  page_size is a power of two of at least 16, head_dim 64 or
+ * code * scale.  Scales are finite and not negative; the write makes powers of two.  Attention answers NaN
+ * in the queries that see a block with any other K or V scale, and rounds code * scale of V to bf16 in the
+ * prefill part (exact for powers of two).  page_size is a power of two of at least 16, head_dim 64 or
  * 128; codes and their strides are multiples of 16 bytes (else
  * NQ_ERR_UNSUPPORTED).
  *

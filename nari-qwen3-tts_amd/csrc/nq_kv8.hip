@@ -52,6 +52,9 @@ __device__ __forceinline__ float scale_for(float amax) {
     return e < 1 ? kMinScale : __uint_as_float(static_cast<uint32_t>(e) << 23);
 }
 
+// What scales are: anything else (NaN, an infinity, a negative number) makes the queries that see its block NaN.
+__device__ __forceinline__ bool is_scale(float s) { return s >= 0.f && s < __builtin_inff(); }
+
 __device__ __forceinline__ uint32_t pack4_i8(float a, float b, float c, float d) {
     const int ia = static_cast<int>(rintf(a)), ib = static_cast<int>(rintf(b)), ic = static_cast<int>(rintf(c)),
               id = static_cast<int>(rintf(d));
@@ -393,12 +396,13 @@ kv8_decode_kernel(Attend8 a, Pool8 pool, int waves, float2 *__restrict__ part_ml
             const int pid = a.kv_indices[mine >> a.bpp_log2];
             if (pid >= 0 && pid < pool.num_pages) {
                 const float *s = pool.scales + pid * pool.s_page + (mine & in_page) * pool.s_block + head * pool.s_head;
-                // A scale that is not finite, K's or V's, answers through the scores of the rows that see the block: its
-                // V factor alone would be lost where a probability vanishes, and infinite ones can cancel.
-                const bool fine = fabsf(s[0]) < __builtin_inff() && fabsf(s[pool.s_kind]) < __builtin_inff();
+                // What is no scale, K's or V's, answers through the scores of the rows that see the block: as a V factor
+                // it would be lost where a probability vanishes, and infinite K factors can drop a block's keys.
+                const float ks = s[0], vs = s[pool.s_kind];
+                const bool fine = is_scale(ks) && is_scale(vs);
                 w_pid = pid;
-                w_ks = fine ? s[0] : __builtin_nanf("");
-                w_vs = fine ? s[pool.s_kind] : 0.f;
+                w_ks = fine ? ks : __builtin_nanf("");
+                w_vs = fine ? vs : 0.f;
             } else if (a.status) {
                 *a.status = NQ_ERR_INVALID_ARGUMENT;
             }
@@ -730,8 +734,8 @@ template <int D>
 struct Smem8 {
     u32x4 k[2][kKeys * (D / 8 + 1)];
     u32x4 v[2][D * (kKeys / 8)];
-    float ks[2][kKeys / kBlk];     // K scales of the tile's blocks times sm_scale log2(e), 1 where one is not finite
-    int odd[2][kKeys / kBlk];      // kAbsent: the block's page is not in the pool; kPoison: a scale is not finite
+    float ks[2][kKeys / kBlk];     // K scales of the tile's blocks times sm_scale log2(e), 1 where one is none
+    int odd[2][kKeys / kBlk];      // kAbsent: the block's page is not in the pool; kPoison: a scale is none
     Meta8 meta;
 };
 constexpr int kAbsent = 1, kPoison = 2;
@@ -835,16 +839,16 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int splits, int skip_single, float2 *_
         *reinterpret_cast<bf16x8_t *>(stage + put_k0 + 16 * KT * e + buf * kBufK) = widen8(r.k[e].x, r.k[e].y);
     };
     auto put_scales = [&](const Stage &r, int buf) __attribute__((always_inline)) {
-        // A scale that is not finite, K's or V's, answers through the scores of the queries that see the block, not
-        // through 0 * NaN in those that do not.
-        const bool fine = fabsf(r.ks) < __builtin_inff() && fabsf(r.vs) < __builtin_inff();
+        // What is no scale, K's or V's, answers through the scores of the queries that see the block, not through
+        // 0 * NaN in those that do not.
+        const bool fine = is_scale(r.ks) && is_scale(r.vs);
         const int blk = uwave * NB / NW;
         // above zero, also for a block that was never written: a masked score, minus infinity, stays that
         sm.ks[buf][blk] = r.on && fine ? fmaxf(r.ks * a.scale, kMinScale) : 1.0f;
         sm.odd[buf][blk] = !r.on ? kAbsent : fine ? 0 : kPoison;
     };
     auto put_v = [&](const Stage &r, int col, int buf) __attribute__((always_inline)) {
-        const float vs = fabsf(r.v_vs) < __builtin_inff() ? r.v_vs : 0.f;
+        const float vs = is_scale(r.v_vs) ? r.v_vs : 0.f;
         uint32_t x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

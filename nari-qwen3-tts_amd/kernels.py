@@ -464,6 +464,7 @@ def paged_attention_int8(query: torch.Tensor, layer_cache: torch.Tensor, layer_s
     ``parts`` as ``paged_attention_noalloc`` takes them: NQ_ATTN_DECODE for the rows with one query,
     NQ_ATTN_PREFILL for those with several (alone: for all of them); both by default, NQ_ATTN_DECODE where the
     metadata has no qo_indptr.  A query that sees no key gets zeros; tokens of no row keep what ``out`` held.
+    A block whose K or V scale is negative or not finite makes the queries that see it NaN.
     ``workspace`` (``paged_attention_int8_workspace_bytes``; allocated if None) belongs to one call at a
     time.  The same inputs give the same bits.  No counterpart in the reference."""
 

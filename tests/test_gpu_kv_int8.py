@@ -506,3 +506,26 @@ def _check_poisoned(device, queries, kind, value):
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
 def test_visible_scales_that_are_not_finite_answer_nan(nq, device, queries, kind, value):
     _check_poisoned(device, queries, kind, value)
+
+
+@pytest.mark.parametrize("queries", [None, [3, 40]])
+@pytest.mark.parametrize("kind", [0, 1])
+def test_visible_negative_scales_answer_nan(nq, device, queries, kind):
+    """No write leaves one: it is held to be as little a scale as infinity, in decode as in prefill."""
+
+    _check_poisoned(device, queries, kind, -(2.0**-5))
+
+
+def test_scales_that_are_no_powers_of_two(nq, device):
+    """Any finite scale of at least zero is taken.  Prefill rounds V's code * scale to bf16, as the read back does: 2^-8 of
+    sum P |v| more than the oracle's bound allows."""
+
+    for queries in (None, [20, 70]):
+        q, codes, scales, meta = _batch(device, 341, [90, 400], queries, hq=4, hkv=2, d=128, ps=16)
+        scales.mul_(torch.rand(scales.shape, device=device) + 0.5)
+        scales[meta.paged_kv_indices[1]] = 0.0
+        want, bound = _want(q, codes, scales, meta)
+        sizes, _ = _want(q, torch.stack((codes[:, 0], codes[:, 1].abs()), 1), scales, meta)
+        from nari_qwen3_tts_amd.kernels import paged_attention_int8
+
+        _compare(paged_attention_int8(q, codes, scales, meta), want, bound + (1 + 2.0**-6) * 2.0**-8 * sizes)
