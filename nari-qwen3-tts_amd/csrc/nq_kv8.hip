@@ -1090,7 +1090,9 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int splits, int skip_single, float2 *_
                           pack2_bf16(acc[j][i + 2] * inv, acc[j][i + 3] * inv)};
     } else {
         const int64_t at = ((static_cast<int64_t>(slot) * a.heads + head) * splits + piece) * COLS + col;
-        if (half == 0) part_ml[at] = make_float2(any ? m_run : -__builtin_inff(), l_run);
+        // Minus infinity says that the piece saw no key.  One whose scores are all minus infinity has no weight beside
+        // other pieces, and if there are no others the sum of 0 makes the row NaN.
+        if (half == 0) part_ml[at] = make_float2(any ? fmaxf(m_run, -__FLT_MAX__) : -__builtin_inff(), l_run);
         float *o = part_o + at * D + 4 * half;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)

@@ -529,3 +529,20 @@ def test_scales_that_are_no_powers_of_two(nq, device):
         from nari_qwen3_tts_amd.kernels import paged_attention_int8
 
         _compare(paged_attention_int8(q, codes, scales, meta), want, bound + (1 + 2.0**-6) * 2.0**-8 * sizes)
+
+
+@pytest.mark.parametrize("keys,queries", [([60], None), ([600], None), ([60], [4]), ([600], [4]), ([600, 9], [4, 1])])
+def test_scores_of_minus_infinity_answer_nan(nq, device, keys, queries):
+    """A query whose every score is minus infinity has seen keys: NaN, as the softmax of the definition, whether its keys
+    are read in one piece or in several; not the zeros of a query without keys."""
+
+    from nari_qwen3_tts_amd.kernels import paged_attention_int8
+
+    q, codes, scales, meta = _batch(device, 342, keys, queries, hq=4, hkv=2, d=128, ps=16)
+    codes[:, 0] = codes[:, 0].abs().clamp(1)
+    want, bound = _want(q, codes, scales, meta)
+    q[0, 1, 5] = float("-inf")
+    out = paged_attention_int8(q, codes, scales, meta)
+    assert out[0, 1].isnan().all()
+    _compare(out[0, [0, 2, 3]], want[0, [0, 2, 3]], bound[0, [0, 2, 3]])
+    _compare(out[1:], want[1:], bound[1:])
