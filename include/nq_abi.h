@@ -257,7 +257,8 @@ int nq_kv_int8_read(const int8_t *codes, int64_t c_page, int64_t c_kind, int64_t
  * with one query too, NQ_ATTN_DECODE alone leaves rows with several out.
  * qo_indptr may be NULL with NQ_ATTN_DECODE alone: row r then owns query r.  A
  * query that sees no key (a row without pages, or more queries than keys) gets
- * zeros; query tokens of no row are left as they were.  A page id outside
+ * zeros; query tokens of no row are left as they were.  sm_scale times log2(e) is finite, else
+ * NQ_ERR_INVALID_ARGUMENT.  A page id outside
  * [0, num_pages) is skipped and sets status (may be NULL) to
  * NQ_ERR_INVALID_ARGUMENT.  Up to 16 query heads per kv head; q, out and their
  * strides are multiples of 16 bytes.  workspace holds the partial results of

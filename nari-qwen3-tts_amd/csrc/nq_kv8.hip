@@ -1336,6 +1336,7 @@ extern "C" int nq_paged_attention_int8(const int32_t *qo_indptr, const int32_t *
     NQ_CHECK_ARG(num_qo_heads >= num_kv_heads && num_qo_heads % num_kv_heads == 0);
     NQ_CHECK_ARG(parts >= 1 && parts <= (NQ_ATTN_DECODE | NQ_ATTN_PREFILL));
     NQ_CHECK_ARG(qo_indptr || parts == NQ_ATTN_DECODE);
+    NQ_CHECK_ARG(fabsf(sm_scale) * kLog2e8 <= __FLT_MAX__);  // not NaN either
     const Pool8 pool = {const_cast<int8_t *>(codes), c_page, c_kind, c_slot, c_head, const_cast<float *>(scales),
                         s_page, s_kind, s_block, s_head, num_pages, page_size};
     const int rc = check_pool(pool, num_kv_heads, head_dim);

@@ -342,6 +342,7 @@ def paged_attention_noalloc(query: torch.Tensor, layer_cache: torch.Tensor, meta
 
 INT8_BLOCK = 16  # cache slots that share a scale
 _INT8_SLOTS = 0x7FFF0000  # slots that a call's page list may name
+_INT8_SM_SCALE = 2.3e38  # times log2(e) still a float32
 
 
 def _int8_cache(layer_cache: torch.Tensor, layer_scales: torch.Tensor) -> tuple:
@@ -494,6 +495,9 @@ def paged_attention_int8(query: torch.Tensor, layer_cache: torch.Tensor, layer_s
         parts = _lib.NQ_ATTN_DECODE if qo is None else _lib.NQ_ATTN_DECODE | _lib.NQ_ATTN_PREFILL
     if qo is None and (parts != _lib.NQ_ATTN_DECODE or rows > tokens):
         raise ValueError("without qo_indptr every row has one query and only NQ_ATTN_DECODE runs")
+    sm_scale = float(d) ** -0.5 if sm_scale is None else float(sm_scale)
+    if not -_INT8_SM_SCALE < sm_scale < _INT8_SM_SCALE:
+        raise ValueError("sm_scale must be finite, also times log2(e) in float32")
     index = _lib.one_device(query, layer_cache, layer_scales, out, qo, kv, ids, last, status, workspace)
     # paged_kv_indptr says which entries count.  A planner's paged_kv_indices is the part of its buffer that one step fills:
     # a captured call reads the lists of later steps from the same buffer, so the bound is what the buffer holds.
@@ -515,8 +519,8 @@ def paged_attention_int8(query: torch.Tensor, layer_cache: torch.Tensor, layer_s
     _lib.launch(
         index, "nq_paged_attention_int8", None if qo is None else qo.data_ptr(), kv.data_ptr(), last.data_ptr(),
         ids.data_ptr(), rows, entries, query.data_ptr(), strides[0], strides[1], tokens, *cache, hq, hkv, d,
-        float(d) ** -0.5 if sm_scale is None else float(sm_scale), out.data_ptr(), o_strides[0], o_strides[1],
-        int(parts), workspace.data_ptr(), size, _int8_status(status),
+        sm_scale, out.data_ptr(), o_strides[0], o_strides[1], int(parts), workspace.data_ptr(), size,
+        _int8_status(status),
     )
     return out
 

@@ -173,3 +173,18 @@ def test_host_checks_of_the_c_entries(nq):
     assert attend(qo=None, parts=1, n=5) == -1  # more rows than queries
     assert attend(q=8) == -2 and attend(q_s0=1020) == -2 and attend(ps=8) == -2
     assert attend(ids=1 << 28) == -2  # 2^32 slots
+
+
+def test_sm_scale_that_is_not_finite_is_refused(nq):
+    """Also where the factor log2(e) or the entry's fp32 takes it there."""
+
+    from nari_qwen3_tts_amd import _lib, kernels
+
+    a = _args()
+    lib = _lib.load()
+    for bad in (float("nan"), float("inf"), float("-inf"), 3e38, 1e300):
+        with pytest.raises(ValueError, match="sm_scale"):
+            kernels.paged_attention_int8(torch.zeros(2, 4, 64, dtype=torch.bfloat16), a.layer_cache, a.layer_scales,
+                                         _metadata(), sm_scale=bad)
+        assert lib.nq_paged_attention_int8(16, 16, 16, 16, 2, 2, 16, 1024, 64, 4, 16, 32768, 16384, 1024, 128, 16, 16, 8, 8,
+                                           1, 4, 16, 16, 8, 128, bad, 16, 2048, 128, 3, 16, 1 << 40, None, None) == -1
