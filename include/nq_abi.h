@@ -225,8 +225,8 @@ int nq_paged_attention_noalloc(const int32_t *qo_indptr, const int32_t *kv_indpt
  * scale becomes e(a) if o == 0, else max(scale, e(a)), e(a) = the least power
  * of two >= 2^-126 with a / e <= 127; the codes of slots below o are rescaled
  * (rint, ties to even) when the scale grows, slots behind the run keep their
- * codes and count as empty.  A NaN or infinity in the run, or a scale that is
- * not finite, makes the block's scale NaN.  A slot outside the pool is skipped
+ * codes and count as empty.  A NaN or infinity in the run, or an earlier scale
+ * that is negative or not finite (o > 0), makes the block's scale NaN.  A slot outside the pool is skipped
  * and sets status (device int32, may be NULL) to NQ_ERR_INVALID_ARGUMENT.  The
  * runs of one call are in different blocks: what a block that two runs share
  * holds afterwards is not specified.

@@ -146,8 +146,8 @@ kv8_write_kernel(const uint16_t *__restrict__ key, int64_t k_s0, int64_t k_s1, c
             }
         }
         amax = group_max<kWave>(amax);
-        // a scale that is NaN stays: every query that reads the block answers NaN
-        const bool bad = __any(odd) || !(old < __builtin_inff());
+        // what was no scale becomes NaN and stays: every query that reads the block answers NaN
+        const bool bad = __any(odd) || !is_scale(old);
         const float own = scale_for(amax);
         const float s = bad ? __builtin_nanf("") : (first && old > own ? old : own);
         const float inv = bad ? 0.f : 1.0f / s;  // exact: s is a power of two, at most 2^122

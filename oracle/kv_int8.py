@@ -49,7 +49,7 @@ def write(codes: np.ndarray, scales: np.ndarray, key: np.ndarray, value: np.ndar
                 new = x[t : t + run, h].astype(np.float64)
                 old = float(scales[p, kind, b, h]) if first else 0.0
                 before = codes[p, kind, b * BLOCK : o, h].astype(np.float64)
-                if not np.isfinite(new).all() or not np.isfinite(old):
+                if not np.isfinite(new).all() or not 0 <= old < np.inf:
                     scales[p, kind, b, h] = np.nan
                     codes[p, kind, o : o + run, h] = 0
                     continue

@@ -546,3 +546,17 @@ def test_scores_of_minus_infinity_answer_nan(nq, device, keys, queries):
     assert out[0, 1].isnan().all()
     _compare(out[0, [0, 2, 3]], want[0, [0, 2, 3]], bound[0, [0, 2, 3]])
     _compare(out[1:], want[1:], bound[1:])
+
+
+@pytest.mark.parametrize("old", [float("-inf"), float("inf"), float("nan"), -0.25])
+def test_write_beside_a_scale_that_is_none(nq, device, old):
+    """A block whose scale is not finite, or negative, stays unusable until a write at its first slot."""
+
+    rng = np.random.default_rng(17)
+    codes, scales = _pool(device, rng, 2, 16, 2, 64)
+    scales[1, :, 0, 1] = old
+    x = _bf16(rng, device, 2, 3, 2, 64)
+    _check_write(codes, scales, x[0, :1], x[1, :1], *_slots(device, [1], [4]))
+    assert scales[1, :, 0, 1].isnan().all() and scales[1, :, 0, 0].isfinite().all()
+    _check_write(codes, scales, x[0], x[1], *_slots(device, [1, 1, 1], [0, 1, 2]))
+    assert scales[1].isfinite().all()
