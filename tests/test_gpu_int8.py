@@ -171,3 +171,17 @@ def test_graph(nq, device):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("m", [3, 40, 300, 700])
+def test_linear_scales_of_far_apart_sizes(nq, device, m):
+    """Large activations against small weights: the result fits bf16 where sum * sx would not fit fp32."""
+
+    from nari_qwen3_tts_amd.layers import linear_int8
+
+    rng = np.random.default_rng(m)
+    n = 3000 if m == 700 else 96
+    q, w = _codes(rng, device, m, 512), _codes(rng, device, n, 512)
+    s = torch.from_numpy(rng.uniform(1e35, 1e36, m).astype(np.float32)).to(device)
+    sw = torch.from_numpy(rng.uniform(1e-6, 1e-5, n).astype(np.float32)).to(device)
+    _check(linear_int8(q, s, w, sw), q, s, w, sw)
