@@ -251,7 +251,8 @@ int nq_kv_int8_read(const int8_t *codes, int64_t c_page, int64_t c_kind, int64_t
  * nq_paged_attention over the 8-bit cache, without a plan: the launches read
  * the ragged metadata themselves.  kv_indptr [n_rows + 1] starts at 0 and does
  * not decrease; entries are held to [0, num_indices], the entries that kv_indices has room for (a captured
- * call may find more of them in use at a later replay).
+ * call may find more of them in use at a later replay), and to what precedes them, and status is set where that
+ * changes one: rows in such a batch may get any value, memory outside the arguments is not touched.
  * parts: NQ_ATTN_DECODE (rows with one query), NQ_ATTN_PREFILL (rows with
  * several, bottom-right causal), or both; NQ_ATTN_PREFILL alone takes the rows
  * with one query too, NQ_ATTN_DECODE alone leaves rows with several out.

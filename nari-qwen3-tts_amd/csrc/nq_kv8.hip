@@ -304,9 +304,10 @@ struct Row8 {
 template <typename R>
 __device__ __forceinline__ Row8 row_of(const Attend8 &a, const R &rows, int r) {
     Row8 w;
-    int b = __builtin_amdgcn_readfirstlane(rows.kv(r)), e = __builtin_amdgcn_readfirstlane(rows.kv(r + 1));
-    b = b < 0 ? 0 : (b > a.n_indices ? a.n_indices : b);
-    e = e < b ? b : (e > a.n_indices ? a.n_indices : e);
+    const int first = __builtin_amdgcn_readfirstlane(rows.kv(r)), end = __builtin_amdgcn_readfirstlane(rows.kv(r + 1));
+    const int b = first < 0 ? 0 : (first > a.n_indices ? a.n_indices : first);
+    const int e = end < b ? b : (end > a.n_indices ? a.n_indices : end);
+    if ((b != first || e != end) && a.status) *a.status = NQ_ERR_INVALID_ARGUMENT;
     w.first_page = b;
     w.n_pages = e - b;
     const int ps = kBlk << a.bpp_log2;
@@ -607,7 +608,9 @@ kv8_merge_kernel(Attend8 a, int waves, const float2 *__restrict__ part_ml, const
     const Row8 row = row_of(a, rows, r);
     if (row.q_len != 1) return;
     uint16_t *out = a.out + row.q0 * a.o_s0 + (head * a.group + g) * a.o_s1;
-    if (row.n_pages == 0) {
+    // a row behind the batch's last page (a kv_indptr that decreases) was in no span
+    const bool outside = (static_cast<int64_t>(row.first_page + row.n_pages) << a.bpp_log2) > sp.blocks;
+    if (row.n_pages == 0 || outside) {
         if (threadIdx.x < TP) *reinterpret_cast<u32x2 *>(out + 4 * threadIdx.x) = u32x2{0, 0};
         return;
     }

@@ -560,3 +560,23 @@ def test_write_beside_a_scale_that_is_none(nq, device, old):
     assert scales[1, :, 0, 1].isnan().all() and scales[1, :, 0, 0].isfinite().all()
     _check_write(codes, scales, x[0], x[1], *_slots(device, [1, 1, 1], [0, 1, 2]))
     assert scales[1].isfinite().all()
+
+
+@pytest.mark.parametrize("queries", [None, [3, 1, 20]])
+@pytest.mark.parametrize("indptr", [[0, 3, 6, 9], [0, 4, 3, 6], [0, 6, 2, 2], [0, 6, 3, 1], [0, -5, 2, 6], [0, 6, 6, 0],
+                                    [2, 1 << 30, 6, 6]])
+def test_page_ranges_outside_the_list(nq, device, queries, indptr):
+    """Ranges that decrease or pass the list's six pages set status; reads and writes stay inside the arguments (the workspace's
+    partials included), and a call behind it is right."""
+
+    from nari_qwen3_tts_amd.kernels import paged_attention_int8
+
+    q, codes, scales, meta = _batch(device, 350, [30, 40, 20], queries, hq=4, hkv=2, d=64, ps=16, spare=2)
+    meta.paged_kv_indices = meta.paged_kv_indices[:6].clone()
+    good = meta.paged_kv_indptr.clone()
+    meta.paged_kv_indptr.copy_(torch.tensor(indptr, dtype=torch.int32))
+    status = torch.zeros(1, dtype=torch.int32, device=device)
+    paged_attention_int8(q, codes, scales, meta, status=status)
+    assert int(status) == -1
+    meta.paged_kv_indptr.copy_(good.clamp(max=6))
+    _check(q, codes, scales, meta)
