@@ -253,6 +253,7 @@ int nq_kv_int8_read(const int8_t *codes, int64_t c_page, int64_t c_kind, int64_t
  * not decrease; entries are held to [0, num_indices], the entries that kv_indices has room for (a captured
  * call may find more of them in use at a later replay), and to what precedes them, and status is set where that
  * changes one: rows in such a batch may get any value, memory outside the arguments is not touched.
+ * num_indices times page_size is at most 0x7fff0000 (else NQ_ERR_UNSUPPORTED).
  * parts: NQ_ATTN_DECODE (rows with one query), NQ_ATTN_PREFILL (rows with
  * several, bottom-right causal), or both; NQ_ATTN_PREFILL alone takes the rows
  * with one query too, NQ_ATTN_DECODE alone leaves rows with several out.

@@ -1358,7 +1358,7 @@ extern "C" int nq_paged_attention_int8(const int32_t *qo_indptr, const int32_t *
     while ((kBlk << bpp) < page_size) ++bpp;
     const Prefill8 p = prefill_plan(tokens, n_rows, num_qo_heads / num_kv_heads, num_kv_heads, head_dim);
     if (static_cast<int64_t>(p.slots) * num_kv_heads > 0x3fffffff || num_kv_heads > 65535 ||
-        (static_cast<int64_t>(num_indices) * page_size) > 0x7fffffffll)
+        (static_cast<int64_t>(num_indices) * page_size) > 0x7fff0000ll)  // a tile behind the last key is still an int
         return NQ_ERR_UNSUPPORTED;
     const Attend8 a = {q,     q_s0,        q_s1,   out,         o_s0,
                        o_s1,  qo_indptr,   kv_indptr, kv_indices,  last_page_len,

@@ -188,3 +188,14 @@ def test_sm_scale_that_is_not_finite_is_refused(nq):
                                          _metadata(), sm_scale=bad)
         assert lib.nq_paged_attention_int8(16, 16, 16, 16, 2, 2, 16, 1024, 64, 4, 16, 32768, 16384, 1024, 128, 16, 16, 8, 8,
                                            1, 4, 16, 16, 8, 128, bad, 16, 2048, 128, 3, 16, 1 << 40, None, None) == -1
+
+
+def test_page_lists_near_2_31_slots_are_refused(nq):
+    """The last key tile of such a row would pass 2^31."""
+
+    from nari_qwen3_tts_amd import _lib
+
+    lib = _lib.load()
+    for ids, d in ((0x7FFFFFFF // 16, 128), (0x7FFF0000 // 16 + 1, 64)):
+        assert lib.nq_paged_attention_int8(16, 16, 16, 16, 2, ids, 16, 1024, 64, 4, 16, 32768, 16384, 1024, 128, 16, 16, 8,
+                                           8, 1, 4, 16, 16, 8, d, 0.1, 16, 2048, 128, 3, 16, 1 << 40, None, None) == -2
