@@ -113,3 +113,40 @@ def attention(q, codes, scales, kv_indptr, kv_indices, last_page_len, qo_indptr=
                 out[q0 + i, h] = mean
                 bound[q0 + i, h] = 2.0**-8 * np.abs(mean) + loss * (1 + 2.0**-7) * size + 1e-38
     return out, bound
+
+
+def attention_rows(q, codes, scales, kv_indptr, kv_indices, last_page_len, qo_indptr, num_pages=None):
+    """``attention`` a row and head at a time, for rows of many queries; page ids outside [0, num_pages) have no
+    keys.  The same bound (``num_pages``: how many pages the call was given, all by default)."""
+
+    q = np.asarray(q, dtype=np.float64)
+    tokens, hq, d = q.shape
+    ps, hkv = codes.shape[2], codes.shape[3]
+    pages = codes.shape[0] if num_pages is None else num_pages
+    out, bound = np.full(q.shape, np.nan), np.full(q.shape, np.nan)
+    u = 2.0**-24
+    for r in range(len(kv_indptr) - 1):
+        q0, q1 = int(qo_indptr[r]), int(qo_indptr[r + 1])
+        ids = np.asarray(kv_indices[kv_indptr[r] : kv_indptr[r + 1]])
+        kv_len = (len(ids) - 1) * ps + int(last_page_len[r]) if len(ids) else 0
+        if kv_len == 0:
+            out[q0:q1] = bound[q0:q1] = 0.0
+            continue
+        there = (ids >= 0) & (ids < pages)
+        held = values(codes[np.where(there, ids, 0)], scales[np.where(there, ids, 0)])
+        limit = np.clip(kv_len - (q1 - q0) + np.arange(q1 - q0) + 1, 0, kv_len)
+        seen = (np.arange(kv_len) < limit[:, None]) & np.repeat(there, ps)[:kv_len]
+        n = seen.sum(1, keepdims=True)
+        for h in range(hq):
+            k, v = (held[:, i, :, h // (hq // hkv)].reshape(-1, d)[:kv_len] for i in (0, 1))
+            x = q[q0:q1, h]
+            s = np.where(seen, x @ k.T * d**-0.5, -np.inf)
+            top = np.where(n > 0, s.max(1, keepdims=True), 0.0)
+            p = np.exp(s - top)
+            p /= np.where(n > 0, p.sum(1, keepdims=True), 1.0)
+            largest = np.where(seen, np.abs(x) @ np.abs(k).T, 0.0).max(1, keepdims=True) * d**-0.5
+            size = np.where(seen, np.abs(x @ k.T) * d**-0.5, 0.0).max(1, keepdims=True)
+            loss = 2 * (2 * d + 4) * u * largest + 8 * u * size + 8 * u + 2.0**-8 + 2 * n * u
+            out[q0:q1, h] = p @ v
+            bound[q0:q1, h] = np.where(n > 0, 2.0**-8 * np.abs(p @ v) + loss * (1 + 2.0**-7) * (p @ np.abs(v)) + 1e-38, 0.0)
+    return out, bound

@@ -580,3 +580,112 @@ def test_page_ranges_outside_the_list(nq, device, queries, indptr):
     assert int(status) == -1
     meta.paged_kv_indptr.copy_(good.clamp(max=6))
     _check(q, codes, scales, meta)
+
+
+# -- one long prompt: tiles of 256 columns, eight waves ---------------------------------------------------
+
+
+def _tile_columns(tokens, rows, hq, hkv, d):
+    """Columns of a prefill tile, from the workspace: (tokens // (columns // group) + rows) tiles of each kv head, in 2 to 8
+    pieces of a maximum, a sum and d values a column, or none where the pieces are one."""
+
+    from nari_qwen3_tts_amd import _lib, kernels
+
+    size = kernels.paged_attention_int8_workspace_bytes(tokens, rows, hq, hkv, d, _lib.NQ_ATTN_PREFILL)
+    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    found = {columns for columns in (128, 256) for pieces in range(2, 9)
+             for n in [(tokens // (columns * hkv // hq) + rows) * hkv * pieces * columns]
+             if up(8 * n) + up(4 * n * d) == size}
+    assert len(found) == 1, "sizes whose workspace tells the tiles apart"
+    return found.pop()
+
+
+def _want_rows(q, codes, scales, meta):
+    return o_kv.attention_rows(to_np(q), codes.cpu().numpy(), scales.cpu().numpy(), *(t.cpu().numpy() for t in (
+        meta.paged_kv_indptr, meta.paged_kv_indices, meta.paged_kv_last_page_len, meta.qo_indptr)))
+
+
+WIDE = [  # keys, queries, query heads, kv heads, page size
+    ([1500], [1040], 16, 8, 16), ([1040], [1040], 16, 8, 64), ([2900], [1037], 16, 8, 16),
+    ([900], [160], 16, 1, 16), ([100], [160], 16, 1, 64),  # the first 60 queries see no key
+    ([800], [700], 6, 2, 16), ([730], [700], 6, 2, 64),  # a group that does not divide the columns
+    ([700, 650], [700, 650], 16, 4, 128), ([500, 0, 300], [350, 1, 49], 16, 1, 16), ([2100], [2060], 4, 4, 32),
+]
+
+
+@pytest.mark.parametrize("case", range(len(WIDE)))
+def test_prefill_of_a_long_prompt(nq, device, case):
+    """Tiles of one piece, of two and of several; last tiles that are not full; empty rows and rows of one query beside."""
+
+    from nari_qwen3_tts_amd import _lib
+    from nari_qwen3_tts_amd.kernels import paged_attention_int8
+
+    keys, queries, hq, hkv, ps = WIDE[case]
+    q, codes, scales, meta = _batch(device, 360 + case, keys, queries, hq=hq, hkv=hkv, d=128, ps=ps, tail=2)
+    assert _tile_columns(q.shape[0], len(keys), hq, hkv, 128) == 256
+    want, bound = _want_rows(q, codes, scales, meta)
+    for parts in (_lib.NQ_ATTN_PREFILL, None):
+        outs = []
+        for _ in range(2):
+            outs.append(torch.full_like(q, 7.0))
+            paged_attention_int8(q, codes, scales, meta, parts=parts, out=outs[-1])
+        _compare(outs[0], want, bound, f"{WIDE[case]}")
+        assert (outs[0][sum(queries):] == 7.0).all()
+        assert torch.equal(outs[0].view(torch.int16), outs[1].view(torch.int16))
+
+
+@pytest.mark.parametrize("hq,hkv,ps,keys,queries", [(16, 8, 16, 1500, 1040), (16, 1, 64, 900, 160), (6, 2, 16, 800, 700)])
+def test_prefill_of_a_long_prompt_with_odd_blocks(nq, device, hq, hkv, ps, keys, queries):
+    """A page outside the pool among the keys, blocks of NaN and infinite scales that the last queries alone see, codes and
+    scales in other orders, queries and outputs as slices."""
+
+    from nari_qwen3_tts_amd import _lib
+    from nari_qwen3_tts_amd.kernels import paged_attention_int8
+
+    q, codes, scales, meta = _batch(device, 380 + hq, [keys], [queries], hq=hq, hkv=hkv, d=128, ps=ps)
+    assert _tile_columns(queries, 1, hq, hkv, 128) == 256
+    meta.paged_kv_indices[3] = codes.shape[0] + 7
+    want, bound = _want_rows(q, codes, scales, meta)
+    late = keys - 37  # a block that the last 37 queries see, a whole tile and a part of one behind
+    page, block = int(meta.paged_kv_indices[late // ps]), late % ps // 16
+    first = late // 16 * 16 - (keys - queries)  # the first query that sees it
+    scales[page, 0, block], scales[page, 1, block] = float("nan"), 2.0**-5
+    other = late + 16
+    page, block = int(meta.paged_kv_indices[other // ps]), other % ps // 16
+    scales[page, 1, block] = float("inf")
+    packed = torch.zeros(queries, hq + 3, 128, dtype=torch.bfloat16, device=device)
+    packed[:, 1:hq + 1] = q
+    out = torch.full((queries, 2, hq, 128), 7.0, dtype=torch.bfloat16, device=device)
+    status = torch.zeros(1, dtype=torch.int32, device=device)
+    heads_first = codes.transpose(2, 3).contiguous().transpose(2, 3)
+    blocks_last = scales.permute(3, 1, 0, 2).contiguous().permute(2, 1, 3, 0)
+    paged_attention_int8(packed[:, 1:hq + 1], heads_first, blocks_last, meta, parts=_lib.NQ_ATTN_PREFILL, status=status,
+                         out=out[:, 1])
+    assert int(status) == -1 and (out[:, 0] == 7.0).all()
+    assert out[first:, 1].isnan().all()
+    _compare(out[:first, 1], want[:first], bound[:first])
+
+
+def test_prefill_of_a_long_prompt_in_a_graph(nq, device):
+    """Captured, replayed with other queries, keys and lengths, eager work between."""
+
+    from nari_qwen3_tts_amd.kernels import paged_attention_int8
+
+    q, codes, scales, meta = _batch(device, 390, [1300], [1040], hq=16, hkv=8, d=128, ps=16)
+    assert _tile_columns(1040, 1, 16, 8, 128) == 256
+    out = torch.zeros_like(q)
+    paged_attention_int8(q, codes, scales, meta, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged_attention_int8(q, codes, scales, meta, out=out)
+    for last in (4, 1, 16, 9):
+        q.normal_()
+        codes.random_(-127, 128)
+        meta.paged_kv_last_page_len.fill_(last)
+        meta.qo_indptr[1] = 1000 + last
+        want = paged_attention_int8(q, codes, scales, meta, out=torch.full_like(q, 7.0))
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(torch.int16), want.view(torch.int16)) and want[:1000 + last].isfinite().all()

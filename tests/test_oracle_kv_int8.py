@@ -66,6 +66,22 @@ def test_attention_closed_forms():
     assert np.allclose(out[0], v.mean(0), rtol=1e-12) and (bound[0] < 0.03 * np.abs(v).max()).all()
 
 
+def test_attention_by_rows_is_attention():
+    """Rows at once against query by query: values and bounds; and a page outside the pool against the same keys left out."""
+
+    rng = np.random.default_rng(5)
+    codes = rng.integers(-127, 128, (9, 2, 16, 2, 8)).astype(np.int8)
+    scales = (2.0 ** rng.integers(-8, -4, (9, 2, 1, 2))).astype(np.float32)
+    q = rng.standard_normal((24, 4, 8))
+    where = ([0, 3, 3, 8], [4, 0, 7, 1, 2, 3, 8, 5], [5, 1, 16], [0, 9, 11, 24])
+    for got, want in zip(o_kv.attention_rows(q, codes, scales, *where), o_kv.attention(q, codes, scales, *where)):
+        assert np.allclose(got, want, rtol=1e-9, atol=1e-300)
+    assert (o_kv.attention_rows(q, codes, scales, *where)[0][9:11] == 0).all()
+    out, bound = o_kv.attention_rows(q[:1], codes, scales, [0, 3], [4, 9, 2], [16], [0, 1])
+    want, wide = o_kv.attention(q[:1], codes, scales, [0, 2], [4, 2], [16], [0, 1])
+    assert np.allclose(out, want, rtol=1e-12) and np.allclose(bound, wide, rtol=1e-9)
+
+
 # -- refusals ------------------------------------------------------------------------------------------
 
 
