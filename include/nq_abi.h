@@ -877,10 +877,12 @@ int nq_codec_transconv_overlap(const int32_t *offsets, int B, int u_in, int stri
  * nq_linear_int8: out[m, n] = bf16(sum_k xq[m, k] wq[n, k] * sw[n] * sx[m]),
  * the sum in int32, exact for codes within +-127, then two fp32 products in this order.  K is a multiple of 16, up to 2^17 for the product; codes
  * and their row strides are multiples of 16 bytes (x of the quantisation and its codes' rows: of 8
- * elements).  M, N: any.
+ * elements).  M, N: any.  nq_linear_int8_tile: rows << 16 | columns of out that one workgroup of the product
+ * takes (-1 where M or N is below 1).
  */
 int nq_quantize_int8_rows(const uint16_t *x, int64_t x_s0, int M, int K, int8_t *q, int64_t q_s0,
                           float *scales, void *stream);
+int nq_linear_int8_tile(int M, int N);
 int nq_linear_int8(const int8_t *xq, int64_t x_s0, const float *sx, const int8_t *wq, int64_t w_s0,
                    const float *sw, int M, int N, int K, uint16_t *out, int64_t o_s0, void *stream);
 

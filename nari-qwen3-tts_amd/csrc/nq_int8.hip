@@ -397,6 +397,24 @@ void launch_tiles(const Int8Args &a, hipStream_t st) {
                        tiles_m, tiles);
 }
 
+// Rows and columns of out a workgroup takes.  Few tiles: the waves split K.  Otherwise the largest tile that still gives every
+// CU one: a stage of 128 bytes takes 0.29, 0.38 and 1.0 us at 64 x 64, 64 x 128 and 128 x 256.  Measured, K 2048, us:
+//   M 64  N 4096:  64-row pieces 5.5, 32-row pieces 6.6, 64 x 64 tiles 8.4;   N 6144: 9.8, 9.4, 8.4
+//   M 32  N 6144:  32-row pieces 6.8, 64 x 64 tiles 8.2;                      N 12288: 10.0, 8.4
+//   M 256 N 4096:  64 x 64 tiles 9.1, 64 x 128 9.6, 128 x 256 19;             N 6144: 11.0, 10.1, 20
+//   M 640 N 6144:  64 x 128 tiles 15.8, 128 x 256 21.0;                       N 12288: 28.0, 24.4 (22.9 since)
+constexpr int tile_id(int rows, int columns) { return rows << 16 | columns; }
+int tile_for(int M, int N) {
+    auto count = [&](int bm, int bn) { return static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+    auto rounds = [](int64_t tiles) { return (tiles + 255) / 256; };
+    if (M <= 16) return tile_id(16, 16);
+    if (count(32, 16) <= (M <= 32 ? 512 : 256)) return tile_id(32, 16);
+    if (count(64, 16) <= 256) return tile_id(64, 16);
+    if (count(64, 64) <= 256) return tile_id(64, 64);
+    if (3 * rounds(count(128, 256)) > rounds(count(64, 128))) return tile_id(64, 128);
+    return tile_id(128, 256);
+}
+
 }  // namespace
 }  // namespace nq
 
@@ -413,6 +431,10 @@ extern "C" int nq_quantize_int8_rows(const uint16_t *x, int64_t x_s0, int M, int
     return NQ_LAUNCH_STATUS();
 }
 
+extern "C" int nq_linear_int8_tile(int M, int N) {
+    return M < 1 || N < 1 || M > 0x7fffff00 || N > 0x7fffff00 ? -1 : tile_for(M, N);
+}
+
 extern "C" int nq_linear_int8(const int8_t *xq, int64_t x_s0, const float *sx, const int8_t *wq, int64_t w_s0,
                               const float *sw, int M, int N, int K, uint16_t *out, int64_t o_s0, void *stream) {
     NQ_CHECK_ARG(M >= 0 && N >= 0 && K >= 0);
@@ -426,19 +448,13 @@ extern "C" int nq_linear_int8(const int8_t *xq, int64_t x_s0, const float *sx, c
     const Int8Args a = {xq,  x_s0, sx,   wq, w_s0, sw, M, N, K, out, o_s0,
                         (M == 1 || o_s0 % 8 == 0) && al(out, 16)};
     hipStream_t st = static_cast<hipStream_t>(stream);
-    // Few tiles: the waves split K.  Otherwise the largest tile that still gives every CU one: a stage of 128 bytes takes
-    // 0.29, 0.38 and 1.0 us at 64 x 64, 64 x 128 and 128 x 256.  Measured, K 2048, us:
-    //   M 64  N 4096:  64-row pieces 5.5, 32-row pieces 6.6, 64 x 64 tiles 8.4;   N 6144: 9.8, 9.4, 8.4
-    //   M 32  N 6144:  32-row pieces 6.8, 64 x 64 tiles 8.2;                      N 12288: 10.0, 8.4
-    //   M 256 N 4096:  64 x 64 tiles 9.1, 64 x 128 9.6, 128 x 256 19;             N 6144: 11.0, 10.1, 20
-    //   M 640 N 6144:  64 x 128 tiles 15.8, 128 x 256 21.0;                       N 12288: 28.0, 24.4 (22.9 since)
-    auto count = [&](int bm, int bn) { return static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-    auto rounds = [](int64_t tiles) { return (tiles + 255) / 256; };
-    if (M <= 16) launch_rows<1>(a, st);
-    else if (count(32, 16) <= (M <= 32 ? 512 : 256)) launch_rows<2>(a, st);
-    else if (count(64, 16) <= 256) launch_rows<4>(a, st);
-    else if (count(64, 64) <= 256) launch_tiles<2, 2, 1, 1>(a, st);
-    else if (3 * rounds(count(128, 256)) > rounds(count(64, 128))) launch_tiles<2, 4, 1, 1>(a, st);
-    else launch_tiles<2, 4, 2, 2>(a, st);
+    switch (tile_for(M, N)) {
+        case tile_id(16, 16): launch_rows<1>(a, st); break;
+        case tile_id(32, 16): launch_rows<2>(a, st); break;
+        case tile_id(64, 16): launch_rows<4>(a, st); break;
+        case tile_id(64, 64): launch_tiles<2, 2, 1, 1>(a, st); break;
+        case tile_id(64, 128): launch_tiles<2, 4, 1, 1>(a, st); break;
+        default: launch_tiles<2, 4, 2, 2>(a, st);  // 128 x 256
+    }
     return NQ_LAUNCH_STATUS();
 }

@@ -185,3 +185,28 @@ def test_linear_scales_of_far_apart_sizes(nq, device, m):
     s = torch.from_numpy(rng.uniform(1e35, 1e36, m).astype(np.float32)).to(device)
     sw = torch.from_numpy(rng.uniform(1e-6, 1e-5, n).astype(np.float32)).to(device)
     _check(linear_int8(q, s, w, sw), q, s, w, sw)
+
+
+@pytest.mark.parametrize("m,n,k,tile", [
+    (640, 12288, 2048, (128, 256)), (4001, 2040, 1040, (128, 256)), (2050, 2100, 384, (128, 256)),
+    (2050, 2100, 400, (128, 256)), (2050, 2100, 512, (128, 256)), (2050, 2100, 528, (128, 256)),
+    (2050, 2100, 16, (128, 256)), (1900, 2305, 6144, (128, 256)),
+    (300, 5001, 2064, (64, 128)), (640, 6144, 1040, (64, 128)), (250, 4090, 1552, (64, 64)), (129, 700, 6160, (32, 16)),
+    (64, 4096, 2064, (64, 16)), (50, 2040, 1040, (32, 16)), (16, 5000, 3088, (16, 16)),
+])
+def test_linear_long_sums(nq, device, m, n, k, tile):
+    """Each kernel through its loop over whole stages, around the loop's bounds and with a part of a stage behind it."""
+
+    from nari_qwen3_tts_amd import _lib
+    from nari_qwen3_tts_amd.layers import linear_int8
+
+    assert _lib.load().nq_linear_int8_tile(m, n) == tile[0] << 16 | tile[1]
+    rng = np.random.default_rng(m + n + k)
+    q, w = _codes(rng, device, m, k), _codes(rng, device, n, k)
+    s, sw = torch.rand(m, device=device) + 0.01, torch.rand(n, device=device) + 0.01
+    out = torch.full((m, n + 8), 7.0, dtype=torch.bfloat16, device=device)
+    linear_int8(q, s, w, sw, out=out[:, :n])
+    assert (out[:, n:] == 7.0).all()
+    _check(out[:, :n], q, s, w, sw)
+    again = linear_int8(q, s, w, sw)
+    assert torch.equal(again.view(torch.int16), out[:, :n].contiguous().view(torch.int16))
