@@ -2,8 +2,12 @@
 //   out[m, n] = bf16(float(sum_k cx[m, k] cw[n, k]) * sw[n] * sx[m])
 // with the sum in int32 (exact for K <= 2^17), and the quantisation of rows that
 // makes both operands: s = max |x| / 127, c = rint(127 x / max |x|).  127 x is exact
-// in fp32 for a bf16 x and the quotient correctly rounded, and a quotient that is
-// no tie lies at least 1 / 512 from one, so the codes are those of exact arithmetic.
+// in fp32 for a bf16 x.  With significands a of x and b of max |x| (integers below
+// 256) and 2^k between their exponents a quotient is 127 a / (b 2^k); from a tie,
+// (2n + 1) / 2, it differs by |254 a - (2n + 1) b 2^k| / (b 2^(k + 1)), whose
+// numerator is an integer: by nothing, or by at least 1 / (254 a) > 2^-16 of the
+// quotient itself.  The computed one is within 2^-23 of itself, and a tie, a float,
+// comes out as it is; so the codes are those of exact arithmetic.
 //
 // Few rows: a workgroup owns 16 output channels and all of K, its waves interleave K in
 // pieces of 128 bytes, each through LDS of its own, and add their int32 sums at the end.
@@ -25,8 +29,8 @@ constexpr int kQThreads = 256;
 constexpr int kQVec = 4;  // 8-value vectors a thread keeps; longer rows are read twice
 
 // rint(127 x / top) as the low byte of a float: t = 127 x is exact, q = t / top follows from t * (1 / top) by one
-// correction, which gives the quotient itself where that is a float (every tie is) and within its last place elsewhere,
-// far from any tie; adding 1.5 * 2^23 rounds it to an integer, ties to even.  A fifth of the instructions of a
+// correction, which gives the quotient itself where that is a float (every tie is) and within its last place elsewhere;
+// adding 1.5 * 2^23 rounds it to an integer, ties to even.  A fifth of the instructions of a
 // division and a conversion.
 __device__ __forceinline__ uint32_t code_bits(float x, float top, float inv) {
     const float t = x * 127.0f;

@@ -210,3 +210,26 @@ def test_linear_long_sums(nq, device, m, n, k, tile):
     _check(out[:, :n], q, s, w, sw)
     again = linear_int8(q, s, w, sw)
     assert torch.equal(again.view(torch.int16), out[:, :n].contiguous().view(torch.int16))
+
+
+def test_quantize_every_quotient(nq, device):
+    """Every significand under every maximum's, eleven exponents down (below them every code is 0), both signs, against integer
+    arithmetic; the same rows near the ends of bf16's range."""
+
+    from nari_qwen3_tts_amd.layers import quantize_int8_rows
+
+    a, k, b = np.arange(128, 256), np.arange(11), np.arange(128, 256)
+    x = (a[None, :] * 2.0 ** -k[:, None].astype(np.float64)).reshape(-1)  # [11 * 128]
+    rows = np.minimum(x, b[:, None])  # what lies above a row's maximum is the maximum
+    rows[:, 1::2] *= -1
+    rows = np.concatenate((rows, np.repeat(b[:, None], 16, 1)), 1)
+    halves = np.abs(rows) * 2**10  # integers
+    num, den = (254 * halves).astype(np.int64), (b[:, None] << 10).astype(np.int64)
+    whole, rest = num // (2 * den), num % (2 * den)
+    codes = np.sign(rows) * (whole + ((rest > den) | ((rest == den) & (whole % 2 == 1))))
+    for power in (0, 100, 119, -60, -100):
+        t = torch.from_numpy(rows * 2.0**power).to(device).to(torch.bfloat16)
+        assert np.array_equal(to_np(t), (rows * 2.0**power).astype(np.float32))  # bf16 holds them
+        q, s = quantize_int8_rows(t)
+        assert np.array_equal(q.cpu().numpy(), codes)
+        assert torch.equal(s.cpu(), torch.from_numpy((b * 2.0**power).astype(np.float32) / np.float32(127)))

@@ -27,6 +27,24 @@ def test_quantize_rows_against_fractions():
         assert got.tolist() == [round(127 * Fraction(float(v)) / top) for v in row]  # round: ties to even
 
 
+def test_quotients_keep_away_from_ties():
+    """Every pair of bf16 significands and every exponent between them that matters: 127 a / (b 2^k) is a tie or at least
+    1 / (254 a) > 2^-16 of itself from one, in integers; and float64 quotients round as the exact ones."""
+
+    a, b = np.arange(1, 256)[:, None], np.arange(128, 256)[None, :]
+    for k in range(12):
+        num, den = 254 * a, b << k  # the quotient in halves
+        if k == 0:
+            a_max = np.minimum(a, b)
+            num = 254 * a_max
+        near = 2 * ((num // den) // 2) + 1  # the odd number of halves around it
+        off = np.abs(num - near * den)
+        assert (((off == 0) | (off * 254 * np.minimum(a, 255) >= num)).all()) and ((off == 0) | (off * 2**16 > num)).all()
+        whole, rest = num // (2 * den), num % (2 * den)
+        exact = whole + ((rest > den) | ((rest == den) & (whole % 2 == 1)))
+        assert np.array_equal(np.rint(num / (2 * den)).astype(np.int64), exact)
+
+
 def test_linear_closed_form():
     q, w = np.array([[1, 2], [-127, 127]], np.int8), np.array([[3, 4], [127, -127], [0, 1]], np.int8)
     y = o_int8.linear(q, [0.5, 2.0], w, [1.0, 1.0, 4.0])
