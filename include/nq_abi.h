@@ -227,7 +227,9 @@ int nq_paged_attention_noalloc(const int32_t *qo_indptr, const int32_t *kv_indpt
  * (rint, ties to even) when the scale grows, slots behind the run keep their
  * codes and count as empty.  A NaN or infinity in the run, or an earlier scale
  * that is negative or not finite (o > 0), makes the block's scale NaN.  A slot outside the pool is skipped
- * and sets status (device int32, may be NULL) to NQ_ERR_INVALID_ARGUMENT.  The
+ * and sets status (device int32, may be NULL) to NQ_ERR_INVALID_ARGUMENT.  A slot may be
+ * written again (a token was discarded): the block keeps a scale that the discarded one
+ * raised, or made NaN, until a run that begins at its first slot.  The
  * runs of one call are in different blocks: what a block that two runs share
  * holds afterwards is not specified.
  *

@@ -134,6 +134,30 @@ def test_read_outside_the_pool(nq, device):
     assert int(status) == -1 and not k[1:].any() and not v[1:].any() and k[0].any()
 
 
+def test_write_over_discarded_tokens(nq, device):
+    """A slot written again: the block keeps the step of a discarded outlier, at most one step off, and a discarded NaN, until
+    it is written from its first slot."""
+
+    from nari_qwen3_tts_amd.kernels import paged_cache_read_int8
+
+    rng = np.random.default_rng(18)
+    codes, scales = _pool(device, rng, 2, 16, 2, 64)
+    x = _bf16(rng, device, 2, 8, 2, 64)
+    at = _slots(device, [1] * 8, list(range(8)))
+    for slots, values in ((slice(0, 5), x[:, :5]), (slice(5, 6), x[:, 5:6] * 64.0), (slice(5, 8), x[:, 5:])):
+        _check_write(codes, scales, values[0], values[1], at[0][slots], at[1][slots])
+    for got, want, step in zip(paged_cache_read_int8(codes, scales, *at), x, scales[1, :, 0]):
+        off = (got.float() - want.float()).abs()
+        assert (off < step[:, None]).all() and step.min() >= 0.5  # 64 times values of some 2 in 127 codes
+    bad = x[:, 5:6].clone()
+    bad[0, 0, 1, 3] = float("nan")
+    for values in (bad, x[:, 5:6]):
+        _check_write(codes, scales, values[0], values[1], at[0][5:6], at[1][5:6])
+        assert scales[1, 0, 0, 1].isnan() and scales[1, 1].isfinite().all()
+    _check_write(codes, scales, x[0], x[1], *at)
+    assert scales[1].isfinite().all() and (scales[1] <= 2.0**-4).all()
+
+
 # -- attention -----------------------------------------------------------------------------------------
 
 
