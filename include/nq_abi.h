@@ -266,7 +266,8 @@ int nq_kv_int8_read(const int8_t *codes, int64_t c_page, int64_t c_kind, int64_t
  * [0, num_pages) is skipped and sets status (may be NULL) to
  * NQ_ERR_INVALID_ARGUMENT.  Up to 16 query heads per kv head; q, out and their
  * strides are multiples of 16 bytes.  workspace holds the partial results of
- * rows cut over workgroups; calls that overlap in time need one each.  Results do not depend on
+ * rows cut over workgroups; calls that overlap in time need one each.  The scores are fp32 sums of q times
+ * code: |q| stays below 2^114.  Results do not depend on
  * the order in which workgroups run.
  */
 int64_t nq_paged_attention_int8_workspace_bytes(int tokens, int rows, int num_qo_heads,

@@ -43,7 +43,7 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
 }
 
 // A workgroup a row, which stays in registers between the maximum and the codes up to 8192 values.  Bound by HBM:
-// 4001 rows of 6144 (74 MB) 14.9 us, 4.9 TB/s; by its launch and one round trip at 1 row of 2048, 2.4 us.
+// 4001 rows of 6144 (74 MB) 14.6 us, 5.1 TB/s; by its launch and one round trip at 1 row of 2048, 2.4 us.
 __global__ void __launch_bounds__(kQThreads)
 quantize_int8_rows_kernel(const uint16_t *__restrict__ x, int64_t x_s0, int K, int8_t *__restrict__ q, int64_t q_s0,
                           float *__restrict__ scales) {
@@ -241,10 +241,12 @@ int8_rows_kernel(Int8Args a) {
 // loads themselves (a register on the way would cost its write to LDS: 0.14 us a stage of 128 x 256).  Step k: stage k
 // has arrived, the loads of stage k + 2 are issued; the operands of each 32 bytes are read while the MFMAs of the 32
 // before run, also across the barrier.  The results cross LDS once more, so that they leave in whole lines.
-// Bound by LDS: 128 x 256 reads 128 KB and writes 48 KB a stage, 0.65 us at 128 bytes a clock, beside 0.51 us of MFMAs;
-// the stage takes 1.0 us, and launch, first loads and results 9 us.  640 x 12288 (K 2048) 22.9 us = 1410 TOP/s, 4001 x
-// 2048 (K 6144) 57.4 us = 1750 TOP/s (2496 is what a library's 8192^3 reaches).  Other waves for that tile at the same
-// sizes: 2 x 2 of 64 x 128 33 and 69 us, 1 x 4 of 128 x 64 32 and 68, 4 x 2 of 32 x 64 (128 x 128) 30 and 70.
+// No unit is full: at 4001 x 2048 (K 6144) the MFMAs run in 38 % of the clocks and LDS in 21 % (128 KB read a stage, at 256
+// bytes a clock), while the waves wait to issue in 54 % of theirs: the eight waves of a CU's one workgroup (its buffers
+// take the LDS) meet at every stage's barrier.  A stage takes 1.0 us with every CU busy, launch, first loads and results
+// 9 us.  640 x 12288 (K 2048) 22.5 us = 1430 TOP/s, 4001 x 2048 (K 6144) 56.6 us = 1780 TOP/s (2496 is what a library's
+// 8192^3 reaches).  Other waves for that tile at the same sizes: 2 x 2 of 64 x 128 33 and 69 us, 1 x 4 of 128 x 64 32 and
+// 68, 4 x 2 of 32 x 64 (128 x 128) 30 and 70 (24.4 and 67.9 since).
 template <int WM, int WN, int TM, int TN>
 __global__ void __launch_bounds__(WM * WN * kWave)
 int8_tile_kernel(Int8Args a, int tiles_m, int tiles) {
@@ -402,11 +404,14 @@ void launch_tiles(const Int8Args &a, hipStream_t st) {
 }
 
 // Rows and columns of out a workgroup takes.  Few tiles: the waves split K.  Otherwise the largest tile that still gives every
-// CU one: a stage of 128 bytes takes 0.29, 0.38 and 1.0 us at 64 x 64, 64 x 128 and 128 x 256.  Measured, K 2048, us:
-//   M 64  N 4096:  64-row pieces 5.5, 32-row pieces 6.6, 64 x 64 tiles 8.4;   N 6144: 9.8, 9.4, 8.4
-//   M 32  N 6144:  32-row pieces 6.8, 64 x 64 tiles 8.2;                      N 12288: 10.0, 8.4
-//   M 256 N 4096:  64 x 64 tiles 9.1, 64 x 128 9.6, 128 x 256 19;             N 6144: 11.0, 10.1, 20
-//   M 640 N 6144:  64 x 128 tiles 15.8, 128 x 256 21.0;                       N 12288: 28.0, 24.4 (22.9 since)
+// CU one: a stage of 128 bytes takes 0.28, 0.34 and 0.72 us at 64 x 64, 64 x 128 and 128 x 256 (1.0 with every CU busy).
+// Measured, K 2048, us (the rule's own first):
+//   M 16  N 4096:  16-row pieces 3.1, 32-row 3.6;                 N 12288: 7.3, 64 x 64 tiles 7.4
+//   M 32  N 6144:  32-row pieces 7.1, 64 x 64 tiles 7.2;          N 12288: 64 x 64 tiles 7.5, 32-row pieces 10.2
+//   M 64  N 4096:  64-row pieces 5.2, 32-row 6.2, 64 x 64 6.4;    N 6144: 64 x 64 tiles 7.4, 64-row pieces 9.9
+//   M 256 N 4096:  64 x 64 tiles 7.6, 64 x 128 8.7;               N 6144: 64 x 128 tiles 8.9, 64 x 64 9.6, 128 x 256 17.5
+//   M 640 N 6144:  64 x 128 tiles 15.0, 128 x 256 18.5;           N 12288: 128 x 256 tiles 21.9, 64 x 128 26.8
+//   M 1000 N 12288: 128 x 256 tiles 37.4, 64 x 128 39.0 (128 x 128, which is not kept, 35.6; at 640 x 6144 13.6)
 constexpr int tile_id(int rows, int columns) { return rows << 16 | columns; }
 int tile_for(int M, int N) {
     auto count = [&](int bm, int bn) { return static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn); };

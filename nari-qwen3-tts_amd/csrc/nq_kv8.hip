@@ -10,9 +10,11 @@
 // step (1/2 + 1/4 + ...).  The price is a step of up to twice max |x| / 127.
 //
 // Attention.  S = q . c_K with the codes widened to bf16 (exact), each block's
-// scale applied to its 16 columns of fp32 scores; P times the V scale of its
-// block rounded to bf16, the codes of V widened, fp32 sums.  So the cache moves half
-// the bytes of a bf16 one and is never written out wider.
+// scale applied to its 16 columns of fp32 scores.  P V in bf16 with fp32 sums: in
+// decode V's scale multiplies P before it is rounded to bf16 and V's codes are
+// widened as they are; in prefill P is rounded alone (2^-8 of a weight either way, as
+// the bf16 cache's attention rounds it) and V's codes are widened times their scale.
+// So the cache moves half the bytes of a bf16 one and is never written out wider.
 #include <stddef.h>
 
 #include <type_traits>
@@ -84,8 +86,9 @@ __device__ __forceinline__ bf16x8_t widen8(uint32_t a, uint32_t b) {
 // quantised with one scale, and a block's earlier slots are read only by the wave that may rescale them.
 // Lane l holds slots l / (D/8) + i * (512/D), values 8 (l % (D/8)) .. + 7.
 // Bound by its chain of loads (slots, then the block's scale and tokens) where tokens are few: 64 single tokens 4.5 us,
-// 4 of them the launch and the chain; by HBM where they are many: 7677 tokens of 8 heads of 128 (47 MB) 14.8 us, 3.2 TB/s,
-// one round of waves that all load first and store last.
+// 4 of them the launch and the chain.  Where they are many, 7677 tokens of 8 heads of 128 (47 MB) 14.8 us, 3.2 TB/s: 95 VGPRs
+// hold five waves a SIMD, so its 7680 waves are a round and a half, each of which loads first and stores last (they wait in 51 %
+// of their clocks, the vector units run in 31 %).
 template <int D>
 __global__ void __launch_bounds__(kKv8Threads)
 kv8_write_kernel(const uint16_t *__restrict__ key, int64_t k_s0, int64_t k_s1, const uint16_t *__restrict__ value,
@@ -176,8 +179,8 @@ kv8_write_kernel(const uint16_t *__restrict__ key, int64_t k_s0, int64_t k_s1, c
 }
 
 // ---------------------------------------------------------------------------------------------
-// Read back: thread per 16 codes of one (token, kind, head).  Bound by HBM: 7677 tokens of 8 heads of 128 (47 MB) 11.3 us,
-// 4.2 TB/s.
+// Read back: thread per 16 codes of one (token, kind, head).  Bound by HBM: 7677 tokens of 8 heads of 128 (47 MB) 10.7 us,
+// 4.4 TB/s.
 template <int D>
 __global__ void __launch_bounds__(kKv8Threads)
 kv8_read_kernel(Pool8 pool, const int64_t *__restrict__ pages, const int64_t *__restrict__ offsets, int tokens,
@@ -678,13 +681,14 @@ kv8_merge_kernel(Attend8 a, int waves, const float2 *__restrict__ part_ml, const
 // tile's loads are in flight while the one before it is multiplied.  Sums are rescaled only when a maximum has grown
 // by more than 2^8 (P stays below that, and bf16 and fp32 lose nothing by it).  With few tiles the key range is
 // cut into pieces, joined by kv8_join_kernel.
-// 1856 queries of 16 heads over 6001 keys (77 GFLOP): 127 us and 10 for the join, 610 TFLOP/s; 64 rows of 128 queries over
-// 512 keys 67 us.  A step of eight waves takes 1.25 us: 0.49 us of MFMAs (two waves a SIMD), 0.8 of vector instructions,
-// 0.6 of LDS (139 KB read, 17 KB written a workgroup), the loads' issue, and the barrier, which overlap in part only;
-// without the loads it takes 0.17 us less.  With uniform pieces the longest one takes 94 tiles where 79 is the mean.
+// 1856 queries of 16 heads over 6001 keys (77 GFLOP): 108 us and 10 for the join, 716 TFLOP/s at the clocks of a steady
+// load (124 us in the first milliseconds of one); 64 rows of 128 queries over 512 keys 60 us.  No unit is full: the vector
+// units run in 42 % of the clocks, the MFMAs in 29 %, LDS in 27 % (a fifth of that the conflicts of V's writes); they overlap
+// in part only, around one barrier a step.  The loads' issue takes 0.17 us of a step of 1.25 (at the first milliseconds'
+// clocks).  With uniform pieces the longest one takes 94 tiles where 79 is the mean.
 // 64-key tiles take 1 to 10 % less where one long prompt fills the card and up to 1.6 times as long for batches
-// (registers spill, one workgroup a CU).  Tried and no faster: 64 columns a wave at one wave a SIMD (156 us), spans that
-// cross tiles for even work (143 us), staging two steps ahead.
+// (registers spill, one workgroup a CU).  Tried and no faster (against 127 us): 64 columns a wave at one wave a SIMD (156
+// us), spans that cross tiles for even work (143 us), staging two steps ahead.
 constexpr int kKeys = 32;
 constexpr float kLag = 8.0f;
 
@@ -742,8 +746,9 @@ struct Smem8 {
     Meta8 meta;
 };
 constexpr int kAbsent = 1, kPoison = 2;
-// Places of 16-byte chunks, free of conflicts for the operand reads (32 rows, two chunks each): rows of K one chunk longer
-// than their values, V's chunks exclusive-ored with bits of their row.
+// Places of 16-byte chunks, free of conflicts for the operand reads (32 rows, two chunks each) and for K's writes: rows of K
+// one chunk longer than their values, V's chunks exclusive-ored with bits of their row.  V's writes, eight bytes in each of
+// 16 rows and four quads, take 16 clocks for the 4 of neighbouring ones.
 template <int D>
 __device__ __forceinline__ int k_chunk(int key, int chunk) {
     return key * (D / 8 + 1) + chunk;
@@ -1107,7 +1112,7 @@ kv8_prefill_kernel(Attend8 a, Pool8 pool, int splits, int skip_single, float2 *_
 }
 
 // Joins the pieces of a tile, in order: D/8 threads a column, every piece's values in flight at once.  Bound by its reads:
-// 66 MB of partials 9.2 us.
+// 31 MB of partials 10 us.
 constexpr int kMaxPieces = 8;
 template <int D>
 __global__ void __launch_bounds__(kKv8Threads)
@@ -1171,8 +1176,9 @@ struct Prefill8 {
 // Four waves, two workgroups a CU: their starts, barriers and ends overlap.  Eight (one a CU) stage each tile half as often
 // per column, which counts where few tiles have long key ranges, of heads of 128: rows of 2000 columns and more that still
 // leave two pieces a workgroup.  Measured with four and eight waves, us, 16 query heads of 128 on 8:
-//   1 row of 1800 queries over 6001 keys 145, 137;  1 of 2000 over 2000 60, 57;  1 of 1000 over 12000 139, 131
-//   1 of 4000 over 4000 128, 148;  4 of 2000 over 2000 116, 137;  64 of 128 over 512 67, 78;  1 of 300 over 300 17.4, 20.3
+//   1 row of 1800 queries over 6001 keys 129, 117;  1 of 2000 over 2000 56, 52;  1 of 1000 over 12000 137, 123
+//   1 of 4000 over 4000 117, 129;  4 of 2000 over 2000 115, 126;  64 of 128 over 512 60, 68;  1 of 300 over 300 15.3, 18.6
+// (past what two pieces tell, where the rule takes four: 2 of 2000 over 4000 161, 139;  1 of 8000 over 8000 348, 302)
 // Pieces: as many as fit the CUs at once, up to kMaxPieces.
 Prefill8 prefill_plan(int tokens, int rows, int group, int heads, int D) {
     const int64_t columns = static_cast<int64_t>(tokens) * group;
