@@ -405,8 +405,9 @@ def paged_cache_write_int8_(key: torch.Tensor, value: torch.Tensor, layer_cache:
     on takes the slots before it as held and those behind the written ones as empty.  Tokens that
     share a block stand next to each other in slot order (as a request's do); two separate runs into one block in
     one call leave that block unspecified.  A NaN or infinity makes its block's scale NaN.  A slot may be
-    written again where its token was discarded, but scales do not shrink: the block's other tokens keep the coarser step that a
-    discarded outlier brought, and a discarded NaN leaves the block NaN, until the block is written from its first slot again.  A slot outside the pool is skipped and
+    written again where its token was discarded, but scales do not shrink: the block's other tokens keep the coarser
+    step that a discarded outlier brought, and a discarded NaN leaves the block NaN, until the block is written from
+    its first slot again.  A slot outside the pool is skipped and
     ``status`` (int32, optional) set to NQ_ERR_INVALID_ARGUMENT.  No counterpart in the reference."""
 
     heads, d, cache = _int8_cache(layer_cache, layer_scales)
