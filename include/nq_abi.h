@@ -877,8 +877,9 @@ int nq_codec_transconv_overlap(const int32_t *offsets, int B, int u_in, int stri
  * |x|) (ties to even) and the scale max |x| / 127: activations per token, or
  * weights [N, K] per output channel.  A row of zeros has scale 1, a row that holds a NaN
  * or an infinity codes of 0 and a NaN scale.
- * nq_linear_int8: out[m, n] = bf16(sum_k xq[m, k] wq[n, k] * sw[n] * sx[m]),
- * the sum in int32, exact for codes within +-127, then two fp32 products in this order.  K is a
+ * nq_linear_int8: out[m, n] = bf16(sum_k xq[m, k] wq[n, k] * sx[m] * sw[n]),
+ * the sum in int32, exact for codes within +-127, then two fp32 products in this order (sw first where
+ * sx is above 2^96, so that it is the result that has to fit).  K is a
  * multiple of 16, up to 2^17 for the product; codes
  * and their row strides are multiples of 16 bytes (x of the quantisation and its codes' rows: of 8
  * elements).  M, N: any.  nq_linear_int8_tile: rows << 16 | columns of out that one workgroup of the product

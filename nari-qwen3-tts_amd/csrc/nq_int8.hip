@@ -1,5 +1,5 @@
 // Products of 8-bit integers with a scale for each token and output channel:
-//   out[m, n] = bf16(float(sum_k cx[m, k] cw[n, k]) * sw[n] * sx[m])
+//   out[m, n] = bf16(float(sum_k cx[m, k] cw[n, k]) * sx[m] * sw[n])
 // with the sum in int32 (exact for K <= 2^17), and the quantisation of rows that
 // makes both operands: s = max |x| / 127, c = rint(127 x / max |x|).  127 x is exact
 // in fp32 for a bf16 x.  With significands a of x and b of max |x| (integers below
@@ -126,9 +126,12 @@ struct Int8Args {
     int wide;  // out rows take 16-byte stores
 };
 
-// The weights' scale first: a model's weights keep sum * sw far inside fp32, so that what the activations' scale makes of it
-// is the result, or beyond bf16 with it.
-__device__ __forceinline__ float scaled(int sum, float sx, float sw) { return static_cast<float>(sum) * sw * sx; }
+// |sum| <= 2^31, so that sum * sx stays inside fp32 up to sx = 2^96; a larger sx comes last, when a model's weights have
+// made sum * sw small enough for the result, where that fits.
+__device__ __forceinline__ float scaled(int sum, float sx, float sw) {
+    const bool far = sx > 0x1p96f;
+    return static_cast<float>(sum) * (far ? sw : sx) * (far ? sx : sw);
+}
 
 constexpr int kStage = 128;         // bytes of K a stage
 constexpr int kChunks = kStage / 16;

@@ -783,7 +783,7 @@ def quantize_int8_rows(x: torch.Tensor, q: torch.Tensor | None = None,
 
 def linear_int8(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, weight_scales: torch.Tensor,
                 out: torch.Tensor | None = None) -> torch.Tensor:
-    """out[m, n] = bf16(sum_k q[m, k] weight_q[n, k] * weight_scales[n] * scales[m]) for int8 codes [rows, in] and
+    """out[m, n] = bf16(sum_k q[m, k] weight_q[n, k] * scales[m] * weight_scales[n]) for int8 codes [rows, in] and
     [out, in] with the scales of ``quantize_int8_rows``; the sum is exact (int32), so the same codes give the
     same bits at any number of rows.  ``in`` a multiple of 16 up to 131072 (codes within +-127), any rows and out."""
 
