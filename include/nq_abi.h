@@ -891,6 +891,22 @@ int nq_linear_int8_tile(int M, int N);
 int nq_linear_int8(const int8_t *xq, int64_t x_s0, const float *sx, const int8_t *wq, int64_t w_s0,
                    const float *sw, int M, int N, int K, uint16_t *out, int64_t o_s0, void *stream);
 
+/*
+ * RMS norm of bf16 rows answered in the operands of nq_linear_int8 (no counterpart in the reference, whose 8-bit
+ * norm output is FP8 with block scales).  nq_add_rmsnorm_int8: residual = bf16(residual + hidden), stored; with
+ * y = residual * weight / sqrt(mean(residual^2) + eps), never rounded, scales[r] = max |y| / 127 and codes rint(y /
+ * scale) (ties to even), which are those of exact arithmetic.  nq_rmsnorm_int8: the same of x, which it does not
+ * change.  A row whose weighted values are all zero has scale 1, one that holds a NaN or an infinity (in a row or
+ * in the weight) codes of 0 and a NaN scale.  width is a multiple of 16; rows and weight are 16-byte aligned, row
+ * strides and the codes' address multiples of 8 elements; eps is not negative.  hidden and residual do not overlap,
+ * nor the rows of residual.
+ */
+int nq_add_rmsnorm_int8(const uint16_t *hidden, int64_t h_s0, uint16_t *residual, int64_t r_s0,
+                        const uint16_t *weight, int rows, int width, float eps, int8_t *q, int64_t q_s0,
+                        float *scales, void *stream);
+int nq_rmsnorm_int8(const uint16_t *x, int64_t x_s0, const uint16_t *weight, int rows, int width, float eps,
+                    int8_t *q, int64_t q_s0, float *scales, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -92,6 +92,8 @@ _SIGNATURES: dict[str, list] = {
     "nq_add_rmsnorm_fp8": [_P, _P, _P, _I, _I, _F, _P, _L, _P, _L, _P],
     "nq_linear_add_rmsnorm_fp8": [_P, _L, _P, _L, _I, _I, _I, _P, _P, _F, _P, _L, _P, _L, _P, _L, _P],
     "nq_quantize_int8_rows": [_P, _L, _I, _I, _P, _L, _P, _P],
+    "nq_add_rmsnorm_int8": [_P, _L, _P, _L, _P, _I, _I, _F, _P, _L, _P, _P],
+    "nq_rmsnorm_int8": [_P, _L, _P, _I, _I, _F, _P, _L, _P, _P],
     "nq_linear_int8_tile": [_I, _I],
     "nq_linear_int8": [_P, _L, _P, _P, _L, _P, _I, _I, _I, _P, _L, _P],
     "nq_linear_fp8_splits": [_I, _I, _I],

@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "nq_common.h"
+#include "nq_int8_codes.h"
 #include "nq_internal.h"
 
 namespace nq {
@@ -27,20 +28,6 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kQThreads = 256;
 constexpr int kQVec = 4;  // 8-value vectors a thread keeps; longer rows are read twice
-
-// rint(127 x / top) as the low byte of a float: t = 127 x is exact, q = t / top follows from t * (1 / top) by one
-// correction, which gives the quotient itself where that is a float (every tie is) and within its last place elsewhere;
-// adding 1.5 * 2^23 rounds it to an integer, ties to even.  A fifth of the instructions of a
-// division and a conversion.
-__device__ __forceinline__ uint32_t code_bits(float x, float top, float inv) {
-    const float t = x * 127.0f;
-    const float q = t * inv;
-    return __float_as_uint(fmaf(fmaf(-q, top, t), inv, q) + 12582912.0f);
-}
-__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u),
-                                 0x05040100u);
-}
 
 // A workgroup a row, which stays in registers between the maximum and the codes up to 8192 values.  Bound by HBM:
 // 4001 rows of 6144 (74 MB) 14.6 us, 5.1 TB/s; by its launch and one round trip at 1 row of 2048, 2.4 us.

@@ -747,6 +747,74 @@ def linear_fp8_swiglu(q: torch.Tensor, scales: torch.Tensor, packed: torch.Tenso
     return out
 
 
+def _int8_out(rows: int, k: int, device, q: torch.Tensor | None, scales: torch.Tensor | None):
+    """Codes, their row stride and scales of ``rows`` quantised rows: the caller's, checked, or new ones."""
+
+    q_row = k
+    if q is None:
+        q = torch.empty(rows, k, dtype=torch.int8, device=device)  # sizes as numbers parse faster than as a tuple
+    elif q.dtype is not torch.int8:
+        raise TypeError("int8 codes expected")
+    elif q.shape != (rows, k) or q.stride(1) != 1:
+        raise ValueError(f"codes must be [{rows}, {k}] with unit inner stride")
+    else:
+        q_row = q.stride(0)
+    if scales is None:
+        scales = torch.empty(rows, dtype=torch.float32, device=device)
+    elif scales.dtype is not torch.float32:
+        raise TypeError("float32 scales expected")
+    elif scales.shape != (rows,) or not scales.is_contiguous():
+        raise ValueError(f"scales must be [{rows}], contiguous")
+    return q, q_row, scales
+
+
+def _norm_int8_args(x: torch.Tensor, weight: torch.Tensor, eps: float):
+    if x.dtype is not torch.bfloat16 or weight.dtype is not torch.bfloat16:
+        raise TypeError("the int8 norm needs bf16 rows and a bf16 weight")
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 2 or strides[1] != 1:
+        raise ValueError("the int8 norm needs [rows, width] with unit inner stride")
+    rows, width = shape
+    if width < 16 or width % 16:
+        raise ValueError("the int8 norm needs a multiple of 16 columns")
+    if weight.shape != (width,) or not weight.is_contiguous():
+        raise ValueError("norm weight must match the hidden width, contiguous")
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative")
+    return rows, width, strides[0]
+
+
+def add_rmsnorm_int8(hidden: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float,
+                     q: torch.Tensor | None = None,
+                     scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """residual <- bf16(residual + hidden), in place; its rmsnorm, in one launch, as ``linear_int8`` takes it: int8 codes
+    [rows, width] and float32 scales [rows].  The normalised row is quantised unrounded, so a code may differ by one
+    from ``add_rmsnorm`` followed by ``quantize_int8_rows``.  Rows bf16 with any stride (of 8 elements' multiples),
+    width a multiple of 16; zero, NaN and infinite rows as in ``quantize_int8_rows``."""
+
+    rows, width, r_row = _norm_int8_args(residual, weight, eps)
+    if hidden.dtype is not torch.bfloat16:
+        raise TypeError("hidden_states must be bf16")
+    if hidden.shape != residual.shape or hidden.stride(1) != 1 or (rows and hidden.data_ptr() == residual.data_ptr()):
+        raise ValueError("fused add-RMSNorm needs distinct tensors of one shape with unit inner stride")
+    q, q_row, scales = _int8_out(rows, width, residual.device, q, scales)
+    _lib.launch(_lib.one_device(hidden, residual, weight, q, scales), "nq_add_rmsnorm_int8", hidden.data_ptr(),
+                hidden.stride(0), residual.data_ptr(), r_row, weight.data_ptr(), rows, width, eps, q.data_ptr(), q_row,
+                scales.data_ptr())
+    return q, scales
+
+
+def rmsnorm_int8(hidden: torch.Tensor, weight: torch.Tensor, eps: float, q: torch.Tensor | None = None,
+                 scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``add_rmsnorm_int8`` without an addition (a first layer's norm): the rmsnorm of ``hidden``, which stays as it is."""
+
+    rows, width, h_row = _norm_int8_args(hidden, weight, eps)
+    q, q_row, scales = _int8_out(rows, width, hidden.device, q, scales)
+    _lib.launch(_lib.one_device(hidden, weight, q, scales), "nq_rmsnorm_int8", hidden.data_ptr(), h_row,
+                weight.data_ptr(), rows, width, eps, q.data_ptr(), q_row, scales.data_ptr())
+    return q, scales
+
+
 def quantize_int8_rows(x: torch.Tensor, q: torch.Tensor | None = None,
                        scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """bf16 [rows, K] -> (int8 codes rint(127 x / max|x|), float32 scales max|x| / 127 [rows]): activations per
@@ -761,21 +829,7 @@ def quantize_int8_rows(x: torch.Tensor, q: torch.Tensor | None = None,
     rows, k = shape
     if k < 16 or k % 16:
         raise ValueError("int8 row quantization needs a multiple of 16 columns")
-    q_row = k
-    if q is None:
-        q = torch.empty(rows, k, dtype=torch.int8, device=x.device)  # sizes as numbers parse faster than as a tuple
-    elif q.dtype is not torch.int8:
-        raise TypeError("int8 codes expected")
-    elif q.shape != shape or q.stride(1) != 1:
-        raise ValueError(f"codes must be [{rows}, {k}] with unit inner stride")
-    else:
-        q_row = q.stride(0)
-    if scales is None:
-        scales = torch.empty(rows, dtype=torch.float32, device=x.device)
-    elif scales.dtype is not torch.float32:
-        raise TypeError("float32 scales expected")
-    elif scales.shape != (rows,) or not scales.is_contiguous():
-        raise ValueError(f"scales must be [{rows}], contiguous")
+    q, q_row, scales = _int8_out(rows, k, x.device, q, scales)
     _lib.launch(_lib.one_device(x, q, scales), "nq_quantize_int8_rows", x.data_ptr(), strides[0], rows, k,
                 q.data_ptr(), q_row, scales.data_ptr())
     return q, scales
@@ -814,6 +868,8 @@ def linear_int8(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, w
 
 
 __all__ = [
+    "add_rmsnorm_int8",
+    "rmsnorm_int8",
     "linear_int8",
     "quantize_int8_rows",
     "NormRows",
