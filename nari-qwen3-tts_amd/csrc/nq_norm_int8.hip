@@ -19,7 +19,7 @@ struct NormInt8Args {
     uint16_t *residual;
     int64_t r_s0;
     const uint16_t *weight;
-    int width;
+    int rows, width;
     float eps;
     int8_t *q;
     int64_t q_s0;
@@ -27,16 +27,19 @@ struct NormInt8Args {
 };
 
 // Rows whose sums or products leave fp32's comfort (values beyond 2^60 or all below 2^-30, NaN, infinities, zeros) are
-// worked in double, which holds every product and square of bf16 values: a workgroup's second look at the row, from
-// what it stored.
-template <int T>
-__device__ __attribute__((noinline)) void norm_int8_row_wide(const NormInt8Args &a, int64_t row) {
-    __shared__ double s_ss[T / kWave], s_top[T / kWave];
+// worked in double, which holds every product and square of bf16 values: a second look at the row, from what its own
+// kWaves waves stored.
+template <int kWaves>
+__device__ __forceinline__ void norm_int8_row_wide(const NormInt8Args &a, int64_t row) {
+    __shared__ double s_ss[kWaves], s_top[kWaves];
+    constexpr int T = kWaves * kWave;
+    const int tid = threadIdx.x;
     const uint16_t *x = a.residual + row * a.r_s0;
-    __syncthreads();  // the row's stores, by other threads too
     double ss = 0.0, top = 0.0;
-    bool odd = false;
-    for (int i = threadIdx.x; i < a.width; i += T) {
+    int odd = 0;
+    if constexpr (kWaves > 1) __syncthreads();  // the row's stores, by other waves too
+    else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    for (int i = tid; i < a.width; i += T) {
         const double v = bf16_to_f32(x[i]), p = v * bf16_to_f32(a.weight[i]);
         ss += v * v;
         top = fmax(top, fabs(p));
@@ -47,34 +50,40 @@ __device__ __attribute__((noinline)) void norm_int8_row_wide(const NormInt8Args 
         ss += __shfl_xor(ss, m, kWave);
         top = fmax(top, __shfl_xor(top, m, kWave));
     }
-    odd = __syncthreads_or(odd);
-    if (threadIdx.x % kWave == 0) {
-        s_ss[threadIdx.x / kWave] = ss;
-        s_top[threadIdx.x / kWave] = top;
-    }
-    __syncthreads();
-    ss = 0.0;
-    for (int w = 0; w < T / kWave; ++w) {
-        ss += s_ss[w];
-        top = fmax(top, s_top[w]);
+    odd = __any(odd);
+    if constexpr (kWaves > 1) {
+        odd = __syncthreads_or(odd);
+        if (tid % kWave == 0) {
+            s_ss[tid / kWave] = ss;
+            s_top[tid / kWave] = top;
+        }
+        __syncthreads();
+        ss = 0.0;
+        for (int w = 0; w < kWaves; ++w) {
+            ss += s_ss[w];
+            top = fmax(top, s_top[w]);
+        }
     }
     const bool zero = odd || top == 0.0;
-    for (int i = threadIdx.x; i < a.width; i += T) {
+    for (int i = tid; i < a.width; i += T) {
         const double p = static_cast<double>(bf16_to_f32(x[i])) * bf16_to_f32(a.weight[i]);
         a.q[row * a.q_s0 + i] = zero ? 0 : static_cast<int8_t>(static_cast<int>(rint(127.0 * p / top)));
     }
-    if (threadIdx.x == 0)
+    if (tid == 0)
         a.scales[row] = odd ? __builtin_nanf("")
                             : zero ? 1.0f : static_cast<float>(top / (127.0 * sqrt(ss / a.width + a.eps)));
 }
 
-// A workgroup of T threads a row, which stays in registers between the sums and the codes up to 8 T kVec values; what is
-// longer is read twice.
-template <bool kAdd, int T, int kVec>
-__global__ void __launch_bounds__(T)
+// A workgroup of kWaves waves a row, which stays in registers between the sums and the codes up to 512 kWaves kVec
+// values; what is longer is read twice.  Bound by HBM where rows are many: 4001 x 2048 (57 MB) 11.8 us, 4.9 TB/s, 5000 x
+// 6144 39.7 us, 5.4 TB/s; by its launch and one round trip where they are few: 1 x 2048 2.7 us, replayed.
+template <bool kAdd, int kWaves, int kVec>
+__global__ void __launch_bounds__(kWaves * kWave)
 norm_int8_kernel(NormInt8Args a) {
-    __shared__ float s_ss[T / kWave], s_top[T / kWave];
-    __shared__ int s_odd[T / kWave];
+    constexpr int T = kWaves * kWave;
+    __shared__ float s_ss[kWaves], s_top[kWaves];
+    __shared__ int s_odd[kWaves];
+    const int tid = threadIdx.x;
     const int64_t row = blockIdx.x;
     const int nvec = a.width / 8;
     const uint16_t *h = a.hidden + row * a.h_s0;
@@ -83,7 +92,7 @@ norm_int8_kernel(NormInt8Args a) {
     float ss = 0.f, top = 0.f;
     bool odd = false;
     // the new residual (stored) and its products with the weight
-    auto sum = [&](uint4 rv, const uint4 &hv, const uint4 &wv, uint16_t *to, float (&out)[8]) {
+    auto sum = [&](uint4 rv, const uint4 &hv, const uint4 &wv, uint16_t *to, float (&out)[8]) __attribute__((always_inline)) {
         float x[8], w[8];
         if constexpr (kAdd) {
             float y[8];
@@ -106,7 +115,7 @@ norm_int8_kernel(NormInt8Args a) {
     uint4 rv[kVec], hv[kVec], wv[kVec];
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
-        const int vi = threadIdx.x + i * T;
+        const int vi = tid + i * T;
         const bool in = vi < nvec;
         rv[i] = in ? *reinterpret_cast<const uint4 *>(r + vi * 8) : make_uint4(0, 0, 0, 0);
         hv[i] = kAdd && in ? *reinterpret_cast<const uint4 *>(h + vi * 8) : make_uint4(0, 0, 0, 0);
@@ -114,10 +123,10 @@ norm_int8_kernel(NormInt8Args a) {
     }
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
-        const int vi = threadIdx.x + i * T;
+        const int vi = tid + i * T;
         if (vi < nvec) sum(rv[i], hv[i], wv[i], r + vi * 8, p[i]);
     }
-    for (int vi = threadIdx.x + kVec * T; vi < nvec; vi += T) {
+    for (int vi = tid + kVec * T; vi < nvec; vi += T) {
         float out[8];
         sum(*reinterpret_cast<const uint4 *>(r + vi * 8),
             kAdd ? *reinterpret_cast<const uint4 *>(h + vi * 8) : make_uint4(0, 0, 0, 0),
@@ -126,8 +135,8 @@ norm_int8_kernel(NormInt8Args a) {
     ss = group_sum<kWave>(ss);
     top = group_max<kWave>(top);
     odd = __any(odd);
-    if constexpr (T > kWave) {
-        const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    if constexpr (kWaves > 1) {
+        const int lane = tid & (kWave - 1), wave = tid / kWave;
         if (lane == 0) {
             s_ss[wave] = ss;
             s_top[wave] = top;
@@ -137,7 +146,7 @@ norm_int8_kernel(NormInt8Args a) {
         ss = 0.f;
         int bad = 0;
 #pragma unroll
-        for (int w = 0; w < T / kWave; ++w) {
+        for (int w = 0; w < kWaves; ++w) {
             ss += s_ss[w];
             top = fmaxf(top, s_top[w]);
             bad |= s_odd[w];
@@ -146,11 +155,11 @@ norm_int8_kernel(NormInt8Args a) {
     }
     // 127 p, 1 / top and the products that decide a code are normal between these; so is the sum of squares
     if (odd || !(top > 0x1p-100f && top < 0x1p100f) || !(ss > 0x1p-60f && ss < 0x1p120f)) {
-        norm_int8_row_wide<T>(a, row);  // the row's every thread: the tests are of its sums
+        norm_int8_row_wide<kWaves>(a, row);  // the row's every thread: the tests are of its sums
         return;
     }
     const float inv = 1.0f / top;
-    auto put = [&](int vi, const float (&v)[8]) {
+    auto put = [&](int vi, const float (&v)[8]) __attribute__((always_inline)) {
         uint32_t c[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) c[e] = code_bits(v[e], top, inv);
@@ -159,10 +168,10 @@ norm_int8_kernel(NormInt8Args a) {
     };
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
-        const int vi = threadIdx.x + i * T;
+        const int vi = tid + i * T;
         if (vi < nvec) put(vi, p[i]);
     }
-    for (int vi = threadIdx.x + kVec * T; vi < nvec; vi += T) {
+    for (int vi = tid + kVec * T; vi < nvec; vi += T) {
         float x[8], w[8], v[8];
         unpack8(*reinterpret_cast<const uint4 *>(r + vi * 8), x);  // this thread's own store
         unpack8(*reinterpret_cast<const uint4 *>(a.weight + vi * 8), w);
@@ -170,19 +179,21 @@ norm_int8_kernel(NormInt8Args a) {
         for (int e = 0; e < 8; ++e) v[e] = x[e] * w[e];
         put(vi, v);
     }
-    if (threadIdx.x == 0) a.scales[row] = top / (127.0f * sqrtf(ss / static_cast<float>(a.width) + a.eps));
+    if (tid == 0) a.scales[row] = top / (127.0f * sqrtf(ss / static_cast<float>(a.width) + a.eps));
 }
 
 bool al(const void *p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-template <bool kAdd, int T, int kVec>
-int launch_as(const NormInt8Args &a, int rows, hipStream_t st) {
-    hipLaunchKernelGGL((norm_int8_kernel<kAdd, T, kVec>), dim3(rows), dim3(T), 0, st, a);
+template <bool kAdd, int kWaves, int kVec>
+int launch_as(const NormInt8Args &a, void *stream) {
+    hipLaunchKernelGGL((norm_int8_kernel<kAdd, kWaves, kVec>), dim3(a.rows), dim3(kWaves * kWave), 0,
+                       static_cast<hipStream_t>(stream), a);
     return NQ_LAUNCH_STATUS();
 }
 
 template <bool kAdd>
-int launch(const NormInt8Args &a, int rows, void *stream) {
+int launch(const NormInt8Args &a, void *stream) {
+    const int rows = a.rows;
     NQ_CHECK_ARG(rows >= 0 && a.width >= 0);
     if (rows == 0) return NQ_OK;
     NQ_CHECK_ARG(a.residual && a.weight && a.q && a.scales && a.width >= 16 && a.eps >= 0.f);
@@ -194,9 +205,15 @@ int launch(const NormInt8Args &a, int rows, void *stream) {
         NQ_CHECK_ARG(a.hidden && a.h_s0 >= 0);
         if (!al(a.hidden, 16) || (rows > 1 && a.h_s0 % 8)) return NQ_ERR_UNSUPPORTED;
     }
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    if (a.width <= 2048) return launch_as<kAdd, 256, 1>(a, rows, st);
-    return launch_as<kAdd, 256, 4>(a, rows, st);
+    // One vector of 8 a thread while that fills whole waves, up to four of them: a round trip less than with more a
+    // thread, and fewer idle or waiting waves than with more threads.  Measured, us, replayed, with 1, 2 and 4 waves of one
+    // vector: 100 x 512 2.76, 2.86, 2.93; 5000 x 512 5.3, 6.2, 7.9; 500 x 1024 3.67, 3.27, 3.35; 8000 x 1024 12.0, 11.9,
+    // 13.2; 64 x 2048 with 1, 2, 4 waves of one and 8 of two 4.9, -, 3.0, 3.0; 4001 x 2048 12.3, -, 11.8, 15.1.  Longer
+    // rows with 4 of one, 4 of four, 8 of two and 16 of one: 1 x 6144 4.0, 3.3, 3.0, 3.0; 5000 x 6144 41.5, 42.3, 39.7, 40.9.
+    if (a.width <= 512) return launch_as<kAdd, 1, 1>(a, stream);
+    if (a.width <= 1024) return launch_as<kAdd, 2, 1>(a, stream);
+    if (a.width <= 2048) return launch_as<kAdd, 4, 1>(a, stream);
+    return launch_as<kAdd, 8, 2>(a, stream);
 }
 
 }  // namespace
@@ -205,11 +222,11 @@ int launch(const NormInt8Args &a, int rows, void *stream) {
 extern "C" int nq_add_rmsnorm_int8(const uint16_t *hidden, int64_t h_s0, uint16_t *residual, int64_t r_s0,
                                    const uint16_t *weight, int rows, int width, float eps, int8_t *q, int64_t q_s0,
                                    float *scales, void *stream) {
-    return nq::launch<true>({hidden, h_s0, residual, r_s0, weight, width, eps, q, q_s0, scales}, rows, stream);
+    return nq::launch<true>({hidden, h_s0, residual, r_s0, weight, rows, width, eps, q, q_s0, scales}, stream);
 }
 
 extern "C" int nq_rmsnorm_int8(const uint16_t *x, int64_t x_s0, const uint16_t *weight, int rows, int width, float eps,
                                int8_t *q, int64_t q_s0, float *scales, void *stream) {
     // the rows are read alone: the kernel without the addition stores none
-    return nq::launch<false>({nullptr, 0, const_cast<uint16_t *>(x), x_s0, weight, width, eps, q, q_s0, scales}, rows, stream);
+    return nq::launch<false>({nullptr, 0, const_cast<uint16_t *>(x), x_s0, weight, rows, width, eps, q, q_s0, scales}, stream);
 }
