@@ -907,6 +907,23 @@ int nq_add_rmsnorm_int8(const uint16_t *hidden, int64_t h_s0, uint16_t *residual
 int nq_rmsnorm_int8(const uint16_t *x, int64_t x_s0, const uint16_t *weight, int rows, int width, float eps,
                     int8_t *q, int64_t q_s0, float *scales, void *stream);
 
+/*
+ * One token a row with temperature, min-p, top-k and top-p, for a caller's uniform number and a vocabulary of up to
+ * 2^20 (no counterpart in the reference, whose samplers have no min-p, executor/sampling.py:156-336).
+ * logits: fp32 or bf16 (NQ_F32, NQ_BF16) [rows, vocab], rows logits_s0 apart; the parameters one a row.
+ * With x the logits (a NaN counts as minus infinity), e = exp((x - max x) / temperature) in double and w =
+ * rint(2^42 e), or 0 where e < min_p, the ranks are in the order of (x descending, id ascending) and
+ *   total = the sum of w over the first top_k ranks (top_k <= 0: all),
+ *   kept  = the sum of w up to the first rank at which it reaches top_p * total,
+ *   token = the id of the first rank at which the sum of w reaches u * kept.
+ * The sums are integers, so a token does not depend on the launch or on other rows.  temperature not above 0 (or
+ * NaN): the first rank.  min_p, top_p and u are held to [0, 1] (NaN: no min-p, no top-p, u = 0); a row without a
+ * logit above minus infinity answers 0, one with infinite logits one of those.
+ */
+int nq_sample_min_p(const void *logits, int logits_dtype, int64_t logits_s0, int rows, int vocab,
+                    const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                    const float *uniforms, int64_t *tokens, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -144,6 +144,47 @@ def sample_with_counter_from_planes(planes, temperature, top_k, top_p, seed, off
                    **kwargs)
 
 
+def sample_min_p(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor,
+                 min_p: torch.Tensor, uniforms: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """One token per row: temperature, min-p, top-k, top-p and the inverse-CDF draw with the caller's uniforms, over up
+    to 2^20 ids (``sample_with_uniforms`` takes 4096).  A token is kept while its probability is at least ``min_p`` of the
+    likeliest's; top-p takes its share of what min-p and top-k leave.  Weights are fixed-point integers of double
+    exponentials, so tokens do not depend on the batch; they are not those of ``sample_with_uniforms``, whose sums
+    are float32, next to a border.  float32 or bfloat16 logits [rows, vocabulary] with contiguous rows at any stride, row
+    vectors float32 (``top_k`` int32), tokens int64."""
+
+    shape = logits.shape
+    if len(shape) != 2:
+        raise ValueError("logits must have shape (rows, vocabulary)")
+    if logits.dtype is torch.bfloat16:
+        code = _lib.NQ_BF16
+    elif logits.dtype is torch.float32:
+        code = _lib.NQ_F32
+    else:
+        raise TypeError("logits must be float32 or bfloat16")
+    rows, vocab = shape
+    row, unit = logits.stride()
+    if vocab < 1 or unit != 1:
+        raise ValueError("logits rows must be contiguous and hold at least one id")
+    for name, t, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32),
+                           ("uniforms", uniforms, torch.float32)):
+        if t.dtype is not dtype:
+            raise TypeError(f"{name} must use {dtype}, got {t.dtype}")
+        if t.shape != (rows,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous row vector with {rows} entries")
+    if out is None:
+        out = torch.empty(rows, dtype=torch.long, device=logits.device)
+    elif out.dtype is not torch.long:
+        raise TypeError("out must use torch.int64")
+    elif out.shape != (rows,) or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous row vector with {rows} entries")
+    _lib.launch(_lib.one_device(logits, temperature, top_k, top_p, min_p, uniforms, out), "nq_sample_min_p",
+                logits.data_ptr(), code, row, rows, vocab, temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
+                min_p.data_ptr(), uniforms.data_ptr(), out.data_ptr())
+    return out
+
+
 def sample_talker_cuda_graph(
     logits: torch.Tensor,
     temperature: torch.Tensor,
@@ -177,6 +218,7 @@ def sample_code_predictor_cuda_graph(logits, temperature, top_k, top_p, seed, of
 __all__ = [
     "sample_code_predictor_cuda_graph",
     "sample_logits_cuda_graph",
+    "sample_min_p",
     "sample_talker_cuda_graph",
     "sample_with_counter",
     "sample_with_counter_from_planes",

@@ -196,3 +196,42 @@ def uniform_from_counter(seed: int, offset: int) -> np.float32:
     o = int(offset) & 0xFFFFFFFFFFFFFFFF
     x0 = philox4x32((o & _MASK, o >> 32, 0, 0), (s & _MASK, s >> 32))[0]
     return F(x0 >> 8) * F(1.0 / 16777216.0)
+
+
+# --- min-p over large vocabularies ------------------------------------------
+
+
+def min_p_weights(x: np.ndarray, temperature: float, min_p: float) -> np.ndarray:
+    """Integer weights rint(2^42 exp((x - max) / T)) of one row, 0 where the exponential is below ``min_p``; float64."""
+
+    x = np.where(np.isnan(x), -np.inf, np.asarray(x, np.float64))
+    top = x.max()
+    with np.errstate(invalid="ignore", over="ignore", under="ignore"):
+        e = np.exp((x - top) * (1.0 / float(F(temperature))))
+    e = np.where(x == top, 1.0, np.where(np.isnan(e), 0.0, e))
+    return np.where(e >= min(max(float(F(min_p)), 0.0), 1.0), np.rint(e * 2.0**42), 0.0).astype(np.int64)
+
+
+def sample_min_p_row(logits: np.ndarray, temperature: float, top_k: int, top_p: float, min_p: float, u: float) -> int:
+    """The token of one row (the contract of ``nq_sample_min_p``), with the whole row sorted and exact integer sums."""
+
+    x = np.where(np.isnan(logits), -np.inf, np.asarray(logits, np.float64))
+    order = np.argsort(-x, kind="stable")
+    if not temperature > 0 or x[order[0]] == -np.inf:
+        return int(order[0])
+    hold = lambda v, nan: nan if np.isnan(v) else min(max(float(F(v)), 0.0), 1.0)  # noqa: E731
+    sums = np.cumsum(min_p_weights(x, temperature, hold(min_p, 0.0))[order])
+    k = top_k if 0 < top_k < len(x) else len(x)
+
+    def reached(share: float, mass: int) -> int:  # the first rank at which the sum reaches that share
+        return int(np.argmax(sums >= min(mass, max(1, int(np.ceil(share * float(mass)))))))
+
+    kept = int(sums[k - 1])
+    if hold(top_p, 1.0) < 1.0:
+        kept = int(sums[reached(hold(top_p, 1.0), kept)])
+    return int(order[reached(hold(u, 0.0), kept)])
+
+
+def sample_min_p(logits, temperature, top_k, top_p, min_p, uniforms) -> np.ndarray:
+    return np.array([sample_min_p_row(r, float(t), int(k), float(p), float(m), float(u))
+                     for r, t, k, p, m, u in zip(logits, temperature, top_k, top_p, min_p, uniforms)], dtype=np.int64)
