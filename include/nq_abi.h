@@ -908,6 +908,23 @@ int nq_rmsnorm_int8(const uint16_t *x, int64_t x_s0, const uint16_t *weight, int
                     int8_t *q, int64_t q_s0, float *scales, void *stream);
 
 /*
+ * Matrix products with a bias, an activation and a residual in their epilogue, for any M and N (the reference's
+ * projections are nn.Linear, model/layers.py:195-306; a bias and silu follow it in its text projection):
+ *   nq_linear_act:      out = bf16(residual + act(x w^T + bias)), bf16 x [M, K] and w [N, K], sums in fp32;
+ *   nq_linear_int8_act: the same of nq_linear_int8's value before its rounding, codes, scales and limits as there.
+ * bias (bf16 [N]) and residual (bf16 [M, N], rows r_s0 apart) may be NULL; out may be the residual itself (the same
+ * address and stride) but overlaps no operand otherwise.  Rounded once, from fp32.  K of nq_linear_act is a multiple of 8 up
+ * to 2^24, x, w and their row strides multiples of 16 bytes.
+ */
+enum nq_activation { NQ_ACT_NONE = 0, NQ_ACT_RELU = 1, NQ_ACT_GELU = 2, NQ_ACT_GELU_TANH = 3, NQ_ACT_SILU = 4 };
+int nq_linear_act(const uint16_t *x, int64_t x_s0, const uint16_t *w, int64_t w_s0, int M, int N, int K,
+                  const uint16_t *bias, int act, const uint16_t *residual, int64_t r_s0, uint16_t *out,
+                  int64_t o_s0, void *stream);
+int nq_linear_int8_act(const int8_t *xq, int64_t x_s0, const float *sx, const int8_t *wq, int64_t w_s0,
+                       const float *sw, int M, int N, int K, const uint16_t *bias, int act,
+                       const uint16_t *residual, int64_t r_s0, uint16_t *out, int64_t o_s0, void *stream);
+
+/*
  * One token a row with temperature, min-p, top-k and top-p, for a caller's uniform number and a vocabulary of up to
  * 2^20 (no counterpart in the reference, whose samplers have no min-p, executor/sampling.py:156-336).
  * logits: fp32 or bf16 (NQ_F32, NQ_BF16) [rows, vocab], rows logits_s0 apart; the parameters one a row.

@@ -29,6 +29,11 @@ NQ_EPI_NONE = 0
 NQ_EPI_ADD_RMSNORM = 1
 NQ_EPI_SILU_MUL = 2
 NQ_EPI_PARTIALS = 3
+NQ_ACT_NONE = 0
+NQ_ACT_RELU = 1
+NQ_ACT_GELU = 2
+NQ_ACT_GELU_TANH = 3
+NQ_ACT_SILU = 4
 NQ_MATMUL_HIGHEST = 0
 NQ_MATMUL_HIGH = 1
 NQ_ATTN_DECODE = 1
@@ -97,6 +102,8 @@ _SIGNATURES: dict[str, list] = {
     "nq_rmsnorm_int8": [_P, _L, _P, _I, _I, _F, _P, _L, _P, _P],
     "nq_linear_int8_tile": [_I, _I],
     "nq_linear_int8": [_P, _L, _P, _P, _L, _P, _I, _I, _I, _P, _L, _P],
+    "nq_linear_act": [_P, _L, _P, _L, _I, _I, _I, _P, _I, _P, _L, _P, _L, _P],
+    "nq_linear_int8_act": [_P, _L, _P, _P, _L, _P, _I, _I, _I, _P, _I, _P, _L, _P, _L, _P],
     "nq_linear_fp8_splits": [_I, _I, _I],
     "nq_linear_fp8_workspace_bytes": [_I, _I, _I, _I],
     "nq_linear_fp8": [_P, _L, _P, _L, _P, _L, _P, _L, _I, _I, _I, _I, _P, _L, _P, _L, _P],

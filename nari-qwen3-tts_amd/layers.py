@@ -18,7 +18,10 @@ quantized per row and 128 columns by the add-RMSNorm that produces them
 
 8-bit integers (no reference counterpart): ``quantize_int8_rows`` gives codes with
 one scale per row, of activations (per token) as of weights (per output
-channel), and ``linear_int8`` runs their product for any number of rows.
+channel), and ``linear_int8`` runs their product for any number of rows;
+``add_rmsnorm_int8`` / ``rmsnorm_int8`` answer a norm in such codes.
+``linear_act`` (bf16) and ``linear_int8`` take a bias, an activation and a
+residual in the product's epilogue.
 """
 
 from __future__ import annotations
@@ -835,11 +838,66 @@ def quantize_int8_rows(x: torch.Tensor, q: torch.Tensor | None = None,
     return q, scales
 
 
+ACTIVATIONS = {None: _lib.NQ_ACT_NONE, "relu": _lib.NQ_ACT_RELU, "gelu": _lib.NQ_ACT_GELU,
+               "gelu_tanh": _lib.NQ_ACT_GELU_TANH, "silu": _lib.NQ_ACT_SILU}
+
+
+def _epilogue(rows: int, n: int, bias, activation, residual, out):
+    """Checks of a product's epilogue and output: the activation's code, the row strides of residual and output."""
+
+    act = ACTIVATIONS.get(activation, -1)
+    if act < 0:
+        raise ValueError(f"activation must be one of {', '.join(map(repr, ACTIVATIONS))}")
+    if bias is not None:
+        if bias.dtype is not torch.bfloat16:
+            raise TypeError("bias must be bf16")
+        if bias.shape != (n,) or not bias.is_contiguous():
+            raise ValueError("bias must match out_features, contiguous")
+    r_row, o_row = 0, n
+    if residual is not None:
+        if residual.dtype is not torch.bfloat16:
+            raise TypeError("residual must be bf16")
+        if residual.shape != (rows, n) or residual.stride(1) != 1:
+            raise ValueError(f"residual must be [{rows}, {n}] with unit inner stride")
+        r_row = residual.stride(0)
+    if out is not None:
+        if out.dtype is not torch.bfloat16 or out.shape != (rows, n) or out.stride(1) != 1:
+            raise ValueError(f"out must be bf16 [{rows}, {n}] with unit inner stride")
+        o_row = out.stride(0)
+    return act, r_row, o_row
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+               residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """out = residual + act(x @ weight.T + bias) in one launch, for any number of rows: bf16 x [rows, in] and weight [out,
+    in] (row strides free, of 8 elements' multiples), bf16 bias [out] and residual [rows, out], each optional;
+    activation None, "relu", "gelu" (erf), "gelu_tanh" or "silu".  fp32 sums and epilogue, one rounding to bf16.  ``out``
+    may be ``residual`` itself.  ``in`` a multiple of 8."""
+
+    if x.dtype is not torch.bfloat16 or weight.dtype is not torch.bfloat16:
+        raise TypeError("linear_act needs bf16 activations and weights")
+    x_strides, w_strides, w_shape = x.stride(), weight.stride(), weight.shape
+    if len(x_strides) != 2 or len(w_shape) != 2 or x_strides[1] != 1 or w_strides[1] != 1:
+        raise ValueError("linear_act needs matrices with unit inner stride")
+    (rows, k), n = x.shape, w_shape[0]
+    if w_shape[1] != k or k < 8 or k % 8:
+        raise ValueError("x and weight must share an inner size that is a multiple of 8")
+    act, r_row, o_row = _epilogue(rows, n, bias, activation, residual, out)
+    if out is None:
+        out = torch.empty(rows, n, dtype=torch.bfloat16, device=x.device)
+    _lib.launch(_lib.one_device(x, weight, bias, residual, out), "nq_linear_act", x.data_ptr(), x_strides[0],
+                weight.data_ptr(), w_strides[0], rows, n, k, _lib.ptr(bias), act, _lib.ptr(residual), r_row,
+                out.data_ptr(), o_row)
+    return out
+
+
 def linear_int8(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, weight_scales: torch.Tensor,
-                out: torch.Tensor | None = None) -> torch.Tensor:
+                out: torch.Tensor | None = None, *, bias: torch.Tensor | None = None, activation: str | None = None,
+                residual: torch.Tensor | None = None) -> torch.Tensor:
     """out[m, n] = bf16(sum_k q[m, k] weight_q[n, k] * scales[m] * weight_scales[n]) for int8 codes [rows, in] and
     [out, in] with the scales of ``quantize_int8_rows``; the sum is exact (int32), so the same codes give the
-    same bits at any number of rows.  ``in`` a multiple of 16 up to 131072 (codes within +-127), any rows and out."""
+    same bits at any number of rows.  ``in`` a multiple of 16 up to 131072 (codes within +-127), any rows and out.
+    bias, activation and residual as in ``linear_act``, applied to the fp32 value: one rounding to bf16."""
 
     if q.dtype is not torch.int8 or weight_q.dtype is not torch.int8:
         raise TypeError("the int8 projection needs int8 codes")
@@ -854,20 +912,23 @@ def linear_int8(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, w
     if scales.shape != (rows,) or weight_scales.shape != (n,) or not (
             scales.is_contiguous() and weight_scales.is_contiguous()):
         raise ValueError("int8 scales must be contiguous, one per row and one per output")
-    o_row = n
+    act, r_row, o_row = _epilogue(rows, n, bias, activation, residual, out)
     if out is None:
         out = torch.empty(rows, n, dtype=torch.bfloat16, device=q.device)
-    elif out.dtype is not torch.bfloat16 or out.shape != (rows, n) or out.stride(1) != 1:
-        raise ValueError(f"out must be bf16 [{rows}, {n}] with unit inner stride")
+    index = _lib.one_device(q, scales, weight_q, weight_scales, bias, residual, out)
+    if bias is None and residual is None and not act:
+        _lib.launch(index, "nq_linear_int8", q.data_ptr(), q_strides[0], scales.data_ptr(), weight_q.data_ptr(),
+                    w_strides[0], weight_scales.data_ptr(), rows, n, k, out.data_ptr(), o_row)
     else:
-        o_row = out.stride(0)
-    _lib.launch(_lib.one_device(q, scales, weight_q, weight_scales, out), "nq_linear_int8", q.data_ptr(),
-                q_strides[0], scales.data_ptr(), weight_q.data_ptr(), w_strides[0], weight_scales.data_ptr(), rows, n,
-                k, out.data_ptr(), o_row)
+        _lib.launch(index, "nq_linear_int8_act", q.data_ptr(), q_strides[0], scales.data_ptr(), weight_q.data_ptr(),
+                    w_strides[0], weight_scales.data_ptr(), rows, n, k, _lib.ptr(bias), act, _lib.ptr(residual), r_row,
+                    out.data_ptr(), o_row)
     return out
 
 
 __all__ = [
+    "ACTIVATIONS",
+    "linear_act",
     "add_rmsnorm_int8",
     "rmsnorm_int8",
     "linear_int8",
