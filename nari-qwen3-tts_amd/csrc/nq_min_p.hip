@@ -10,21 +10,24 @@
 // T not above zero: the first rank.  All three cuts and the draw are the same question, the first rank whose count or
 // mass reaches a target, so a row is asked it up to three times and never sorted whole.
 //
-// A workgroup a row.  The logits that can have a weight (by their distance from the maximum) usually fit a list in
-// LDS, which is sorted and summed there.  Where they do not, a radix descent finds the digits of the rank in question from
-// histograms of counts and masses, until the ranks that share those digits fit the list.
+// A workgroup a row.  Where min-p leaves few logits, one pass collects them in LDS, by the maximum so far (what a later
+// one drops is dropped behind the pass), and they are sorted and summed there.  Otherwise a histogram over the distance
+// from the maximum, of counts for top-k and of masses for the shares, says which bin a rank lies in, and that bin's logits
+// alone are collected and sorted; a bin too full for the list (equal logits) is cut by the digits of its entries.
+#include <type_traits>
+
 #include "nq_common.h"
 #include "nq_internal.h"
 
 namespace nq {
 namespace {
 
-constexpr int kMinPThreads = 1024;
-constexpr int kMinPWaves = kMinPThreads / kWave;
-constexpr int kMinPList = 4096;           // entries of the list
+constexpr int kMinPList = 4096;  // entries of the list
+constexpr int kMinPSorted = 512; // entries that are rather sorted than cut by a histogram
+constexpr int kMinPRanked = 256; // entries that are sorted by counting those above each
 constexpr int kMinPBins = 2048;
+constexpr int kMinPHeld = 8;     // logits a thread keeps in registers where the row fits
 constexpr int kMinPVocab = 1 << 20;
-constexpr double kMinPOne = 4398046511104.0;  // 2^42
 
 struct MinPArgs {
     const void *logits;
@@ -38,8 +41,9 @@ struct MinPArgs {
     int64_t *tokens;
 };
 
-__device__ __forceinline__ uint64_t min_p_entry(float x, int id) {  // larger: earlier in the order
-    const uint32_t u = __float_as_uint(x);
+// An entry of the order: the larger the earlier.
+__device__ __forceinline__ uint64_t min_p_entry(float x, int id) {
+    const uint32_t u = __float_as_uint(x + 0.0f);  // -0 as 0
     const uint32_t key = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
     return (static_cast<uint64_t>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(id));
 }
@@ -50,17 +54,12 @@ __device__ __forceinline__ float entry_value(uint64_t e) {
 __device__ __forceinline__ int entry_id(uint64_t e) {
     return static_cast<int>(0xffffffffu - static_cast<uint32_t>(e));
 }
-// NaN as -inf, -0 as 0
-__device__ __forceinline__ float plain_logit(float x) { return x == x ? x + 0.0f : -__builtin_inff(); }
+// The larger of the two; b where a is NaN (fmaxf answers NaN to a signalling one).
+__device__ __forceinline__ float larger(float a, float b) { return a > b ? a : b; }
 
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
     const uint32_t lo = __shfl_up(static_cast<uint32_t>(v), d, kWave);
     const uint32_t hi = __shfl_up(static_cast<uint32_t>(v >> 32), d, kWave);
-    return (static_cast<uint64_t>(hi) << 32) | lo;
-}
-__device__ __forceinline__ uint64_t shfl64(uint64_t v, int lane) {
-    const uint32_t lo = __shfl(static_cast<uint32_t>(v), lane, kWave);
-    const uint32_t hi = __shfl(static_cast<uint32_t>(v >> 32), lane, kWave);
     return (static_cast<uint64_t>(hi) << 32) | lo;
 }
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
@@ -78,92 +77,294 @@ __device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {  // inclusive
     return v;
 }
 
+template <int T>
 struct MinPShared {
+    static constexpr int kWaves = T / kWave;
     uint64_t list[kMinPList];
-    uint64_t mass[2][kMinPBins];
-    uint32_t count[2][kMinPBins];
-    uint64_t part[2][kMinPWaves];
-    uint64_t found_mass;
-    uint64_t above_mass;
-    uint32_t above_count, bin, bin_count, n;
-    int found_id;
+    uint64_t hist[2][kMinPBins];  // of the row, and of what one bin is cut by; counts take 32 bits a bin
+    double table[32];
+    uint64_t part[kWaves];
+    float max[2][kWaves];
+    uint64_t found_mass, found, above;
+    uint32_t rank[kMinPRanked];
+    uint32_t bin, n;
+    int id;
 };
 
-// Sums over the workgroup of the threads before this one; two barriers.
-__device__ __forceinline__ uint64_t block_before(uint64_t v, uint64_t *part) {
+// Sums over the workgroup of the threads before this one, and of all; two barriers.
+template <int T>
+__device__ __forceinline__ uint64_t block_before(uint64_t v, uint64_t *part, uint64_t &total) {
     const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
     const uint64_t incl = wave_scan64(v);
     if (lane == kWave - 1) part[wave] = incl;
     __syncthreads();
     uint64_t before = incl - v;
-    for (int w = 0; w < wave; ++w) before += part[w];
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < T / kWave; ++w) {
+        before += w < wave ? part[w] : 0;
+        total += part[w];
+    }
     __syncthreads();
     return before;
 }
 
-// What a row's weights follow from.
+// 2^(i / 32)
+__device__ const double kExp2Table[32] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
+};
+
+// What a row's weights follow from.  With t = 32 log2(e) (x - max) / T and i = rint(t), e = 2^(i / 32) 2^((t - i) / 32): a
+// table, the Taylor series of 2^f for |f| <= 1 / 64 to its fifth power, whose rest is below 3e-15 of it, and an
+// exponent; and -i is the logit's bin in the row's histogram, 32 an octave.  A weight of 1 needs e >= 2^-43, so t is held to 45
+// octaves.
 struct RowRule {
-    float max, least;  // least: no logit below it has a weight (a bound)
-    double inv_t, min_p;
+    static constexpr int kPer = 32, kLast = 45 * kPer;
+    static_assert(kLast < kMinPBins, "the row's bins");
+    const double *table;  // in LDS
+    double max, turns;    // turns: 32 log2(e) / T
+    double min_p;
+    float least;          // no logit below it has a weight (a bound); NaN and -inf are never from it on
+    uint64_t last;        // top-k's last entry: none behind it has a weight
+    __device__ __forceinline__ double turn(float x) const {
+        // an infinite maximum is held as the largest finite logit, which only infinite ones then reach
+        const double d = static_cast<double>(fminf(x, 3.4028234663852886e38f)) - max;
+        return fmax(d * turns, -1.0 * kLast);
+    }
+    __device__ __forceinline__ int bin(float x) const {  // does not decrease as x falls
+        return -static_cast<int>(rint(turn(x)));
+    }
+    __device__ __forceinline__ uint64_t weight(float x, int &bin) const {
+        const double t = turn(x), n = rint(t), f = t - n;
+        const int i = static_cast<int>(n);
+        double p = 3.973709984549416e-11;  // (ln 2 / 32)^5 / 5!, and so on
+        p = fma(p, f, 9.172562701824643e-09);
+        p = fma(p, f, 1.693850972437182e-06);
+        p = fma(p, f, 0.0002345961982022468);
+        p = fma(p, f, 0.02166084939249829);
+        p = fma(p, f, 1.0);
+        p *= table[i & (kPer - 1)];
+        // its exponent, and 42 more: then the integer is in the low bits behind 2^52, rounded
+        const double w = __longlong_as_double(__double_as_longlong(p) + (static_cast<int64_t>((i >> 5) + 42) << 52));
+        bin = -i;
+        const uint64_t whole = static_cast<uint64_t>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
+        return w >= min_p ? whole : 0;
+    }
     __device__ __forceinline__ uint64_t weight(float x) const {
-        if (x == max) return static_cast<uint64_t>(kMinPOne);  // an infinite one too
-        const double e = exp((static_cast<double>(x) - static_cast<double>(max)) * inv_t);
-        return e >= min_p ? static_cast<uint64_t>(rint(e * kMinPOne)) : 0;
+        int bin;
+        return weight(x, bin);
+    }
+    __device__ __forceinline__ bool counts(float x) const { return x >= least; }
+};
+
+template <typename InT>
+__device__ __forceinline__ float logit_at(const InT *row, int id) {
+    if constexpr (sizeof(InT) == 2) return bf16_to_f32(row[id]);
+    else return row[id];
+}
+
+// A row in registers, thread t the ids t, t + T, ..
+template <typename InT, int T>
+struct HeldRow {
+    float x[kMinPHeld];
+    int vocab;
+    __device__ __forceinline__ HeldRow(const InT *row, int v) : vocab(v) {
+#pragma unroll
+        for (int i = 0; i < kMinPHeld; ++i) {
+            const int id = static_cast<int>(threadIdx.x) + i * T;
+            x[i] = id < v ? logit_at(row, id) : -__builtin_inff();
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+        for (int i = 0; i < kMinPHeld; ++i) {
+            const int id = static_cast<int>(threadIdx.x) + i * T;
+            if (id < vocab) f(id, x[i]);
+        }
     }
 };
 
-// f(id, logit) for every logit of the row, 16 bytes a load where the row's alignment allows.
-template <typename InT, typename F>
-__device__ __forceinline__ void each_logit(const InT *row, int vocab, F f) {
-    constexpr int V = 16 / sizeof(InT), U = 4;
-    const int tid = threadIdx.x;
-    const int head = min(vocab, static_cast<int>((16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(InT)));
-    const int nv = (vocab - head) / V;
-    auto one = [&](int id) __attribute__((always_inline)) {
-        if constexpr (sizeof(InT) == 2) f(id, plain_logit(bf16_to_f32(row[id])));
-        else f(id, plain_logit(row[id]));
-    };
-    if (tid < head) one(tid);
-    const uint4 *body = reinterpret_cast<const uint4 *>(row + head);
-    for (int j0 = tid; j0 < nv; j0 += U * kMinPThreads) {
-        uint4 v[U];
+// What is left of a row, the n entries of a list, in registers: the list is free for others behind the constructor.
+template <int T>
+struct HeldList {
+    static constexpr int kEach = kMinPList / T;
+    uint64_t e[kEach];
+    __device__ __forceinline__ HeldList(const MinPShared<T> &s, int n) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int j = j0 + u * kMinPThreads;
-            v[u] = j < nv ? body[j] : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kEach; ++i) {
+            const int at = static_cast<int>(threadIdx.x) + i * T;
+            e[i] = at < n ? s.list[at] : 0;  // no entry is 0
         }
+        __syncthreads();
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int j = j0 + u * kMinPThreads;
-            if (j >= nv) break;
-            const int id = head + j * V;
-            if constexpr (sizeof(InT) == 2) {
-                float x[8];
-                unpack8(v[u], x);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f(id + e, plain_logit(x[e]));
-            } else {
-                f(id, plain_logit(__uint_as_float(v[u].x)));
-                f(id + 1, plain_logit(__uint_as_float(v[u].y)));
-                f(id + 2, plain_logit(__uint_as_float(v[u].z)));
-                f(id + 3, plain_logit(__uint_as_float(v[u].w)));
-            }
+        for (int i = 0; i < kEach; ++i)
+            if (e[i]) f(entry_id(e[i]), entry_value(e[i]));
+    }
+};
+
+// A row in memory: 16 bytes a load from the first address that allows them, head logits before and some behind.
+template <typename InT, int T>
+struct FarRow {
+    const InT *row;
+    int vocab, head, nv;
+    static constexpr int V = 16 / sizeof(InT);
+    __device__ __forceinline__ FarRow(const InT *r, int v) : row(r), vocab(v) {
+        head = min(v, static_cast<int>((16 - reinterpret_cast<uintptr_t>(r) % 16) % 16 / sizeof(InT)));
+        nv = (v - head) / V;
+    }
+    __device__ __forceinline__ uint4 load(int j) const {
+        return j < nv ? reinterpret_cast<const uint4 *>(row + head)[j] : make_uint4(0, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void unpack(const uint4 &v, float (&x)[V]) {
+        if constexpr (V == 8) {
+            unpack8(v, x);
+        } else {
+            x[0] = __uint_as_float(v.x);
+            x[1] = __uint_as_float(v.y);
+            x[2] = __uint_as_float(v.z);
+            x[3] = __uint_as_float(v.w);
         }
     }
-    const int tail = head + nv * V + tid;
-    if (tail < vocab) one(tail);
-}
+    // f for the logits outside the whole vectors (fewer than T)
+    template <typename F>
+    __device__ __forceinline__ void few(F f) const {
+        const int i = threadIdx.x, id = i < head ? i : i + nv * V;
+        if (id < vocab) f(id, logit_at(row, id));
+    }
+    // Three vectors of a thread are in flight; the body is one's, since code that is run through once costs its fetch.
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        const int tid = threadIdx.x;
+        uint4 v0 = load(tid), v1 = load(tid + T), v2 = load(tid + 2 * T);
+        few(f);
+#pragma unroll 1
+        for (int j = tid; j < nv; j += T) {
+            const uint4 v = v0;
+            v0 = v1;
+            v1 = v2;
+            v2 = load(j + 3 * T);
+            float x[V];
+            unpack(v, x);
+#pragma unroll
+            for (int e = 0; e < V; ++e) f(head + j * V + e, x[e]);
+        }
+    }
+    // The largest logit of this thread's part, and in `where` the first vector that holds its vectors' largest (-1: none).  With
+    // collect, after each batch of loads: the largest so far of all threads goes through least(), and put takes every logit of
+    // the batch from that on.
+    template <typename L, typename P>
+    __device__ __forceinline__ float first_pass(MinPShared<T> &s, bool collect, L least, P put, int &where) const {
+        constexpr int U = 8;
+        const int tid = threadIdx.x;
+        float top = -__builtin_inff();
+        where = -1;
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = load(tid + u * T);
+#pragma unroll 1
+        for (int b = 0, turn = 0; b < nv; b += U * T, turn ^= 1) {
+            float high[U];
+            uint4 next[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int j = b + tid + u * T;
+                float x[V];
+                unpack(v[u], x);
+                high[u] = larger(x[0], -__builtin_inff());
+#pragma unroll
+                for (int e = 1; e < V; ++e) high[u] = larger(x[e], high[u]);
+                high[u] = j < nv ? high[u] : -__builtin_inff();
+                where = high[u] > top ? j : where;
+                top = larger(high[u], top);
+                next[u] = load(j + U * T);
+            }
+            if (collect) {
+                const float m = group_max<kWave>(top);
+                if (tid % kWave == 0) s.max[turn][tid / kWave] = m;
+                __syncthreads();
+                float all = s.max[turn][0];
+#pragma unroll
+                for (int w = 1; w < T / kWave; ++w) all = fmaxf(all, s.max[turn][w]);
+                const float from = least(all);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (!(high[u] >= from)) continue;
+                    const int id = head + (b + tid + u * T) * V;
+                    uint4 r = v[u];
+#pragma unroll 1
+                    for (int e = 0; e < V; ++e) {
+                        const float x = __uint_as_float(V == 8 ? r.x << 16 : r.x);
+                        if (V == 8) {
+                            r.x = __builtin_amdgcn_alignbit(r.y, r.x, 16);
+                            r.y = __builtin_amdgcn_alignbit(r.z, r.y, 16);
+                            r.z = __builtin_amdgcn_alignbit(r.w, r.z, 16);
+                            r.w >>= 16;
+                        } else {
+                            r = make_uint4(r.y, r.z, r.w, 0);
+                        }
+                        put(id + e, x, from);
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = next[u];
+        }
+        few([&](int id, float x) {
+            top = larger(x, top);
+            if (collect) put(id, x, -3.4028234663852886e38f);
+        });
+        return top;
+    }
+    // f for this thread's logits outside whole vectors and those of one
+    template <typename F>
+    __device__ __forceinline__ void vector(int j, F f) const {
+        few(f);
+        if (j < 0) return;
+#pragma unroll 1
+        for (int e = 0; e < V; ++e) f(head + j * V + e, logit_at(row, head + j * V + e));
+    }
+};
 
-// Sorts the list's n entries in descending order (all threads).
-__device__ __forceinline__ void sort_list(MinPShared &s, int n) {
-    int n2 = 2;
+// Sorts the list's n entries in descending order (all threads): a few by counting those above each, several threads a
+// counted entry; more by a network.
+template <int T>
+__device__ __forceinline__ void sort_list(MinPShared<T> &s, int n) {
+    const int tid = threadIdx.x;
+    if (n <= kMinPRanked) {
+        const int span = n <= 64 ? 64 : n <= 128 ? 128 : 256, parts = T / span;  // span <= T
+        const int i = tid & (span - 1), each = (n + parts - 1) / parts;
+        const int from = min(n, tid / span * each), to = min(n, from + each);
+        for (int j = tid; j < span; j += T) s.rank[j] = 0;
+        const uint64_t mine = i < n ? s.list[i] : 0;
+        uint32_t above = 0;
+#pragma unroll 4
+        for (int j = from; j < to; ++j) above += s.list[j] > mine ? 1u : 0u;
+        __syncthreads();
+        if (i < n && above) atomicAdd(&s.rank[i], above);
+        __syncthreads();
+        if (tid < n) s.list[s.rank[tid]] = mine;  // thread tid < span holds entry tid
+        __syncthreads();
+        return;
+    }
+    int n2 = 2 * kMinPRanked;
     while (n2 < n) n2 <<= 1;
-    for (int i = n + threadIdx.x; i < n2; i += kMinPThreads) s.list[i] = 0;
+    for (int i = n + tid; i < n2; i += T) s.list[i] = 0;
     __syncthreads();
     for (int kk = 2; kk <= n2; kk <<= 1)
         for (int j = kk >> 1; j > 0; j >>= 1) {
-            for (int i = threadIdx.x; i < n2 / 2; i += kMinPThreads) {
-                const int lo = 2 * j * (i / j) + i % j;
+            for (int i = tid; i < n2 / 2; i += T) {
+                const int lo = 2 * i - (i & (j - 1));
                 const uint64_t a = s.list[lo], b = s.list[lo + j];
                 if (((lo & kk) == 0) == (a < b)) {
                     s.list[lo] = b;
@@ -174,245 +375,378 @@ __device__ __forceinline__ void sort_list(MinPShared &s, int n) {
         }
 }
 
-constexpr int kMinPEach = kMinPList / kMinPThreads;
-
-// The sums of a sorted list: thread t has the ranks t E .. t E + E - 1, E = ceil(n / threads).
+// The sums of a sorted list: thread t has the ranks t E .. t E + E - 1, E = ceil(n / T).
+template <int T>
 struct ListSums {
-    uint64_t cum[kMinPEach];
+    static constexpr int kEach = kMinPList / T;
+    uint64_t cum[kEach];
     uint64_t before;
     int first, end;
-};
-__device__ __forceinline__ ListSums sum_list(MinPShared &s, int n, uint64_t above, const RowRule &rule) {
-    ListSums r;
-    const int each = (n + kMinPThreads - 1) / kMinPThreads;
-    r.first = min(n, static_cast<int>(threadIdx.x) * each);
-    r.end = min(n, r.first + each);
-    uint64_t own = 0;
+    __device__ __forceinline__ ListSums(MinPShared<T> &s, int n, uint64_t above, const RowRule &rule) {
+        const int each = (n + T - 1) / T;
+        first = min(n, static_cast<int>(threadIdx.x) * each);
+        end = min(n, first + each);
+        uint64_t own = 0;
 #pragma unroll
-    for (int i = 0; i < kMinPEach; ++i) {
-        if (r.first + i < r.end) own += rule.weight(entry_value(s.list[r.first + i]));
-        r.cum[i] = own;
-    }
-    r.before = above + block_before(own, s.part[0]);
-#pragma unroll
-    for (int i = 0; i < kMinPEach; ++i) r.cum[i] += r.before;
-    return r;
-}
-// The first rank whose mass reaches the target (which the list's last does): its mass and id, for every thread.
-__device__ __forceinline__ void find_mass(MinPShared &s, const ListSums &r, uint64_t target) {
-    uint64_t last = r.before;
-#pragma unroll
-    for (int i = 0; i < kMinPEach; ++i) {
-        if (r.first + i < r.end && last < target && target <= r.cum[i]) {
-            s.found_mass = r.cum[i];
-            s.found_id = entry_id(s.list[r.first + i]);
+        for (int i = 0; i < kEach; ++i) {
+            if (first + i < end) own += rule.weight(entry_value(s.list[first + i]));
+            cum[i] = own;
         }
-        last = r.cum[i];
-    }
-    __syncthreads();
-}
-__device__ __forceinline__ void find_rank(MinPShared &s, const ListSums &r, int rank) {
+        uint64_t total;
+        before = above + block_before<T>(own, s.part, total);
 #pragma unroll
-    for (int i = 0; i < kMinPEach; ++i)
-        if (r.first + i < r.end && r.first + i == rank) s.found_mass = r.cum[i];
-    __syncthreads();
-}
+        for (int i = 0; i < kEach; ++i) cum[i] += before;
+    }
+    // The first rank whose mass reaches the target, which the list's last does.
+    __device__ __forceinline__ void find_mass(MinPShared<T> &s, uint64_t target) const {
+        uint64_t last = before;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (first + i < end && last < target && target <= cum[i]) {
+                s.found_mass = cum[i];
+                s.found = s.list[first + i];
+            }
+            last = cum[i];
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ void find_rank(MinPShared<T> &s, int rank) const {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (first + i < end && first + i == rank) s.found_mass = cum[i];
+        __syncthreads();
+    }
+};
 
-// least integer target that p (in [0, 1]) of a mass asks for, at least 1
+// The least integer that p (in [0, 1]) of a mass asks for, at least 1.
 __device__ __forceinline__ uint64_t share(double p, uint64_t mass) {
     const uint64_t t = static_cast<uint64_t>(ceil(p * static_cast<double>(mass)));
     return t < 1 ? 1 : t > mass ? mass : t;
 }
 
-template <typename InT>
-__global__ void __launch_bounds__(kMinPThreads)
-min_p_kernel(MinPArgs a) {
-    __shared__ MinPShared s;
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    const InT *x = static_cast<const InT *>(a.logits) + row * a.s0;
+struct RowCuts {
+    int k;
+    double p, u;
+};
 
-    // 1. the first of the order
-    uint64_t best = 0;
-    each_logit(x, a.vocab, [&](int id, float v) {
-        const uint64_t e = min_p_entry(v, id);
-        best = e > best ? e : best;
-    });
+// The token of a row whose weights are all among the list's n <= 64 entries, by one wave: lane r has rank r.  Sums of 64
+// weights are exact in double.
+template <int T>
+__device__ __forceinline__ int draw_from_few(const MinPShared<T> &s, int n, const RowRule &rule, const RowCuts &c) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const uint64_t mine = lane < n ? s.list[lane] : 0;
+    int above = lane < n ? 0 : lane;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) above += lane < n && s.list[j] > mine ? 1 : 0;
+    const uint32_t lo = __builtin_amdgcn_ds_permute(4 * above, static_cast<int>(static_cast<uint32_t>(mine)));
+    const uint32_t hi = __builtin_amdgcn_ds_permute(4 * above, static_cast<int>(static_cast<uint32_t>(mine >> 32)));
+    const uint64_t e = (static_cast<uint64_t>(hi) << 32) | lo;
+    double cum = lane < n && lane < c.k ? static_cast<double>(rule.weight(entry_value(e))) : 0.0;
 #pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) {
-        const uint64_t o = shfl_xor64(best, m);
-        best = o > best ? o : best;
+    for (int d = 1; d < kWave; d <<= 1) {
+        const double o = __shfl_up(cum, d, kWave);
+        if (lane >= d) cum += o;
     }
-    if (lane == 0) s.part[0][wave] = best;
-    if (tid == 0) s.n = 0;
-    __syncthreads();
-    best = s.part[0][0];
-#pragma unroll
-    for (int w = 1; w < kMinPWaves; ++w) best = s.part[0][w] > best ? s.part[0][w] : best;
-    const float temperature = a.temperature[row];
-    RowRule rule;
-    rule.max = entry_value(best);
-    if (!(temperature > 0.f) || rule.max == -__builtin_inff()) {
-        if (tid == 0) a.tokens[row] = entry_id(best);
-        return;
-    }
-    rule.inv_t = 1.0 / temperature;
-    const float mp = a.min_p[row];
-    rule.min_p = mp > 0.f ? (mp < 1.f ? mp : 1.0) : 0.0;
-    const int kq = a.top_k[row];
-    const int k = kq > 0 && kq < a.vocab ? kq : a.vocab;
-    const float pq = a.top_p[row];
-    const double p = pq < 1.f ? (pq > 0.f ? pq : 0.0) : 1.0;
-    const float uq = a.uniforms[row];
-    const double u = uq > 0.f ? (uq < 1.f ? uq : 1.0) : 0.0;
-    // w >= 1 needs e >= 2^-43; the margin covers the roundings of this bound many times over
-    const double reach = temperature * log(fmax(rule.min_p, 0x1p-43));
-    rule.least = rule.max == __builtin_inff()
-                     ? rule.max
-                     : static_cast<float>(rule.max + reach - 1e-6 * (fabs(static_cast<double>(rule.max)) - reach));
+    double kept = __shfl(cum, kWave - 1, kWave);
+    auto reached = [&](double target) {  // the first lane, which the last one reaches
+        return __ffsll(static_cast<long long>(__ballot(cum >= fmin(fmax(target, 1.0), kept)))) - 1;
+    };
+    if (c.p < 1.0) kept = __shfl(cum, reached(ceil(c.p * kept)), kWave);
+    return __shfl(entry_id(e), reached(ceil(c.u * kept)), kWave);
+}
 
-    // 2. the list of those
-    each_logit(x, a.vocab, [&](int id, float v) {
-        if (v >= rule.least) {
-            const uint32_t at = atomicAdd(&s.n, 1u);
-            if (at < kMinPList) s.list[at] = min_p_entry(v, id);
-        }
-    });
+// The token of a row whose weights are all in the list (of every thread).
+template <int T>
+__device__ __forceinline__ int draw_from_list(MinPShared<T> &s, int n, const RowRule &rule, const RowCuts &c) {
+    if (n <= kWave) return draw_from_few<T>(s, n, rule, c);
+    sort_list<T>(s, n);
+    const ListSums<T> sums(s, n, 0, rule);
+    sums.find_rank(s, min(c.k, n) - 1);
+    uint64_t kept = s.found_mass;
     __syncthreads();
-    const int n = static_cast<int>(s.n);
-    if (n <= kMinPList) {
-        sort_list(s, n);
-        const ListSums sums = sum_list(s, n, 0, rule);
-        find_rank(s, sums, min(k, n) - 1);
-        uint64_t kept = s.found_mass;
+    if (c.p < 1.0) {
+        sums.find_mass(s, share(c.p, kept));
+        kept = s.found_mass;
         __syncthreads();
-        if (p < 1.0) {
-            find_mass(s, sums, share(p, kept));
-            kept = s.found_mass;
-            __syncthreads();
-        }
-        find_mass(s, sums, share(u, kept));
-        if (tid == 0) a.tokens[row] = s.found_id;
-        return;
     }
+    sums.find_mass(s, share(c.u, kept));
+    return entry_id(s.found);
+}
 
-    // 3. too many: histograms of the order's digits, first of its top 11 bits
-    for (int i = tid; i < kMinPBins; i += kMinPThreads) {
-        s.mass[0][i] = 0;
-        s.count[0][i] = 0;
-    }
+// The row's histogram: of counts (kMass false) or of masses.  The list's counter is cleared besides.
+template <bool kMass, int T, typename Row>
+__device__ __forceinline__ void row_histogram(MinPShared<T> &s, const Row &row, const RowRule &rule) {
+    for (int i = threadIdx.x; i < kMinPBins; i += T) s.hist[0][i] = 0;
+    if (threadIdx.x == 0) s.n = 0;
     __syncthreads();
-    each_logit(x, a.vocab, [&](int id, float v) {
-        if (v >= rule.least) {
-            const uint64_t w = rule.weight(v);
-            if (w) {
-                const int bin = static_cast<int>(min_p_entry(v, id) >> 53);
-                atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[0][bin]), w);
-                atomicAdd(&s.count[0][bin], 1u);
-            }
+    const bool all = rule.last == 0;
+    row.each([&](int id, float v) {
+        if (!rule.counts(v)) return;
+        if constexpr (kMass) {
+            int bin;
+            uint64_t w = rule.weight(v, bin);
+            if (!all && min_p_entry(v, id) < rule.last) w = 0;
+            if (w) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[0][bin]), w);
+        } else {
+            atomicAdd(reinterpret_cast<uint32_t *>(s.hist[0]) + rule.bin(v), 1u);
         }
     });
     __syncthreads();
+}
 
-    // The first rank whose count (by_mass false) or mass reaches the target, which all of them reach: s.found_mass its mass,
-    // s.found_id its id.  Digits of an entry: 11, 11 and 10 bits of the logit, 10 and 10 of the id (below 2^20).
-    auto locate = [&](uint64_t target, bool by_mass) {
-        uint64_t prefix = 0xfff00000ull, mask = 0xfff00000ull, above_mass = 0;
-        uint32_t above_count = 0;
-        int shift = 64, level = 0;
-        for (;; ++level) {
-            const int bits = level < 2 ? 11 : 10;
-            shift = level == 3 ? 10 : shift - bits;
-            const int bins = 1 << bits, h = level > 0;
-            if (level > 0) {
-                for (int i = tid; i < bins; i += kMinPThreads) {
-                    s.mass[1][i] = 0;
-                    s.count[1][i] = 0;
-                }
-                __syncthreads();
-                each_logit(x, a.vocab, [&](int id, float v) {
-                    const uint64_t e = min_p_entry(v, id);
-                    if (v >= rule.least && (e & mask) == prefix) {
-                        const uint64_t w = rule.weight(v);
-                        if (w) {
-                            const int bin = static_cast<int>(e >> shift) & (bins - 1);
-                            atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[1][bin]), w);
-                            atomicAdd(&s.count[1][bin], 1u);
-                        }
-                    }
-                });
-                __syncthreads();
-            }
-            // thread t: the digits bins - 1 - 2 t and the next below
-            uint64_t m[2] = {0, 0};
-            uint32_t c[2] = {0, 0};
+// A histogram's sums: thread t has the bins t E .. t E + E - 1.
+template <bool kMass, int T>
+struct BinSums {
+    static constexpr int kEach = kMinPBins / T;
+    uint64_t h[kEach], before, total;
+    __device__ __forceinline__ BinSums(MinPShared<T> &s, const uint64_t *hist, uint64_t above) {
+        uint64_t own = 0;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int bin = bins - 1 - 2 * tid - i;
-                if (bin >= 0) {
-                    m[i] = s.mass[h][bin];
-                    c[i] = s.count[h][bin];
-                }
-            }
-            uint64_t bm = above_mass + block_before(m[0] + m[1], s.part[0]);
-            uint32_t bc = above_count + static_cast<uint32_t>(block_before(c[0] + c[1], s.part[1]));
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint64_t from = by_mass ? bm : bc, to = from + (by_mass ? m[i] : c[i]);
-                if (from < target && target <= to) {
-                    s.bin = static_cast<uint32_t>(bins - 1 - 2 * tid - i);
-                    s.bin_count = c[i];
-                    s.above_mass = bm;
-                    s.above_count = bc;
-                }
-                bm += m[i];
-                bc += c[i];
-            }
-            if (tid == 0) s.n = 0;
-            __syncthreads();
-            above_mass = s.above_mass;
-            above_count = s.above_count;
-            prefix |= static_cast<uint64_t>(s.bin) << shift;
-            mask |= static_cast<uint64_t>(bins - 1) << shift;
-            const bool fits = s.bin_count <= kMinPList;
-            __syncthreads();
-            if (fits) break;  // at the last level: one entry
+        for (int i = 0; i < kEach; ++i) {
+            const int bin = kEach * threadIdx.x + i;
+            h[i] = kMass ? hist[bin] : reinterpret_cast<const uint32_t *>(hist)[bin];
+            own += h[i];
         }
-        each_logit(x, a.vocab, [&](int id, float v) {
-            const uint64_t e = min_p_entry(v, id);
-            if (v >= rule.least && (e & mask) == prefix && rule.weight(v)) {
+        before = above + block_before<T>(own, s.part, total);
+    }
+    // The first bin at which the sum reaches the target (the last does): s.bin, s.above before it, s.found_mass through it.
+    __device__ __forceinline__ void find(MinPShared<T> &s, uint64_t target) const {
+        uint64_t at = before;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (at < target && target <= at + h[i]) {
+                s.bin = kEach * threadIdx.x + i;
+                s.above = at;
+                s.found_mass = at + h[i];
+            }
+            at += h[i];
+        }
+        __syncthreads();
+    }
+};
+
+// The entry at which the sum of counts or masses reaches the target, s.found, and the mass through it, s.found_mass, from the
+// row's histogram of that kind, whose whole sum reaches it.  A bin that overflows the list is cut by the digits of an
+// entry, ten or eleven bits at a time (32 of the logit, 20 of the id), until one does not; the last digits leave one entry.
+template <bool kMass, int T, typename Row>
+__device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const RowRule &rule, const BinSums<kMass, T> &sums,
+                                       uint64_t target) {
+    uint64_t prefix = 0, mask = 0;
+    sums.find(s, target);
+    const int bin = static_cast<int>(s.bin);
+    uint64_t above = s.above;
+    // the bin's logits lie between these (with room for roundings): a look at the bin itself for few others
+    const double unit = 1.0 / rule.turns, room = 1e-6 * (fabs(rule.max) + fabs(bin * unit));
+    const float from = bin == RowRule::kLast ? rule.least  // with what is beyond it
+                                             : larger(static_cast<float>(rule.max - (bin + 0.5) * unit - room), rule.least);
+    const float to = static_cast<float>(rule.max - (bin - 0.5) * unit + room);
+    auto in_question = [&](int id, float v, uint64_t &e) {
+        if (!(v >= from) || v > to || rule.bin(v) != bin) return false;
+        e = min_p_entry(v, id);
+        return e >= rule.last && (e & mask) == prefix;
+    };
+    constexpr int kBits = 11;
+    static_assert(1 << kBits == kMinPBins, "a digit fills the histogram");
+    for (int top = 64;;) {  // the digits down to bit `top` are known
+        row.each([&](int id, float v) {
+            uint64_t e;
+            if (in_question(id, v, e)) {
                 const uint32_t at = atomicAdd(&s.n, 1u);
                 if (at < kMinPList) s.list[at] = e;
             }
         });
         __syncthreads();
-        const int m = min(static_cast<int>(s.n), kMinPList);
-        sort_list(s, m);
-        const ListSums sums = sum_list(s, m, above_mass, rule);
-        if (by_mass) find_mass(s, sums, target);
-        else find_rank(s, sums, static_cast<int>(target - above_count) - 1);
-        const uint64_t mass = s.found_mass;
+        if (s.n <= kMinPList) break;
+        if (top == 32) {  // bits 20 .. 31 are ones in every entry
+            top = 20;
+            mask |= 0xfff00000ull;
+            prefix |= 0xfff00000ull;
+        }
+        const int low = top > 32 ? 32 : 0, bits = min(kBits, top - low), shift = top - bits, bins = 1 << bits;
+        for (int i = threadIdx.x; i < kMinPBins; i += T) s.hist[1][i] = 0;
         __syncthreads();
-        return mass;
+        if (threadIdx.x == 0) s.n = 0;
+        row.each([&](int id, float v) {
+            uint64_t e;
+            if (in_question(id, v, e)) {
+                const int at = bins - 1 - (static_cast<int>(e >> shift) & (bins - 1));
+                if constexpr (kMass) {
+                    const uint64_t w = rule.weight(v);
+                    if (w) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[1][at]), w);
+                } else {
+                    atomicAdd(reinterpret_cast<uint32_t *>(s.hist[1]) + at, 1u);
+                }
+            }
+        });
+        __syncthreads();
+        BinSums<kMass, T>(s, s.hist[1], above).find(s, target);
+        above = s.above;
+        prefix |= static_cast<uint64_t>(bins - 1 - s.bin) << shift;
+        mask |= static_cast<uint64_t>(bins - 1) << shift;
+        top = shift;
+    }
+    const int n = static_cast<int>(s.n);
+    sort_list<T>(s, n);
+    if constexpr (kMass) {
+        ListSums<T>(s, n, above, rule).find_mass(s, target);
+    } else {
+        if (threadIdx.x == 0) s.found = s.list[target - above - 1];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) s.n = 0;
+}
+
+// The token of a row by its histograms.
+template <int T, typename Row>
+__device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, RowRule &rule, const RowCuts &c, int vocab) {
+    // top-k: its last entry, or, where few are before it, those
+    if (c.k < vocab) {
+        row_histogram<false, T>(s, row, rule);
+        const BinSums<false, T> sums(s, s.hist[0], 0);
+        if (sums.total > static_cast<uint64_t>(c.k)) {
+            if (c.k <= kMinPSorted) {
+                sums.find(s, c.k);
+                const int bin = static_cast<int>(s.bin);
+                if (s.found_mass <= kMinPSorted) {
+                    row.each([&](int id, float v) {
+                        if (rule.counts(v) && rule.bin(v) <= bin) s.list[atomicAdd(&s.n, 1u)] = min_p_entry(v, id);
+                    });
+                    __syncthreads();
+                    return draw_from_list<T>(s, static_cast<int>(s.n), rule, c);
+                }
+                __syncthreads();
+            }
+            locate<false, T>(s, row, rule, sums, c.k);
+            rule.last = s.found;
+            __syncthreads();
+        }
+    }
+    // top-p's last entry and the drawn one, by their masses
+    row_histogram<true, T>(s, row, rule);
+    const BinSums<true, T> sums(s, s.hist[0], 0);
+    uint64_t kept = sums.total;
+    if (c.p < 1.0) {
+        locate<true, T>(s, row, rule, sums, share(c.p, kept));
+        kept = s.found_mass;
+        __syncthreads();
+    }
+    locate<true, T>(s, row, rule, sums, share(c.u, kept));
+    return entry_id(s.found);
+}
+
+template <typename InT, int T, bool kHeld>
+__global__ void __launch_bounds__(T)
+min_p_kernel(MinPArgs a) {
+    __shared__ MinPShared<T> s;
+    typedef typename std::conditional<kHeld, HeldRow<InT, T>, FarRow<InT, T>>::type Row;
+    const int64_t r = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    const Row row(static_cast<const InT *>(a.logits) + r * a.s0, a.vocab);
+    const float temperature = a.temperature[r], mp = a.min_p[r], pq = a.top_p[r], uq = a.uniforms[r];
+    const int kq = a.top_k[r];
+    const bool greedy = !(temperature > 0.f);
+    const double min_p = mp > 0.f ? (mp < 1.f ? mp : 1.0) : 0.0;
+    const RowCuts cuts = {kq > 0 && kq < a.vocab ? kq : a.vocab, pq < 1.f ? (pq > 0.f ? pq : 0.0) : 1.0,
+                          uq > 0.f ? (uq < 1.f ? uq : 1.0) : 0.0};
+    const double reach = temperature * log(fmax(min_p, 0x1p-43));
+    // The least logit that can have a weight beside a maximum; the margins cover the roundings many times over.
+    constexpr float kLargest = 3.4028234663852886e38f;
+    auto least = [&](float max) {
+        return max > kLargest ? max
+                              : larger(static_cast<float>(max + reach - 1e-6 * (fabs(static_cast<double>(max)) - reach)), -kLargest);
     };
-    // all of them, from the histogram
-    uint64_t m = 0, c = 0;
-    for (int i = tid; i < kMinPBins; i += kMinPThreads) {
-        m += s.mass[0][i];
-        c += s.count[0][i];
-    }
-    const uint64_t m0 = block_before(m, s.part[0]), c0 = block_before(c, s.part[1]);
-    if (tid == kMinPThreads - 1) {
-        s.found_mass = m0 + m;
-        s.above_mass = c0 + c;
+    if (tid < 32) s.table[tid] = kExp2Table[tid];
+    if (tid == 0) {
+        s.n = 0;
+        s.id = a.vocab;
     }
     __syncthreads();
-    uint64_t total = s.found_mass;
-    const uint64_t weighted = s.above_mass;
+
+    // 1. the maximum, and, where min-p may leave few, the list of what it leaves
+    float top = -__builtin_inff();
+    int where = -1;
+    if constexpr (kHeld) {
+        row.each([&](int, float v) { top = larger(v, top); });
+    } else {
+        top = row.first_pass(s, !greedy && min_p > 0.0, least, [&](int id, float v, float from) {
+            if (v >= from) {
+                const uint32_t at = atomicAdd(&s.n, 1u);
+                if (at < kMinPList) s.list[at] = min_p_entry(v, id);
+            }
+        }, where);
+        __syncthreads();  // the batches' maxima are read
+    }
+    const float own = top;
+    top = group_max<kWave>(top);
+    if (lane == 0) s.max[0][wave] = top;
     __syncthreads();
-    if (static_cast<uint64_t>(k) < weighted) total = locate(k, false);
-    const uint64_t kept = p < 1.0 ? locate(share(p, total), true) : total;
-    locate(share(u, kept), true);
-    if (tid == 0) a.tokens[row] = s.found_id;
+    top = s.max[0][0];
+#pragma unroll
+    for (int w = 1; w < T / kWave; ++w) top = fmaxf(top, s.max[0][w]);
+    if (greedy || top == -__builtin_inff()) {
+        if (own == top) {
+            auto first = [&](int id, float v) {
+                if (v == top) atomicMin(&s.id, id);
+            };
+            if constexpr (kHeld) row.each(first);
+            else row.vector(where, first);
+        }
+        __syncthreads();
+        if (tid == 0) a.tokens[r] = top == -__builtin_inff() ? 0 : s.id;
+        return;
+    }
+    RowRule rule;
+    rule.table = s.table;
+    rule.max = fminf(top, kLargest);
+    rule.turns = top > kLargest ? 0.0 : 32.0 * 1.4426950408889634 / temperature;
+    rule.min_p = min_p * 4398046511104.0;  // in weights
+    rule.least = least(top);
+    rule.last = 0;
+    const int found = static_cast<int>(s.n);
+    __syncthreads();
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    if constexpr (kHeld) {
+        row.each([&](int id, float v) {
+            if (rule.counts(v)) {
+                const uint32_t at = atomicAdd(&s.n, 1u);
+                if (at < kMinPList) s.list[at] = min_p_entry(v, id);
+            }
+        });
+    } else if (found > 0 && found <= kMinPList) {
+        const HeldList<T> list(s, found);
+        list.each([&](int id, float v) {
+            if (rule.counts(v)) s.list[atomicAdd(&s.n, 1u)] = min_p_entry(v, id);
+        });
+    }
+    __syncthreads();
+    const int n = static_cast<int>(s.n);
+    int token;
+    if (n > 0 && n <= kMinPSorted) {
+        token = draw_from_list<T>(s, n, rule, cuts);
+    } else {
+        __syncthreads();
+        if constexpr (kHeld) {
+            token = draw_by_bins<T>(s, row, rule, cuts, a.vocab);
+        } else if (n > 0) {
+            const HeldList<T> list(s, n);
+            token = draw_by_bins<T>(s, list, rule, cuts, a.vocab);
+        } else {
+            token = draw_by_bins<T>(s, row, rule, cuts, a.vocab);
+        }
+    }
+    if (tid == 0) a.tokens[r] = token;
+}
+
+// Threads a row: enough to hold it, or to keep a CU's loads in flight.
+template <typename InT>
+void launch_min_p(const MinPArgs &a, int rows, hipStream_t st) {
+    if (a.vocab <= 256 * kMinPHeld)
+        hipLaunchKernelGGL((min_p_kernel<InT, 256, true>), dim3(rows), dim3(256), 0, st, a);
+    else if (a.vocab <= 1024 * kMinPHeld)
+        hipLaunchKernelGGL((min_p_kernel<InT, 1024, true>), dim3(rows), dim3(1024), 0, st, a);
+    else
+        hipLaunchKernelGGL((min_p_kernel<InT, 1024, false>), dim3(rows), dim3(1024), 0, st, a);
 }
 
 }  // namespace
@@ -430,9 +764,7 @@ extern "C" int nq_sample_min_p(const void *logits, int logits_dtype, int64_t log
     if (reinterpret_cast<uintptr_t>(logits) % (logits_dtype == NQ_F32 ? 4 : 2)) return NQ_ERR_UNSUPPORTED;
     const MinPArgs a = {logits, logits_s0, vocab, temperature, top_k, top_p, min_p, uniforms, tokens};
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (logits_dtype == NQ_F32)
-        hipLaunchKernelGGL(min_p_kernel<float>, dim3(rows), dim3(kMinPThreads), 0, st, a);
-    else
-        hipLaunchKernelGGL(min_p_kernel<uint16_t>, dim3(rows), dim3(kMinPThreads), 0, st, a);
+    if (logits_dtype == NQ_F32) launch_min_p<float>(a, rows, st);
+    else launch_min_p<uint16_t>(a, rows, st);
     return NQ_LAUNCH_STATUS();
 }

@@ -119,6 +119,53 @@ def test_masked_and_infinite_logits(nq, device, vocab):
             _run(device, x.to(torch.bfloat16), [t] * 16, [k] * 16, [p] * 16, [m] * 16, _uniforms(rng, 16))
 
 
+@pytest.mark.parametrize("vocab", [65, 3000, 9001])
+def test_every_kind_of_nan(nq, device, vocab):
+    """Quiet and signalling NaN of both signs, in the first places and the last, are never the maximum."""
+
+    rng = np.random.default_rng(vocab)
+    x = _logits(rng, device, 12, vocab, torch.bfloat16, 1.0)
+    bits = x.view(torch.int16)
+    for i, nan in enumerate((0x7f81, 0x7fff, 0x7fc0, -0x7f, -1, -0x40)):
+        bits[i, ::2], bits[i + 6, 1::2] = nan, nan
+        bits[i, -1] = bits[i + 6, 0] = nan
+    assert (x.isnan().sum(1) >= vocab // 2).all()
+    for t, m in ((1.0, 0.0), (1.0, 0.05), (0.0, 0.0)):
+        got = _run(device, x, [t] * 12, [0, 20] * 6, [0.9, 1.0, 1.0] * 4, [m] * 12, _uniforms(rng, 12))
+        assert not x.cpu()[torch.arange(12), torch.from_numpy(got)].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_greedy_ties_take_the_lowest_id(nq, device, dtype):
+    """Maxima in the first and last places, which rows at odd addresses load alone, and between them."""
+
+    vocab = 20011
+    wide = torch.zeros(24, vocab + 7, dtype=dtype, device=device)
+    for at in range(7):
+        x = wide[:, at:at + vocab]
+        x.fill_(-1.0)
+        want = np.zeros(24, np.int64)
+        for r in range(24):
+            ids = [vocab - 1 - r % 3, vocab // 2 + 37 * r, 8191 + r, 8 + r] + ([r % 9] if r % 2 else [])
+            x[r, ids] = 0.0
+            if r % 4 == 0:
+                x[r, ids[-1]] = -0.0
+            want[r] = min(ids)
+        assert np.array_equal(_run(device, x, [0.0] * 24, [0] * 24, [1.0] * 24, [0.0] * 24, [0.5] * 24), want)
+        _run(device, x, [1.0] * 24, [3] * 24, [1.0] * 24, [0.0, 0.99] * 12, [0.9] * 24)
+
+
+def test_large_offsets_beside_a_small_temperature(nq, device):
+    """Where a bound on the logits that count is looser than the weights' range: those are counted and weigh nothing."""
+
+    rng = np.random.default_rng(12)
+    x = torch.from_numpy((1e6 + rng.random((12, 9000)) * 8).astype(np.float32)).to(device)
+    for t in (1e-3, 0.01, 0.3):
+        for k, p, m in ((0, 1.0, 0.0), (8500, 1.0, 0.0), (4000, 0.9, 0.0), (300, 1.0, 0.0), (0, 0.9, 0.1)):
+            _run(device, x, [t] * 12, [k] * 12, [p] * 12, [m] * 12, _uniforms(rng, 12))
+            _run(device, -x, [t] * 12, [k] * 12, [p] * 12, [m] * 12, _uniforms(rng, 12))
+
+
 def test_parameters_out_of_range(nq, device):
     rng = np.random.default_rng(9)
     for vocab in (300, 9000):
