@@ -127,25 +127,36 @@ __device__ const double kExp2Table[32] = {
 // octaves.
 struct RowRule {
     static constexpr int kPer = 32, kLast = 45 * kPer;
+    static constexpr float kLargest = 3.4028234663852886e38f;
     static_assert(kLast < kMinPBins, "the row's bins");
     const double *table;  // in LDS
     double max, turns;    // turns: 32 log2(e) / T
     double min_p;
-    float least;          // no logit below it has a weight (a bound); NaN and -inf are never from it on
-    uint64_t last;        // top-k's last entry: none behind it has a weight
+    float least;          // no logit below it has a weight (a bound, or top-k's last one); NaN and -inf never reach it
+    float tie;            // of the logits that equal it (NaN: none do) those with ids behind tie_id have none either
+    int tie_id;
     __device__ __forceinline__ double turn(float x) const {
         // an infinite maximum is held as the largest finite logit, which only infinite ones then reach
-        const double d = static_cast<double>(fminf(x, 3.4028234663852886e38f)) - max;
+        const double d = static_cast<double>(__builtin_amdgcn_fmed3f(x, -kLargest, kLargest)) - max;
         return fmax(d * turns, -1.0 * kLast);
     }
     __device__ __forceinline__ int bin(float x) const {  // does not decrease as x falls
         return -static_cast<int>(rint(turn(x)));
     }
-    __device__ __forceinline__ uint64_t weight(float x, int &bin) const {
+    // The bin's logits lie between these two, with room for their roundings; the last bin's reach down to any that counts.
+    __device__ __forceinline__ float bin_from(int bin) const {
+        const double at = (bin + 0.5) / turns;
+        return bin == kLast ? least : larger(static_cast<float>(max - at - 1e-6 * (fabs(max) + at)), least);
+    }
+    __device__ __forceinline__ float bin_to(int bin) const {
+        const double at = (bin - 0.5) / turns;
+        return static_cast<float>(max - at + 1e-6 * (fabs(max) + fabs(at)));
+    }
+    // 0 for what does not count
+    __device__ __forceinline__ uint64_t weight(float x, int id, int &bin) const {
         const double t = turn(x), n = rint(t), f = t - n;
         const int i = static_cast<int>(n);
-        double p = 3.973709984549416e-11;  // (ln 2 / 32)^5 / 5!, and so on
-        p = fma(p, f, 9.172562701824643e-09);
+        double p = fma(3.973709984549416e-11, f, 9.172562701824643e-09);  // (ln 2 / 32)^5 / 5!, and so on
         p = fma(p, f, 1.693850972437182e-06);
         p = fma(p, f, 0.0002345961982022468);
         p = fma(p, f, 0.02166084939249829);
@@ -155,13 +166,13 @@ struct RowRule {
         const double w = __longlong_as_double(__double_as_longlong(p) + (static_cast<int64_t>((i >> 5) + 42) << 52));
         bin = -i;
         const uint64_t whole = static_cast<uint64_t>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
-        return w >= min_p ? whole : 0;
+        return w >= min_p && counts(x, id) ? whole : 0;
     }
-    __device__ __forceinline__ uint64_t weight(float x) const {
+    __device__ __forceinline__ uint64_t weight(uint64_t entry) const {
         int bin;
-        return weight(x, bin);
+        return weight(entry_value(entry), entry_id(entry), bin);
     }
-    __device__ __forceinline__ bool counts(float x) const { return x >= least; }
+    __device__ __forceinline__ bool counts(float x, int id) const { return x >= least && !(x == tie && id > tie_id); }
 };
 
 template <typename InT>
@@ -190,7 +201,19 @@ struct HeldRow {
             if (id < vocab) f(id, x[i]);
         }
     }
+    // f for several logits at once: an id, the step to the next, and the logits, NaN where there is none
+    template <typename F>
+    __device__ __forceinline__ void several(F f) const {
+#pragma unroll 1
+        for (int i = 0; i < kMinPHeld; i += 4) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = static_cast<int>(threadIdx.x) + (i + e) * T < vocab ? (i ? x[e + 4] : x[e]) : __builtin_nanf("");
+            f(static_cast<int>(threadIdx.x) + i * T, T, v);
+        }
+    }
 };
+static_assert(kMinPHeld == 8, "two groups of four");
 
 // What is left of a row, the n entries of a list, in registers: the list is free for others behind the constructor.
 template <int T>
@@ -210,6 +233,14 @@ struct HeldList {
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
             if (e[i]) f(entry_id(e[i]), entry_value(e[i]));
+    }
+    template <typename F>
+    __device__ __forceinline__ void several(F f) const {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const float v[1] = {e[i] ? entry_value(e[i]) : __builtin_nanf("")};
+            f(entry_id(e[i]), 1, v);
+        }
     }
 };
 
@@ -244,10 +275,13 @@ struct FarRow {
     }
     // Three vectors of a thread are in flight; the body is one's, since code that is run through once costs its fetch.
     template <typename F>
-    __device__ __forceinline__ void each(F f) const {
+    __device__ __forceinline__ void several(F f) const {
         const int tid = threadIdx.x;
         uint4 v0 = load(tid), v1 = load(tid + T), v2 = load(tid + 2 * T);
-        few(f);
+        few([&](int id, float x) {
+            const float v[1] = {x};
+            f(id, 1, v);
+        });
 #pragma unroll 1
         for (int j = tid; j < nv; j += T) {
             const uint4 v = v0;
@@ -256,9 +290,16 @@ struct FarRow {
             v2 = load(j + 3 * T);
             float x[V];
             unpack(v, x);
-#pragma unroll
-            for (int e = 0; e < V; ++e) f(head + j * V + e, x[e]);
+            f(head + j * V, 1, x);
         }
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        several([&](int id, int step, const auto &x) {
+            constexpr int N = sizeof(x) / sizeof(float);
+#pragma unroll
+            for (int e = 0; e < N; ++e) f(id + e * step, x[e]);
+        });
     }
     // The largest logit of this thread's part, and in `where` the first vector that holds its vectors' largest (-1: none).  With
     // collect, after each batch of loads: the largest so far of all threads goes through least(), and put takes every logit of
@@ -389,7 +430,7 @@ struct ListSums {
         uint64_t own = 0;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            if (first + i < end) own += rule.weight(entry_value(s.list[first + i]));
+            if (first + i < end) own += rule.weight(s.list[first + i]);
             cum[i] = own;
         }
         uint64_t total;
@@ -441,7 +482,7 @@ __device__ __forceinline__ int draw_from_few(const MinPShared<T> &s, int n, cons
     const uint32_t lo = __builtin_amdgcn_ds_permute(4 * above, static_cast<int>(static_cast<uint32_t>(mine)));
     const uint32_t hi = __builtin_amdgcn_ds_permute(4 * above, static_cast<int>(static_cast<uint32_t>(mine >> 32)));
     const uint64_t e = (static_cast<uint64_t>(hi) << 32) | lo;
-    double cum = lane < n && lane < c.k ? static_cast<double>(rule.weight(entry_value(e))) : 0.0;
+    double cum = lane < n && lane < c.k ? static_cast<double>(rule.weight(e)) : 0.0;
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) {
         const double o = __shfl_up(cum, d, kWave);
@@ -479,16 +520,22 @@ __device__ __forceinline__ void row_histogram(MinPShared<T> &s, const Row &row, 
     for (int i = threadIdx.x; i < kMinPBins; i += T) s.hist[0][i] = 0;
     if (threadIdx.x == 0) s.n = 0;
     __syncthreads();
-    const bool all = rule.last == 0;
-    row.each([&](int id, float v) {
-        if (!rule.counts(v)) return;
+    row.several([&](int id, int step, const auto &x) {
+        constexpr int N = sizeof(x) / sizeof(float);
+        int bin[N];
         if constexpr (kMass) {
-            int bin;
-            uint64_t w = rule.weight(v, bin);
-            if (!all && min_p_entry(v, id) < rule.last) w = 0;
-            if (w) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[0][bin]), w);
+            uint64_t w[N];  // side by side: one's instructions alone would wait for each other
+#pragma unroll
+            for (int e = 0; e < N; ++e) w[e] = rule.weight(x[e], id + e * step, bin[e]);
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (w[e]) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[0][bin[e]]), w[e]);
         } else {
-            atomicAdd(reinterpret_cast<uint32_t *>(s.hist[0]) + rule.bin(v), 1u);
+#pragma unroll
+            for (int e = 0; e < N; ++e) bin[e] = rule.bin(x[e]);
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (rule.counts(x[e], id + e * step)) atomicAdd(reinterpret_cast<uint32_t *>(s.hist[0]) + bin[e], 1u);
         }
     });
     __syncthreads();
@@ -535,15 +582,11 @@ __device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const R
     sums.find(s, target);
     const int bin = static_cast<int>(s.bin);
     uint64_t above = s.above;
-    // the bin's logits lie between these (with room for roundings): a look at the bin itself for few others
-    const double unit = 1.0 / rule.turns, room = 1e-6 * (fabs(rule.max) + fabs(bin * unit));
-    const float from = bin == RowRule::kLast ? rule.least  // with what is beyond it
-                                             : larger(static_cast<float>(rule.max - (bin + 0.5) * unit - room), rule.least);
-    const float to = static_cast<float>(rule.max - (bin - 0.5) * unit + room);
+    const float from = rule.bin_from(bin), to = rule.bin_to(bin);  // a look at the bin itself for few others
     auto in_question = [&](int id, float v, uint64_t &e) {
-        if (!(v >= from) || v > to || rule.bin(v) != bin) return false;
+        if (!(v >= from) || v > to || rule.bin(v) != bin || !rule.counts(v, id)) return false;
         e = min_p_entry(v, id);
-        return e >= rule.last && (e & mask) == prefix;
+        return (e & mask) == prefix;
     };
     constexpr int kBits = 11;
     static_assert(1 << kBits == kMinPBins, "a digit fills the histogram");
@@ -571,7 +614,7 @@ __device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const R
             if (in_question(id, v, e)) {
                 const int at = bins - 1 - (static_cast<int>(e >> shift) & (bins - 1));
                 if constexpr (kMass) {
-                    const uint64_t w = rule.weight(v);
+                    const uint64_t w = rule.weight(e);
                     if (w) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[1][at]), w);
                 } else {
                     atomicAdd(reinterpret_cast<uint32_t *>(s.hist[1]) + at, 1u);
@@ -609,7 +652,7 @@ __device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, Ro
                 const int bin = static_cast<int>(s.bin);
                 if (s.found_mass <= kMinPSorted) {
                     row.each([&](int id, float v) {
-                        if (rule.counts(v) && rule.bin(v) <= bin) s.list[atomicAdd(&s.n, 1u)] = min_p_entry(v, id);
+                        if (rule.counts(v, id) && rule.bin(v) <= bin) s.list[atomicAdd(&s.n, 1u)] = min_p_entry(v, id);
                     });
                     __syncthreads();
                     return draw_from_list<T>(s, static_cast<int>(s.n), rule, c);
@@ -617,7 +660,8 @@ __device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, Ro
                 __syncthreads();
             }
             locate<false, T>(s, row, rule, sums, c.k);
-            rule.last = s.found;
+            rule.least = rule.tie = entry_value(s.found);  // at least what it was
+            rule.tie_id = entry_id(s.found);
             __syncthreads();
         }
     }
@@ -650,7 +694,7 @@ min_p_kernel(MinPArgs a) {
                           uq > 0.f ? (uq < 1.f ? uq : 1.0) : 0.0};
     const double reach = temperature * log(fmax(min_p, 0x1p-43));
     // The least logit that can have a weight beside a maximum; the margins cover the roundings many times over.
-    constexpr float kLargest = 3.4028234663852886e38f;
+    constexpr float kLargest = RowRule::kLargest;
     auto least = [&](float max) {
         return max > kLargest ? max
                               : larger(static_cast<float>(max + reach - 1e-6 * (fabs(static_cast<double>(max)) - reach)), -kLargest);
@@ -701,14 +745,15 @@ min_p_kernel(MinPArgs a) {
     rule.turns = top > kLargest ? 0.0 : 32.0 * 1.4426950408889634 / temperature;
     rule.min_p = min_p * 4398046511104.0;  // in weights
     rule.least = least(top);
-    rule.last = 0;
+    rule.tie = __builtin_nanf("");
+    rule.tie_id = 0;
     const int found = static_cast<int>(s.n);
     __syncthreads();
     if (tid == 0) s.n = 0;
     __syncthreads();
     if constexpr (kHeld) {
         row.each([&](int id, float v) {
-            if (rule.counts(v)) {
+            if (rule.counts(v, id)) {
                 const uint32_t at = atomicAdd(&s.n, 1u);
                 if (at < kMinPList) s.list[at] = min_p_entry(v, id);
             }
@@ -716,8 +761,25 @@ min_p_kernel(MinPArgs a) {
     } else if (found > 0 && found <= kMinPList) {
         const HeldList<T> list(s, found);
         list.each([&](int id, float v) {
-            if (rule.counts(v)) s.list[atomicAdd(&s.n, 1u)] = min_p_entry(v, id);
+            if (rule.counts(v, id)) s.list[atomicAdd(&s.n, 1u)] = min_p_entry(v, id);
         });
+    } else if (cuts.k <= T / 2) {
+        // the k-th largest of the threads' own maxima, or its bin: as many logits reach it, and few more
+        for (int i = tid; i < kMinPBins; i += T) s.hist[0][i] = 0;
+        __syncthreads();
+        if (own >= rule.least) atomicAdd(reinterpret_cast<uint32_t *>(s.hist[0]) + rule.bin(own), 1u);
+        __syncthreads();
+        const BinSums<false, T> sums(s, s.hist[0], 0);
+        if (sums.total >= static_cast<uint64_t>(cuts.k)) {
+            sums.find(s, cuts.k);
+            const float from = rule.bin_from(static_cast<int>(s.bin));
+            row.each([&](int id, float v) {
+                if (v >= from) {
+                    const uint32_t at = atomicAdd(&s.n, 1u);
+                    if (at < kMinPList) s.list[at] = min_p_entry(v, id);
+                }
+            });
+        }
     }
     __syncthreads();
     const int n = static_cast<int>(s.n);
@@ -728,7 +790,7 @@ min_p_kernel(MinPArgs a) {
         __syncthreads();
         if constexpr (kHeld) {
             token = draw_by_bins<T>(s, row, rule, cuts, a.vocab);
-        } else if (n > 0) {
+        } else if (n > 0 && n <= kMinPList) {
             const HeldList<T> list(s, n);
             token = draw_by_bins<T>(s, list, rule, cuts, a.vocab);
         } else {
