@@ -929,7 +929,7 @@ int nq_linear_int8_act(const int8_t *xq, int64_t x_s0, const float *sx, const in
  * 2^20 (no counterpart in the reference, whose samplers have no min-p, executor/sampling.py:156-336).
  * logits: fp32 or bf16 (NQ_F32, NQ_BF16) [rows, vocab], rows logits_s0 apart; the parameters one a row.
  * With x the logits (a NaN counts as minus infinity), e = exp((x - max x) / temperature) in double and w =
- * rint(2^42 e), or 0 where e < min_p, the ranks are in the order of (x descending, id ascending) and
+ * rint(2^42 e), or 0 where that is below 2^42 min_p, the ranks are in the order of (x descending, id ascending) and
  *   total = the sum of w over the first top_k ranks (top_k <= 0: all),
  *   kept  = the sum of w up to the first rank at which it reaches top_p * total,
  *   token = the id of the first rank at which the sum of w reaches u * kept.

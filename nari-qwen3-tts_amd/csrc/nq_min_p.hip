@@ -1,7 +1,7 @@
 // A token a row from logits over a vocabulary of any size up to 2^20: temperature, min-p, top-k, top-p and the draw for a
 // given uniform number.
 //   e_i   = exp((x_i - max x) / T)          in double;  NaN logits count as -inf, -0 as 0
-//   w_i   = rint(2^42 e_i), 0 where e_i < min_p: an integer, so that every sum is exact in any order and the token does
+//   w_i   = rint(2^42 e_i), or 0 where that is below 2^42 min_p: an integer, so that every sum is exact in any order and the token does
 //           not depend on how the work is cut; 2^20 of them stay below 2^62
 //   order : by (x desc, id asc); F(r) = sum of w over the ranks 0 .. r
 //   total = F(min(k, V) - 1), k = top_k > 0 ? top_k : V
@@ -22,10 +22,8 @@
 namespace nq {
 namespace {
 
-constexpr int kMinPList = 4096;  // entries of the list
-constexpr int kMinPSorted = 512; // entries that are rather sorted than cut by a histogram
-constexpr int kMinPRanked = 256; // entries that are sorted by counting those above each
-constexpr int kMinPBins = 2048;
+constexpr int kMinPSorted = 256;  // entries that are rather sorted, by counting those above each, than cut by a histogram
+constexpr int kMinPDigits = 2048; // values of a digit that cuts a bin
 constexpr int kMinPHeld = 8;     // logits a thread keeps in registers where the row fits
 constexpr int kMinPVocab = 1 << 20;
 
@@ -57,36 +55,44 @@ __device__ __forceinline__ int entry_id(uint64_t e) {
 // The larger of the two; b where a is NaN (fmaxf answers NaN to a signalling one).
 __device__ __forceinline__ float larger(float a, float b) { return a > b ? a : b; }
 
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
-    const uint32_t lo = __shfl_up(static_cast<uint32_t>(v), d, kWave);
-    const uint32_t hi = __shfl_up(static_cast<uint32_t>(v >> 32), d, kWave);
+// v of lanes moved by a DPP control word, 0 where none comes from
+template <int Ctrl, int Rows>
+__device__ __forceinline__ uint64_t dpp64(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(v)), Ctrl, Rows, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(v >> 32)), Ctrl, Rows, 0xF, false);
     return (static_cast<uint64_t>(hi) << 32) | lo;
 }
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
-    const uint32_t lo = __shfl_xor(static_cast<uint32_t>(v), m, kWave);
-    const uint32_t hi = __shfl_xor(static_cast<uint32_t>(v >> 32), m, kWave);
-    return (static_cast<uint64_t>(hi) << 32) | lo;
-}
-__device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {  // inclusive
-    const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const uint64_t o = shfl_up64(v, d);
-        if (lane >= d) v += o;
-    }
+// Inclusive sums over the 64 lanes: wave_incl_scan's steps.
+__device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {
+    v += dpp64<0x111, 0xF>(v);
+    v += dpp64<0x112, 0xF>(v);
+    v += dpp64<0x114, 0xF>(v);
+    v += dpp64<0x118, 0xF>(v);
+    v += dpp64<0x142, 0xA>(v);
+    v += dpp64<0x143, 0xC>(v);
     return v;
 }
+
+// Sizes by the threads of a row: 1024, or 256 for what they hold in registers.
+template <int T>
+struct MinPSizes {
+    static constexpr int kList = T == 1024 ? 4096 : T * kMinPHeld;  // entries of the list
+    static constexpr int kShift = T == 1024 ? 0 : 3;                // the row's histogram has 128 bins an octave, or 16
+    static constexpr int kLast = 45 * (128 >> kShift);
+    static constexpr int kEach = kLast / T + 1, kBins = kEach * T;  // bins a thread, and of them all
+};
 
 template <int T>
 struct MinPShared {
     static constexpr int kWaves = T / kWave;
-    uint64_t list[kMinPList];
-    uint64_t hist[2][kMinPBins];  // of the row, and of what one bin is cut by; counts take 32 bits a bin
-    double table[32];
+    uint64_t list[MinPSizes<T>::kList];
+    uint64_t hist[MinPSizes<T>::kBins];  // of the row; counts take 32 bits a bin
+    uint64_t digits[T == 1024 ? kMinPDigits : 1];
+    double table[128];
     uint64_t part[kWaves];
     float max[2][kWaves];
     uint64_t found_mass, found, above;
-    uint32_t rank[kMinPRanked];
+    uint32_t rank[kMinPSorted];
     uint32_t bin, n;
     int id;
 };
@@ -109,71 +115,106 @@ __device__ __forceinline__ uint64_t block_before(uint64_t v, uint64_t *part, uin
     return before;
 }
 
-// 2^(i / 32)
-__device__ const double kExp2Table[32] = {
-    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
-    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
-    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
-    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
-    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
-    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
-    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
-    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
+// 2^(42 + i / 128)
+__device__ const double kExp2Table[128] = {
+    4398046511104.0, 4421927468748.802, 4445938097632.095, 4470079101855.88,
+    4494351189345.363, 4518755071869.717, 4543291465062.945, 4567961088444.878,
+    4592764665442.265, 4617702923409.991, 4642776593652.408, 4667986411444.776,
+    4693333116054.829, 4718817450764.449, 4744440162891.469, 4770202003811.579,
+    4796103728980.37, 4822146097955.479, 4848329874418.864, 4874655826199.207,
+    4901124725294.416, 4927737347894.278, 4954494474403.209, 4981396889463.146,
+    5008445381976.555, 5035640745129.562, 5062983776415.216, 5090475277656.876,
+    5118116055031.72, 5145906919094.391, 5173848684800.761, 5201942171531.834,
+    5230188203117.7705, 5258587607862.048, 5287141218565.749, 5315849872551.985,
+    5344714411690.448, 5373735682422.1, 5402914535783.991, 5432251827434.224,
+    5461748417677.033, 5491405171488.027, 5521222958539.541, 5551202653226.147,
+    5581345134690.294, 5611651286848.085, 5642121998415.203, 5672758162932.967,
+    5703560678794.538, 5734530449271.263, 5765668382539.163, 5796975391705.564,
+    5828452394835.877, 5860100314980.515, 5891920080201.963, 5923912623601.997,
+    5956078883349.04, 5988419802705.679, 6020936330056.32, 6053629418935.009,
+    6086500028053.38, 6119549121328.781, 6152777667912.536, 6186186642218.362,
+    6219777023950.95, 6253549798134.687, 6287505955142.546, 6321646490725.129,
+    6355972406039.863, 6390484707680.363, 6425184407705.946, 6460072523671.312,
+    6495150078656.382, 6530418101296.299, 6565877625811.596, 6601529692038.518,
+    6637375345459.519, 6673415637233.919, 6709651624228.731, 6746084369049.649,
+    6782714940072.214, 6819544411473.137, 6856573863261.803, 6893804381311.943,
+    6931237057393.474, 6968872989204.515, 7006713280403.578, 7044759040641.932,
+    7083011385596.141, 7121471437000.784, 7160140322681.349, 7199019176587.3,
+    7238109138825.341, 7277411355692.836, 7316926979711.437, 7356657169660.869,
+    7396603090612.919, 7436765913965.6, 7477146817477.495, 7517746985302.307,
+    7558567608023.569, 7599609882689.572, 7640875012848.455, 7682364208583.509,
+    7724078686548.652, 7766019670004.119, 7808188388852.323, 7850586079673.927,
+    7893213985764.103, 7936073357168.994, 7979165450722.371, 8022491530082.486,
+    8066052865769.132, 8109850735200.898, 8153886422732.63, 8198161219693.094,
+    8242676424422.843, 8287433342312.29, 8332433285839.99, 8377677574611.128,
+    8423167535396.213, 8468904502169.985, 8514889816150.538, 8561124825838.647,
+    8607610887057.3125, 8654349362991.52, 8701341624228.211, 8748589048796.485,
 };
 
-// What a row's weights follow from.  With t = 32 log2(e) (x - max) / T and i = rint(t), e = 2^(i / 32) 2^((t - i) / 32): a
-// table, the Taylor series of 2^f for |f| <= 1 / 64 to its fifth power, whose rest is below 3e-15 of it, and an
-// exponent; and -i is the logit's bin in the row's histogram, 32 an octave.  A weight of 1 needs e >= 2^-43, so t is held to 45
-// octaves.
+// What a row's weights follow from.  With t = 128 log2(e) (x - max) / T and i = rint(t), e = 2^(i / 128) 2^((t - i) / 128): a
+// table, the Taylor series of 2^f for |f| <= 1 / 256 to its fourth power, whose rest is below 2e-15 of it, and an
+// exponent; and -i, or -i / 8, is the logit's bin in the row's histogram.  A weight of 1 needs e >= 2^-43, so t is held to
+// 45 octaves.
+template <int kShift>
 struct RowRule {
-    static constexpr int kPer = 32, kLast = 45 * kPer;
+    static constexpr int kPer = 128, kLast = 45 * (kPer >> kShift);
     static constexpr float kLargest = 3.4028234663852886e38f;
-    static_assert(kLast < kMinPBins, "the row's bins");
     const double *table;  // in LDS
-    double max, turns;    // turns: 32 log2(e) / T
-    double min_p;
+    double max, turns;    // turns: 128 log2(e) / T
+    double lowest;        // of t: -45 octaves
+    uint64_t least_weight;  // a smaller one is none (min-p)
     float least;          // no logit below it has a weight (a bound, or top-k's last one); NaN and -inf never reach it
     float tie;            // of the logits that equal it (NaN: none do) those with ids behind tie_id have none either
     int tie_id;
+    bool plain;           // t keeps above its bound by itself, and neither least_weight nor tie drop a logit
     __device__ __forceinline__ double turn(float x) const {
-        // an infinite maximum is held as the largest finite logit, which only infinite ones then reach
-        const double d = static_cast<double>(__builtin_amdgcn_fmed3f(x, -kLargest, kLargest)) - max;
-        return fmax(d * turns, -1.0 * kLast);
+        // beside an infinite maximum max, turns and lowest are 0 and infinite logits alone count: NaN becomes 0
+        return fmax((static_cast<double>(x) - max) * turns, lowest);
     }
     __device__ __forceinline__ int bin(float x) const {  // does not decrease as x falls
-        return -static_cast<int>(rint(turn(x)));
+        return -static_cast<int>(rint(turn(x))) >> kShift;
     }
     // The bin's logits lie between these two, with room for their roundings; the last bin's reach down to any that counts.
     __device__ __forceinline__ float bin_from(int bin) const {
-        const double at = (bin + 0.5) / turns;
+        const double at = (((bin + 1) << kShift) - 0.5) / turns;
         return bin == kLast ? least : larger(static_cast<float>(max - at - 1e-6 * (fabs(max) + at)), least);
     }
     __device__ __forceinline__ float bin_to(int bin) const {
-        const double at = (bin - 0.5) / turns;
+        const double at = ((bin << kShift) - 0.5) / turns;
         return static_cast<float>(max - at + 1e-6 * (fabs(max) + fabs(at)));
     }
-    // 0 for what does not count
-    __device__ __forceinline__ uint64_t weight(float x, int id, int &bin) const {
-        const double t = turn(x), n = rint(t), f = t - n;
+    // The weight by t, whether or not the logit counts.
+    __device__ __forceinline__ uint64_t weight(double t, int &bin) const {
+        const double n = rint(t), f = t - n;
         const int i = static_cast<int>(n);
-        double p = fma(3.973709984549416e-11, f, 9.172562701824643e-09);  // (ln 2 / 32)^5 / 5!, and so on
-        p = fma(p, f, 1.693850972437182e-06);
-        p = fma(p, f, 0.0002345961982022468);
-        p = fma(p, f, 0.02166084939249829);
+        double p = fma(3.583199206380349e-11, f, 2.6466421444330903e-08);  // (ln 2 / 128)^4 / 4!, and so on
+        p = fma(p, f, 1.4662262387640426e-05);
+        p = fma(p, f, 0.005415212348124573);
         p = fma(p, f, 1.0);
-        p *= table[i & (kPer - 1)];
-        // its exponent, and 42 more: then the integer is in the low bits behind 2^52, rounded
-        const double w = __longlong_as_double(__double_as_longlong(p) + (static_cast<int64_t>((i >> 5) + 42) << 52));
-        bin = -i;
-        const uint64_t whole = static_cast<uint64_t>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
-        return w >= min_p && counts(x, id) ? whole : 0;
+        const uint64_t e = __double_as_longlong(table[i & (kPer - 1)]);
+        const uint32_t high = static_cast<uint32_t>(e >> 32) + (static_cast<uint32_t>(i & -kPer) << 13);  // its exponent + i / 128
+        // behind 2^52 the integer is in the low bits, rounded
+        const double w = fma(p, __longlong_as_double((static_cast<uint64_t>(high) << 32) | static_cast<uint32_t>(e)), 4503599627370496.0);
+        bin = -i >> kShift;
+        return static_cast<uint64_t>(__double_as_longlong(w)) & 0xfffffffffffffull;
+    }
+    __device__ __forceinline__ uint64_t weight(float x, int &bin) const {
+        const uint64_t w = weight(turn(x), bin);
+        return w >= least_weight ? w : 0;
+    }
+    __device__ __forceinline__ uint64_t plain_weight(float x, int &bin) const {
+        return weight((static_cast<double>(x) - max) * turns, bin);
     }
     __device__ __forceinline__ uint64_t weight(uint64_t entry) const {
         int bin;
-        return weight(entry_value(entry), entry_id(entry), bin);
+        const float x = entry_value(entry);
+        const uint64_t w = weight(x, bin);
+        return counts(x, entry_id(entry)) ? w : 0;
     }
     __device__ __forceinline__ bool counts(float x, int id) const { return x >= least && !(x == tie && id > tie_id); }
 };
+template <int T>
+using Rule = RowRule<MinPSizes<T>::kShift>;
 
 template <typename InT>
 __device__ __forceinline__ float logit_at(const InT *row, int id) {
@@ -184,6 +225,7 @@ __device__ __forceinline__ float logit_at(const InT *row, int id) {
 // A row in registers, thread t the ids t, t + T, ..
 template <typename InT, int T>
 struct HeldRow {
+    static constexpr bool kShort = false;  // whether its logits are bf16 and many
     float x[kMinPHeld];
     int vocab;
     __device__ __forceinline__ HeldRow(const InT *row, int v) : vocab(v) {
@@ -218,7 +260,8 @@ static_assert(kMinPHeld == 8, "two groups of four");
 // What is left of a row, the n entries of a list, in registers: the list is free for others behind the constructor.
 template <int T>
 struct HeldList {
-    static constexpr int kEach = kMinPList / T;
+    static constexpr bool kShort = false;
+    static constexpr int kEach = MinPSizes<T>::kList / T;
     uint64_t e[kEach];
     __device__ __forceinline__ HeldList(const MinPShared<T> &s, int n) {
 #pragma unroll
@@ -250,6 +293,7 @@ struct FarRow {
     const InT *row;
     int vocab, head, nv;
     static constexpr int V = 16 / sizeof(InT);
+    static constexpr bool kShort = sizeof(InT) == 2;
     __device__ __forceinline__ FarRow(const InT *r, int v) : row(r), vocab(v) {
         head = min(v, static_cast<int>((16 - reinterpret_cast<uintptr_t>(r) % 16) % 16 / sizeof(InT)));
         nv = (v - head) / V;
@@ -273,24 +317,28 @@ struct FarRow {
         const int i = threadIdx.x, id = i < head ? i : i + nv * V;
         if (id < vocab) f(id, logit_at(row, id));
     }
-    // Three vectors of a thread are in flight; the body is one's, since code that is run through once costs its fetch.
+    // f for several logits at once: an id, the step to the next, and the logits.  Four vectors of a thread are in flight.
     template <typename F>
     __device__ __forceinline__ void several(F f) const {
+        constexpr int U = 4;
         const int tid = threadIdx.x;
-        uint4 v0 = load(tid), v1 = load(tid + T), v2 = load(tid + 2 * T);
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = load(tid + u * T);
         few([&](int id, float x) {
             const float v[1] = {x};
             f(id, 1, v);
         });
 #pragma unroll 1
-        for (int j = tid; j < nv; j += T) {
-            const uint4 v = v0;
-            v0 = v1;
-            v1 = v2;
-            v2 = load(j + 3 * T);
-            float x[V];
-            unpack(v, x);
-            f(head + j * V, 1, x);
+        for (int j = tid; j < nv; j += U * T) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (j + u * T >= nv) break;
+                float x[V];
+                unpack(v[u], x);
+                v[u] = load(j + (u + U) * T);
+                f(head + (j + u * T) * V, 1, x);
+            }
         }
     }
     template <typename F>
@@ -301,69 +349,75 @@ struct FarRow {
             for (int e = 0; e < N; ++e) f(id + e * step, x[e]);
         });
     }
-    // The largest logit of this thread's part, and in `where` the first vector that holds its vectors' largest (-1: none).  With
-    // collect, after each batch of loads: the largest so far of all threads goes through least(), and put takes every logit of
-    // the batch from that on.
+    // The largest logit of this thread's part, and in `where` the first vector that holds its vectors' largest (-1: none).
+    __device__ __forceinline__ float first_pass(int &where) const {
+        float top = -__builtin_inff();
+        where = -1;
+        several([&](int id, int, const auto &x) {
+            constexpr int N = sizeof(x) / sizeof(float);
+            float high = larger(x[0], -__builtin_inff());
+#pragma unroll
+            for (int e = 1; e < N; ++e) high = larger(x[e], high);
+            if (N == V) where = high > top ? (id - head) / V : where;
+            if (N == V) top = larger(high, top);
+        });
+        few([&](int, float x) { top = larger(x, top); });
+        return top;
+    }
+    // The same without `where`, and after each batch of loads: the largest so far of all threads goes through least(), and put takes
+    // every logit of the batch from that on.
     template <typename L, typename P>
-    __device__ __forceinline__ float first_pass(MinPShared<T> &s, bool collect, L least, P put, int &where) const {
+    __device__ __forceinline__ float first_pass(MinPShared<T> &s, L least, P put) const {
         constexpr int U = 8;
         const int tid = threadIdx.x;
         float top = -__builtin_inff();
-        where = -1;
         uint4 v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = load(tid + u * T);
 #pragma unroll 1
         for (int b = 0, turn = 0; b < nv; b += U * T, turn ^= 1) {
             float high[U];
-            uint4 next[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int j = b + tid + u * T;
                 float x[V];
                 unpack(v[u], x);
                 high[u] = larger(x[0], -__builtin_inff());
 #pragma unroll
                 for (int e = 1; e < V; ++e) high[u] = larger(x[e], high[u]);
-                high[u] = j < nv ? high[u] : -__builtin_inff();
-                where = high[u] > top ? j : where;
+                high[u] = b + tid + u * T < nv ? high[u] : -__builtin_inff();
                 top = larger(high[u], top);
-                next[u] = load(j + U * T);
             }
-            if (collect) {
-                const float m = group_max<kWave>(top);
-                if (tid % kWave == 0) s.max[turn][tid / kWave] = m;
-                __syncthreads();
-                float all = s.max[turn][0];
+            const float m = group_max<kWave>(top);
+            if (tid % kWave == 0) s.max[turn][tid / kWave] = m;
+            __syncthreads();
+            float all = s.max[turn][0];
 #pragma unroll
-                for (int w = 1; w < T / kWave; ++w) all = fmaxf(all, s.max[turn][w]);
-                const float from = least(all);
+            for (int w = 1; w < T / kWave; ++w) all = fmaxf(all, s.max[turn][w]);
+            const float from = least(all);
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (!(high[u] >= from)) continue;
-                    const int id = head + (b + tid + u * T) * V;
-                    uint4 r = v[u];
+            for (int u = 0; u < U; ++u) {
+                uint4 r = v[u];
+                v[u] = load(b + tid + (u + U) * T);
+                if (!(high[u] >= from)) continue;
+                const int id = head + (b + tid + u * T) * V;
 #pragma unroll 1
-                    for (int e = 0; e < V; ++e) {
-                        const float x = __uint_as_float(V == 8 ? r.x << 16 : r.x);
-                        if (V == 8) {
-                            r.x = __builtin_amdgcn_alignbit(r.y, r.x, 16);
-                            r.y = __builtin_amdgcn_alignbit(r.z, r.y, 16);
-                            r.z = __builtin_amdgcn_alignbit(r.w, r.z, 16);
-                            r.w >>= 16;
-                        } else {
-                            r = make_uint4(r.y, r.z, r.w, 0);
-                        }
-                        put(id + e, x, from);
+                for (int e = 0; e < V; ++e) {
+                    const float x = __uint_as_float(V == 8 ? r.x << 16 : r.x);
+                    if (V == 8) {
+                        r.x = __builtin_amdgcn_alignbit(r.y, r.x, 16);
+                        r.y = __builtin_amdgcn_alignbit(r.z, r.y, 16);
+                        r.z = __builtin_amdgcn_alignbit(r.w, r.z, 16);
+                        r.w >>= 16;
+                    } else {
+                        r = make_uint4(r.y, r.z, r.w, 0);
                     }
+                    put(id + e, x, from);
                 }
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = next[u];
         }
         few([&](int id, float x) {
             top = larger(x, top);
-            if (collect) put(id, x, -3.4028234663852886e38f);
+            put(id, x, -3.4028234663852886e38f);
         });
         return top;
     }
@@ -382,7 +436,7 @@ struct FarRow {
 template <int T>
 __device__ __forceinline__ void sort_list(MinPShared<T> &s, int n) {
     const int tid = threadIdx.x;
-    if (n <= kMinPRanked) {
+    if (n <= kMinPSorted) {
         const int span = n <= 64 ? 64 : n <= 128 ? 128 : 256, parts = T / span;  // span <= T
         const int i = tid & (span - 1), each = (n + parts - 1) / parts;
         const int from = min(n, tid / span * each), to = min(n, from + each);
@@ -398,7 +452,7 @@ __device__ __forceinline__ void sort_list(MinPShared<T> &s, int n) {
         __syncthreads();
         return;
     }
-    int n2 = 2 * kMinPRanked;
+    int n2 = 2 * kMinPSorted;
     while (n2 < n) n2 <<= 1;
     for (int i = n + tid; i < n2; i += T) s.list[i] = 0;
     __syncthreads();
@@ -419,11 +473,11 @@ __device__ __forceinline__ void sort_list(MinPShared<T> &s, int n) {
 // The sums of a sorted list: thread t has the ranks t E .. t E + E - 1, E = ceil(n / T).
 template <int T>
 struct ListSums {
-    static constexpr int kEach = kMinPList / T;
+    static constexpr int kEach = MinPSizes<T>::kList / T;
     uint64_t cum[kEach];
     uint64_t before;
     int first, end;
-    __device__ __forceinline__ ListSums(MinPShared<T> &s, int n, uint64_t above, const RowRule &rule) {
+    __device__ __forceinline__ ListSums(MinPShared<T> &s, int n, uint64_t above, const Rule<T> &rule) {
         const int each = (n + T - 1) / T;
         first = min(n, static_cast<int>(threadIdx.x) * each);
         end = min(n, first + each);
@@ -473,7 +527,7 @@ struct RowCuts {
 // The token of a row whose weights are all among the list's n <= 64 entries, by one wave: lane r has rank r.  Sums of 64
 // weights are exact in double.
 template <int T>
-__device__ __forceinline__ int draw_from_few(const MinPShared<T> &s, int n, const RowRule &rule, const RowCuts &c) {
+__device__ __forceinline__ int draw_from_few(const MinPShared<T> &s, int n, const Rule<T> &rule, const RowCuts &c) {
     const int lane = threadIdx.x & (kWave - 1);
     const uint64_t mine = lane < n ? s.list[lane] : 0;
     int above = lane < n ? 0 : lane;
@@ -496,10 +550,10 @@ __device__ __forceinline__ int draw_from_few(const MinPShared<T> &s, int n, cons
     return __shfl(entry_id(e), reached(ceil(c.u * kept)), kWave);
 }
 
-// The token of a row whose weights are all in the list (of every thread).
+// The token of a row whose weights are all in the list (for thread 0).
 template <int T>
-__device__ __forceinline__ int draw_from_list(MinPShared<T> &s, int n, const RowRule &rule, const RowCuts &c) {
-    if (n <= kWave) return draw_from_few<T>(s, n, rule, c);
+__device__ __forceinline__ int draw_from_list(MinPShared<T> &s, int n, const Rule<T> &rule, const RowCuts &c) {
+    if (n <= kWave) return threadIdx.x < kWave ? draw_from_few<T>(s, n, rule, c) : 0;
     sort_list<T>(s, n);
     const ListSums<T> sums(s, n, 0, rule);
     sums.find_rank(s, min(c.k, n) - 1);
@@ -516,35 +570,84 @@ __device__ __forceinline__ int draw_from_list(MinPShared<T> &s, int n, const Row
 
 // The row's histogram: of counts (kMass false) or of masses.  The list's counter is cleared besides.
 template <bool kMass, int T, typename Row>
-__device__ __forceinline__ void row_histogram(MinPShared<T> &s, const Row &row, const RowRule &rule) {
-    for (int i = threadIdx.x; i < kMinPBins; i += T) s.hist[0][i] = 0;
+__device__ __forceinline__ void row_histogram(MinPShared<T> &s, const Row &row, const Rule<T> &rule) {
+    for (int i = threadIdx.x; i < MinPSizes<T>::kBins; i += T) s.hist[i] = 0;
     if (threadIdx.x == 0) s.n = 0;
-    __syncthreads();
-    row.several([&](int id, int step, const auto &x) {
+    auto weigh = [&](int id, int step, const auto &x) {
         constexpr int N = sizeof(x) / sizeof(float);
         int bin[N];
-        if constexpr (kMass) {
-            uint64_t w[N];  // side by side: one's instructions alone would wait for each other
+        uint64_t w[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) w[e] = rule.weight(x[e], id + e * step, bin[e]);
+        for (int e = 0; e < N; ++e) w[e] = rule.weight(x[e], bin[e]);
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (rule.counts(x[e], id + e * step)) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[bin[e]]), w[e]);
+    };
+    // A pass is bound by its vector instructions: without what a row does not need they are 21 a logit instead of 31.
+    auto weigh_plain = [&](int, int, const auto &x) {
+        constexpr int N = sizeof(x) / sizeof(float);
+        int bin[N];
+        uint64_t w[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = rule.plain_weight(x[e], bin[e]);
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (x[e] >= rule.least) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[bin[e]]), w[e]);
+    };
+    if constexpr (!kMass) {
+        __syncthreads();
+        row.several([&](int id, int step, const auto &x) {
+            constexpr int N = sizeof(x) / sizeof(float);
 #pragma unroll
             for (int e = 0; e < N; ++e)
-                if (w[e]) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[0][bin[e]]), w[e]);
-        } else {
+                if (rule.counts(x[e], id + e * step)) atomicAdd(reinterpret_cast<uint32_t *>(s.hist) + rule.bin(x[e]), 1u);
+        });
+    } else if constexpr (!Row::kShort) {
+        __syncthreads();
+        if (rule.plain) row.several(weigh_plain);
+        else row.several(weigh);
+    } else {
+        // A bf16 row repeats its values: they are counted where the list will be, 32 binades of either sign down from the
+        // largest that counts (and zero), and each is weighed once, 5 instructions a logit instead of 25.  What is smaller yet is
+        // weighed alone.
+        constexpr int kHalf = MinPSizes<T>::kList;  // 32-bit counters of a sign
+        uint32_t *const count = reinterpret_cast<uint32_t *>(s.list);
+        for (int i = threadIdx.x; i < 2 * kHalf; i += T) count[i] = 0;
+        __syncthreads();
+        const float high = fmaxf(fabsf(static_cast<float>(rule.max)), fabsf(rule.least));
+        const int base = max(0, static_cast<int>((__float_as_uint(high) >> 16) & 0x7f80u) + 128 - kHalf);
+        row.several([&](int id, int step, const auto &x) {
+            constexpr int N = sizeof(x) / sizeof(float);
 #pragma unroll
-            for (int e = 0; e < N; ++e) bin[e] = rule.bin(x[e]);
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (rule.counts(x[e], id + e * step)) atomicAdd(reinterpret_cast<uint32_t *>(s.hist[0]) + bin[e], 1u);
+            for (int e = 0; e < N; ++e) {
+                if (!rule.counts(x[e], id + e * step)) continue;
+                const uint32_t bits = __float_as_uint(x[e]);
+                const int key = static_cast<int>((bits >> 16) & 0x7fffu), at = max(0, key - base);
+                if (at > 0 || key == 0) {
+                    atomicAdd(&count[(bits >> 31) * kHalf + at], 1u);
+                } else {
+                    const float one[1] = {x[e]};
+                    weigh(id + e * step, 1, one);
+                }
+            }
+        });
+        __syncthreads();
+#pragma unroll 1
+        for (int i = threadIdx.x; i < 2 * kHalf; i += T) {
+            const uint32_t c = count[i];
+            if (c == 0) continue;
+            const uint32_t key = i % kHalf ? i % kHalf + base : 0;
+            int bin;
+            const uint64_t w = rule.weight(__uint_as_float((key << 16) | (i >= kHalf ? 0x80000000u : 0u)), bin);
+            atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[bin]), c * w);
         }
-    });
+    }
     __syncthreads();
 }
 
 // A histogram's sums: thread t has the bins t E .. t E + E - 1.
-template <bool kMass, int T>
+template <bool kMass, int T, int kEach = MinPSizes<T>::kEach>
 struct BinSums {
-    static constexpr int kEach = kMinPBins / T;
     uint64_t h[kEach], before, total;
     __device__ __forceinline__ BinSums(MinPShared<T> &s, const uint64_t *hist, uint64_t above) {
         uint64_t own = 0;
@@ -576,7 +679,7 @@ struct BinSums {
 // row's histogram of that kind, whose whole sum reaches it.  A bin that overflows the list is cut by the digits of an
 // entry, ten or eleven bits at a time (32 of the logit, 20 of the id), until one does not; the last digits leave one entry.
 template <bool kMass, int T, typename Row>
-__device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const RowRule &rule, const BinSums<kMass, T> &sums,
+__device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const Rule<T> &rule, const BinSums<kMass, T> &sums,
                                        uint64_t target) {
     uint64_t prefix = 0, mask = 0;
     sums.find(s, target);
@@ -589,24 +692,24 @@ __device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const R
         return (e & mask) == prefix;
     };
     constexpr int kBits = 11;
-    static_assert(1 << kBits == kMinPBins, "a digit fills the histogram");
+    static_assert(1 << kBits == kMinPDigits, "a digit fills the histogram");
     for (int top = 64;;) {  // the digits down to bit `top` are known
         row.each([&](int id, float v) {
             uint64_t e;
             if (in_question(id, v, e)) {
                 const uint32_t at = atomicAdd(&s.n, 1u);
-                if (at < kMinPList) s.list[at] = e;
+                if (at < MinPSizes<T>::kList) s.list[at] = e;
             }
         });
         __syncthreads();
-        if (s.n <= kMinPList) break;
+        if (T < 1024 || s.n <= MinPSizes<T>::kList) break;
         if (top == 32) {  // bits 20 .. 31 are ones in every entry
             top = 20;
             mask |= 0xfff00000ull;
             prefix |= 0xfff00000ull;
         }
         const int low = top > 32 ? 32 : 0, bits = min(kBits, top - low), shift = top - bits, bins = 1 << bits;
-        for (int i = threadIdx.x; i < kMinPBins; i += T) s.hist[1][i] = 0;
+        for (int i = threadIdx.x; i < kMinPDigits; i += T) s.digits[i] = 0;
         __syncthreads();
         if (threadIdx.x == 0) s.n = 0;
         row.each([&](int id, float v) {
@@ -615,14 +718,14 @@ __device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const R
                 const int at = bins - 1 - (static_cast<int>(e >> shift) & (bins - 1));
                 if constexpr (kMass) {
                     const uint64_t w = rule.weight(e);
-                    if (w) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[1][at]), w);
+                    if (w) atomicAdd(reinterpret_cast<unsigned long long *>(&s.digits[at]), w);
                 } else {
-                    atomicAdd(reinterpret_cast<uint32_t *>(s.hist[1]) + at, 1u);
+                    atomicAdd(reinterpret_cast<uint32_t *>(s.digits) + at, 1u);
                 }
             }
         });
         __syncthreads();
-        BinSums<kMass, T>(s, s.hist[1], above).find(s, target);
+        BinSums<kMass, T, kMinPDigits / T>(s, s.digits, above).find(s, target);
         above = s.above;
         prefix |= static_cast<uint64_t>(bins - 1 - s.bin) << shift;
         mask |= static_cast<uint64_t>(bins - 1) << shift;
@@ -641,11 +744,11 @@ __device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const R
 
 // The token of a row by its histograms.
 template <int T, typename Row>
-__device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, RowRule &rule, const RowCuts &c, int vocab) {
+__device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, Rule<T> &rule, const RowCuts &c, int vocab) {
     // top-k: its last entry, or, where few are before it, those
     if (c.k < vocab) {
         row_histogram<false, T>(s, row, rule);
-        const BinSums<false, T> sums(s, s.hist[0], 0);
+        const BinSums<false, T> sums(s, s.hist, 0);
         if (sums.total > static_cast<uint64_t>(c.k)) {
             if (c.k <= kMinPSorted) {
                 sums.find(s, c.k);
@@ -662,12 +765,13 @@ __device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, Ro
             locate<false, T>(s, row, rule, sums, c.k);
             rule.least = rule.tie = entry_value(s.found);  // at least what it was
             rule.tie_id = entry_id(s.found);
+            rule.plain = false;
             __syncthreads();
         }
     }
     // top-p's last entry and the drawn one, by their masses
     row_histogram<true, T>(s, row, rule);
-    const BinSums<true, T> sums(s, s.hist[0], 0);
+    const BinSums<true, T> sums(s, s.hist, 0);
     uint64_t kept = sums.total;
     if (c.p < 1.0) {
         locate<true, T>(s, row, rule, sums, share(c.p, kept));
@@ -694,12 +798,12 @@ min_p_kernel(MinPArgs a) {
                           uq > 0.f ? (uq < 1.f ? uq : 1.0) : 0.0};
     const double reach = temperature * log(fmax(min_p, 0x1p-43));
     // The least logit that can have a weight beside a maximum; the margins cover the roundings many times over.
-    constexpr float kLargest = RowRule::kLargest;
+    constexpr float kLargest = Rule<T>::kLargest;
     auto least = [&](float max) {
         return max > kLargest ? max
                               : larger(static_cast<float>(max + reach - 1e-6 * (fabs(static_cast<double>(max)) - reach)), -kLargest);
     };
-    if (tid < 32) s.table[tid] = kExp2Table[tid];
+    if (tid < 128) s.table[tid] = kExp2Table[tid];
     if (tid == 0) {
         s.n = 0;
         s.id = a.vocab;
@@ -712,13 +816,17 @@ min_p_kernel(MinPArgs a) {
     if constexpr (kHeld) {
         row.each([&](int, float v) { top = larger(v, top); });
     } else {
-        top = row.first_pass(s, !greedy && min_p > 0.0, least, [&](int id, float v, float from) {
-            if (v >= from) {
-                const uint32_t at = atomicAdd(&s.n, 1u);
-                if (at < kMinPList) s.list[at] = min_p_entry(v, id);
-            }
-        }, where);
-        __syncthreads();  // the batches' maxima are read
+        if (!greedy && min_p > 0.0) {
+            top = row.first_pass(s, least, [&](int id, float v, float from) {
+                if (v >= from) {
+                    const uint32_t at = atomicAdd(&s.n, 1u);
+                    if (at < MinPSizes<T>::kList) s.list[at] = min_p_entry(v, id);
+                }
+            });
+            __syncthreads();  // the batches' maxima are read
+        } else {
+            top = row.first_pass(where);
+        }
     }
     const float own = top;
     top = group_max<kWave>(top);
@@ -739,12 +847,14 @@ min_p_kernel(MinPArgs a) {
         if (tid == 0) a.tokens[r] = top == -__builtin_inff() ? 0 : s.id;
         return;
     }
-    RowRule rule;
+    Rule<T> rule;
     rule.table = s.table;
-    rule.max = fminf(top, kLargest);
-    rule.turns = top > kLargest ? 0.0 : 32.0 * 1.4426950408889634 / temperature;
-    rule.min_p = min_p * 4398046511104.0;  // in weights
+    rule.max = top > kLargest ? 0.0 : top;
+    rule.turns = top > kLargest ? 0.0 : 128.0 * 1.4426950408889634 / temperature;
+    rule.lowest = top > kLargest ? 0.0 : -45.0 * 128.0;
+    rule.least_weight = static_cast<uint64_t>(ceil(min_p * 4398046511104.0));
     rule.least = least(top);
+    rule.plain = rule.least_weight == 0 && top <= kLargest && (rule.least - rule.max) * rule.turns >= rule.lowest;
     rule.tie = __builtin_nanf("");
     rule.tie_id = 0;
     const int found = static_cast<int>(s.n);
@@ -755,28 +865,28 @@ min_p_kernel(MinPArgs a) {
         row.each([&](int id, float v) {
             if (rule.counts(v, id)) {
                 const uint32_t at = atomicAdd(&s.n, 1u);
-                if (at < kMinPList) s.list[at] = min_p_entry(v, id);
+                if (at < MinPSizes<T>::kList) s.list[at] = min_p_entry(v, id);
             }
         });
-    } else if (found > 0 && found <= kMinPList) {
+    } else if (found > 0 && found <= MinPSizes<T>::kList) {
         const HeldList<T> list(s, found);
         list.each([&](int id, float v) {
             if (rule.counts(v, id)) s.list[atomicAdd(&s.n, 1u)] = min_p_entry(v, id);
         });
     } else if (cuts.k <= T / 2) {
         // the k-th largest of the threads' own maxima, or its bin: as many logits reach it, and few more
-        for (int i = tid; i < kMinPBins; i += T) s.hist[0][i] = 0;
+        for (int i = tid; i < MinPSizes<T>::kBins; i += T) s.hist[i] = 0;
         __syncthreads();
-        if (own >= rule.least) atomicAdd(reinterpret_cast<uint32_t *>(s.hist[0]) + rule.bin(own), 1u);
+        if (own >= rule.least) atomicAdd(reinterpret_cast<uint32_t *>(s.hist) + rule.bin(own), 1u);
         __syncthreads();
-        const BinSums<false, T> sums(s, s.hist[0], 0);
+        const BinSums<false, T> sums(s, s.hist, 0);
         if (sums.total >= static_cast<uint64_t>(cuts.k)) {
             sums.find(s, cuts.k);
             const float from = rule.bin_from(static_cast<int>(s.bin));
             row.each([&](int id, float v) {
                 if (v >= from) {
                     const uint32_t at = atomicAdd(&s.n, 1u);
-                    if (at < kMinPList) s.list[at] = min_p_entry(v, id);
+                    if (at < MinPSizes<T>::kList) s.list[at] = min_p_entry(v, id);
                 }
             });
         }
@@ -790,7 +900,7 @@ min_p_kernel(MinPArgs a) {
         __syncthreads();
         if constexpr (kHeld) {
             token = draw_by_bins<T>(s, row, rule, cuts, a.vocab);
-        } else if (n > 0 && n <= kMinPList) {
+        } else if (n > 0 && n <= MinPSizes<T>::kList) {
             const HeldList<T> list(s, n);
             token = draw_by_bins<T>(s, list, rule, cuts, a.vocab);
         } else {

@@ -202,14 +202,15 @@ def uniform_from_counter(seed: int, offset: int) -> np.float32:
 
 
 def min_p_weights(x: np.ndarray, temperature: float, min_p: float) -> np.ndarray:
-    """Integer weights rint(2^42 exp((x - max) / T)) of one row, 0 where the exponential is below ``min_p``; float64."""
+    """Integer weights rint(2^42 exp((x - max) / T)) of one row, 0 where that is below 2^42 ``min_p``; float64."""
 
     x = np.where(np.isnan(x), -np.inf, np.asarray(x, np.float64))
     top = x.max()
     with np.errstate(invalid="ignore", over="ignore", under="ignore"):
         e = np.exp((x - top) * (1.0 / float(F(temperature))))
     e = np.where(x == top, 1.0, np.where(np.isnan(e), 0.0, e))
-    return np.where(e >= min(max(float(F(min_p)), 0.0), 1.0), np.rint(e * 2.0**42), 0.0).astype(np.int64)
+    w = np.rint(e * 2.0**42)
+    return np.where(w >= min(max(float(F(min_p)), 0.0), 1.0) * 2.0**42, w, 0.0).astype(np.int64)
 
 
 def sample_min_p_row(logits: np.ndarray, temperature: float, top_k: int, top_p: float, min_p: float, u: float) -> int:
