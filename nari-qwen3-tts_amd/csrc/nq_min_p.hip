@@ -52,6 +52,8 @@ __device__ __forceinline__ float entry_value(uint64_t e) {
 __device__ __forceinline__ int entry_id(uint64_t e) {
     return static_cast<int>(0xffffffffu - static_cast<uint32_t>(e));
 }
+constexpr float kLargest = 3.4028234663852886e38f;
+
 // The larger of the two; b where a is NaN (fmaxf answers NaN to a signalling one).
 __device__ __forceinline__ float larger(float a, float b) { return a > b ? a : b; }
 
@@ -86,7 +88,7 @@ template <int T>
 struct MinPShared {
     static constexpr int kWaves = T / kWave;
     uint64_t list[MinPSizes<T>::kList];
-    uint64_t hist[MinPSizes<T>::kBins];  // of the row; counts take 32 bits a bin
+    uint64_t hist[MinPSizes<T>::kBins];  // of the row
     uint64_t digits[T == 1024 ? kMinPDigits : 1];
     double table[128];
     uint64_t part[kWaves];
@@ -158,7 +160,6 @@ __device__ const double kExp2Table[128] = {
 template <int kShift>
 struct RowRule {
     static constexpr int kPer = 128, kLast = 45 * (kPer >> kShift);
-    static constexpr float kLargest = 3.4028234663852886e38f;
     const double *table;  // in LDS
     double max, turns;    // turns: 128 log2(e) / T
     double lowest;        // of t: -45 octaves
@@ -243,6 +244,13 @@ struct HeldRow {
             if (id < vocab) f(id, x[i]);
         }
     }
+    // f for the logits between two bounds
+    template <typename F>
+    __device__ __forceinline__ void each_in(float from, float to, F f) const {
+        each([&](int id, float v) {
+            if (v >= from && v <= to) f(id, v);
+        });
+    }
     // f for several logits at once: an id, the step to the next, and the logits, NaN where there is none
     template <typename F>
     __device__ __forceinline__ void several(F f) const {
@@ -276,6 +284,18 @@ struct HeldList {
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
             if (e[i]) f(entry_id(e[i]), entry_value(e[i]));
+    }
+    template <typename F>
+    __device__ __forceinline__ void entries(F f) const {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (e[i]) f(e[i]);
+    }
+    template <typename F>
+    __device__ __forceinline__ void each_in(float from, float to, F f) const {
+        each([&](int id, float v) {
+            if (v >= from && v <= to) f(id, v);
+        });
     }
     template <typename F>
     __device__ __forceinline__ void several(F f) const {
@@ -342,11 +362,16 @@ struct FarRow {
         }
     }
     template <typename F>
-    __device__ __forceinline__ void each(F f) const {
-        several([&](int id, int step, const auto &x) {
+    __device__ __forceinline__ void each_in(float from, float to, F f) const {
+        several([&](int id, int, const auto &x) {
             constexpr int N = sizeof(x) / sizeof(float);
+            bool any = false;  // one branch a vector: they are few
 #pragma unroll
-            for (int e = 0; e < N; ++e) f(id + e * step, x[e]);
+            for (int e = 0; e < N; ++e) any |= x[e] >= from && x[e] <= to;
+            if (!any) return;
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (x[e] >= from && x[e] <= to) f(id + e, x[e]);
         });
     }
     // The largest logit of this thread's part, and in `where` the first vector that holds its vectors' largest (-1: none).
@@ -530,9 +555,14 @@ template <int T>
 __device__ __forceinline__ int draw_from_few(const MinPShared<T> &s, int n, const Rule<T> &rule, const RowCuts &c) {
     const int lane = threadIdx.x & (kWave - 1);
     const uint64_t mine = lane < n ? s.list[lane] : 0;
-    int above = lane < n ? 0 : lane;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) above += lane < n && s.list[j] > mine ? 1 : 0;
+    int above = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(mine)), j);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(mine >> 32)), j);
+        above += ((static_cast<uint64_t>(hi) << 32) | lo) > mine ? 1 : 0;
+    }
+    if (lane >= n) above = lane;
     const uint32_t lo = __builtin_amdgcn_ds_permute(4 * above, static_cast<int>(static_cast<uint32_t>(mine)));
     const uint32_t hi = __builtin_amdgcn_ds_permute(4 * above, static_cast<int>(static_cast<uint32_t>(mine >> 32)));
     const uint64_t e = (static_cast<uint64_t>(hi) << 32) | lo;
@@ -600,7 +630,7 @@ __device__ __forceinline__ void row_histogram(MinPShared<T> &s, const Row &row, 
             constexpr int N = sizeof(x) / sizeof(float);
 #pragma unroll
             for (int e = 0; e < N; ++e)
-                if (rule.counts(x[e], id + e * step)) atomicAdd(reinterpret_cast<uint32_t *>(s.hist) + rule.bin(x[e]), 1u);
+                if (rule.counts(x[e], id + e * step)) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[rule.bin(x[e])]), 1ull);
         });
     } else if constexpr (!Row::kShort) {
         __syncthreads();
@@ -620,11 +650,11 @@ __device__ __forceinline__ void row_histogram(MinPShared<T> &s, const Row &row, 
             constexpr int N = sizeof(x) / sizeof(float);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                if (!rule.counts(x[e], id + e * step)) continue;
+                if (!(x[e] >= rule.least) || (!rule.plain && !rule.counts(x[e], id + e * step))) continue;
                 const uint32_t bits = __float_as_uint(x[e]);
-                const int key = static_cast<int>((bits >> 16) & 0x7fffu), at = max(0, key - base);
+                const int key = static_cast<int>((bits >> 16) & 0x7fffu), at = key - base;
                 if (at > 0 || key == 0) {
-                    atomicAdd(&count[(bits >> 31) * kHalf + at], 1u);
+                    atomicAdd(&count[static_cast<int>(bits >> 31) * kHalf + max(at, 0)], 1u);
                 } else {
                     const float one[1] = {x[e]};
                     weigh(id + e * step, 1, one);
@@ -646,7 +676,7 @@ __device__ __forceinline__ void row_histogram(MinPShared<T> &s, const Row &row, 
 }
 
 // A histogram's sums: thread t has the bins t E .. t E + E - 1.
-template <bool kMass, int T, int kEach = MinPSizes<T>::kEach>
+template <int T, int kEach = MinPSizes<T>::kEach>
 struct BinSums {
     uint64_t h[kEach], before, total;
     __device__ __forceinline__ BinSums(MinPShared<T> &s, const uint64_t *hist, uint64_t above) {
@@ -654,7 +684,7 @@ struct BinSums {
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             const int bin = kEach * threadIdx.x + i;
-            h[i] = kMass ? hist[bin] : reinterpret_cast<const uint32_t *>(hist)[bin];
+            h[i] = hist[bin];
             own += h[i];
         }
         before = above + block_before<T>(own, s.part, total);
@@ -678,62 +708,70 @@ struct BinSums {
 // The entry at which the sum of counts or masses reaches the target, s.found, and the mass through it, s.found_mass, from the
 // row's histogram of that kind, whose whole sum reaches it.  A bin that overflows the list is cut by the digits of an
 // entry, ten or eleven bits at a time (32 of the logit, 20 of the id), until one does not; the last digits leave one entry.
-template <bool kMass, int T, typename Row>
-__device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const Rule<T> &rule, const BinSums<kMass, T> &sums,
-                                       uint64_t target) {
+template <int T, typename Row>
+__device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const Rule<T> &rule, const BinSums<T> &sums,
+                                       uint64_t target, bool mass) {
     uint64_t prefix = 0, mask = 0;
     sums.find(s, target);
     const int bin = static_cast<int>(s.bin);
     uint64_t above = s.above;
-    const float from = rule.bin_from(bin), to = rule.bin_to(bin);  // a look at the bin itself for few others
-    auto in_question = [&](int id, float v, uint64_t &e) {
-        if (!(v >= from) || v > to || rule.bin(v) != bin || !rule.counts(v, id)) return false;
-        e = min_p_entry(v, id);
-        return (e & mask) == prefix;
+    const float from = rule.bin_from(bin), to = rule.bin_to(bin);
+    auto in_question = [&](uint64_t e) {
+        const float v = entry_value(e);
+        return rule.bin(v) == bin && rule.counts(v, entry_id(e)) && (e & mask) == prefix;
     };
     constexpr int kBits = 11;
     static_assert(1 << kBits == kMinPDigits, "a digit fills the histogram");
-    for (int top = 64;;) {  // the digits down to bit `top` are known
-        row.each([&](int id, float v) {
-            uint64_t e;
-            if (in_question(id, v, e)) {
+    int shift = 64, bins = 0;  // the digits down to bit `shift` are known
+    for (bool list = true;; list = !list) {
+        if (!list) {
+            if (shift == 32) {  // bits 20 .. 31 are ones in every entry
+                shift = 20;
+                mask |= 0xfff00000ull;
+                prefix |= 0xfff00000ull;
+            }
+            const int bits = min(kBits, shift > 32 ? shift - 32 : shift);
+            shift -= bits;
+            bins = 1 << bits;
+            for (int i = threadIdx.x; i < kMinPDigits && T == 1024; i += T) s.digits[i] = 0;
+            if (threadIdx.x == 0) s.n = 0;
+            __syncthreads();
+        }
+        // a few logits beside the bin's own come along at first: the look at them waits until they are listed
+        row.each_in(from, to, [&](int id, float v) {
+            const uint64_t e = min_p_entry(v, id);
+            if (mask != 0 || !list) {
+                if (!in_question(e)) return;
+            }
+            if (list) {
                 const uint32_t at = atomicAdd(&s.n, 1u);
                 if (at < MinPSizes<T>::kList) s.list[at] = e;
-            }
-        });
-        __syncthreads();
-        if (T < 1024 || s.n <= MinPSizes<T>::kList) break;
-        if (top == 32) {  // bits 20 .. 31 are ones in every entry
-            top = 20;
-            mask |= 0xfff00000ull;
-            prefix |= 0xfff00000ull;
-        }
-        const int low = top > 32 ? 32 : 0, bits = min(kBits, top - low), shift = top - bits, bins = 1 << bits;
-        for (int i = threadIdx.x; i < kMinPDigits; i += T) s.digits[i] = 0;
-        __syncthreads();
-        if (threadIdx.x == 0) s.n = 0;
-        row.each([&](int id, float v) {
-            uint64_t e;
-            if (in_question(id, v, e)) {
+            } else {
                 const int at = bins - 1 - (static_cast<int>(e >> shift) & (bins - 1));
-                if constexpr (kMass) {
-                    const uint64_t w = rule.weight(e);
-                    if (w) atomicAdd(reinterpret_cast<unsigned long long *>(&s.digits[at]), w);
-                } else {
-                    atomicAdd(reinterpret_cast<uint32_t *>(s.digits) + at, 1u);
-                }
+                atomicAdd(reinterpret_cast<unsigned long long *>(&s.digits[at]), mass ? rule.weight(e) : 1);
             }
         });
         __syncthreads();
-        BinSums<kMass, T, kMinPDigits / T>(s, s.digits, above).find(s, target);
-        above = s.above;
-        prefix |= static_cast<uint64_t>(bins - 1 - s.bin) << shift;
-        mask |= static_cast<uint64_t>(bins - 1) << shift;
-        top = shift;
+        if (list) {
+            if (T < 1024 || s.n <= MinPSizes<T>::kList) break;
+        } else {
+            BinSums<T, T == 1024 ? kMinPDigits / T : 1>(s, s.digits, above).find(s, target);
+            above = s.above;
+            prefix |= static_cast<uint64_t>(bins - 1 - s.bin) << shift;
+            mask |= static_cast<uint64_t>(bins - 1) << shift;
+        }
     }
-    const int n = static_cast<int>(s.n);
+    int n = static_cast<int>(s.n);
+    const HeldList<T> raw(s, n);
+    if (threadIdx.x == 0) s.n = 0;
+    __syncthreads();
+    raw.entries([&](uint64_t e) {
+        if (in_question(e)) s.list[atomicAdd(&s.n, 1u)] = e;
+    });
+    __syncthreads();
+    n = static_cast<int>(s.n);
     sort_list<T>(s, n);
-    if constexpr (kMass) {
+    if (mass) {
         ListSums<T>(s, n, above, rule).find_mass(s, target);
     } else {
         if (threadIdx.x == 0) s.found = s.list[target - above - 1];
@@ -748,13 +786,13 @@ __device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, Ru
     // top-k: its last entry, or, where few are before it, those
     if (c.k < vocab) {
         row_histogram<false, T>(s, row, rule);
-        const BinSums<false, T> sums(s, s.hist, 0);
+        const BinSums<T> sums(s, s.hist, 0);
         if (sums.total > static_cast<uint64_t>(c.k)) {
             if (c.k <= kMinPSorted) {
                 sums.find(s, c.k);
                 const int bin = static_cast<int>(s.bin);
                 if (s.found_mass <= kMinPSorted) {
-                    row.each([&](int id, float v) {
+                    row.each_in(rule.bin_from(bin), __builtin_inff(), [&](int id, float v) {
                         if (rule.counts(v, id) && rule.bin(v) <= bin) s.list[atomicAdd(&s.n, 1u)] = min_p_entry(v, id);
                     });
                     __syncthreads();
@@ -762,7 +800,7 @@ __device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, Ru
                 }
                 __syncthreads();
             }
-            locate<false, T>(s, row, rule, sums, c.k);
+            locate<T>(s, row, rule, sums, c.k, false);
             rule.least = rule.tie = entry_value(s.found);  // at least what it was
             rule.tie_id = entry_id(s.found);
             rule.plain = false;
@@ -771,14 +809,14 @@ __device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, Ru
     }
     // top-p's last entry and the drawn one, by their masses
     row_histogram<true, T>(s, row, rule);
-    const BinSums<true, T> sums(s, s.hist, 0);
+    const BinSums<T> sums(s, s.hist, 0);
     uint64_t kept = sums.total;
     if (c.p < 1.0) {
-        locate<true, T>(s, row, rule, sums, share(c.p, kept));
+        locate<T>(s, row, rule, sums, share(c.p, kept), true);
         kept = s.found_mass;
         __syncthreads();
     }
-    locate<true, T>(s, row, rule, sums, share(c.u, kept));
+    locate<T>(s, row, rule, sums, share(c.u, kept), true);
     return entry_id(s.found);
 }
 
@@ -798,7 +836,6 @@ min_p_kernel(MinPArgs a) {
                           uq > 0.f ? (uq < 1.f ? uq : 1.0) : 0.0};
     const double reach = temperature * log(fmax(min_p, 0x1p-43));
     // The least logit that can have a weight beside a maximum; the margins cover the roundings many times over.
-    constexpr float kLargest = Rule<T>::kLargest;
     auto least = [&](float max) {
         return max > kLargest ? max
                               : larger(static_cast<float>(max + reach - 1e-6 * (fabs(static_cast<double>(max)) - reach)), -kLargest);
@@ -877,17 +914,15 @@ min_p_kernel(MinPArgs a) {
         // the k-th largest of the threads' own maxima, or its bin: as many logits reach it, and few more
         for (int i = tid; i < MinPSizes<T>::kBins; i += T) s.hist[i] = 0;
         __syncthreads();
-        if (own >= rule.least) atomicAdd(reinterpret_cast<uint32_t *>(s.hist) + rule.bin(own), 1u);
+        if (own >= rule.least) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[rule.bin(own)]), 1ull);
         __syncthreads();
-        const BinSums<false, T> sums(s, s.hist, 0);
+        const BinSums<T> sums(s, s.hist, 0);
         if (sums.total >= static_cast<uint64_t>(cuts.k)) {
             sums.find(s, cuts.k);
             const float from = rule.bin_from(static_cast<int>(s.bin));
-            row.each([&](int id, float v) {
-                if (v >= from) {
-                    const uint32_t at = atomicAdd(&s.n, 1u);
-                    if (at < MinPSizes<T>::kList) s.list[at] = min_p_entry(v, id);
-                }
+            row.each_in(from, __builtin_inff(), [&](int id, float v) {
+                const uint32_t at = atomicAdd(&s.n, 1u);
+                if (at < MinPSizes<T>::kList) s.list[at] = min_p_entry(v, id);
             });
         }
     }
