@@ -22,7 +22,6 @@
 namespace nq {
 namespace {
 
-constexpr int kMinPSorted = 256;  // entries that are rather sorted, by counting those above each, than cut by a histogram
 constexpr int kMinPDigits = 2048; // values of a digit that cuts a bin
 constexpr int kMinPHeld = 8;     // logits a thread keeps in registers where the row fits
 constexpr int kMinPVocab = 1 << 20;
@@ -79,6 +78,7 @@ __device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {
 template <int T>
 struct MinPSizes {
     static constexpr int kList = T == 1024 ? 4096 : T * kMinPHeld;  // entries of the list
+    static constexpr int kSorted = T / 2 < 256 ? 256 : T / 2;        // entries that are rather sorted, by counting those above each, than cut
     static constexpr int kShift = T == 1024 ? 0 : 3;                // the row's histogram has 128 bins an octave, or 16
     static constexpr int kLast = 45 * (128 >> kShift);
     static constexpr int kEach = kLast / T + 1, kBins = kEach * T;  // bins a thread, and of them all
@@ -87,17 +87,28 @@ struct MinPSizes {
 template <int T>
 struct MinPShared {
     static constexpr int kWaves = T / kWave;
-    uint64_t list[MinPSizes<T>::kList];
+    alignas(16) uint64_t list[MinPSizes<T>::kList];
     uint64_t hist[MinPSizes<T>::kBins];  // of the row
     uint64_t digits[T == 1024 ? kMinPDigits : 1];
     double table[128];
     uint64_t part[kWaves];
     float max[2][kWaves];
     uint64_t found_mass, found, above;
-    uint32_t rank[kMinPSorted];
+    uint32_t rank[MinPSizes<T>::kSorted];
     uint32_t bin, n;
     int id;
 };
+
+// Appends a logit to the list (past its end it is counted alone) as it is: the entry is made when it is read.
+template <int T>
+__device__ __forceinline__ void append(MinPShared<T> &s, int id, float x) {
+    const uint32_t at = __hip_atomic_fetch_add(&s.n, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    if (at < MinPSizes<T>::kList) s.list[at] = (static_cast<uint64_t>(__float_as_uint(x)) << 32) | static_cast<uint32_t>(id);
+}
+
+__device__ __forceinline__ uint64_t listed_entry(uint64_t v) {
+    return min_p_entry(__uint_as_float(static_cast<uint32_t>(v >> 32)), static_cast<int>(static_cast<uint32_t>(v)));
+}
 
 // Sums over the workgroup of the threads before this one, and of all; two barriers.
 template <int T>
@@ -265,7 +276,8 @@ struct HeldRow {
 };
 static_assert(kMinPHeld == 8, "two groups of four");
 
-// What is left of a row, the n entries of a list, in registers: the list is free for others behind the constructor.
+// What is left of a row, the n logits of a list as append() left them, in registers: the list is free for others behind the
+// constructor.  No entry is 0.
 template <int T>
 struct HeldList {
     static constexpr bool kShort = false;
@@ -275,7 +287,7 @@ struct HeldList {
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             const int at = static_cast<int>(threadIdx.x) + i * T;
-            e[i] = at < n ? s.list[at] : 0;  // no entry is 0
+            e[i] = at < n ? listed_entry(s.list[at]) : 0;
         }
         __syncthreads();
     }
@@ -361,18 +373,47 @@ struct FarRow {
             }
         }
     }
+    // f for the logits between two bounds, which are few: one branch for four vectors.
     template <typename F>
     __device__ __forceinline__ void each_in(float from, float to, F f) const {
-        several([&](int id, int, const auto &x) {
-            constexpr int N = sizeof(x) / sizeof(float);
-            bool any = false;  // one branch a vector: they are few
+        constexpr int U = 4;
+        const int tid = threadIdx.x;
+        uint4 v[U];
 #pragma unroll
-            for (int e = 0; e < N; ++e) any |= x[e] >= from && x[e] <= to;
-            if (!any) return;
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (x[e] >= from && x[e] <= to) f(id + e, x[e]);
+        for (int u = 0; u < U; ++u) v[u] = load(tid + u * T);
+        few([&](int id, float x) {
+            if (x >= from && x <= to) f(id, x);
         });
+#pragma unroll 1
+        for (int j0 = tid; j0 < nv; j0 += U * T) {
+            bool any = false;
+            uint4 r[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float x[V];
+                unpack(v[u], x);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    // quiet: the comparisons' disjunction becomes one of a maximum, which a signalling NaN would spoil
+                    const float q = __builtin_canonicalizef(x[e]);
+                    any |= (q >= from) & (q <= to);
+                }
+                r[u] = v[u];
+                v[u] = load(j0 + (u + U) * T);
+            }
+            if (!any) continue;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int j = j0 + u * T;
+                float x[V];
+                // compared again: kept, the answers above would spill
+                asm volatile("" : "+v"(r[u].x), "+v"(r[u].y), "+v"(r[u].z), "+v"(r[u].w));
+                unpack(r[u], x);
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if ((x[e] >= from) & (x[e] <= to) & (j < nv)) f(head + j * V + e, x[e]);
+            }
+        }
     }
     // The largest logit of this thread's part, and in `where` the first vector that holds its vectors' largest (-1: none).
     __device__ __forceinline__ float first_pass(int &where) const {
@@ -461,23 +502,28 @@ struct FarRow {
 template <int T>
 __device__ __forceinline__ void sort_list(MinPShared<T> &s, int n) {
     const int tid = threadIdx.x;
-    if (n <= kMinPSorted) {
-        const int span = n <= 64 ? 64 : n <= 128 ? 128 : 256, parts = T / span;  // span <= T
-        const int i = tid & (span - 1), each = (n + parts - 1) / parts;
+    if (n <= MinPSizes<T>::kSorted) {
+        const int span = n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512, parts = T / span;
+        static_assert(MinPSizes<T>::kSorted <= T, "a thread an entry at least");
+        const int i = tid & (span - 1), each = ((n + parts - 1) / parts + 1) & ~1;
         const int from = min(n, tid / span * each), to = min(n, from + each);
         for (int j = tid; j < span; j += T) s.rank[j] = 0;
         const uint64_t mine = i < n ? s.list[i] : 0;
+        if (tid == 0 && n % 2) s.list[n] = 0;  // entries are read in pairs
+        __syncthreads();
         uint32_t above = 0;
 #pragma unroll 4
-        for (int j = from; j < to; ++j) above += s.list[j] > mine ? 1u : 0u;
-        __syncthreads();
+        for (int j = from; j < to; j += 2) {
+            const ulonglong2 e = *reinterpret_cast<const ulonglong2 *>(s.list + j);
+            above += (e.x > mine ? 1u : 0u) + (e.y > mine ? 1u : 0u);
+        }
         if (i < n && above) atomicAdd(&s.rank[i], above);
         __syncthreads();
         if (tid < n) s.list[s.rank[tid]] = mine;  // thread tid < span holds entry tid
         __syncthreads();
         return;
     }
-    int n2 = 2 * kMinPSorted;
+    int n2 = 2;
     while (n2 < n) n2 <<= 1;
     for (int i = n + tid; i < n2; i += T) s.list[i] = 0;
     __syncthreads();
@@ -549,12 +595,12 @@ struct RowCuts {
     double p, u;
 };
 
-// The token of a row whose weights are all among the list's n <= 64 entries, by one wave: lane r has rank r.  Sums of 64
+// The token of a row whose weights are all among the list's n <= 64 logits, by one wave: lane r has rank r.  Sums of 64
 // weights are exact in double.
 template <int T>
 __device__ __forceinline__ int draw_from_few(const MinPShared<T> &s, int n, const Rule<T> &rule, const RowCuts &c) {
     const int lane = threadIdx.x & (kWave - 1);
-    const uint64_t mine = lane < n ? s.list[lane] : 0;
+    const uint64_t mine = lane < n ? listed_entry(s.list[lane]) : 0;
     int above = 0;
 #pragma unroll 4
     for (int j = 0; j < n; ++j) {
@@ -584,6 +630,8 @@ __device__ __forceinline__ int draw_from_few(const MinPShared<T> &s, int n, cons
 template <int T>
 __device__ __forceinline__ int draw_from_list(MinPShared<T> &s, int n, const Rule<T> &rule, const RowCuts &c) {
     if (n <= kWave) return threadIdx.x < kWave ? draw_from_few<T>(s, n, rule, c) : 0;
+    for (int i = threadIdx.x; i < n; i += T) s.list[i] = listed_entry(s.list[i]);
+    __syncthreads();
     sort_list<T>(s, n);
     const ListSums<T> sums(s, n, 0, rule);
     sums.find_rank(s, min(c.k, n) - 1);
@@ -737,20 +785,22 @@ __device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const R
             if (threadIdx.x == 0) s.n = 0;
             __syncthreads();
         }
-        // a few logits beside the bin's own come along at first: the look at them waits until they are listed
-        row.each_in(from, to, [&](int id, float v) {
-            const uint64_t e = min_p_entry(v, id);
-            if (mask != 0 || !list) {
-                if (!in_question(e)) return;
-            }
-            if (list) {
-                const uint32_t at = atomicAdd(&s.n, 1u);
-                if (at < MinPSizes<T>::kList) s.list[at] = e;
+        if (list) {
+            // a few logits beside the bin's own come along at first: the look at them waits until they are listed
+            if (mask == 0) {
+                row.each_in(from, to, [&](int id, float v) { append<T>(s, id, v); });
             } else {
-                const int at = bins - 1 - (static_cast<int>(e >> shift) & (bins - 1));
-                atomicAdd(reinterpret_cast<unsigned long long *>(&s.digits[at]), mass ? rule.weight(e) : 1);
+                row.each_in(from, to, [&](int id, float v) {
+                    if (in_question(min_p_entry(v, id))) append<T>(s, id, v);
+                });
             }
-        });
+        } else {
+            row.each_in(from, to, [&](int id, float v) {
+                const uint64_t e = min_p_entry(v, id);
+                const int at = bins - 1 - (static_cast<int>(e >> shift) & (bins - 1));
+                if (in_question(e)) atomicAdd(reinterpret_cast<unsigned long long *>(&s.digits[at]), mass ? rule.weight(e) : 1);
+            });
+        }
         __syncthreads();
         if (list) {
             if (T < 1024 || s.n <= MinPSizes<T>::kList) break;
@@ -788,13 +838,13 @@ __device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, Ru
         row_histogram<false, T>(s, row, rule);
         const BinSums<T> sums(s, s.hist, 0);
         if (sums.total > static_cast<uint64_t>(c.k)) {
-            if (c.k <= kMinPSorted) {
+            if (c.k <= MinPSizes<T>::kSorted) {
                 sums.find(s, c.k);
                 const int bin = static_cast<int>(s.bin);
-                if (s.found_mass <= kMinPSorted) {
+                if (s.found_mass <= MinPSizes<T>::kSorted) {
                     row.each_in(rule.bin_from(bin), __builtin_inff(), [&](int id, float v) {
-                        if (rule.counts(v, id) && rule.bin(v) <= bin) s.list[atomicAdd(&s.n, 1u)] = min_p_entry(v, id);
-                    });
+                        if (rule.counts(v, id) && rule.bin(v) <= bin) append<T>(s, id, v);
+                    });  // at most MinPSizes<T>::kSorted
                     __syncthreads();
                     return draw_from_list<T>(s, static_cast<int>(s.n), rule, c);
                 }
@@ -855,10 +905,7 @@ min_p_kernel(MinPArgs a) {
     } else {
         if (!greedy && min_p > 0.0) {
             top = row.first_pass(s, least, [&](int id, float v, float from) {
-                if (v >= from) {
-                    const uint32_t at = atomicAdd(&s.n, 1u);
-                    if (at < MinPSizes<T>::kList) s.list[at] = min_p_entry(v, id);
-                }
+                if (v >= from) append<T>(s, id, v);
             });
             __syncthreads();  // the batches' maxima are read
         } else {
@@ -900,15 +947,12 @@ min_p_kernel(MinPArgs a) {
     __syncthreads();
     if constexpr (kHeld) {
         row.each([&](int id, float v) {
-            if (rule.counts(v, id)) {
-                const uint32_t at = atomicAdd(&s.n, 1u);
-                if (at < MinPSizes<T>::kList) s.list[at] = min_p_entry(v, id);
-            }
+            if (rule.counts(v, id)) append<T>(s, id, v);
         });
     } else if (found > 0 && found <= MinPSizes<T>::kList) {
         const HeldList<T> list(s, found);
         list.each([&](int id, float v) {
-            if (rule.counts(v, id)) s.list[atomicAdd(&s.n, 1u)] = min_p_entry(v, id);
+            if (rule.counts(v, id)) append<T>(s, id, v);
         });
     } else if (cuts.k <= T / 2) {
         // the k-th largest of the threads' own maxima, or its bin: as many logits reach it, and few more
@@ -920,16 +964,13 @@ min_p_kernel(MinPArgs a) {
         if (sums.total >= static_cast<uint64_t>(cuts.k)) {
             sums.find(s, cuts.k);
             const float from = rule.bin_from(static_cast<int>(s.bin));
-            row.each_in(from, __builtin_inff(), [&](int id, float v) {
-                const uint32_t at = atomicAdd(&s.n, 1u);
-                if (at < MinPSizes<T>::kList) s.list[at] = min_p_entry(v, id);
-            });
+            row.each_in(from, __builtin_inff(), [&](int id, float v) { append<T>(s, id, v); });
         }
     }
     __syncthreads();
     const int n = static_cast<int>(s.n);
     int token;
-    if (n > 0 && n <= kMinPSorted) {
+    if (n > 0 && n <= MinPSizes<T>::kSorted) {
         token = draw_from_list<T>(s, n, rule, cuts);
     } else {
         __syncthreads();
