@@ -72,18 +72,55 @@ struct Bf16Op {
     static __device__ __forceinline__ float value(float sum, float, float) { return sum; }
 };
 
-// 1 / (1 + exp(-y)) by the hardware's exponential and reciprocal (an ulp each): 1 and 0 at the ends
-__device__ __forceinline__ float sigmoid(float y) {
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * y));
+// The activations in fp32, by the hardware's exponential and reciprocal (an ulp each); the bf16 result's half step is far
+// above their roundings.  y / (1 + exp(-z)) with z = y (silu) or 2 sqrt(2 / pi) (y + 0.044715 y^3) (gelu_tanh, since (1 + tanh(z /
+// 2)) / 2 is that factor); at the ends the exponential is infinite or 0.  gelu is max(y, 0) - |y| erfc(|y| / sqrt 2) / 2, which
+// does not cancel in its tail as 1 + erf would: erfc(a) = k 2^(q(k) - a^2 log2 e) with k = 1 / (1 + 0.3 a), and q a polynomial
+// fitted to log2(erfc(a) exp(a^2) / k) at Chebyshev nodes for a up to 10.5, 8e-7 off there; behind it all is 0.
+template <int kAct>
+__device__ __forceinline__ float activate(float y) {
+    if constexpr (kAct == NQ_ACT_RELU) return y < 0.f ? 0.f : y;
+    if constexpr (kAct == NQ_ACT_SILU) return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * y));
+    if constexpr (kAct == NQ_ACT_GELU_TANH) {
+        const float z = y * fmaf(-0.10294324f, y * y, -2.3022082f);  // -2 sqrt(2 / pi) log2 e (0.044715 y^3 + y)
+        return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z));
+    }
+    if constexpr (kAct == NQ_ACT_GELU) {
+        const float m = fabsf(y), k = __builtin_amdgcn_rcpf(fmaf(0.21213203f, m, 1.0f));
+        float q = fmaf(0.6919735f, k, -2.821275f);
+        q = fmaf(q, k, 4.1087608f);
+        q = fmaf(q, k, -2.9656343f);
+        q = fmaf(q, k, 1.7799832f);
+        q = fmaf(q, k, 0.27396405f);
+        q = fmaf(q, k, 1.4983267f);
+        q = fmaf(q, k, -2.5660994f);
+        const float g = 0.5f * m * k * __builtin_amdgcn_exp2f(fmaf(-0.72134752f * y, y, q));
+        return (y < 0.f ? 0.f : y) - g;  // NaN stays
+    }
+    return y;
 }
-// In fp32; the bf16 result's half step, 2^-9 of it, is far above their roundings.
-__device__ __forceinline__ float activate(float y, int act) {
-    switch (act) {
-        case NQ_ACT_RELU: return y < 0.f ? 0.f : y;
-        case NQ_ACT_GELU: return 0.5f * y * erfcf(-0.70710678f * y);  // accurate where 1 + erf would cancel
-        case NQ_ACT_GELU_TANH: return y * sigmoid(1.59576912f * fmaf(0.044715f * y * y, y, y));  // (1 + tanh z) / 2
-        case NQ_ACT_SILU: return y * sigmoid(y);
-        default: return y;
+
+// N values' activation
+template <int N>
+__device__ __forceinline__ void activate_all(float (&v)[N], int act) {
+    switch (act) {  // once for all of them: straight code for every one costs its fetch
+        case NQ_ACT_RELU:
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = activate<NQ_ACT_RELU>(v[e]);
+            break;
+        case NQ_ACT_GELU:
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = activate<NQ_ACT_GELU>(v[e]);
+            break;
+        case NQ_ACT_GELU_TANH:
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = activate<NQ_ACT_GELU_TANH>(v[e]);
+            break;
+        case NQ_ACT_SILU:
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = activate<NQ_ACT_SILU>(v[e]);
+            break;
+        default: break;
     }
 }
 
@@ -192,7 +229,9 @@ product_rows_kernel(ProductArgs a) {
         float v = Op::kScales ? Op::value(sum, a.sx[r], a.sw[n0 + n]) : Op::value(sum, 0.f, 0.f);
         if constexpr (kEpi) {
             if (a.bias) v += bf16_to_f32(a.bias[n0 + n]);
-            v = activate(v, a.act);
+            float one[1] = {v};
+            activate_all(one, a.act);
+            v = one[0];
             if (a.residual) v += bf16_to_f32(a.residual[r * a.r_s0 + n0 + n]);
         }
         a.out[r * a.o_s0 + n0 + n] = f32_to_bf16(v);
@@ -332,10 +371,7 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles) {
                 float4 v = make_float4(Op::value(acc[m][n][i], sx, sw.x), Op::value(acc[m][n][i + 1], sx, sw.y),
                                        Op::value(acc[m][n][i + 2], sx, sw.z), Op::value(acc[m][n][i + 3], sx, sw.w));
                 if constexpr (kEpi) {
-                    const float4 b = *reinterpret_cast<const float4 *>(s_b + c);
-                    *reinterpret_cast<float4 *>(lds + r * kOutPitch + 4 * c) =
-                        make_float4(activate(v.x + b.x, a.act), activate(v.y + b.y, a.act), activate(v.z + b.z, a.act),
-                                    activate(v.w + b.w, a.act));
+                    *reinterpret_cast<float4 *>(lds + r * kOutPitch + 4 * c) = v;
                 } else {
                     *reinterpret_cast<uint2 *>(lds + r * kOutPitch + 2 * c) =
                         make_uint2(pack2_bf16(v.x, v.y), pack2_bf16(v.z, v.w));
@@ -343,6 +379,7 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles) {
             }
     }
     __syncthreads();
+#pragma unroll 1
     for (int i = threadIdx.x; i < BM * BN / 8; i += T) {
         const int r = i / (BN / 8), c = i % (BN / 8) * 8;
         if (m0 + r >= a.M || n0 + c >= a.N) continue;
@@ -351,7 +388,9 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles) {
         const bool whole = a.wide && n0 + c + 8 <= a.N;
         if constexpr (kEpi) {
             const float4 lo = *reinterpret_cast<const float4 *>(src), hi = *reinterpret_cast<const float4 *>(src + 16);
-            float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            const float4 bl = *reinterpret_cast<const float4 *>(s_b + c), bh = *reinterpret_cast<const float4 *>(s_b + c + 4);
+            float v[8] = {lo.x + bl.x, lo.y + bl.y, lo.z + bl.z, lo.w + bl.w, hi.x + bh.x, hi.y + bh.y, hi.z + bh.z, hi.w + bh.w};
+            activate_all(v, a.act);
             const uint16_t *res = a.residual + (m0 + r) * a.r_s0 + n0 + c;
             if (whole) {
                 if (a.residual) {
