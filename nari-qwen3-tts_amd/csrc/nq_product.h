@@ -124,6 +124,13 @@ __device__ __forceinline__ void activate_all(float (&v)[N], int act) {
     }
 }
 
+#ifndef BAND
+#define BAND 8
+#endif
+#ifndef EARLY
+#define EARLY 1
+#endif
+constexpr int kBand = BAND;
 constexpr int kStage = 128;         // bytes of K a stage
 constexpr int kChunks = kStage / 16;
 
@@ -135,9 +142,11 @@ __device__ const i32x4 kZero16 = {0, 0, 0, 0};  // what a chunk behind K is read
 
 // Waits until at most N of the wave's loads are under way (and all its LDS reads are back), then the barrier: what those
 // loads wrote to LDS is there for every wave, and what they read there may be overwritten.
+constexpr int wait_for(int vm, int lgkm) { return (vm & 15) | (vm >> 4) << 14 | 7 << 4 | lgkm << 8; }  // s_waitcnt's operand
 template <int N>
 __device__ __forceinline__ void arrive() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(wait_for(N, 0));
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
@@ -248,25 +257,30 @@ product_rows_kernel(ProductArgs a) {
 // 9 us.  640 x 12288 (K 2048) 22.5 us = 1430 TOP/s, 4001 x 2048 (K 6144) 56.6 us = 1780 TOP/s (2496 is what a library's
 // 8192^3 reaches).  Other waves for that tile at the same sizes: 2 x 2 of 64 x 128 33 and 69 us, 1 x 4 of 128 x 64 32 and
 // 68, 4 x 2 of 32 x 64 (128 x 128) 30 and 70 (24.4 and 67.9 since).
-template <typename Op, bool kEpi, int WM, int WN, int TM, int TN>
+template <typename Op, bool kEpi, int WM, int WN, int TM, int TN, int NB>
 __global__ void __launch_bounds__(WM * WN * kWave)
-product_tile_kernel(ProductArgs a, int tiles_m, int tiles) {
+product_tile_kernel(ProductArgs a, int tiles_m, int tiles_n) {
     constexpr int NW = WM * WN, T = NW * kWave, BM = 32 * TM * WM, BN = 32 * TN * WN;
     constexpr int V = (BM + BN) / 8 / NW;  // loads of 1 KB (eight rows) a wave and stage
     constexpr int STEPS = kStage / 32;
     static_assert(V * NW * 8 == BM + BN && STEPS == 4, "a stage splits evenly over the waves");
     constexpr int kBuf = (BM + BN) * kStage;     // bytes of a stage: weights, then x
     constexpr int kOutPitch = BN * (kEpi ? 4 : 2) + 16;  // bytes of a result row, fp32 where a residual may follow
-    constexpr int kOut = BM * kOutPitch;
-    constexpr int kScales = 3 * kBuf > kOut ? 3 * kBuf : kOut;  // behind the buffers: the tile's scales, there when the sums are
+    // the results leave in passes of PM of a wave's TM parts, as many as fit
+    constexpr int kMost = 150 * 1024, PM = TM * WM * 32 * kOutPitch <= kMost ? TM : TM / 2;
+    constexpr int kOut = PM * WM * 32 * kOutPitch;
+    static_assert(TM % PM == 0 && kOut <= kMost, "one or two passes");
+    constexpr int kScales = NB * kBuf > kOut ? NB * kBuf : kOut;  // behind the buffers: the tile's scales, there when the sums are
     // one array: with a second one the compiler waits for every load in flight before it reads LDS (57 us become 87)
     __shared__ __attribute__((aligned(16))) char lds[kScales + 4 * (BM + 2 * BN)];
     float *const s_w = reinterpret_cast<float *>(lds + kScales), *const s_x = s_w + BN, *const s_b = s_x + BM;
-    // XCD b % 8 takes tiles (b % 8) per ..: neighbours in m share their weights in one L2
-    const int per = (tiles + 7) / 8;
+    // XCD b % 8 takes tiles (b % 8) per .., in bands of kBand tiles in m: those under way at a time share rows and weights in
+    // one L2
+    const int tiles = tiles_m * tiles_n, per = (tiles + 7) / 8;
     const int t = static_cast<int>(blockIdx.x % 8) * per + static_cast<int>(blockIdx.x / 8);
     if (t >= tiles) return;
-    const int m0 = t % tiles_m * BM, n0 = t / tiles_m * BN;
+    const int band = t / (kBand * tiles_n), high = min(kBand, tiles_m - band * kBand), inside = t - band * kBand * tiles_n;
+    const int m0 = (band * kBand + inside % high) * BM, n0 = inside / high * BN;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int r32 = lane & 31, half = lane >> 5;
     const int wm = wave / WN, wn = wave % WN;
@@ -321,15 +335,16 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles) {
             for (int n = 0; n < TN; ++n)
                 acc[m][n] = Op::mfma(wf[j & 1][n], xf[j & 1][m], acc[m][n]);
     };
-    int b0 = 0, b1 = kBuf, b2 = 2 * kBuf;  // buffers of stages k, k + 1, k + 2
+    // buffers of stages k, k + 1 and, of three, k + 2; loads run NB - 1 stages ahead
+    int b0 = 0, b1 = kBuf, b2 = 2 * kBuf;
     constexpr std::true_type whole{};      // stages inside K: no look at the chunks, 14 vector instructions instead of 40
     constexpr std::false_type part{};
 #pragma unroll
     for (int v = 0; v < V; ++v) load(part, 0, b0, v);
 #pragma unroll
-    for (int v = 0; v < V; ++v) load(part, 1, b1, v);
+    for (int v = 0; v < V && NB == 3; ++v) load(part, 1, b1, v);
     auto step = [&](auto next, int k) __attribute__((always_inline)) {
-        arrive<V>();  // stage k is there; stage k + 1 may be under way
+        arrive<(NB - 2) * V>();  // stage k is there; of three buffers, stage k + 1 may be under way
         read(b0, 0);
         __builtin_amdgcn_sched_barrier(0);
         if (k > 0) multiply(STEPS - 1);  // the last operands of stage k - 1
@@ -337,9 +352,14 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles) {
         for (int j = 0; j < STEPS; ++j) {
             // into the buffer that the barrier freed; stages behind the last read zeros, so that the waits can count
 #pragma unroll
-            for (int v = V * j / STEPS; v < V * (j + 1) / STEPS; ++v) load(next, k + 2, b2, v);
+            for (int v = 0; v < V; ++v)
+                if (v * (NB == 3 ? STEPS : EARLY) / V == j) load(next, k + NB - 1, NB == 3 ? b2 : b1, v);
             __builtin_amdgcn_sched_barrier(0);
             if (j + 1 < STEPS) {
+                // operands j, before the next are asked for: the compiler's own wait, behind that, would be for all, since a load
+                // that writes LDS is under way
+                __builtin_amdgcn_s_waitcnt(wait_for(63, 0));
+                __builtin_amdgcn_sched_barrier(0);
                 read(b0, j + 1);
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(j);
@@ -348,20 +368,23 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles) {
         }
         const int b = b0;
         b0 = b1;
-        b1 = b2;
+        b1 = NB == 3 ? b2 : b;
         b2 = b;
     };
     int k = 0;
-    for (; (k + 3) * kStage <= a.K; ++k) step(whole, k);
+    for (; (k + NB) * kStage <= a.K; ++k) step(whole, k);
     for (; k < stages; ++k) step(part, k);
     multiply(STEPS - 1);
     arrive<0>();  // no load is left that would write over the results
 
     // the lane holds x row r32, weight rows 8 (i / 4) + 4 half + i % 4 of each part
 #pragma unroll
-    for (int m = 0; m < TM; ++m) {
-        const int r = (wm * TM + m) * 32 + r32;
-        const float sx = Op::kScales ? s_x[r] : 0.f;
+  for (int p = 0; p < TM; p += PM) {
+    if (p > 0) __syncthreads();
+#pragma unroll
+    for (int m = p; m < p + PM; ++m) {
+        const int at = (wm * PM + m - p) * 32 + r32;  // the row's place in LDS
+        const float sx = Op::kScales ? s_x[(wm * TM + m) * 32 + r32] : 0.f;
 #pragma unroll
         for (int n = 0; n < TN; ++n)
 #pragma unroll
@@ -371,19 +394,20 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles) {
                 float4 v = make_float4(Op::value(acc[m][n][i], sx, sw.x), Op::value(acc[m][n][i + 1], sx, sw.y),
                                        Op::value(acc[m][n][i + 2], sx, sw.z), Op::value(acc[m][n][i + 3], sx, sw.w));
                 if constexpr (kEpi) {
-                    *reinterpret_cast<float4 *>(lds + r * kOutPitch + 4 * c) = v;
+                    *reinterpret_cast<float4 *>(lds + at * kOutPitch + 4 * c) = v;
                 } else {
-                    *reinterpret_cast<uint2 *>(lds + r * kOutPitch + 2 * c) =
+                    *reinterpret_cast<uint2 *>(lds + at * kOutPitch + 2 * c) =
                         make_uint2(pack2_bf16(v.x, v.y), pack2_bf16(v.z, v.w));
                 }
             }
     }
     __syncthreads();
 #pragma unroll 1
-    for (int i = threadIdx.x; i < BM * BN / 8; i += T) {
-        const int r = i / (BN / 8), c = i % (BN / 8) * 8;
+    for (int i = threadIdx.x; i < PM * WM * 32 * BN / 8; i += T) {
+        const int at = i / (BN / 8), c = i % (BN / 8) * 8;
+        const int r = (at / (32 * PM) * TM + p + at / 32 % PM) * 32 + at % 32;
         if (m0 + r >= a.M || n0 + c >= a.N) continue;
-        const char *src = lds + r * kOutPitch + (kEpi ? 4 : 2) * c;
+        const char *src = lds + at * kOutPitch + (kEpi ? 4 : 2) * c;
         uint16_t *dst = a.out + (m0 + r) * a.o_s0 + n0 + c;
         const bool whole = a.wide && n0 + c + 8 <= a.N;
         if constexpr (kEpi) {
@@ -412,6 +436,7 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles) {
             for (int e = 0; e < 8 && n0 + c + e < a.N; ++e) dst[e] = reinterpret_cast<const uint16_t *>(src)[e];
         }
     }
+  }
 }
 
 bool al(const void *p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -422,12 +447,12 @@ void launch_rows(const ProductArgs &a, hipStream_t st) {
                        dim3(kRowWaves * kWave), 0, st, a);
 }
 
-template <typename Op, bool kEpi, int WM, int WN, int TM, int TN>
+template <typename Op, bool kEpi, int WM, int WN, int TM, int TN, int NB = 3>
 void launch_tiles(const ProductArgs &a, hipStream_t st) {
     constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN;
-    const int tiles_m = (a.M + BM - 1) / BM, tiles = tiles_m * ((a.N + BN - 1) / BN);
-    hipLaunchKernelGGL((product_tile_kernel<Op, kEpi, WM, WN, TM, TN>), dim3((tiles + 7) / 8 * 8),
-                       dim3(WM * WN * kWave), 0, st, a, tiles_m, tiles);
+    const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (a.N + BN - 1) / BN;
+    hipLaunchKernelGGL((product_tile_kernel<Op, kEpi, WM, WN, TM, TN, NB>), dim3((tiles_m * tiles_n + 7) / 8 * 8),
+                       dim3(WM * WN * kWave), 0, st, a, tiles_m, tiles_n);
 }
 
 // Rows and columns of out a workgroup takes.  Few tiles: the waves split K.  Otherwise the largest tile that still gives every
@@ -453,6 +478,19 @@ int tile_for(int M, int N) {
 
 template <typename Op, bool kEpi>
 int launch_product(const ProductArgs &a, hipStream_t st) {
+#ifdef FORCE
+    if (a.M >= 300) {
+        if (FORCE == 1) launch_tiles<Op, kEpi, 4, 2, 2, 4, 2>(a, st);
+        if (FORCE == 2) launch_tiles<Op, kEpi, 4, 2, 2, 3, 2>(a, st);
+        if (FORCE == 3) launch_tiles<Op, kEpi, 2, 4, 4, 2, 2>(a, st);
+        if (FORCE == 4) launch_tiles<Op, kEpi, 2, 4, 2, 2, 3>(a, st);
+        if (FORCE == 5) launch_tiles<Op, kEpi, 2, 4, 2, 2, 2>(a, st);
+        if (FORCE == 6) launch_tiles<Op, kEpi, 2, 4, 2, 1, 3>(a, st);  // 128 x 128
+        if (FORCE == 7) launch_tiles<Op, kEpi, 2, 2, 2, 2, 2>(a, st);  // 128 x 128, 4 waves, two a CU
+        if (FORCE == 8) launch_tiles<Op, kEpi, 4, 2, 1, 3, 3>(a, st);  // 128 x 192
+        return NQ_LAUNCH_STATUS();
+    }
+#endif
     switch (tile_for(a.M, a.N)) {
         case tile_id(16, 16): launch_rows<Op, kEpi, 1>(a, st); break;
         case tile_id(32, 16): launch_rows<Op, kEpi, 2>(a, st); break;
