@@ -124,13 +124,7 @@ __device__ __forceinline__ void activate_all(float (&v)[N], int act) {
     }
 }
 
-#ifndef BAND
-#define BAND 8
-#endif
-#ifndef EARLY
-#define EARLY 1
-#endif
-constexpr int kBand = BAND;
+constexpr int kBand = 8;            // tiles in m of a band
 constexpr int kStage = 128;         // bytes of K a stage
 constexpr int kChunks = kStage / 16;
 
@@ -251,13 +245,14 @@ product_rows_kernel(ProductArgs a) {
 // loads themselves (a register on the way would cost its write to LDS: 0.14 us a stage of 128 x 256).  Step k: stage k
 // has arrived, the loads of stage k + 2 are issued; the operands of each 32 bytes are read while the MFMAs of the 32
 // before run, also across the barrier.  The results cross LDS once more, so that they leave in whole lines.
-// No unit is full: at 4001 x 2048 (K 6144) the MFMAs run in 38 % of the clocks and LDS in 21 % (128 KB read a stage, at 256
-// bytes a clock), while the waves wait to issue in 54 % of theirs: the eight waves of a CU's one workgroup (its buffers
-// take the LDS) meet at every stage's barrier.  A stage takes 1.0 us with every CU busy, launch, first loads and results
-// 9 us.  640 x 12288 (K 2048) 22.5 us = 1430 TOP/s, 4001 x 2048 (K 6144) 56.6 us = 1780 TOP/s (2496 is what a library's
-// 8192^3 reaches).  Other waves for that tile at the same sizes: 2 x 2 of 64 x 128 33 and 69 us, 1 x 4 of 128 x 64 32 and
-// 68, 4 x 2 of 32 x 64 (128 x 128) 30 and 70 (24.4 and 67.9 since).
-template <typename Op, bool kEpi, int WM, int WN, int TM, int TN, int NB>
+// 4001 x 2048 (K 6144) bf16 94 us = 1070 TFLOP/s, int8 55.5 us = 1810 TOP/s; 4096^3 124 us = 1105 TFLOP/s and 73 us = 1880
+// TOP/s (a library's bf16: 86 and 92 us).  No unit is full: the MFMAs run in half of the clocks, of the eight waves of a
+// CU's one workgroup (its buffers take the LDS) two share a matrix unit and all meet at every stage's barrier.  Without the
+// stages' loads it would be 84 us at 4096^3, with loads of one and the same cached tile 119: their way into LDS beside the
+// operand reads costs, not the memory behind them.  Waiting for operands before the next are asked for gave 7 %, bands of
+// tiles 3 %, an MFMA ahead of the reads and the loads between MFMAs 6 %.  Other tiles and depths at 4096^3, us: 256 x 256 in
+// two buffers 118, but 137 where that leaves CUs idle (4001 x 2048); in four buffers of 64 bytes 124; four waves 129 to 150.
+template <typename Op, bool kEpi, int WM, int WN, int TM, int TN>
 __global__ void __launch_bounds__(WM * WN * kWave)
 product_tile_kernel(ProductArgs a, int tiles_m, int tiles_n) {
     constexpr int NW = WM * WN, T = NW * kWave, BM = 32 * TM * WM, BN = 32 * TN * WN;
@@ -266,11 +261,8 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles_n) {
     static_assert(V * NW * 8 == BM + BN && STEPS == 4, "a stage splits evenly over the waves");
     constexpr int kBuf = (BM + BN) * kStage;     // bytes of a stage: weights, then x
     constexpr int kOutPitch = BN * (kEpi ? 4 : 2) + 16;  // bytes of a result row, fp32 where a residual may follow
-    // the results leave in passes of PM of a wave's TM parts, as many as fit
-    constexpr int kMost = 150 * 1024, PM = TM * WM * 32 * kOutPitch <= kMost ? TM : TM / 2;
-    constexpr int kOut = PM * WM * 32 * kOutPitch;
-    static_assert(TM % PM == 0 && kOut <= kMost, "one or two passes");
-    constexpr int kScales = NB * kBuf > kOut ? NB * kBuf : kOut;  // behind the buffers: the tile's scales, there when the sums are
+    constexpr int kOut = BM * kOutPitch;
+    constexpr int kScales = 3 * kBuf > kOut ? 3 * kBuf : kOut;  // behind the buffers: the tile's scales, there when the sums are
     // one array: with a second one the compiler waits for every load in flight before it reads LDS (57 us become 87)
     __shared__ __attribute__((aligned(16))) char lds[kScales + 4 * (BM + 2 * BN)];
     float *const s_w = reinterpret_cast<float *>(lds + kScales), *const s_x = s_w + BN, *const s_b = s_x + BM;
@@ -335,56 +327,54 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles_n) {
             for (int n = 0; n < TN; ++n)
                 acc[m][n] = Op::mfma(wf[j & 1][n], xf[j & 1][m], acc[m][n]);
     };
-    // buffers of stages k, k + 1 and, of three, k + 2; loads run NB - 1 stages ahead
-    int b0 = 0, b1 = kBuf, b2 = 2 * kBuf;
+    int b0 = 0, b2 = 2 * kBuf;  // the buffers of stage k and of stage k + 2, whose loads step k issues
     constexpr std::true_type whole{};      // stages inside K: no look at the chunks, 14 vector instructions instead of 40
     constexpr std::false_type part{};
 #pragma unroll
-    for (int v = 0; v < V; ++v) load(part, 0, b0, v);
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int v = 0; v < V && NB == 3; ++v) load(part, 1, b1, v);
+        for (int v = 0; v < V; ++v) load(part, i, i * kBuf, v);
     auto step = [&](auto next, int k) __attribute__((always_inline)) {
-        arrive<(NB - 2) * V>();  // stage k is there; of three buffers, stage k + 1 may be under way
+        arrive<V>();  // stage k is there; stage k + 1 may be under way
         read(b0, 0);
         __builtin_amdgcn_sched_barrier(0);
         if (k > 0) multiply(STEPS - 1);  // the last operands of stage k - 1
 #pragma unroll
-        for (int j = 0; j < STEPS; ++j) {
+        for (int j = 0; j + 1 < STEPS; ++j) {
+            // operands j, before the next are asked for: the compiler's own wait, behind that, would be for all, since a load
+            // that writes LDS is under way
+            __builtin_amdgcn_s_waitcnt(wait_for(63, 0));
+            __builtin_amdgcn_sched_barrier(0);
+            read(b0, j + 1);
             // into the buffer that the barrier freed; stages behind the last read zeros, so that the waits can count
 #pragma unroll
             for (int v = 0; v < V; ++v)
-                if (v * (NB == 3 ? STEPS : EARLY) / V == j) load(next, k + NB - 1, NB == 3 ? b2 : b1, v);
-            __builtin_amdgcn_sched_barrier(0);
-            if (j + 1 < STEPS) {
-                // operands j, before the next are asked for: the compiler's own wait, behind that, would be for all, since a load
-                // that writes LDS is under way
-                __builtin_amdgcn_s_waitcnt(wait_for(63, 0));
-                __builtin_amdgcn_sched_barrier(0);
-                read(b0, j + 1);
-                __builtin_amdgcn_sched_barrier(0);
-                multiply(j);
-                __builtin_amdgcn_sched_barrier(0);
+                if (v * (STEPS - 1) / V == j) load(next, k + 2, b2, v);
+            multiply(j);
+            // an MFMA, the reads, then a load behind each of the other MFMAs: the matrix unit has work at once
+            __builtin_amdgcn_sched_group_barrier(8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, TM + TN, 0);
+#pragma unroll
+            for (int i = 1; i < TM * TN; ++i) {
+                __builtin_amdgcn_sched_group_barrier(8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        const int b = b0;
-        b0 = b1;
-        b1 = NB == 3 ? b2 : b;
-        b2 = b;
+        b2 = b0;
+        b0 = b0 == 2 * kBuf ? 0 : b0 + kBuf;
     };
     int k = 0;
-    for (; (k + NB) * kStage <= a.K; ++k) step(whole, k);
+    for (; (k + 3) * kStage <= a.K; ++k) step(whole, k);
     for (; k < stages; ++k) step(part, k);
     multiply(STEPS - 1);
     arrive<0>();  // no load is left that would write over the results
 
     // the lane holds x row r32, weight rows 8 (i / 4) + 4 half + i % 4 of each part
 #pragma unroll
-  for (int p = 0; p < TM; p += PM) {
-    if (p > 0) __syncthreads();
-#pragma unroll
-    for (int m = p; m < p + PM; ++m) {
-        const int at = (wm * PM + m - p) * 32 + r32;  // the row's place in LDS
-        const float sx = Op::kScales ? s_x[(wm * TM + m) * 32 + r32] : 0.f;
+    for (int m = 0; m < TM; ++m) {
+        const int r = (wm * TM + m) * 32 + r32;
+        const float sx = Op::kScales ? s_x[r] : 0.f;
 #pragma unroll
         for (int n = 0; n < TN; ++n)
 #pragma unroll
@@ -394,20 +384,19 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles_n) {
                 float4 v = make_float4(Op::value(acc[m][n][i], sx, sw.x), Op::value(acc[m][n][i + 1], sx, sw.y),
                                        Op::value(acc[m][n][i + 2], sx, sw.z), Op::value(acc[m][n][i + 3], sx, sw.w));
                 if constexpr (kEpi) {
-                    *reinterpret_cast<float4 *>(lds + at * kOutPitch + 4 * c) = v;
+                    *reinterpret_cast<float4 *>(lds + r * kOutPitch + 4 * c) = v;
                 } else {
-                    *reinterpret_cast<uint2 *>(lds + at * kOutPitch + 2 * c) =
+                    *reinterpret_cast<uint2 *>(lds + r * kOutPitch + 2 * c) =
                         make_uint2(pack2_bf16(v.x, v.y), pack2_bf16(v.z, v.w));
                 }
             }
     }
     __syncthreads();
 #pragma unroll 1
-    for (int i = threadIdx.x; i < PM * WM * 32 * BN / 8; i += T) {
-        const int at = i / (BN / 8), c = i % (BN / 8) * 8;
-        const int r = (at / (32 * PM) * TM + p + at / 32 % PM) * 32 + at % 32;
+    for (int i = threadIdx.x; i < BM * BN / 8; i += T) {
+        const int r = i / (BN / 8), c = i % (BN / 8) * 8;
         if (m0 + r >= a.M || n0 + c >= a.N) continue;
-        const char *src = lds + at * kOutPitch + (kEpi ? 4 : 2) * c;
+        const char *src = lds + r * kOutPitch + (kEpi ? 4 : 2) * c;
         uint16_t *dst = a.out + (m0 + r) * a.o_s0 + n0 + c;
         const bool whole = a.wide && n0 + c + 8 <= a.N;
         if constexpr (kEpi) {
@@ -436,7 +425,6 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles_n) {
             for (int e = 0; e < 8 && n0 + c + e < a.N; ++e) dst[e] = reinterpret_cast<const uint16_t *>(src)[e];
         }
     }
-  }
 }
 
 bool al(const void *p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -447,51 +435,51 @@ void launch_rows(const ProductArgs &a, hipStream_t st) {
                        dim3(kRowWaves * kWave), 0, st, a);
 }
 
-template <typename Op, bool kEpi, int WM, int WN, int TM, int TN, int NB = 3>
+template <typename Op, bool kEpi, int WM, int WN, int TM, int TN>
 void launch_tiles(const ProductArgs &a, hipStream_t st) {
     constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN;
     const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (a.N + BN - 1) / BN;
-    hipLaunchKernelGGL((product_tile_kernel<Op, kEpi, WM, WN, TM, TN, NB>), dim3((tiles_m * tiles_n + 7) / 8 * 8),
+    hipLaunchKernelGGL((product_tile_kernel<Op, kEpi, WM, WN, TM, TN>), dim3((tiles_m * tiles_n + 7) / 8 * 8),
                        dim3(WM * WN * kWave), 0, st, a, tiles_m, tiles_n);
 }
 
 // Rows and columns of out a workgroup takes.  Few tiles: the waves split K.  Otherwise the largest tile that still gives every
-// CU one: a stage of 128 bytes takes 0.28, 0.34 and 0.72 us at 64 x 64, 64 x 128 and 128 x 256 (1.0 with every CU busy).
+// CU one.
 // Measured, K 2048, us (the rule's own first):
 //   M 16  N 4096:  16-row pieces 3.1, 32-row 3.6;                 N 12288: 7.3, 64 x 64 tiles 7.4
 //   M 32  N 6144:  32-row pieces 7.1, 64 x 64 tiles 7.2;          N 12288: 64 x 64 tiles 7.5, 32-row pieces 10.2
 //   M 64  N 4096:  64-row pieces 5.2, 32-row 6.2, 64 x 64 6.4;    N 6144: 64 x 64 tiles 7.4, 64-row pieces 9.9
 //   M 256 N 4096:  64 x 64 tiles 7.6, 64 x 128 8.7;               N 6144: 64 x 128 tiles 8.9, 64 x 64 9.6, 128 x 256 17.5
 //   M 640 N 6144:  64 x 128 tiles 15.0, 128 x 256 18.5;           N 12288: 128 x 256 tiles 21.9, 64 x 128 26.8
-//   M 1000 N 12288: 128 x 256 tiles 37.4, 64 x 128 39.0 (128 x 128, which is not kept, 35.6; at 640 x 6144 13.6)
+//   M 1000 N 12288: 128 x 256 tiles 37.4, 64 x 128 39.0
+// With an epilogue also 128 x 128, where those are one round of the CUs and 64 x 128 are two (the plain product's tiles, which
+// nq_linear_int8_tile tells, stay as they were), 128 x 128 before what the rule would take:
+//   M 500 N 6144:  bf16 19.1 and 23.3, int8 13.6 and 15.2;        M 640 N 6144: 24.3 and 29.3, 16.8 and 17.8
+//   M 1500 N 2048: 21.1 and 23.1, 14.5 and 15.5;                  M 2000 N 2048, K 6144: 57.7 and 66.6, 33.1 and 36.9
+//   one round of 64 x 128 (M 500 N 4096): 18.1 and 15.5, 12.5 and 10.8; two of 128 x 128 (M 800 N 6144): 37.6 and 30.0
 constexpr int tile_id(int rows, int columns) { return rows << 16 | columns; }
-int tile_for(int M, int N) {
+int tile_for(int M, int N, bool epilogue = false) {
     auto count = [&](int bm, int bn) { return static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
     auto rounds = [](int64_t tiles) { return (tiles + 255) / 256; };
     if (M <= 16) return tile_id(16, 16);
     if (count(32, 16) <= (M <= 32 ? 512 : 256)) return tile_id(32, 16);
     if (count(64, 16) <= 256) return tile_id(64, 16);
     if (count(64, 64) <= 256) return tile_id(64, 64);
+    if (epilogue && count(64, 128) > 256 && count(128, 128) <= 256) return tile_id(128, 128);
     if (3 * rounds(count(128, 256)) > rounds(count(64, 128))) return tile_id(64, 128);
     return tile_id(128, 256);
 }
 
 template <typename Op, bool kEpi>
 int launch_product(const ProductArgs &a, hipStream_t st) {
-#ifdef FORCE
-    if (a.M >= 300) {
-        if (FORCE == 1) launch_tiles<Op, kEpi, 4, 2, 2, 4, 2>(a, st);
-        if (FORCE == 2) launch_tiles<Op, kEpi, 4, 2, 2, 3, 2>(a, st);
-        if (FORCE == 3) launch_tiles<Op, kEpi, 2, 4, 4, 2, 2>(a, st);
-        if (FORCE == 4) launch_tiles<Op, kEpi, 2, 4, 2, 2, 3>(a, st);
-        if (FORCE == 5) launch_tiles<Op, kEpi, 2, 4, 2, 2, 2>(a, st);
-        if (FORCE == 6) launch_tiles<Op, kEpi, 2, 4, 2, 1, 3>(a, st);  // 128 x 128
-        if (FORCE == 7) launch_tiles<Op, kEpi, 2, 2, 2, 2, 2>(a, st);  // 128 x 128, 4 waves, two a CU
-        if (FORCE == 8) launch_tiles<Op, kEpi, 4, 2, 1, 3, 3>(a, st);  // 128 x 192
-        return NQ_LAUNCH_STATUS();
+    const int tile = tile_for(a.M, a.N, kEpi);
+    if constexpr (kEpi) {
+        if (tile == tile_id(128, 128)) {
+            launch_tiles<Op, kEpi, 2, 4, 2, 1>(a, st);
+            return NQ_LAUNCH_STATUS();
+        }
     }
-#endif
-    switch (tile_for(a.M, a.N)) {
+    switch (tile) {
         case tile_id(16, 16): launch_rows<Op, kEpi, 1>(a, st); break;
         case tile_id(32, 16): launch_rows<Op, kEpi, 2>(a, st); break;
         case tile_id(64, 16): launch_rows<Op, kEpi, 4>(a, st); break;
