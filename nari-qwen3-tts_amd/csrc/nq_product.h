@@ -449,6 +449,8 @@ void launch_tiles(const ProductArgs &a, hipStream_t st) {
 //   M 16  N 4096:  16-row pieces 3.1, 32-row 3.6;                 N 12288: 7.3, 64 x 64 tiles 7.4
 //   M 32  N 6144:  32-row pieces 7.1, 64 x 64 tiles 7.2;          N 12288: 64 x 64 tiles 7.5, 32-row pieces 10.2
 //   M 64  N 4096:  64-row pieces 5.2, 32-row 6.2, 64 x 64 6.4;    N 6144: 64 x 64 tiles 7.4, 64-row pieces 9.9
+//   M 77  N 2048 (K 6144): 48-row pieces int8 8.2, bf16 12.5, 64-row 9.5, 14.3; M 48 N 4096: 5.2, 8.7 and 5.9, 9.1: pieces of 48
+//   rows where they are no more than pieces of 64, since each reads its rows of x again
 //   M 256 N 4096:  64 x 64 tiles 7.6, 64 x 128 8.7;               N 6144: 64 x 128 tiles 8.9, 64 x 64 9.6, 128 x 256 17.5
 //   M 640 N 6144:  64 x 128 tiles 15.0, 128 x 256 18.5;           N 12288: 128 x 256 tiles 21.9, 64 x 128 26.8
 //   M 1000 N 12288: 128 x 256 tiles 37.4, 64 x 128 39.0
@@ -463,7 +465,7 @@ int tile_for(int M, int N, bool epilogue = false) {
     auto rounds = [](int64_t tiles) { return (tiles + 255) / 256; };
     if (M <= 16) return tile_id(16, 16);
     if (count(32, 16) <= (M <= 32 ? 512 : 256)) return tile_id(32, 16);
-    if (count(64, 16) <= 256) return tile_id(64, 16);
+    if (count(64, 16) <= 256) return (M + 47) / 48 == (M + 63) / 64 ? tile_id(48, 16) : tile_id(64, 16);
     if (count(64, 64) <= 256) return tile_id(64, 64);
     if (epilogue && count(64, 128) > 256 && count(128, 128) <= 256) return tile_id(128, 128);
     if (3 * rounds(count(128, 256)) > rounds(count(64, 128))) return tile_id(64, 128);
@@ -482,6 +484,7 @@ int launch_product(const ProductArgs &a, hipStream_t st) {
     switch (tile) {
         case tile_id(16, 16): launch_rows<Op, kEpi, 1>(a, st); break;
         case tile_id(32, 16): launch_rows<Op, kEpi, 2>(a, st); break;
+        case tile_id(48, 16): launch_rows<Op, kEpi, 3>(a, st); break;
         case tile_id(64, 16): launch_rows<Op, kEpi, 4>(a, st); break;
         case tile_id(64, 64): launch_tiles<Op, kEpi, 2, 2, 1, 1>(a, st); break;
         case tile_id(64, 128): launch_tiles<Op, kEpi, 2, 4, 1, 1>(a, st); break;

@@ -92,7 +92,7 @@ def test_int8(nq, device, m, n, k):
     (640, 12288, 2048), (4001, 2040, 520), (2050, 2100, 192), (2050, 2100, 200), (2050, 2100, 256), (2050, 2100, 264),
     (2050, 2100, 8), (1900, 2305, 3080), (300, 5001, 1032), (640, 6144, 520), (250, 4090, 776), (129, 700, 3088),
     (64, 4096, 1032), (50, 2040, 520), (16, 5000, 1544), (4001, 6144, 2048), (1430, 2001, 8), (1430, 2001, 200),
-    (1430, 2001, 264), (500, 6100, 1544),
+    (1430, 2001, 264), (500, 6100, 1544), (48, 4090, 1032), (77, 2041, 1544),
 ])
 def test_large(nq, device, m, n, k):
     """Each kernel through its loop over whole stages, around the loop's bounds and with a part of a stage behind it."""
