@@ -74,6 +74,81 @@ __device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {
     return v;
 }
 
+// Two bounds of a logit, itself within them.  NaN is in none.
+struct Span {
+    float from, to;
+    __device__ __forceinline__ bool has(float x) const { return x >= from && x <= to; }
+};
+template <int N>
+__device__ __forceinline__ bool in_any(const Span (&in)[N], float x) {
+    bool any = in[0].has(x);
+#pragma unroll
+    for (int i = 1; i < N; ++i) any |= in[i].has(x);
+    return any;
+}
+
+// The same for two bf16 values in a word: with their bits made unsigned integers in the values' order (negative ones
+// inverted, the others' first bit set; -0 before 0), a span is [low, low + size).
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+struct ShortSpan {
+    u16x2 low, size;
+    __device__ __forceinline__ ShortSpan(const Span &s) {
+        auto key = [](float x) {
+            const uint32_t u = __float_as_uint(x);
+            return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+        };
+        // a bf16 value's own 32-bit key ends in zeros, a negative one's in ones: the bounds are rounded inwards
+        const uint32_t f = s.from == 0.f ? key(-0.f) : key(s.from), t = s.to == 0.f ? key(0.f) : key(s.to);
+        const int lo = static_cast<int>(f >= 0x80000000u ? (f - 1 >> 16) + 1 : f >> 16);
+        const int hi = static_cast<int>(t >= 0x80000000u ? t >> 16 : t + 1 >> 16) - (t >= 0x80000000u ? 0 : 1);
+        low = static_cast<uint16_t>(lo);
+        size = static_cast<uint16_t>(s.from <= s.to && hi >= lo ? hi - lo + 1 : 0);
+    }
+    static __device__ __forceinline__ u16x2 keys(uint32_t w) {
+        typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(u16x2, w ^ (__builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, w) >> 15) | 0x80008000u));
+    }
+    // 1 or more where a key is inside
+    __device__ __forceinline__ u16x2 inside(u16x2 key) const { return __builtin_elementwise_sub_sat(size, static_cast<u16x2>(key - low)); }
+};
+
+// Which logits of four vectors some spans hold, a bit a logit, added to a mask a vector at a time: fp32 word w in bit w, bf16's
+// halves of word w in bits 15 - w and 31 - w.
+template <int N>
+struct WordMarks {
+    Span in[N];
+    __device__ __forceinline__ WordMarks(const Span (&of)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) in[i] = of[i];
+    }
+    __device__ __forceinline__ uint32_t add(uint32_t mask, const uint4 &v, int u) const {
+        const float x[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mask |= in_any(in, x[e]) ? 1u << (4 * u + e) : 0u;
+        return mask;
+    }
+    static __device__ __forceinline__ uint32_t first(int vectors) { return (1u << (4 * vectors)) - 1; }
+};
+template <int N>
+struct HalfMarks {
+    ShortSpan in[N];
+    __device__ __forceinline__ HalfMarks(const Span (&of)[1]) : in{of[0]} { static_assert(N == 1); }
+    __device__ __forceinline__ HalfMarks(const Span (&of)[2]) : in{of[0], of[1]} { static_assert(N == 2); }
+    __device__ __forceinline__ uint32_t add(uint32_t mask, const uint4 &v, int) const {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const u16x2 key = ShortSpan::keys(w[e]);
+            u16x2 is = in[0].inside(key);
+#pragma unroll
+            for (int i = 1; i < N; ++i) is = __builtin_elementwise_max(is, in[i].inside(key));
+            mask = mask << 1 | __builtin_bit_cast(uint32_t, __builtin_elementwise_min(is, static_cast<u16x2>(1)));
+        }
+        return mask;
+    }
+    static __device__ __forceinline__ uint32_t first(int vectors) { return (0xffffu << (16 - 4 * vectors) & 0xffffu) * 0x10001u; }
+};
+
 // Sizes by the threads of a row: 1024, or 256 for what they hold in registers.
 template <int T>
 struct MinPSizes {
@@ -255,11 +330,11 @@ struct HeldRow {
             if (id < vocab) f(id, x[i]);
         }
     }
-    // f for the logits between two bounds
-    template <typename F>
-    __device__ __forceinline__ void each_in(float from, float to, F f) const {
+    // f for the logits of some spans
+    template <int N, typename F>
+    __device__ __forceinline__ void each_in(const Span (&in)[N], F f) const {
         each([&](int id, float v) {
-            if (v >= from && v <= to) f(id, v);
+            if (in_any(in, v)) f(id, v);
         });
     }
     // f for several logits at once: an id, the step to the next, and the logits, NaN where there is none
@@ -303,10 +378,10 @@ struct HeldList {
         for (int i = 0; i < kEach; ++i)
             if (e[i]) f(e[i]);
     }
-    template <typename F>
-    __device__ __forceinline__ void each_in(float from, float to, F f) const {
+    template <int N, typename F>
+    __device__ __forceinline__ void each_in(const Span (&in)[N], F f) const {
         each([&](int id, float v) {
-            if (v >= from && v <= to) f(id, v);
+            if (in_any(in, v)) f(id, v);
         });
     }
     template <typename F>
@@ -373,46 +448,53 @@ struct FarRow {
             }
         }
     }
-    // f for the logits between two bounds, which are few: one branch for four vectors.
+    // f for the logits of four vectors, the thread's j, j + T, .., whose bits are set.  A lane's logits come one after the
+    // other, picked out of its registers: f is there once, where a copy behind a test of each logit costs the tests of all and the
+    // fetch of 32 copies.
     template <typename F>
-    __device__ __forceinline__ void each_in(float from, float to, F f) const {
+    __device__ __forceinline__ void marked(const uint4 (&r)[4], uint32_t mask, int j, F f) const {
+        while (mask) {
+            const int at = __builtin_ctz(mask), w = V == 8 ? 15 - (at & 15) : at;
+            mask &= mask - 1;
+            uint32_t q[8];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                q[2 * u] = w & 1 ? r[u].y : r[u].x;
+                q[2 * u + 1] = w & 1 ? r[u].w : r[u].z;
+            }
+#pragma unroll
+            for (int n = 4, bit = 2; n > 0; n >>= 1, bit <<= 1)
+#pragma unroll
+                for (int i = 0; i < n; ++i) q[i] = w & bit ? q[2 * i + 1] : q[2 * i];
+            const int id = head + (j + (w >> 2) * T) * V + (w & 3) * (V / 4);
+            if constexpr (V == 4) f(id, __uint_as_float(q[0]));
+            else f(id + (at >> 4), __uint_as_float(at >= 16 ? q[0] & 0xffff0000u : q[0] << 16));
+        }
+    }
+    // f for the logits of some spans, which are few
+    template <int N, typename F>
+    __device__ __forceinline__ void each_in(const Span (&in)[N], F f) const {
         constexpr int U = 4;
         const int tid = threadIdx.x;
         uint4 v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = load(tid + u * T);
         few([&](int id, float x) {
-            if (x >= from && x <= to) f(id, x);
+            if (in_any(in, x)) f(id, x);
         });
+        const typename std::conditional<V == 8, HalfMarks<N>, WordMarks<N>>::type marks(in);
 #pragma unroll 1
-        for (int j0 = tid; j0 < nv; j0 += U * T) {
-            bool any = false;
+        for (int j = tid; j < nv; j += U * T) {
+            uint32_t mask = 0;
             uint4 r[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                float x[V];
-                unpack(v[u], x);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    // quiet: the comparisons' disjunction becomes one of a maximum, which a signalling NaN would spoil
-                    const float q = __builtin_canonicalizef(x[e]);
-                    any |= (q >= from) & (q <= to);
-                }
+                mask = marks.add(mask, v[u], u);
                 r[u] = v[u];
-                v[u] = load(j0 + (u + U) * T);
+                v[u] = load(j + (u + U) * T);
             }
-            if (!any) continue;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int j = j0 + u * T;
-                float x[V];
-                // compared again: kept, the answers above would spill
-                asm volatile("" : "+v"(r[u].x), "+v"(r[u].y), "+v"(r[u].z), "+v"(r[u].w));
-                unpack(r[u], x);
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if ((x[e] >= from) & (x[e] <= to) & (j < nv)) f(head + j * V + e, x[e]);
-            }
+            const int whole = min(U, (nv - j + T - 1) / T);  // vectors that are there
+            marked(r, mask & marks.first(whole), j, f);
         }
     }
     // The largest logit of this thread's part, and in `where` the first vector that holds its vectors' largest (-1: none).
@@ -753,6 +835,28 @@ struct BinSums {
     }
 };
 
+// Of the listed logits those in question, in order, and the first at which the sum of counts or masses reaches the target
+// (the last does): s.found, and the mass through it, s.found_mass.
+template <int T, typename Q>
+__device__ __forceinline__ void pick(MinPShared<T> &s, const HeldList<T> &listed, const Rule<T> &rule, uint64_t above,
+                                     uint64_t target, bool mass, Q in_question) {
+    if (threadIdx.x == 0) s.n = 0;
+    __syncthreads();
+    listed.entries([&](uint64_t e) {
+        if (in_question(e)) s.list[atomicAdd(&s.n, 1u)] = e;
+    });
+    __syncthreads();
+    const int n = static_cast<int>(s.n);
+    sort_list<T>(s, n);
+    if (mass) {
+        ListSums<T>(s, n, above, rule).find_mass(s, target);
+    } else {
+        if (threadIdx.x == 0) s.found = s.list[target - above - 1];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) s.n = 0;
+}
+
 // The entry at which the sum of counts or masses reaches the target, s.found, and the mass through it, s.found_mass, from the
 // row's histogram of that kind, whose whole sum reaches it.  A bin that overflows the list is cut by the digits of an
 // entry, ten or eleven bits at a time (32 of the logit, 20 of the id), until one does not; the last digits leave one entry.
@@ -763,7 +867,7 @@ __device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const R
     sums.find(s, target);
     const int bin = static_cast<int>(s.bin);
     uint64_t above = s.above;
-    const float from = rule.bin_from(bin), to = rule.bin_to(bin);
+    const Span in[1] = {{rule.bin_from(bin), rule.bin_to(bin)}};
     auto in_question = [&](uint64_t e) {
         const float v = entry_value(e);
         return rule.bin(v) == bin && rule.counts(v, entry_id(e)) && (e & mask) == prefix;
@@ -788,14 +892,14 @@ __device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const R
         if (list) {
             // a few logits beside the bin's own come along at first: the look at them waits until they are listed
             if (mask == 0) {
-                row.each_in(from, to, [&](int id, float v) { append<T>(s, id, v); });
+                row.each_in(in, [&](int id, float v) { append<T>(s, id, v); });
             } else {
-                row.each_in(from, to, [&](int id, float v) {
+                row.each_in(in, [&](int id, float v) {
                     if (in_question(min_p_entry(v, id))) append<T>(s, id, v);
                 });
             }
         } else {
-            row.each_in(from, to, [&](int id, float v) {
+            row.each_in(in, [&](int id, float v) {
                 const uint64_t e = min_p_entry(v, id);
                 const int at = bins - 1 - (static_cast<int>(e >> shift) & (bins - 1));
                 if (in_question(e)) atomicAdd(reinterpret_cast<unsigned long long *>(&s.digits[at]), mass ? rule.weight(e) : 1);
@@ -811,23 +915,7 @@ __device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const R
             mask |= static_cast<uint64_t>(bins - 1) << shift;
         }
     }
-    int n = static_cast<int>(s.n);
-    const HeldList<T> raw(s, n);
-    if (threadIdx.x == 0) s.n = 0;
-    __syncthreads();
-    raw.entries([&](uint64_t e) {
-        if (in_question(e)) s.list[atomicAdd(&s.n, 1u)] = e;
-    });
-    __syncthreads();
-    n = static_cast<int>(s.n);
-    sort_list<T>(s, n);
-    if (mass) {
-        ListSums<T>(s, n, above, rule).find_mass(s, target);
-    } else {
-        if (threadIdx.x == 0) s.found = s.list[target - above - 1];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) s.n = 0;
+    pick<T>(s, HeldList<T>(s, static_cast<int>(s.n)), rule, above, target, mass, in_question);
 }
 
 // The token of a row by its histograms.
@@ -842,7 +930,8 @@ __device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, Ru
                 sums.find(s, c.k);
                 const int bin = static_cast<int>(s.bin);
                 if (s.found_mass <= MinPSizes<T>::kSorted) {
-                    row.each_in(rule.bin_from(bin), __builtin_inff(), [&](int id, float v) {
+                    const Span in[1] = {{rule.bin_from(bin), __builtin_inff()}};
+                    row.each_in(in, [&](int id, float v) {
                         if (rule.counts(v, id) && rule.bin(v) <= bin) append<T>(s, id, v);
                     });  // at most MinPSizes<T>::kSorted
                     __syncthreads();
@@ -862,7 +951,40 @@ __device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, Ru
     const BinSums<T> sums(s, s.hist, 0);
     uint64_t kept = sums.total;
     if (c.p < 1.0) {
-        locate<T>(s, row, rule, sums, share(c.p, kept), true);
+        // top-p's entry is in a bin that the sums tell, so what it keeps lies between two masses, and the drawn entry between
+        // two bins, most often one: all of them are listed in one pass, or, where they are too many, one after the other
+        const uint64_t target = share(c.p, kept);
+        sums.find(s, target);
+        const int cut = static_cast<int>(s.bin);
+        const uint64_t cut_above = s.above, most = s.found_mass;
+        __syncthreads();
+        sums.find(s, share(c.u, cut_above + 1));
+        const int first = static_cast<int>(s.bin);
+        const uint64_t above = s.above;
+        __syncthreads();
+        sums.find(s, share(c.u, most));
+        const int last = static_cast<int>(s.bin);
+        const Span in[2] = {{rule.bin_from(cut), rule.bin_to(cut)}, {rule.bin_from(last), rule.bin_to(first)}};
+        row.each_in(in, [&](int id, float v) { append<T>(s, id, v); });
+        __syncthreads();
+        const int n = static_cast<int>(s.n);
+        if (n <= MinPSizes<T>::kList) {
+            const HeldList<T> listed(s, n);
+            pick<T>(s, listed, rule, cut_above, target, true, [&](uint64_t e) {
+                return rule.bin(entry_value(e)) == cut && rule.counts(entry_value(e), entry_id(e));
+            });
+            kept = s.found_mass;
+            __syncthreads();
+            pick<T>(s, listed, rule, above, share(c.u, kept), true, [&](uint64_t e) {
+                const int bin = rule.bin(entry_value(e));
+                return bin >= first && bin <= last && rule.counts(entry_value(e), entry_id(e));
+            });
+            return entry_id(s.found);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) s.n = 0;
+        __syncthreads();
+        locate<T>(s, row, rule, sums, target, true);
         kept = s.found_mass;
         __syncthreads();
     }
@@ -963,8 +1085,8 @@ min_p_kernel(MinPArgs a) {
         const BinSums<T> sums(s, s.hist, 0);
         if (sums.total >= static_cast<uint64_t>(cuts.k)) {
             sums.find(s, cuts.k);
-            const float from = rule.bin_from(static_cast<int>(s.bin));
-            row.each_in(from, __builtin_inff(), [&](int id, float v) { append<T>(s, id, v); });
+            const Span in[1] = {{rule.bin_from(static_cast<int>(s.bin)), __builtin_inff()}};
+            row.each_in(in, [&](int id, float v) { append<T>(s, id, v); });
         }
     }
     __syncthreads();
