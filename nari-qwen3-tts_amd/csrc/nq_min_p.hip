@@ -14,6 +14,10 @@
 // one drops is dropped behind the pass), and they are sorted and summed there.  Otherwise a histogram over the distance
 // from the maximum, of counts for top-k and of masses for the shares, says which bin a rank lies in, and that bin's logits
 // alone are collected and sorted; a bin too full for the list (equal logits) is cut by the digits of its entries.
+//
+// Bound by the slowest row's passes.  64 x 65537 bf16 (us, replayed): the first rank 7, min-p .05 17, top-k 50 16, no cut 28,
+// top-p .95 35; 256 x 131072 fp32, whose reading takes 26: 28, 38, 54, 84, 94.  Of a row without a cut the maximum takes a pass (2.4 and
+// 17 us), the weights another (11 and 31: its atomics in LDS and its doubles), the drawn bin's logits a third (4 and 18).
 #include <type_traits>
 
 #include "nq_common.h"
@@ -312,7 +316,7 @@ __device__ __forceinline__ float logit_at(const InT *row, int id) {
 // A row in registers, thread t the ids t, t + T, ..
 template <typename InT, int T>
 struct HeldRow {
-    static constexpr bool kShort = false;  // whether its logits are bf16 and many
+    static constexpr bool kShort = false, kMemory = false;  // whether its logits are bf16 and many, and in memory
     float x[kMinPHeld];
     int vocab;
     __device__ __forceinline__ HeldRow(const InT *row, int v) : vocab(v) {
@@ -355,7 +359,7 @@ static_assert(kMinPHeld == 8, "two groups of four");
 // constructor.  No entry is 0.
 template <int T>
 struct HeldList {
-    static constexpr bool kShort = false;
+    static constexpr bool kShort = false, kMemory = false;
     static constexpr int kEach = MinPSizes<T>::kList / T;
     uint64_t e[kEach];
     __device__ __forceinline__ HeldList(const MinPShared<T> &s, int n) {
@@ -400,7 +404,7 @@ struct FarRow {
     const InT *row;
     int vocab, head, nv;
     static constexpr int V = 16 / sizeof(InT);
-    static constexpr bool kShort = sizeof(InT) == 2;
+    static constexpr bool kShort = sizeof(InT) == 2, kMemory = true;
     __device__ __forceinline__ FarRow(const InT *r, int v) : row(r), vocab(v) {
         head = min(v, static_cast<int>((16 - reinterpret_cast<uintptr_t>(r) % 16) % 16 / sizeof(InT)));
         nv = (v - head) / V;
@@ -471,7 +475,8 @@ struct FarRow {
             else f(id + (at >> 4), __uint_as_float(at >= 16 ? q[0] & 0xffff0000u : q[0] << 16));
         }
     }
-    // f for the logits of some spans, which are few
+    // f for the logits of some spans, which are few.  64 x 65537 bf16, a pass 4 us where a test in every logit's place took 6 to 8;
+    // 131072 fp32 logits 10 us alone, 18 beside 255 other rows, which is the memory's rate.
     template <int N, typename F>
     __device__ __forceinline__ void each_in(const Span (&in)[N], F f) const {
         constexpr int U = 4;
@@ -950,9 +955,10 @@ __device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, Ru
     row_histogram<true, T>(s, row, rule);
     const BinSums<T> sums(s, s.hist, 0);
     uint64_t kept = sums.total;
-    if (c.p < 1.0) {
+    if (Row::kMemory && c.p < 1.0) {
         // top-p's entry is in a bin that the sums tell, so what it keeps lies between two masses, and the drawn entry between
-        // two bins, most often one: all of them are listed in one pass, or, where they are too many, one after the other
+        // two bins, most often one: all of them are listed in one pass, or, where they are too many, one after the other, as in
+        // a row in registers, whose passes are short (256 x 8192: 25 us so, 23 in one pass, whose code costs the others 1 to 3)
         const uint64_t target = share(c.p, kept);
         sums.find(s, target);
         const int cut = static_cast<int>(s.bin);
@@ -984,7 +990,9 @@ __device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, Ru
         __syncthreads();
         if (threadIdx.x == 0) s.n = 0;
         __syncthreads();
-        locate<T>(s, row, rule, sums, target, true);
+    }
+    if (c.p < 1.0) {
+        locate<T>(s, row, rule, sums, share(c.p, kept), true);
         kept = s.found_mass;
         __syncthreads();
     }
