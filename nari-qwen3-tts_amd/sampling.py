@@ -7,7 +7,8 @@ same fused kernel draws each row's uniform from its (seed, offset) counter
 with Philox-4x32-10 (``sample_with_counter``, identical to
 ``uniforms_from_counter`` then ``sample_with_uniforms``), so a request's draw
 depends only on its own counter (row-local, batch- and permutation-invariant
-like model/sampling.py:192-195).
+like model/sampling.py:192-195).  ``sample_min_p`` (no reference counterpart)
+adds min-p and takes vocabularies of up to 2^20.
 """
 
 from __future__ import annotations
