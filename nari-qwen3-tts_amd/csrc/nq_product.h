@@ -5,7 +5,7 @@
 // Few rows: a workgroup owns 16 output channels and all of K, its waves interleave K in
 // pieces of 128 bytes, each through LDS of its own, and add their sums at the end, in the order of the waves.
 // Many rows: (32 TM WM) x (32 TN WN) tiles, K staged 128 bytes at a
-// time through three LDS buffers, the next two stages' loads in flight.
+// time through three or four LDS buffers, the next stages' loads in flight.
 #pragma once
 
 #include <type_traits>
@@ -241,9 +241,9 @@ product_rows_kernel(ProductArgs a) {
     }
 }
 
-// WM x WN waves, each TM x TN parts of 32 x 32.  K goes through three LDS buffers, 128 bytes a stage, written by the
+// WM x WN waves, each TM x TN parts of 32 x 32.  K goes through NB LDS buffers, 128 bytes a stage, written by the
 // loads themselves (a register on the way would cost its write to LDS: 0.14 us a stage of 128 x 256).  Step k: stage k
-// has arrived, the loads of stage k + 2 are issued; the operands of each 32 bytes are read while the MFMAs of the 32
+// has arrived, the loads of stage k + NB - 1 are issued; the operands of each 32 bytes are read while the MFMAs of the 32
 // before run, also across the barrier.  The results cross LDS once more, so that they leave in whole lines.
 // 4001 x 2048 (K 6144) bf16 94 us = 1070 TFLOP/s, int8 55.5 us = 1810 TOP/s; 4096^3 124 us = 1105 TFLOP/s and 73 us = 1880
 // TOP/s (a library's bf16: 86 and 92 us).  No unit is full: the MFMAs run in half of the clocks, of the eight waves of a
@@ -251,8 +251,9 @@ product_rows_kernel(ProductArgs a) {
 // stages' loads it would be 84 us at 4096^3, with loads of one and the same cached tile 119: their way into LDS beside the
 // operand reads costs, not the memory behind them.  Waiting for operands before the next are asked for gave 7 %, bands of
 // tiles 3 %, an MFMA ahead of the reads and the loads between MFMAs 6 %.  Other tiles and depths at 4096^3, us: 256 x 256 in
-// two buffers 118, but 137 where that leaves CUs idle (4001 x 2048); in four buffers of 64 bytes 124; four waves 129 to 150.
-template <typename Op, bool kEpi, int WM, int WN, int TM, int TN>
+// two buffers 118, but 137 where that leaves CUs idle (4001 x 2048); in four buffers of 64 bytes 124; four waves 129 to 150; waves
+// in two groups, one reading operands while the other multiplies, 129.
+template <typename Op, bool kEpi, int WM, int WN, int TM, int TN, int NB>
 __global__ void __launch_bounds__(WM * WN * kWave)
 product_tile_kernel(ProductArgs a, int tiles_m, int tiles_n) {
     constexpr int NW = WM * WN, T = NW * kWave, BM = 32 * TM * WM, BN = 32 * TN * WN;
@@ -262,7 +263,7 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles_n) {
     constexpr int kBuf = (BM + BN) * kStage;     // bytes of a stage: weights, then x
     constexpr int kOutPitch = BN * (kEpi ? 4 : 2) + 16;  // bytes of a result row, fp32 where a residual may follow
     constexpr int kOut = BM * kOutPitch;
-    constexpr int kScales = 3 * kBuf > kOut ? 3 * kBuf : kOut;  // behind the buffers: the tile's scales, there when the sums are
+    constexpr int kScales = NB * kBuf > kOut ? NB * kBuf : kOut;  // behind the buffers: the tile's scales, there when the sums are
     // one array: with a second one the compiler waits for every load in flight before it reads LDS (57 us become 87)
     __shared__ __attribute__((aligned(16))) char lds[kScales + 4 * (BM + 2 * BN)];
     float *const s_w = reinterpret_cast<float *>(lds + kScales), *const s_x = s_w + BN, *const s_b = s_x + BM;
@@ -327,15 +328,15 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles_n) {
             for (int n = 0; n < TN; ++n)
                 acc[m][n] = Op::mfma(wf[j & 1][n], xf[j & 1][m], acc[m][n]);
     };
-    int b0 = 0, b2 = 2 * kBuf;  // the buffers of stage k and of stage k + 2, whose loads step k issues
+    int b0 = 0, bl = (NB - 1) * kBuf;      // the buffers of stage k and of stage k + NB - 1, whose loads step k issues
     constexpr std::true_type whole{};      // stages inside K: no look at the chunks, 14 vector instructions instead of 40
     constexpr std::false_type part{};
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < NB - 1; ++i)
 #pragma unroll
         for (int v = 0; v < V; ++v) load(part, i, i * kBuf, v);
     auto step = [&](auto next, int k) __attribute__((always_inline)) {
-        arrive<V>();  // stage k is there; stage k + 1 may be under way
+        arrive<(NB - 2) * V>();  // stage k is there; those behind it may be under way
         read(b0, 0);
         __builtin_amdgcn_sched_barrier(0);
         if (k > 0) multiply(STEPS - 1);  // the last operands of stage k - 1
@@ -349,7 +350,7 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles_n) {
             // into the buffer that the barrier freed; stages behind the last read zeros, so that the waits can count
 #pragma unroll
             for (int v = 0; v < V; ++v)
-                if (v * (STEPS - 1) / V == j) load(next, k + 2, b2, v);
+                if (v * (STEPS - 1) / V == j) load(next, k + NB - 1, bl, v);
             multiply(j);
             // an MFMA, the reads, then a load behind each of the other MFMAs: the matrix unit has work at once
             __builtin_amdgcn_sched_group_barrier(8, 1, 0);
@@ -361,11 +362,11 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles_n) {
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        b2 = b0;
-        b0 = b0 == 2 * kBuf ? 0 : b0 + kBuf;
+        bl = b0;
+        b0 = b0 == (NB - 1) * kBuf ? 0 : b0 + kBuf;
     };
     int k = 0;
-    for (; (k + 3) * kStage <= a.K; ++k) step(whole, k);
+    for (; (k + NB) * kStage <= a.K; ++k) step(whole, k);
     for (; k < stages; ++k) step(part, k);
     multiply(STEPS - 1);
     arrive<0>();  // no load is left that would write over the results
@@ -435,11 +436,11 @@ void launch_rows(const ProductArgs &a, hipStream_t st) {
                        dim3(kRowWaves * kWave), 0, st, a);
 }
 
-template <typename Op, bool kEpi, int WM, int WN, int TM, int TN>
+template <typename Op, bool kEpi, int WM, int WN, int TM, int TN, int NB>
 void launch_tiles(const ProductArgs &a, hipStream_t st) {
     constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN;
     const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (a.N + BN - 1) / BN;
-    hipLaunchKernelGGL((product_tile_kernel<Op, kEpi, WM, WN, TM, TN>), dim3((tiles_m * tiles_n + 7) / 8 * 8),
+    hipLaunchKernelGGL((product_tile_kernel<Op, kEpi, WM, WN, TM, TN, NB>), dim3((tiles_m * tiles_n + 7) / 8 * 8),
                        dim3(WM * WN * kWave), 0, st, a, tiles_m, tiles_n);
 }
 
@@ -472,12 +473,20 @@ int tile_for(int M, int N, bool epilogue = false) {
     return tile_id(128, 256);
 }
 
+bool one_round(int M, int N, int bm, int bn) {
+    return static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn) <= 256;
+}
+
+// Four stages in LDS where a CU has one workgroup of a small tile: three are 48 KB on their way at most, less than the time of a
+// load asks for.  us with four and three, K 2048 unless said, bf16 then int8: M 200 N 4096 10.9 and 11.9, 8.5 and 8.9; M 300 N 2048
+// (K 6144) 22.9 and 27.5, 14.3 and 16.6; M 640 N 2048 (K 6144; 64 x 128) 32.4 and 35.1, 19.1 and 20.7; five to eight
+// no better.  Tiles of 64 x 128 in several rounds keep two workgroups a CU with three (M 1500 N 6144: 56.4 and, with four, 66.5).
 template <typename Op, bool kEpi>
 int launch_product(const ProductArgs &a, hipStream_t st) {
     const int tile = tile_for(a.M, a.N, kEpi);
     if constexpr (kEpi) {
         if (tile == tile_id(128, 128)) {
-            launch_tiles<Op, kEpi, 2, 4, 2, 1>(a, st);
+            launch_tiles<Op, kEpi, 2, 4, 2, 1, 3>(a, st);
             return NQ_LAUNCH_STATUS();
         }
     }
@@ -486,9 +495,12 @@ int launch_product(const ProductArgs &a, hipStream_t st) {
         case tile_id(32, 16): launch_rows<Op, kEpi, 2>(a, st); break;
         case tile_id(48, 16): launch_rows<Op, kEpi, 3>(a, st); break;
         case tile_id(64, 16): launch_rows<Op, kEpi, 4>(a, st); break;
-        case tile_id(64, 64): launch_tiles<Op, kEpi, 2, 2, 1, 1>(a, st); break;
-        case tile_id(64, 128): launch_tiles<Op, kEpi, 2, 4, 1, 1>(a, st); break;
-        default: launch_tiles<Op, kEpi, 2, 4, 2, 2>(a, st);  // 128 x 256
+        case tile_id(64, 64): launch_tiles<Op, kEpi, 2, 2, 1, 1, 4>(a, st); break;
+        case tile_id(64, 128):
+            if (one_round(a.M, a.N, 64, 128)) launch_tiles<Op, kEpi, 2, 4, 1, 1, 4>(a, st);
+            else launch_tiles<Op, kEpi, 2, 4, 1, 1, 3>(a, st);
+            break;
+        default: launch_tiles<Op, kEpi, 2, 4, 2, 2, 3>(a, st);  // 128 x 256
     }
     return NQ_LAUNCH_STATUS();
 }
