@@ -15,9 +15,9 @@
 // from the maximum, of counts for top-k and of masses for the shares, says which bin a rank lies in, and that bin's logits
 // alone are collected and sorted; a bin too full for the list (equal logits) is cut by the digits of its entries.
 //
-// Bound by the slowest row's passes.  64 x 65537 bf16 (us, replayed): the first rank 7, min-p .05 17, top-k 50 16, no cut 28,
-// top-p .95 35; 256 x 131072 fp32, whose reading takes 26: 28, 38, 54, 84, 94.  Of a row without a cut the maximum takes a pass (2.4 and
-// 17 us), the weights another (11 and 31: its atomics in LDS and its doubles), the drawn bin's logits a third (4 and 18).
+// Bound by the slowest row's passes.  64 x 65537 bf16 (us, replayed): the first rank 7, min-p .05 17, top-k 50 16, no cut 24,
+// top-p .95 30; 256 x 131072 fp32, whose reading takes 26: 28, 38, 54, 84, 94.  Of a row without a cut the maximum takes a pass (2.4 and
+// 17 us), the weights another (7 and 31: its atomics in LDS and its doubles), the drawn bin's logits a third (4 and 18).
 #include <type_traits>
 
 #include "nq_common.h"
@@ -428,29 +428,39 @@ struct FarRow {
         const int i = threadIdx.x, id = i < head ? i : i + nv * V;
         if (id < vocab) f(id, logit_at(row, id));
     }
-    // f for several logits at once: an id, the step to the next, and the logits.  Four vectors of a thread are in flight.
-    template <typename F>
-    __device__ __forceinline__ void several(F f) const {
+    // f for each whole vector and its number, one for the logits outside them.  Four vectors of a thread are in flight.
+    template <typename F, typename G>
+    __device__ __forceinline__ void vectors(F f, G one) const {
         constexpr int U = 4;
         const int tid = threadIdx.x;
         uint4 v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = load(tid + u * T);
-        few([&](int id, float x) {
-            const float v[1] = {x};
-            f(id, 1, v);
-        });
+        few(one);
 #pragma unroll 1
         for (int j = tid; j < nv; j += U * T) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (j + u * T >= nv) break;
-                float x[V];
-                unpack(v[u], x);
+                const uint4 r = v[u];
                 v[u] = load(j + (u + U) * T);
-                f(head + (j + u * T) * V, 1, x);
+                f(j + u * T, r);
             }
         }
+    }
+    // f for several logits at once: an id, the step to the next, and the logits
+    template <typename F>
+    __device__ __forceinline__ void several(F f) const {
+        vectors(
+            [&](int j, const uint4 &r) {
+                float x[V];
+                unpack(r, x);
+                f(head + j * V, 1, x);
+            },
+            [&](int id, float x) {
+                const float v[1] = {x};
+                f(id, 1, v);
+            });
     }
     // f for the logits of four vectors, the thread's j, j + T, .., whose bits are set.  A lane's logits come one after the
     // other, picked out of its registers: f is there once, where a copy behind a test of each logit costs the tests of all and the
@@ -479,13 +489,18 @@ struct FarRow {
     // 131072 fp32 logits 10 us alone, 18 beside 255 other rows, which is the memory's rate.
     template <int N, typename F>
     __device__ __forceinline__ void each_in(const Span (&in)[N], F f) const {
+        each_in(in, f, f);
+    }
+    // the same with a function of its own for the logits outside whole vectors
+    template <int N, typename F, typename G>
+    __device__ __forceinline__ void each_in(const Span (&in)[N], F f, G one) const {
         constexpr int U = 4;
         const int tid = threadIdx.x;
         uint4 v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = load(tid + u * T);
         few([&](int id, float x) {
-            if (in_any(in, x)) f(id, x);
+            if (in_any(in, x)) one(id, x);
         });
         const typename std::conditional<V == 8, HalfMarks<N>, WordMarks<N>>::type marks(in);
 #pragma unroll 1
@@ -767,44 +782,57 @@ __device__ __forceinline__ void row_histogram(MinPShared<T> &s, const Row &row, 
             for (int e = 0; e < N; ++e)
                 if (rule.counts(x[e], id + e * step)) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[rule.bin(x[e])]), 1ull);
         });
+    } else if (!rule.plain) {
+        __syncthreads();
+        row.several(weigh);
     } else if constexpr (!Row::kShort) {
         __syncthreads();
-        if (rule.plain) row.several(weigh_plain);
-        else row.several(weigh);
+        row.several(weigh_plain);
     } else {
         // A bf16 row repeats its values: they are counted where the list will be, 32 binades of either sign down from the
-        // largest that counts (and zero), and each is weighed once, 5 instructions a logit instead of 25.  What is smaller yet is
-        // weighed alone.
+        // largest that counts, and each is weighed once, 5 instructions a logit instead of 21 (64 x 65537 without a cut 24 us, 28 with a
+        // test and a branch for each logit).  Counter 0 of a sign has what is smaller and zero, the last one what is larger
+        // (NaN, and what is too far below the maximum to count).
         constexpr int kHalf = MinPSizes<T>::kList;  // 32-bit counters of a sign
+        static_assert(kHalf == 4096, "the sign's bit, moved by three, and the numbers share 16 bits");
         uint32_t *const count = reinterpret_cast<uint32_t *>(s.list);
         for (int i = threadIdx.x; i < 2 * kHalf; i += T) count[i] = 0;
         __syncthreads();
         const float high = fmaxf(fabsf(static_cast<float>(rule.max)), fabsf(rule.least));
-        const int base = max(0, static_cast<int>((__float_as_uint(high) >> 16) & 0x7f80u) + 128 - kHalf);
-        row.several([&](int id, int step, const auto &x) {
-            constexpr int N = sizeof(x) / sizeof(float);
+        const int base = max(0, static_cast<int>((__float_as_uint(high) >> 16) & 0x7f80u) + 128 + 1 - kHalf);
+        auto one = [&](int id, float x) {
+            const float v[1] = {x};
+            weigh(id, 1, v);
+        };
+        row.vectors(
+            [&](int, const uint4 &r) {
+                const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+                const u16x2 low = static_cast<uint16_t>(base), last = static_cast<uint16_t>(kHalf - 1);
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                if (!(x[e] >= rule.least) || (!rule.plain && !rule.counts(x[e], id + e * step))) continue;
-                const uint32_t bits = __float_as_uint(x[e]);
-                const int key = static_cast<int>((bits >> 16) & 0x7fffu), at = key - base;
-                if (at > 0 || key == 0) {
-                    atomicAdd(&count[static_cast<int>(bits >> 31) * kHalf + max(at, 0)], 1u);
-                } else {
-                    const float one[1] = {x[e]};
-                    weigh(id + e * step, 1, one);
+                for (int e = 0; e < 4; ++e) {
+                    const u16x2 size = __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu);
+                    const u16x2 at = __builtin_elementwise_min(__builtin_elementwise_sub_sat(size, low), last);
+                    const uint32_t both = __builtin_bit_cast(uint32_t, at) | (w[e] >> 3 & 0x10001000u);
+                    atomicAdd(&count[both & 0xffffu], 1u);
+                    atomicAdd(&count[both >> 16], 1u);
                 }
-            }
-        });
+            },
+            one);
         __syncthreads();
+        const bool small = base > 0 && count[0] + count[kHalf] > 0;
 #pragma unroll 1
         for (int i = threadIdx.x; i < 2 * kHalf; i += T) {
-            const uint32_t c = count[i];
-            if (c == 0) continue;
-            const uint32_t key = i % kHalf ? i % kHalf + base : 0;
+            const uint32_t c = count[i], at = i % kHalf;
+            const float x = __uint_as_float(((at + base) << 16) | (i >= kHalf ? 0x80000000u : 0u));
+            if (c == 0 || at == kHalf - 1 || (at == 0 && base > 0) || !(x >= rule.least)) continue;
             int bin;
-            const uint64_t w = rule.weight(__uint_as_float((key << 16) | (i >= kHalf ? 0x80000000u : 0u)), bin);
+            const uint64_t w = rule.weight(x, bin);
             atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[bin]), c * w);
+        }
+        if (small) {
+            const float most = __uint_as_float(static_cast<uint32_t>(base) << 16);
+            const Span in[1] = {{-most, most}};
+            row.each_in(in, one, [](int, float) {});  // those outside whole vectors are weighed
         }
     }
     __syncthreads();

@@ -136,6 +136,29 @@ def test_every_kind_of_nan(nq, device, vocab):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale", [1.0, 2.0**-20, 2.0**20, 2.0**-110])
+def test_small_and_zero_logits(nq, device, dtype, scale):
+    """Rows whose logits are far apart in size: zeros of either sign, values 40 binades and more below the largest, the
+    smallest ones; and some that are too far below the maximum to count, or are none."""
+
+    rng = np.random.default_rng(3)
+    rows, vocab = 12, 9003
+    x = torch.from_numpy((rng.standard_normal((rows, vocab)) * np.exp2(rng.integers(-60, 2, (rows, vocab)))).astype(np.float32))
+    x[:, ::5] = 0.0
+    x[:, 1::10] = -0.0
+    x[:, 3::50] = 2.0**-125
+    x[:, 7::70] = -1000.0
+    x[:, 9::90] = -INF
+    x[:, 11::110] = NAN
+    x[6:, 100:8000] = 0.0
+    x[9] = x[9].clamp(max=0.0)
+    x = (x * scale).to(device, dtype)
+    temperature = [float(np.float32(scale * t)) for t in (0.05, 0.3, 1.0, 3.0)] * 3
+    for k, p, m in ((0, 1.0, 0.0), (0, 0.9, 0.0), (3000, 1.0, 0.0), (0, 0.95, 0.2)):
+        _run(device, x, temperature, [k] * rows, [p] * rows, [m] * rows, _uniforms(rng, rows))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_greedy_ties_take_the_lowest_id(nq, device, dtype):
     """Maxima in the first and last places, which rows at odd addresses load alone, and between them."""
 
