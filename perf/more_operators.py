@@ -172,8 +172,8 @@ def _linear(s):
 
 def _sample(s):
     """Plain form in 64 bits, since the draw compares sums: the tokens in order of their logits (ties: the lowest id
-    first), the prefix that min-p and top-k leave, of that the least whose mass reaches top_p of it, and of those the first
-    at which the mass reaches the uniform's share."""
+    first), the prefix that min-p and top-k leave, of that the least whose mass reaches top_p of it, and the first token
+    by id at which the kept mass reaches the uniform's share."""
 
     x = s["logits"].double()
     vocab, greedy = x.shape[1], s["temperature"] == 0
@@ -185,10 +185,10 @@ def _sample(s):
     e = torch.where((rank < k) & (e >= s["min_p"].double()[:, None]), e, 0.0)
     cum = e.cumsum(1)
     e = torch.where((rank == 0) | (cum - e < s["top_p"].double()[:, None] * cum[:, -1:]), e, 0.0)
+    e = torch.zeros_like(e).scatter_(1, order, e)
     cum = e.cumsum(1)
     reached = (e > 0) & (cum >= s["uniforms"].double()[:, None] * cum[:, -1:])
-    first = torch.where(greedy, 0, torch.where(reached, rank, vocab).amin(1))
-    return order.gather(1, first[:, None])[:, 0]
+    return torch.where(greedy, order[:, 0], torch.where(reached, rank, vocab).amin(1))
 
 
 def _package():
