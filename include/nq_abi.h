@@ -931,8 +931,8 @@ int nq_linear_int8_act(const int8_t *xq, int64_t x_s0, const float *sx, const in
  * With x the logits (a NaN counts as minus infinity), e = exp((x - max x) / temperature) in double and w =
  * rint(2^42 e), or 0 where that is below 2^42 min_p, the ranks are in the order of (x descending, id ascending) and
  *   total = the sum of w over the first top_k ranks (top_k <= 0: all),
- *   kept  = the sum of w up to the first rank at which it reaches top_p * total,
- *   token = the id of the first rank at which the sum of w reaches u * kept.
+ *   kept  = the ranks up to the first at which the sum of w reaches top_p * total,
+ *   token = the first id at which the sum of w over the kept ids up to it reaches u * (that of all kept).
  * The sums are integers, so a token does not depend on the launch or on other rows.  temperature not above 0 (or
  * NaN): the first rank.  min_p, top_p and u are held to [0, 1] (NaN: no min-p, no top-p, u = 0); a row without a
  * logit above minus infinity answers 0, one with infinite logits one of those.

@@ -6,14 +6,15 @@
 //   order : by (x desc, id asc); F(r) = sum of w over the ranks 0 .. r
 //   total = F(min(k, V) - 1), k = top_k > 0 ? top_k : V
 //   kept  = the ranks up to the first with F(r) >= p total (min-p and top-k leave a prefix too)
-//   token = id of the first rank with F(r) >= u F(last kept)
-// T not above zero: the first rank.  All three cuts and the draw are the same question, the first rank whose count or
-// mass reaches a target, so a row is asked it up to three times and never sorted whole.
+//   token = the first id at which the sum of w over the kept ids up to it reaches u of its whole
+// T not above zero: the first rank.  Top-k and top-p are the same question, the first rank whose count or mass reaches a
+// target, so a row is asked it up to twice and never sorted whole.
 //
 // A workgroup a row.  Where min-p leaves few logits, one pass collects them in LDS, by the maximum so far (what a later
 // one drops is dropped behind the pass), and they are sorted and summed there.  Otherwise a histogram over the distance
-// from the maximum, of counts for top-k and of masses for the shares, says which bin a rank lies in, and that bin's logits
-// alone are collected and sorted; a bin too full for the list (equal logits) is cut by the digits of its entries.
+// from the maximum, of counts for top-k and of masses for top-p, says which bin the last rank lies in, and that bin's
+// logits alone are collected and sorted; a bin too full for the list (equal logits) is cut by the digits of its entries.
+// The draw sums what is kept over cells of consecutive ids, and looks at the logits of the one cell that it falls into.
 //
 // Bound by the slowest row's passes.  64 x 65537 bf16 (us, replayed): the first rank 7, min-p .05 17, top-k 50 16, no cut 24,
 // top-p .95 30; 256 x 131072 fp32, whose reading takes 26: 28, 38, 54, 84, 94.  Of a row without a cut the maximum takes a pass (2.4 and
@@ -83,13 +84,6 @@ struct Span {
     float from, to;
     __device__ __forceinline__ bool has(float x) const { return x >= from && x <= to; }
 };
-template <int N>
-__device__ __forceinline__ bool in_any(const Span (&in)[N], float x) {
-    bool any = in[0].has(x);
-#pragma unroll
-    for (int i = 1; i < N; ++i) any |= in[i].has(x);
-    return any;
-}
 
 // The same for two bf16 values in a word: with their bits made unsigned integers in the values' order (negative ones
 // inverted, the others' first bit set; -0 before 0), a span is [low, low + size).
@@ -116,36 +110,27 @@ struct ShortSpan {
     __device__ __forceinline__ u16x2 inside(u16x2 key) const { return __builtin_elementwise_sub_sat(size, static_cast<u16x2>(key - low)); }
 };
 
-// Which logits of four vectors some spans hold, a bit a logit, added to a mask a vector at a time: fp32 word w in bit w, bf16's
+// Which logits of four vectors a span holds, a bit a logit, added to a mask a vector at a time: fp32 word w in bit w, bf16's
 // halves of word w in bits 15 - w and 31 - w.
-template <int N>
 struct WordMarks {
-    Span in[N];
-    __device__ __forceinline__ WordMarks(const Span (&of)[N]) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) in[i] = of[i];
-    }
+    Span in;
+    __device__ __forceinline__ WordMarks(const Span &of) : in(of) {}
     __device__ __forceinline__ uint32_t add(uint32_t mask, const uint4 &v, int u) const {
         const float x[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mask |= in_any(in, x[e]) ? 1u << (4 * u + e) : 0u;
+        for (int e = 0; e < 4; ++e) mask |= in.has(x[e]) ? 1u << (4 * u + e) : 0u;
         return mask;
     }
     static __device__ __forceinline__ uint32_t first(int vectors) { return (1u << (4 * vectors)) - 1; }
 };
-template <int N>
 struct HalfMarks {
-    ShortSpan in[N];
-    __device__ __forceinline__ HalfMarks(const Span (&of)[1]) : in{of[0]} { static_assert(N == 1); }
-    __device__ __forceinline__ HalfMarks(const Span (&of)[2]) : in{of[0], of[1]} { static_assert(N == 2); }
+    ShortSpan in;
+    __device__ __forceinline__ HalfMarks(const Span &of) : in(of) {}
     __device__ __forceinline__ uint32_t add(uint32_t mask, const uint4 &v, int) const {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const u16x2 key = ShortSpan::keys(w[e]);
-            u16x2 is = in[0].inside(key);
-#pragma unroll
-            for (int i = 1; i < N; ++i) is = __builtin_elementwise_max(is, in[i].inside(key));
+            const u16x2 is = in.inside(ShortSpan::keys(w[e]));
             mask = mask << 1 | __builtin_bit_cast(uint32_t, __builtin_elementwise_min(is, static_cast<u16x2>(1)));
         }
         return mask;
@@ -254,10 +239,10 @@ struct RowRule {
     double max, turns;    // turns: 128 log2(e) / T
     double lowest;        // of t: -45 octaves
     uint64_t least_weight;  // a smaller one is none (min-p)
-    float least;          // no logit below it has a weight (a bound, or top-k's last one); NaN and -inf never reach it
+    float least;          // no logit below it has a weight (a bound, or the last one kept); NaN and -inf never reach it
     float tie;            // of the logits that equal it (NaN: none do) those with ids behind tie_id have none either
     int tie_id;
-    bool plain;           // t keeps above its bound by itself, and neither least_weight nor tie drop a logit
+    bool bare;            // t keeps above its bound by itself, and least_weight drops no logit
     __device__ __forceinline__ double turn(float x) const {
         // beside an infinite maximum max, turns and lowest are 0 and infinite logits alone count: NaN becomes 0
         return fmax((static_cast<double>(x) - max) * turns, lowest);
@@ -293,7 +278,7 @@ struct RowRule {
         const uint64_t w = weight(turn(x), bin);
         return w >= least_weight ? w : 0;
     }
-    __device__ __forceinline__ uint64_t plain_weight(float x, int &bin) const {
+    __device__ __forceinline__ uint64_t bare_weight(float x, int &bin) const {
         return weight((static_cast<double>(x) - max) * turns, bin);
     }
     __device__ __forceinline__ uint64_t weight(uint64_t entry) const {
@@ -303,6 +288,11 @@ struct RowRule {
         return counts(x, entry_id(entry)) ? w : 0;
     }
     __device__ __forceinline__ bool counts(float x, int id) const { return x >= least && !(x == tie && id > tie_id); }
+    __device__ __forceinline__ bool tied() const { return tie == tie; }
+    __device__ __forceinline__ void end_at(uint64_t entry) {  // an entry that counts: none behind it does
+        least = tie = entry_value(entry);
+        tie_id = entry_id(entry);
+    }
 };
 template <int T>
 using Rule = RowRule<MinPSizes<T>::kShift>;
@@ -312,6 +302,11 @@ __device__ __forceinline__ float logit_at(const InT *row, int id) {
     if constexpr (sizeof(InT) == 2) return bf16_to_f32(row[id]);
     else return row[id];
 }
+
+// The ids of a cell, from .. to - 1, at most 2 T of them.
+struct Ids {
+    int from, to;
+};
 
 // A row in registers, thread t the ids t, t + T, ..
 template <typename InT, int T>
@@ -334,11 +329,11 @@ struct HeldRow {
             if (id < vocab) f(id, x[i]);
         }
     }
-    // f for the logits of some spans
-    template <int N, typename F>
-    __device__ __forceinline__ void each_in(const Span (&in)[N], F f) const {
+    // f for the logits of a span
+    template <typename F>
+    __device__ __forceinline__ void each_in(const Span &in, F f) const {
         each([&](int id, float v) {
-            if (in_any(in, v)) f(id, v);
+            if (in.has(v)) f(id, v);
         });
     }
     // f for several logits at once: an id, the step to the next, and the logits, NaN where there is none
@@ -352,6 +347,20 @@ struct HeldRow {
             f(static_cast<int>(threadIdx.x) + i * T, T, v);
         }
     }
+    // The masses of the cells, 64 ids each.
+    template <typename W>
+    __device__ __forceinline__ void cells(uint64_t *sum, int, W weigh) const {
+        const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+#pragma unroll 1
+        for (int i = 0; i < kMinPHeld; i += 4)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float v[1] = {i ? x[e + 4] : x[e]};  // behind the row's end -inf, which does not count
+                const uint64_t m = wave_scan64(weigh(static_cast<int>(threadIdx.x) + (i + e) * T, v));
+                if (lane == kWave - 1) sum[(i + e) * (T / kWave) + wave] = m;
+            }
+    }
+    __device__ __forceinline__ Ids cell_ids(int cell, int) const { return {cell * kWave, min(vocab, cell * kWave + kWave)}; }
 };
 static_assert(kMinPHeld == 8, "two groups of four");
 
@@ -382,10 +391,10 @@ struct HeldList {
         for (int i = 0; i < kEach; ++i)
             if (e[i]) f(e[i]);
     }
-    template <int N, typename F>
-    __device__ __forceinline__ void each_in(const Span (&in)[N], F f) const {
+    template <typename F>
+    __device__ __forceinline__ void each_in(const Span &in, F f) const {
         each([&](int id, float v) {
-            if (in_any(in, v)) f(id, v);
+            if (in.has(v)) f(id, v);
         });
     }
     template <typename F>
@@ -395,6 +404,23 @@ struct HeldList {
             const float v[1] = {e[i] ? entry_value(e[i]) : __builtin_nanf("")};
             f(entry_id(e[i]), 1, v);
         }
+    }
+    // The masses of the cells, as many ids each, a power of two, as make them 4096 at most.
+    static __device__ __forceinline__ int cell_bits(int vocab) { return max(0, 20 - __clz(max(1, vocab - 1))); }
+    template <typename W>
+    __device__ __forceinline__ void cells(uint64_t *sum, int vocab, W weigh) const {
+        static_assert(kMinPVocab == 1 << 20 && MinPSizes<T>::kBins >= 4096);
+        const int bits = cell_bits(vocab);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (!e[i]) continue;
+            const float v[1] = {entry_value(e[i])};
+            atomicAdd(reinterpret_cast<unsigned long long *>(&sum[entry_id(e[i]) >> bits]), weigh(entry_id(e[i]), v));
+        }
+    }
+    __device__ __forceinline__ Ids cell_ids(int cell, int vocab) const {
+        const int bits = cell_bits(vocab);
+        return {cell << bits, min(vocab, (cell + 1) << bits)};
     }
 };
 
@@ -448,6 +474,42 @@ struct FarRow {
             }
         }
     }
+    // The masses of the cells: the logits before the vectors, those of 256 vectors each, those behind.  A wave takes a cell, so that
+    // its lanes' sums meet once in as many logits; four vectors of a thread are in flight.
+    static constexpr int kCell = 4 * kWave;  // vectors
+    template <typename W>
+    __device__ __forceinline__ void cells(uint64_t *sum, int, W weigh) const {
+        constexpr int U = kCell / kWave, kWaves = T / kWave;
+        static_assert(kMinPVocab / V / kCell + 2 <= MinPSizes<T>::kBins && kCell * V <= 2 * T);
+        const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, n = (nv + kCell - 1) / kCell;
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = load(wave * kCell + u * kWave + lane);
+        few([&](int id, float x) {
+            const float one[1] = {x};
+            atomicAdd(reinterpret_cast<unsigned long long *>(&sum[id < head ? 0 : n + 1]), weigh(id, one));
+        });
+#pragma unroll 1
+        for (int c = wave; c < n; c += kWaves) {
+            uint64_t m = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int j = c * kCell + u * kWave + lane;
+                const uint4 r = v[u];
+                v[u] = load(j + kWaves * kCell);
+                if (j >= nv) continue;
+                float x[V];
+                unpack(r, x);
+                m += weigh(head + j * V, x);
+            }
+            m = wave_scan64(m);
+            if (lane == kWave - 1) sum[c + 1] = m;
+        }
+    }
+    __device__ __forceinline__ Ids cell_ids(int cell, int) const {
+        const int end = head + nv * V, at = head + (cell - 1) * kCell * V;
+        return cell == 0 ? Ids{0, head} : at >= end ? Ids{end, vocab} : Ids{at, min(end, at + kCell * V)};
+    }
     // f for several logits at once: an id, the step to the next, and the logits
     template <typename F>
     __device__ __forceinline__ void several(F f) const {
@@ -485,24 +547,24 @@ struct FarRow {
             else f(id + (at >> 4), __uint_as_float(at >= 16 ? q[0] & 0xffff0000u : q[0] << 16));
         }
     }
-    // f for the logits of some spans, which are few.  64 x 65537 bf16, a pass 4 us where a test in every logit's place took 6 to 8;
+    // f for the logits of a span, which are few.  64 x 65537 bf16, a pass 4 us where a test in every logit's place took 6 to 8;
     // 131072 fp32 logits 10 us alone, 18 beside 255 other rows, which is the memory's rate.
-    template <int N, typename F>
-    __device__ __forceinline__ void each_in(const Span (&in)[N], F f) const {
+    template <typename F>
+    __device__ __forceinline__ void each_in(const Span &in, F f) const {
         each_in(in, f, f);
     }
     // the same with a function of its own for the logits outside whole vectors
-    template <int N, typename F, typename G>
-    __device__ __forceinline__ void each_in(const Span (&in)[N], F f, G one) const {
+    template <typename F, typename G>
+    __device__ __forceinline__ void each_in(const Span &in, F f, G one) const {
         constexpr int U = 4;
         const int tid = threadIdx.x;
         uint4 v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = load(tid + u * T);
         few([&](int id, float x) {
-            if (in_any(in, x)) one(id, x);
+            if (in.has(x)) one(id, x);
         });
-        const typename std::conditional<V == 8, HalfMarks<N>, WordMarks<N>>::type marks(in);
+        const typename std::conditional<V == 8, HalfMarks, WordMarks>::type marks(in);
 #pragma unroll 1
         for (int j = tid; j < nv; j += U * T) {
             uint32_t mask = 0;
@@ -643,12 +705,15 @@ __device__ __forceinline__ void sort_list(MinPShared<T> &s, int n) {
         }
 }
 
-// The sums of a sorted list: thread t has the ranks t E .. t E + E - 1, E = ceil(n / T).
-template <int T>
+// An entry with its halves exchanged: in descending order of these the ids ascend.
+__device__ __forceinline__ uint64_t exchanged(uint64_t e) { return e << 32 | e >> 32; }
+
+// The sums of a sorted list (kIds: of exchanged entries): thread t has the ranks t E .. t E + E - 1, E = ceil(n / T).
+template <int T, bool kIds = false>
 struct ListSums {
     static constexpr int kEach = MinPSizes<T>::kList / T;
     uint64_t cum[kEach];
-    uint64_t before;
+    uint64_t before, total;
     int first, end;
     __device__ __forceinline__ ListSums(MinPShared<T> &s, int n, uint64_t above, const Rule<T> &rule) {
         const int each = (n + T - 1) / T;
@@ -657,20 +722,20 @@ struct ListSums {
         uint64_t own = 0;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            if (first + i < end) own += rule.weight(s.list[first + i]);
+            if (first + i < end) own += rule.weight(kIds ? exchanged(s.list[first + i]) : s.list[first + i]);
             cum[i] = own;
         }
-        uint64_t total;
         before = above + block_before<T>(own, s.part, total);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) cum[i] += before;
     }
-    // The first rank whose mass reaches the target, which the list's last does.
+    // The first rank whose mass reaches the target, which the list's last does: s.bin, its entry and the mass through it.
     __device__ __forceinline__ void find_mass(MinPShared<T> &s, uint64_t target) const {
         uint64_t last = before;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             if (first + i < end && last < target && target <= cum[i]) {
+                s.bin = first + i;
                 s.found_mass = cum[i];
                 s.found = s.list[first + i];
             }
@@ -697,35 +762,43 @@ struct RowCuts {
     double p, u;
 };
 
-// The token of a row whose weights are all among the list's n <= 64 logits, by one wave: lane r has rank r.  Sums of 64
-// weights are exact in double.
+// The token of a row whose weights are all among the list's n <= 64 logits, by one wave, a logit a lane: each lane sums what
+// comes before its own, in the order of the logits for the cuts and of the ids for the draw.  Sums of 64 weights are exact
+// in double.
 template <int T>
 __device__ __forceinline__ int draw_from_few(const MinPShared<T> &s, int n, const Rule<T> &rule, const RowCuts &c) {
     const int lane = threadIdx.x & (kWave - 1);
     const uint64_t mine = lane < n ? listed_entry(s.list[lane]) : 0;
-    int above = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) {
-        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(mine)), j);
-        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(mine >> 32)), j);
-        above += ((static_cast<uint64_t>(hi) << 32) | lo) > mine ? 1 : 0;
-    }
-    if (lane >= n) above = lane;
-    const uint32_t lo = __builtin_amdgcn_ds_permute(4 * above, static_cast<int>(static_cast<uint32_t>(mine)));
-    const uint32_t hi = __builtin_amdgcn_ds_permute(4 * above, static_cast<int>(static_cast<uint32_t>(mine >> 32)));
-    const uint64_t e = (static_cast<uint64_t>(hi) << 32) | lo;
-    double cum = lane < n && lane < c.k ? static_cast<double>(rule.weight(e)) : 0.0;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const double o = __shfl_up(cum, d, kWave);
-        if (lane >= d) cum += o;
-    }
-    double kept = __shfl(cum, kWave - 1, kWave);
-    auto reached = [&](double target) {  // the first lane, which the last one reaches
-        return __ffsll(static_cast<long long>(__ballot(cum >= fmin(fmax(target, 1.0), kept)))) - 1;
+    double own = lane < n ? static_cast<double>(rule.weight(mine)) : 0.0;
+    auto other = [](uint64_t v, int j) {
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v)), j);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v >> 32)), j);
+        return (static_cast<uint64_t>(hi) << 32) | lo;
     };
-    if (c.p < 1.0) kept = __shfl(cum, reached(ceil(c.p * kept)), kWave);
-    return __shfl(entry_id(e), reached(ceil(c.u * kept)), kWave);
+    auto sum = [](double v) {
+#pragma unroll
+        for (int d = 1; d < kWave; d <<= 1) v += __shfl_xor(v, d, kWave);
+        return v;
+    };
+    auto target = [](double p, double mass) { return fmin(fmax(ceil(p * mass), 1.0), mass); };
+    if (c.k < n || c.p < 1.0) {
+        int rank = 0;
+        double above = 0.0;
+        for (int j = 0; j < n; ++j) {
+            const bool first = other(mine, j) > mine;
+            rank += first ? 1 : 0;
+            above += first ? __longlong_as_double(other(__double_as_longlong(own), j)) : 0.0;
+        }
+        if (rank >= c.k) own = 0.0;
+        if (c.p < 1.0 && above >= target(c.p, sum(own))) own = 0.0;
+    }
+    double before = 0.0;
+    for (int j = 0; j < n; ++j) {  // a smaller id has a larger lower half
+        const bool first = static_cast<uint32_t>(other(mine, j)) > static_cast<uint32_t>(mine);
+        before += first ? __longlong_as_double(other(__double_as_longlong(own), j)) : 0.0;
+    }
+    const double at = target(c.u, sum(own));
+    return __shfl(entry_id(mine), __ffsll(static_cast<long long>(__ballot(before < at && at <= before + own))) - 1, kWave);
 }
 
 // The token of a row whose weights are all in the list (for thread 0).
@@ -734,18 +807,24 @@ __device__ __forceinline__ int draw_from_list(MinPShared<T> &s, int n, const Rul
     if (n <= kWave) return threadIdx.x < kWave ? draw_from_few<T>(s, n, rule, c) : 0;
     for (int i = threadIdx.x; i < n; i += T) s.list[i] = listed_entry(s.list[i]);
     __syncthreads();
-    sort_list<T>(s, n);
-    const ListSums<T> sums(s, n, 0, rule);
-    sums.find_rank(s, min(c.k, n) - 1);
-    uint64_t kept = s.found_mass;
-    __syncthreads();
-    if (c.p < 1.0) {
-        sums.find_mass(s, share(c.p, kept));
-        kept = s.found_mass;
-        __syncthreads();
+    int kept = min(c.k, n);
+    if (kept < n || c.p < 1.0) {
+        sort_list<T>(s, n);
+        if (c.p < 1.0) {
+            const ListSums<T> sums(s, n, 0, rule);
+            sums.find_rank(s, kept - 1);
+            const uint64_t mass = s.found_mass;
+            __syncthreads();
+            sums.find_mass(s, share(c.p, mass));
+            kept = static_cast<int>(s.bin) + 1;
+        }
     }
-    sums.find_mass(s, share(c.u, kept));
-    return entry_id(s.found);
+    for (int i = threadIdx.x; i < kept; i += T) s.list[i] = exchanged(s.list[i]);
+    __syncthreads();
+    sort_list<T>(s, kept);
+    const ListSums<T, true> sums(s, kept, 0, rule);
+    sums.find_mass(s, share(c.u, sums.total));
+    return entry_id(exchanged(s.found));
 }
 
 // The row's histogram: of counts (kMass false) or of masses.  The list's counter is cleared besides.
@@ -764,12 +843,12 @@ __device__ __forceinline__ void row_histogram(MinPShared<T> &s, const Row &row, 
             if (rule.counts(x[e], id + e * step)) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[bin[e]]), w[e]);
     };
     // A pass is bound by its vector instructions: without what a row does not need they are 21 a logit instead of 31.
-    auto weigh_plain = [&](int, int, const auto &x) {
+    auto weigh_bare = [&](int, int, const auto &x) {
         constexpr int N = sizeof(x) / sizeof(float);
         int bin[N];
         uint64_t w[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) w[e] = rule.plain_weight(x[e], bin[e]);
+        for (int e = 0; e < N; ++e) w[e] = rule.bare_weight(x[e], bin[e]);
 #pragma unroll
         for (int e = 0; e < N; ++e)
             if (x[e] >= rule.least) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[bin[e]]), w[e]);
@@ -782,12 +861,12 @@ __device__ __forceinline__ void row_histogram(MinPShared<T> &s, const Row &row, 
             for (int e = 0; e < N; ++e)
                 if (rule.counts(x[e], id + e * step)) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[rule.bin(x[e])]), 1ull);
         });
-    } else if (!rule.plain) {
+    } else if (!rule.bare || rule.tied()) {
         __syncthreads();
         row.several(weigh);
     } else if constexpr (!Row::kShort) {
         __syncthreads();
-        row.several(weigh_plain);
+        row.several(weigh_bare);
     } else {
         // A bf16 row repeats its values: they are counted where the list will be, 32 binades of either sign down from the
         // largest that counts, and each is weighed once, 5 instructions a logit instead of 21 (64 x 65537 without a cut 24 us, 28 with a
@@ -831,8 +910,7 @@ __device__ __forceinline__ void row_histogram(MinPShared<T> &s, const Row &row, 
         }
         if (small) {
             const float most = __uint_as_float(static_cast<uint32_t>(base) << 16);
-            const Span in[1] = {{-most, most}};
-            row.each_in(in, one, [](int, float) {});  // those outside whole vectors are weighed
+            row.each_in({-most, most}, one, [](int, float) {});  // those outside whole vectors are weighed
         }
     }
     __syncthreads();
@@ -900,7 +978,7 @@ __device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const R
     sums.find(s, target);
     const int bin = static_cast<int>(s.bin);
     uint64_t above = s.above;
-    const Span in[1] = {{rule.bin_from(bin), rule.bin_to(bin)}};
+    const Span in = {rule.bin_from(bin), rule.bin_to(bin)};
     auto in_question = [&](uint64_t e) {
         const float v = entry_value(e);
         return rule.bin(v) == bin && rule.counts(v, entry_id(e)) && (e & mask) == prefix;
@@ -951,9 +1029,60 @@ __device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const R
     pick<T>(s, HeldList<T>(s, static_cast<int>(s.n)), rule, above, target, mass, in_question);
 }
 
+// The token of a row by what is kept of it: the first id at which the sum of the masses reaches u of the whole.  The cells'
+// masses say in which one, and its logits are read again, two a thread.
+template <int T, typename Row, typename InT>
+__device__ __forceinline__ int draw_by_ids(MinPShared<T> &s, const Row &row, const InT *logits, const Rule<T> &rule,
+                                           double u, int vocab) {
+    for (int i = threadIdx.x; i < MinPSizes<T>::kBins; i += T) s.hist[i] = 0;
+    __syncthreads();
+    auto weigh = [&](int id, const auto &x) {
+        constexpr int N = sizeof(x) / sizeof(float);
+        uint64_t sum = 0;
+        int bin;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const uint64_t w = rule.weight(x[e], bin);
+            sum += rule.counts(x[e], id + e) ? w : 0;
+        }
+        return sum;
+    };
+    auto weigh_bare = [&](int id, const auto &x) {
+        constexpr int N = sizeof(x) / sizeof(float);
+        uint64_t sum = 0;
+        int bin;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const uint64_t w = rule.bare_weight(x[e], bin);
+            sum += rule.counts(x[e], id + e) ? w : 0;
+        }
+        return sum;
+    };
+    if (Row::kMemory && rule.bare) row.cells(s.hist, vocab, weigh_bare);
+    else row.cells(s.hist, vocab, weigh);
+    __syncthreads();
+    const BinSums<T> sums(s, s.hist, 0);
+    const uint64_t target = share(u, sums.total);
+    sums.find(s, target);
+    const Ids ids = row.cell_ids(static_cast<int>(s.bin), vocab);
+    const int id = ids.from + 2 * static_cast<int>(threadIdx.x);
+    uint64_t w[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const float x[1] = {id + e < ids.to ? logit_at(logits, id + e) : -__builtin_inff()};
+        w[e] = weigh(id + e, x);
+    }
+    uint64_t all;
+    const uint64_t before = s.above + block_before<T>(w[0] + w[1], s.part, all);
+    if (before < target && target <= before + w[0] + w[1]) s.id = target <= before + w[0] ? id : id + 1;
+    __syncthreads();
+    return s.id;
+}
+
 // The token of a row by its histograms.
-template <int T, typename Row>
-__device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, Rule<T> &rule, const RowCuts &c, int vocab) {
+template <int T, typename Row, typename InT>
+__device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, const InT *logits, Rule<T> &rule,
+                                            const RowCuts &c, int vocab) {
     // top-k: its last entry, or, where few are before it, those
     if (c.k < vocab) {
         row_histogram<false, T>(s, row, rule);
@@ -963,8 +1092,7 @@ __device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, Ru
                 sums.find(s, c.k);
                 const int bin = static_cast<int>(s.bin);
                 if (s.found_mass <= MinPSizes<T>::kSorted) {
-                    const Span in[1] = {{rule.bin_from(bin), __builtin_inff()}};
-                    row.each_in(in, [&](int id, float v) {
+                    row.each_in({rule.bin_from(bin), __builtin_inff()}, [&](int id, float v) {
                         if (rule.counts(v, id) && rule.bin(v) <= bin) append<T>(s, id, v);
                     });  // at most MinPSizes<T>::kSorted
                     __syncthreads();
@@ -973,59 +1101,19 @@ __device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, Ru
                 __syncthreads();
             }
             locate<T>(s, row, rule, sums, c.k, false);
-            rule.least = rule.tie = entry_value(s.found);  // at least what it was
-            rule.tie_id = entry_id(s.found);
-            rule.plain = false;
+            rule.end_at(s.found);
             __syncthreads();
         }
     }
-    // top-p's last entry and the drawn one, by their masses
-    row_histogram<true, T>(s, row, rule);
-    const BinSums<T> sums(s, s.hist, 0);
-    uint64_t kept = sums.total;
-    if (Row::kMemory && c.p < 1.0) {
-        // top-p's entry is in a bin that the sums tell, so what it keeps lies between two masses, and the drawn entry between
-        // two bins, most often one: all of them are listed in one pass, or, where they are too many, one after the other, as in
-        // a row in registers, whose passes are short (256 x 8192: 25 us so, 23 in one pass, whose code costs the others 1 to 3)
-        const uint64_t target = share(c.p, kept);
-        sums.find(s, target);
-        const int cut = static_cast<int>(s.bin);
-        const uint64_t cut_above = s.above, most = s.found_mass;
-        __syncthreads();
-        sums.find(s, share(c.u, cut_above + 1));
-        const int first = static_cast<int>(s.bin);
-        const uint64_t above = s.above;
-        __syncthreads();
-        sums.find(s, share(c.u, most));
-        const int last = static_cast<int>(s.bin);
-        const Span in[2] = {{rule.bin_from(cut), rule.bin_to(cut)}, {rule.bin_from(last), rule.bin_to(first)}};
-        row.each_in(in, [&](int id, float v) { append<T>(s, id, v); });
-        __syncthreads();
-        const int n = static_cast<int>(s.n);
-        if (n <= MinPSizes<T>::kList) {
-            const HeldList<T> listed(s, n);
-            pick<T>(s, listed, rule, cut_above, target, true, [&](uint64_t e) {
-                return rule.bin(entry_value(e)) == cut && rule.counts(entry_value(e), entry_id(e));
-            });
-            kept = s.found_mass;
-            __syncthreads();
-            pick<T>(s, listed, rule, above, share(c.u, kept), true, [&](uint64_t e) {
-                const int bin = rule.bin(entry_value(e));
-                return bin >= first && bin <= last && rule.counts(entry_value(e), entry_id(e));
-            });
-            return entry_id(s.found);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) s.n = 0;
-        __syncthreads();
-    }
+    // top-p: its last entry, by the masses
     if (c.p < 1.0) {
-        locate<T>(s, row, rule, sums, share(c.p, kept), true);
-        kept = s.found_mass;
+        row_histogram<true, T>(s, row, rule);
+        const BinSums<T> sums(s, s.hist, 0);
+        locate<T>(s, row, rule, sums, share(c.p, sums.total), true);
+        rule.end_at(s.found);
         __syncthreads();
     }
-    locate<T>(s, row, rule, sums, share(c.u, kept), true);
-    return entry_id(s.found);
+    return draw_by_ids<T>(s, row, logits, rule, c.u, vocab);
 }
 
 template <typename InT, int T, bool kHeld>
@@ -1035,7 +1123,8 @@ min_p_kernel(MinPArgs a) {
     typedef typename std::conditional<kHeld, HeldRow<InT, T>, FarRow<InT, T>>::type Row;
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    const Row row(static_cast<const InT *>(a.logits) + r * a.s0, a.vocab);
+    const InT *const logits = static_cast<const InT *>(a.logits) + r * a.s0;
+    const Row row(logits, a.vocab);
     const float temperature = a.temperature[r], mp = a.min_p[r], pq = a.top_p[r], uq = a.uniforms[r];
     const int kq = a.top_k[r];
     const bool greedy = !(temperature > 0.f);
@@ -1096,7 +1185,7 @@ min_p_kernel(MinPArgs a) {
     rule.lowest = top > kLargest ? 0.0 : -45.0 * 128.0;
     rule.least_weight = static_cast<uint64_t>(ceil(min_p * 4398046511104.0));
     rule.least = least(top);
-    rule.plain = rule.least_weight == 0 && top <= kLargest && (rule.least - rule.max) * rule.turns >= rule.lowest;
+    rule.bare = rule.least_weight == 0 && top <= kLargest && (rule.least - rule.max) * rule.turns >= rule.lowest;
     rule.tie = __builtin_nanf("");
     rule.tie_id = 0;
     const int found = static_cast<int>(s.n);
@@ -1121,8 +1210,8 @@ min_p_kernel(MinPArgs a) {
         const BinSums<T> sums(s, s.hist, 0);
         if (sums.total >= static_cast<uint64_t>(cuts.k)) {
             sums.find(s, cuts.k);
-            const Span in[1] = {{rule.bin_from(static_cast<int>(s.bin)), __builtin_inff()}};
-            row.each_in(in, [&](int id, float v) { append<T>(s, id, v); });
+            rule.least = rule.bin_from(static_cast<int>(s.bin));  // nothing below it is kept
+            row.each_in({rule.least, __builtin_inff()}, [&](int id, float v) { append<T>(s, id, v); });
         }
     }
     __syncthreads();
@@ -1133,12 +1222,12 @@ min_p_kernel(MinPArgs a) {
     } else {
         __syncthreads();
         if constexpr (kHeld) {
-            token = draw_by_bins<T>(s, row, rule, cuts, a.vocab);
+            token = draw_by_bins<T>(s, row, logits, rule, cuts, a.vocab);
         } else if (n > 0 && n <= MinPSizes<T>::kList) {
             const HeldList<T> list(s, n);
-            token = draw_by_bins<T>(s, list, rule, cuts, a.vocab);
+            token = draw_by_bins<T>(s, list, logits, rule, cuts, a.vocab);
         } else {
-            token = draw_by_bins<T>(s, row, rule, cuts, a.vocab);
+            token = draw_by_bins<T>(s, row, logits, rule, cuts, a.vocab);
         }
     }
     if (tid == 0) a.tokens[r] = token;

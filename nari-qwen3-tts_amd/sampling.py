@@ -149,9 +149,9 @@ def sample_min_p(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.T
                  min_p: torch.Tensor, uniforms: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """One token per row: temperature, min-p, top-k, top-p and the inverse-CDF draw with the caller's uniforms, over up
     to 2^20 ids (``sample_with_uniforms`` takes 4096).  A token is kept while its probability is at least ``min_p`` of the
-    likeliest's; top-p takes its share of what min-p and top-k leave.  Weights are fixed-point integers of double
-    exponentials, so tokens do not depend on the batch; they are not those of ``sample_with_uniforms``, whose sums
-    are float32, next to a border.  float32 or bfloat16 logits [rows, vocabulary] with contiguous rows at any stride, row
+    likeliest's; top-p takes its share of what min-p and top-k leave; the draw takes the first kept id at which the kept
+    mass, summed by id, reaches its uniform's share.  Weights are fixed-point integers of double exponentials, so
+    tokens do not depend on the batch; ``sample_with_uniforms`` sums by rank, in float32, and draws others.  float32 or bfloat16 logits [rows, vocabulary] with contiguous rows at any stride, row
     vectors float32 (``top_k`` int32), tokens int64."""
 
     shape = logits.shape

@@ -213,26 +213,32 @@ def min_p_weights(x: np.ndarray, temperature: float, min_p: float) -> np.ndarray
     return np.where(w >= min(max(float(F(min_p)), 0.0), 1.0) * 2.0**42, w, 0.0).astype(np.int64)
 
 
-def sample_min_p_row(logits: np.ndarray, temperature: float, top_k: int, top_p: float, min_p: float, u: float) -> int:
-    """The token of one row (the contract of ``nq_sample_min_p``), with the whole row sorted and exact integer sums."""
+def sample_min_p_row(logits: np.ndarray, temperature: float, top_k: int, top_p: float, min_p: float, u: float,
+                     by_id: bool = False) -> int:
+    """The token of one row, with the whole row sorted and exact integer sums: of the kept ranks the first at which the
+    kept mass reaches its share, or, ``by_id`` (the contract of ``nq_sample_min_p``), of the kept ids."""
 
     x = np.where(np.isnan(logits), -np.inf, np.asarray(logits, np.float64))
     order = np.argsort(-x, kind="stable")
     if not temperature > 0 or x[order[0]] == -np.inf:
         return int(order[0])
     hold = lambda v, nan: nan if np.isnan(v) else min(max(float(F(v)), 0.0), 1.0)  # noqa: E731
-    sums = np.cumsum(min_p_weights(x, temperature, hold(min_p, 0.0))[order])
-    k = top_k if 0 < top_k < len(x) else len(x)
+    weights = min_p_weights(x, temperature, hold(min_p, 0.0))
 
-    def reached(share: float, mass: int) -> int:  # the first rank at which the sum reaches that share
+    def reached(sums: np.ndarray, share: float, mass: int) -> int:  # the first place at which the sum reaches that share
         return int(np.argmax(sums >= min(mass, max(1, int(np.ceil(share * float(mass)))))))
 
-    kept = int(sums[k - 1])
+    sums = np.cumsum(weights[order])
+    last = (top_k if 0 < top_k < len(x) else len(x)) - 1
     if hold(top_p, 1.0) < 1.0:
-        kept = int(sums[reached(hold(top_p, 1.0), kept)])
-    return int(order[reached(hold(u, 0.0), kept)])
+        last = reached(sums, hold(top_p, 1.0), int(sums[last]))
+    kept = int(sums[last])
+    if not by_id:
+        return int(order[reached(sums, hold(u, 0.0), kept)])
+    weights[order[last + 1:]] = 0
+    return reached(np.cumsum(weights), hold(u, 0.0), kept)
 
 
 def sample_min_p(logits, temperature, top_k, top_p, min_p, uniforms) -> np.ndarray:
-    return np.array([sample_min_p_row(r, float(t), int(k), float(p), float(m), float(u))
+    return np.array([sample_min_p_row(r, float(t), int(k), float(p), float(m), float(u), by_id=True)
                      for r, t, k, p, m, u in zip(logits, temperature, top_k, top_p, min_p, uniforms)], dtype=np.int64)
