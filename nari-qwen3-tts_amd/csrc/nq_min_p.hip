@@ -1019,6 +1019,7 @@ __device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const R
         __syncthreads();
         if (list) {
             if (T < 1024 || s.n <= MinPSizes<T>::kList) break;
+            __syncthreads();  // all have read the count that the next pass clears
         } else {
             BinSums<T, T == 1024 ? kMinPDigits / T : 1>(s, s.digits, above).find(s, target);
             above = s.above;

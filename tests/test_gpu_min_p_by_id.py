@@ -68,3 +68,31 @@ def test_the_order_of_the_logits_does_not_matter(nq, device, vocab):
             want = [ids[np.argmax(np.cumsum(np.exp(x[r, ids].astype(np.float64))) >=
                                   u[r] * np.exp(x[r, ids].astype(np.float64)).sum())] for r in range(8)]
             assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("vocab", [8192, 9001, 70001, 1 << 20])
+@pytest.mark.parametrize("kind", ["equal", "neighbours", "hot", "two scales"])
+def test_bins_that_overflow_the_list(nq, device, vocab, kind):
+    """More logits in the cut's bin than the list holds, which the digits of logits and ids cut one to five times: the
+    same tokens at each call, and the oracle's."""
+
+    from nari_qwen3_tts_amd.sampling import sample_min_p
+
+    rows = 4 if vocab > 100000 else 32
+    rng = np.random.default_rng(vocab)
+    x = np.full((rows, vocab), 1.5, np.float32)
+    t = 1.0
+    if kind == "neighbours":  # three values that differ in their last digits
+        x = x + rng.integers(0, 3, x.shape).astype(np.float32) * np.float32(2.0**-23)
+    elif kind == "hot":  # all of a bell within few bins
+        x, t = rng.standard_normal(x.shape).astype(np.float32), 500.0
+    elif kind == "two scales":  # equal ones below some that are not
+        x[:, ::7] = rng.standard_normal((rows, len(range(0, vocab, 7)))) * 0.001 + 1.75
+    x = torch.from_numpy(x).to(device)
+    for k, p, m in ((vocab // 2, 1.0, 0.0), (0, 0.6, 0.0), (vocab - 9, 0.3, 0.0), (vocab // 3, 0.5, 0.2)):
+        u = _uniforms(rng, rows)
+        want = _run(device, x, [t] * rows, [k] * rows, [p] * rows, [m] * rows, u)
+        args = [torch.tensor([v] * rows, device=device) for v in (t, k, p, m)] + [torch.tensor(u, device=device)]
+        args[1] = args[1].int()
+        for _ in range(8):
+            assert np.array_equal(sample_min_p(x, *(a if a.dtype == torch.int32 else a.float() for a in args)).cpu().numpy(), want)
