@@ -3,7 +3,7 @@
 Each ``csrc/*.hip`` file compiles to its own object with hipcc and the objects
 link into one shared library that exports the C ABI of ``include/nq_abi.h``.
 Translation units whose results must be bit-identical to the oracle (the
-sampler) are built with ``-ffp-contract=off``.  Nothing here runs a GPU: hipcc
+samplers) are built with ``-ffp-contract=off``.  Nothing here runs a GPU: hipcc
 cross-compiles for gfx950 on any host.
 """
 
@@ -33,7 +33,7 @@ _COMMON = [
     "-Xclang",
     "-packed-fp32-ops",
 ]
-_EXACT_FP = {"nq_sampler.hip"}
+_EXACT_FP = {"nq_sampler.hip", "nq_min_p.hip"}
 
 
 def _hipcc() -> str:

@@ -232,6 +232,9 @@ __device__ const double kExp2Table[128] = {
 // table, the Taylor series of 2^f for |f| <= 1 / 256 to its fourth power, whose rest is below 2e-15 of it, and an
 // exponent; and -i, or -i / 8, is the logit's bin in the row's histogram.  A weight of 1 needs e >= 2^-43, so t is held to
 // 45 octaves.
+// Every pass gives a logit the same weight, to the last unit, since a target taken from one pass's sums is looked for in
+// another's: so this file is built without contraction, and each fma is written out (contracted, t - i took the product
+// unrounded in one pass and rounded in another).
 template <int kShift>
 struct RowRule {
     static constexpr int kPer = 128, kLast = 45 * (kPer >> kShift);

@@ -96,3 +96,20 @@ def test_bins_that_overflow_the_list(nq, device, vocab, kind):
         args[1] = args[1].int()
         for _ in range(8):
             assert np.array_equal(sample_min_p(x, *(a if a.dtype == torch.int32 else a.float() for a in args)).cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("vocab", [8192, 20480])
+def test_the_last_kept_id(nq, device, vocab):
+    """u = 1 asks for the whole mass: the passes that sum a row have to agree to the last unit.  Logits one below the
+    largest, where a rounding of the exponent moves a weight of 2^-42 most often."""
+
+    rows = 256
+    rng = np.random.default_rng(vocab)
+    x = (-1.0 - rng.random((rows, vocab)) * 0.1).astype(np.float32)
+    x[:, 3] = 0.0
+    x = torch.from_numpy(x).to(device)
+    got = _run(device, x, [1.0] * rows, [0] * rows, [1.0] * rows, [0.0] * rows, [1.0] * rows)
+    assert (got == vocab - 1).all()
+    for temperature in (0.9, 1.1):
+        _run(device, x, [temperature] * rows, [0, vocab // 2] * (rows // 2), [1.0, 1.0, 0.75, 0.5] * (rows // 4),
+             [0.0] * rows, [1.0] * rows)
