@@ -76,7 +76,9 @@ struct Bf16Op {
 // above their roundings.  y / (1 + exp(-z)) with z = y (silu) or 2 sqrt(2 / pi) (y + 0.044715 y^3) (gelu_tanh, since (1 + tanh(z /
 // 2)) / 2 is that factor); at the ends the exponential is infinite or 0.  gelu is max(y, 0) - |y| erfc(|y| / sqrt 2) / 2, which
 // does not cancel in its tail as 1 + erf would: erfc(a) = k 2^(q(k) - a^2 log2 e) with k = 1 / (1 + 0.3 a), and q a polynomial
-// fitted to log2(erfc(a) exp(a^2) / k) at Chebyshev nodes for a up to 10.5, 8e-7 off there; behind it all is 0.
+// fitted to log2(erfc(a) exp(a^2) / k) at Chebyshev nodes for a up to 10.5, 8e-7 off there; behind it the exponential is 0, and k is
+// not: |y| is held to 16 on the positive side, so that plus infinity stays.  Minus infinity times 0 is NaN, as in the formulas of
+// the three.
 template <int kAct>
 __device__ __forceinline__ float activate(float y) {
     if constexpr (kAct == NQ_ACT_RELU) return y < 0.f ? 0.f : y;
@@ -86,7 +88,7 @@ __device__ __forceinline__ float activate(float y) {
         return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z));
     }
     if constexpr (kAct == NQ_ACT_GELU) {
-        const float m = fabsf(y), k = __builtin_amdgcn_rcpf(fmaf(0.21213203f, m, 1.0f));
+        const float m = fabsf(fminf(y, 16.0f)), k = __builtin_amdgcn_rcpf(fmaf(0.21213203f, m, 1.0f));
         float q = fmaf(0.6919735f, k, -2.821275f);
         q = fmaf(q, k, 4.1087608f);
         q = fmaf(q, k, -2.9656343f);
@@ -94,8 +96,7 @@ __device__ __forceinline__ float activate(float y) {
         q = fmaf(q, k, 0.27396405f);
         q = fmaf(q, k, 1.4983267f);
         q = fmaf(q, k, -2.5660994f);
-        const float g = 0.5f * m * k * __builtin_amdgcn_exp2f(fmaf(-0.72134752f * y, y, q));
-        return (y < 0.f ? 0.f : y) - g;  // NaN stays
+        return fmaf(-0.5f * m * k, __builtin_amdgcn_exp2f(fmaf(-0.72134752f * y, y, q)), y < 0.f ? 0.f : y);  // NaN stays
     }
     return y;
 }
