@@ -283,7 +283,8 @@ product_tile_kernel(ProductArgs a, int tiles_m, int tiles_n) {
         for (int i = threadIdx.x; i < BM; i += T) s_x[i] = m0 + i < a.M ? a.sx[m0 + i] : 0.f;
     }
     if constexpr (kEpi) {
-        for (int i = threadIdx.x; i < BN; i += T) s_b[i] = a.bias && n0 + i < a.N ? bf16_to_f32(a.bias[n0 + i]) : 0.f;
+        // without a bias -0, which changes no value: with 0 a -0 would lose its sign here and not where rows are few
+        for (int i = threadIdx.x; i < BN; i += T) s_b[i] = a.bias && n0 + i < a.N ? bf16_to_f32(a.bias[n0 + i]) : -0.f;
     }
 
     // load v writes rows 8 (wave V + v) .. + 7 of a stage, lane l place l % 8 of row l / 8

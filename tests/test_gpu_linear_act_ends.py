@@ -1,4 +1,5 @@
-"""Products with an epilogue at the ends of their range: infinite values through every activation."""
+"""Products with an epilogue at the ends of their range: infinite values through every activation, and the same bits of an
+8-bit product, the sign of a zero included, at any number of rows."""
 
 from __future__ import annotations
 
@@ -50,3 +51,28 @@ def test_infinite_values(nq, device, m, act):
     odd = ~np.isfinite(want)
     assert np.isposinf(want).any()
     assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[odd & ~np.isnan(want)], want[odd & ~np.isnan(want)])
+
+
+@pytest.mark.parametrize("act", o_epi.ACTIVATIONS)
+@pytest.mark.parametrize("small", [False, True])
+def test_int8_rows_have_the_same_bits_in_any_batch(nq, device, act, small):
+    """Few-row kernels against tiles, with and without bias and residual; ``small``: products that leave zeros of either sign."""
+
+    from nari_qwen3_tts_amd.layers import linear_int8
+
+    rng = np.random.default_rng(5 + small)
+    m, n, k = 300, 4100, 208
+    q, w = (torch.from_numpy(rng.integers(-127, 128, (r, k)).astype(np.int8)).to(device) for r in (m, n))
+    s, sw = (torch.from_numpy(rng.uniform(0.01, 0.1, r).astype(np.float32)).to(device) for r in (m, n))
+    if small:
+        s, sw = s * 1e-30, sw * 1e-30
+    bias, res = (torch.from_numpy(rng.standard_normal(r).astype(np.float32)).to(device, torch.bfloat16) for r in ((n,), (m, n)))
+    bias[::5] = -0.0
+    res[:, ::3] = -0.0
+    for b in (None, bias):
+        for r in (None, res):
+            out = linear_int8(q, s, w, sw, bias=b, activation=act, residual=r).view(torch.int16)
+            assert not small or b is not None or r is not None or (out == -32768).any()
+            for part in (slice(0, 1), slice(7, 23), slice(100, 140), slice(200, 264)):
+                got = linear_int8(q[part], s[part], w, sw, bias=b, activation=act, residual=None if r is None else r[part])
+                assert torch.equal(got.view(torch.int16), out[part])
