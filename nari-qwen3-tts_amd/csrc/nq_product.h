@@ -457,8 +457,8 @@ void launch_tiles(const ProductArgs &a, hipStream_t st) {
 //   M 256 N 4096:  64 x 64 tiles 7.6, 64 x 128 8.7;               N 6144: 64 x 128 tiles 8.9, 64 x 64 9.6, 128 x 256 17.5
 //   M 640 N 6144:  64 x 128 tiles 15.0, 128 x 256 18.5;           N 12288: 128 x 256 tiles 21.9, 64 x 128 26.8
 //   M 1000 N 12288: 128 x 256 tiles 37.4, 64 x 128 39.0
-// With an epilogue also 128 x 128, where those are one round of the CUs and 64 x 128 are two (the plain product's tiles, which
-// nq_linear_int8_tile tells, stay as they were), 128 x 128 before what the rule would take:
+// With an epilogue also 128 x 128, where those are one round of the CUs and 64 x 128 are two (not in the plain product, whose
+// tiles nq_linear_int8_tile tells), 128 x 128 before what the rule would take:
 //   M 500 N 6144:  bf16 19.1 and 23.3, int8 13.6 and 15.2;        M 640 N 6144: 24.3 and 29.3, 16.8 and 17.8
 //   M 1500 N 2048: 21.1 and 23.1, 14.5 and 15.5;                  M 2000 N 2048, K 6144: 57.7 and 66.6, 33.1 and 36.9
 //   one round of 64 x 128 (M 500 N 4096): 18.1 and 15.5, 12.5 and 10.8; two of 128 x 128 (M 800 N 6144): 37.6 and 30.0

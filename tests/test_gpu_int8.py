@@ -233,3 +233,8 @@ def test_quantize_every_quotient(nq, device):
         q, s = quantize_int8_rows(t)
         assert np.array_equal(q.cpu().numpy(), codes)
         assert torch.equal(s.cpu(), torch.from_numpy((b * 2.0**power).astype(np.float32) / np.float32(127)))
+
+
+@pytest.mark.parametrize("m,n,k", [(48, 4090, 2064), (77, 2041, 3088), (33, 2300, 1024), (140, 1300, 16)])
+def test_linear_long_sums_in_pieces_of_48_rows(nq, device, m, n, k):
+    test_linear_long_sums(nq, device, m, n, k, (48, 16))
