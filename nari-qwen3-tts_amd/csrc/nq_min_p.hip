@@ -154,6 +154,7 @@ struct MinPShared {
     alignas(16) uint64_t list[MinPSizes<T>::kList];
     uint64_t hist[MinPSizes<T>::kBins];  // of the row
     uint64_t digits[T == 1024 ? kMinPDigits : 1];
+    uint64_t cells[T];  // masses of consecutive ids
     double table[128];
     uint64_t part[kWaves];
     float max[2][kWaves];
@@ -306,7 +307,7 @@ __device__ __forceinline__ float logit_at(const InT *row, int id) {
     else return row[id];
 }
 
-// The ids of a cell, from .. to - 1, at most 2 T of them.
+// The ids of a cell, from .. to - 1, at most 2 T of them; a row has T cells at most.
 struct Ids {
     int from, to;
 };
@@ -367,12 +368,12 @@ struct HeldRow {
 };
 static_assert(kMinPHeld == 8, "two groups of four");
 
-// What is left of a row, the n logits of a list as append() left them, in registers: the list is free for others behind the
-// constructor.  No entry is 0.
-template <int T>
+// What is left of a row, the n <= kMost logits of a list as append() left them, in registers: the list is free for others behind
+// the constructor.  No entry is 0.
+template <int T, int kMost = MinPSizes<T>::kList>
 struct HeldList {
     static constexpr bool kShort = false, kMemory = false;
-    static constexpr int kEach = MinPSizes<T>::kList / T;
+    static constexpr int kEach = kMost / T;
     uint64_t e[kEach];
     __device__ __forceinline__ HeldList(const MinPShared<T> &s, int n) {
 #pragma unroll
@@ -408,11 +409,14 @@ struct HeldList {
             f(entry_id(e[i]), 1, v);
         }
     }
-    // The masses of the cells, as many ids each, a power of two, as make them 4096 at most.
-    static __device__ __forceinline__ int cell_bits(int vocab) { return max(0, 20 - __clz(max(1, vocab - 1))); }
+    // The masses of the cells, as many ids each, a power of two, as make them T at most.
+    static __device__ __forceinline__ int cell_bits(int vocab) {
+        constexpr int kBits = T == 1024 ? 10 : 8;
+        static_assert(1 << kBits == T && (T < 1024 || kMinPVocab <= T * 2 * T));
+        return max(0, 32 - kBits - __clz(max(1, vocab - 1)));
+    }
     template <typename W>
     __device__ __forceinline__ void cells(uint64_t *sum, int vocab, W weigh) const {
-        static_assert(kMinPVocab == 1 << 20 && MinPSizes<T>::kBins >= 4096);
         const int bits = cell_bits(vocab);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
@@ -477,37 +481,41 @@ struct FarRow {
             }
         }
     }
-    // The masses of the cells: the logits before the vectors, those of 256 vectors each, those behind.  A wave takes a cell, so that
-    // its lanes' sums meet once in as many logits; four vectors of a thread are in flight.
-    static constexpr int kCell = 4 * kWave;  // vectors
+    // The masses of the cells: the logits before the vectors, those of 256 vectors each (fp32: 512), those behind.  A wave takes 256
+    // vectors, so that its lanes' sums meet once in as many logits; four vectors of a thread are in flight.
+    static constexpr int kPart = 4 * kWave, kCell = kPart * 8 / V;  // vectors
     template <typename W>
     __device__ __forceinline__ void cells(uint64_t *sum, int, W weigh) const {
-        constexpr int U = kCell / kWave, kWaves = T / kWave;
-        static_assert(kMinPVocab / V / kCell + 2 <= MinPSizes<T>::kBins && kCell * V <= 2 * T);
-        const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, n = (nv + kCell - 1) / kCell;
+        constexpr int U = kPart / kWave, kWaves = T / kWave;
+        static_assert(kMinPVocab / V / kCell + 2 <= T && kCell * V <= 2 * T);
+        const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
         uint4 v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = load(wave * kCell + u * kWave + lane);
+        for (int u = 0; u < U; ++u) v[u] = load(wave * kPart + u * kWave + lane);
         few([&](int id, float x) {
             const float one[1] = {x};
-            atomicAdd(reinterpret_cast<unsigned long long *>(&sum[id < head ? 0 : n + 1]), weigh(id, one));
+            atomicAdd(reinterpret_cast<unsigned long long *>(&sum[cell_of(id)]), weigh(id, one));
         });
 #pragma unroll 1
-        for (int c = wave; c < n; c += kWaves) {
+        for (int c = wave; c * kPart < nv; c += kWaves) {
             uint64_t m = 0;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int j = c * kCell + u * kWave + lane;
+                const int j = c * kPart + u * kWave + lane;
                 const uint4 r = v[u];
-                v[u] = load(j + kWaves * kCell);
+                v[u] = load(j + kWaves * kPart);
                 if (j >= nv) continue;
                 float x[V];
                 unpack(r, x);
                 m += weigh(head + j * V, x);
             }
             m = wave_scan64(m);
-            if (lane == kWave - 1) sum[c + 1] = m;
+            if (lane == kWave - 1) atomicAdd(reinterpret_cast<unsigned long long *>(&sum[1 + c * kPart / kCell]), m);
         }
+    }
+    __device__ __forceinline__ int cell_of(int id) const {
+        const int n = (nv + kCell - 1) / kCell;
+        return id < head ? 0 : id >= head + nv * V ? n + 1 : 1 + (id - head) / (kCell * V);
     }
     __device__ __forceinline__ Ids cell_ids(int cell, int) const {
         const int end = head + nv * V, at = head + (cell - 1) * kCell * V;
@@ -708,15 +716,12 @@ __device__ __forceinline__ void sort_list(MinPShared<T> &s, int n) {
         }
 }
 
-// An entry with its halves exchanged: in descending order of these the ids ascend.
-__device__ __forceinline__ uint64_t exchanged(uint64_t e) { return e << 32 | e >> 32; }
-
-// The sums of a sorted list (kIds: of exchanged entries): thread t has the ranks t E .. t E + E - 1, E = ceil(n / T).
-template <int T, bool kIds = false>
+// The sums of a sorted list: thread t has the ranks t E .. t E + E - 1, E = ceil(n / T).
+template <int T>
 struct ListSums {
     static constexpr int kEach = MinPSizes<T>::kList / T;
     uint64_t cum[kEach];
-    uint64_t before, total;
+    uint64_t before;
     int first, end;
     __device__ __forceinline__ ListSums(MinPShared<T> &s, int n, uint64_t above, const Rule<T> &rule) {
         const int each = (n + T - 1) / T;
@@ -725,20 +730,20 @@ struct ListSums {
         uint64_t own = 0;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            if (first + i < end) own += rule.weight(kIds ? exchanged(s.list[first + i]) : s.list[first + i]);
+            if (first + i < end) own += rule.weight(s.list[first + i]);
             cum[i] = own;
         }
+        uint64_t total;
         before = above + block_before<T>(own, s.part, total);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) cum[i] += before;
     }
-    // The first rank whose mass reaches the target, which the list's last does: s.bin, its entry and the mass through it.
+    // The first rank whose mass reaches the target, which the list's last does: its entry, s.found, and the mass through it, s.found_mass.
     __device__ __forceinline__ void find_mass(MinPShared<T> &s, uint64_t target) const {
         uint64_t last = before;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             if (first + i < end && last < target && target <= cum[i]) {
-                s.bin = first + i;
                 s.found_mass = cum[i];
                 s.found = s.list[first + i];
             }
@@ -765,69 +770,141 @@ struct RowCuts {
     double p, u;
 };
 
-// The token of a row whose weights are all among the list's n <= 64 logits, by one wave, a logit a lane: each lane sums what
-// comes before its own, in the order of the logits for the cuts and of the ids for the draw.  Sums of 64 weights are exact
-// in double.
+// The token of a row whose weights are all among the list's n <= 64 logits, by one wave, a logit a lane: each counts the logits
+// and the ids before its own, and the weights are summed in either order.
 template <int T>
 __device__ __forceinline__ int draw_from_few(const MinPShared<T> &s, int n, const Rule<T> &rule, const RowCuts &c) {
     const int lane = threadIdx.x & (kWave - 1);
     const uint64_t mine = lane < n ? listed_entry(s.list[lane]) : 0;
-    double own = lane < n ? static_cast<double>(rule.weight(mine)) : 0.0;
-    auto other = [](uint64_t v, int j) {
-        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v)), j);
-        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v >> 32)), j);
-        return (static_cast<uint64_t>(hi) << 32) | lo;
+    uint64_t own = lane < n ? rule.weight(mine) : 0;
+    int rank = 0, place = 0;
+    for (int j = 0; j < n; ++j) {
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(mine)), j);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(mine >> 32)), j);
+        rank += ((static_cast<uint64_t>(hi) << 32) | lo) > mine ? 1 : 0;
+        place += lo > static_cast<uint32_t>(mine) ? 1 : 0;  // a smaller id's lower half is larger
+    }
+    if (lane >= n) rank = place = lane;
+    auto sums = [&](int to) {  // of the weights, lane r's first moved to lane `to`
+        const uint32_t lo = __builtin_amdgcn_ds_permute(4 * to, static_cast<int>(static_cast<uint32_t>(own)));
+        const uint32_t hi = __builtin_amdgcn_ds_permute(4 * to, static_cast<int>(static_cast<uint32_t>(own >> 32)));
+        return wave_scan64((static_cast<uint64_t>(hi) << 32) | lo);
     };
-    auto sum = [](double v) {
-#pragma unroll
-        for (int d = 1; d < kWave; d <<= 1) v += __shfl_xor(v, d, kWave);
-        return v;
-    };
-    auto target = [](double p, double mass) { return fmin(fmax(ceil(p * mass), 1.0), mass); };
+    auto at = [](uint64_t v, int j) { return static_cast<uint64_t>(__shfl(static_cast<unsigned long long>(v), j, kWave)); };
+    auto first = [](bool reached) { return __ffsll(static_cast<long long>(__ballot(reached))) - 1; };
     if (c.k < n || c.p < 1.0) {
-        int rank = 0;
-        double above = 0.0;
-        for (int j = 0; j < n; ++j) {
-            const bool first = other(mine, j) > mine;
-            rank += first ? 1 : 0;
-            above += first ? __longlong_as_double(other(__double_as_longlong(own), j)) : 0.0;
-        }
-        if (rank >= c.k) own = 0.0;
-        if (c.p < 1.0 && above >= target(c.p, sum(own))) own = 0.0;
+        const uint64_t cum = sums(rank), mass = at(cum, min(c.k, n) - 1);
+        if (rank > first(cum >= (c.p < 1.0 ? share(c.p, mass) : mass))) own = 0;
     }
-    double before = 0.0;
-    for (int j = 0; j < n; ++j) {  // a smaller id has a larger lower half
-        const bool first = static_cast<uint32_t>(other(mine, j)) > static_cast<uint32_t>(mine);
-        before += first ? __longlong_as_double(other(__double_as_longlong(own), j)) : 0.0;
-    }
-    const double at = target(c.u, sum(own));
-    return __shfl(entry_id(mine), __ffsll(static_cast<long long>(__ballot(before < at && at <= before + own))) - 1, kWave);
+    const uint64_t cum = sums(place);
+    const int id = __builtin_amdgcn_ds_permute(4 * place, entry_id(mine));
+    return __shfl(id, first(cum >= share(c.u, at(cum, kWave - 1))), kWave);
 }
 
-// The token of a row whose weights are all in the list (for thread 0).
-template <int T>
-__device__ __forceinline__ int draw_from_list(MinPShared<T> &s, int n, const Rule<T> &rule, const RowCuts &c) {
-    if (n <= kWave) return threadIdx.x < kWave ? draw_from_few<T>(s, n, rule, c) : 0;
-    for (int i = threadIdx.x; i < n; i += T) s.list[i] = listed_entry(s.list[i]);
+// A histogram's sums: thread t has the bins t E .. t E + E - 1.
+template <int T, int kEach = MinPSizes<T>::kEach>
+struct BinSums {
+    uint64_t h[kEach], before, total;
+    __device__ __forceinline__ BinSums(MinPShared<T> &s, const uint64_t *hist, uint64_t above) {
+        uint64_t own = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int bin = kEach * threadIdx.x + i;
+            h[i] = hist[bin];
+            own += h[i];
+        }
+        before = above + block_before<T>(own, s.part, total);
+    }
+    // The first bin at which the sum reaches the target (the last does): s.bin, s.above before it, s.found_mass through it.
+    __device__ __forceinline__ void find(MinPShared<T> &s, uint64_t target) const {
+        uint64_t at = before;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (at < target && target <= at + h[i]) {
+                s.bin = kEach * threadIdx.x + i;
+                s.above = at;
+                s.found_mass = at + h[i];
+            }
+            at += h[i];
+        }
+        __syncthreads();
+    }
+};
+
+// The token of a row by what is kept of it: the first id at which the sum of the masses reaches u of the whole.  The cells'
+// masses say in which one, and its logits are read again, two a thread.
+template <int T, typename Row, typename InT>
+__device__ __forceinline__ int draw_by_ids(MinPShared<T> &s, const Row &row, const InT *logits, const Rule<T> &rule,
+                                           double u, int vocab) {
+    s.cells[threadIdx.x] = 0;
     __syncthreads();
-    int kept = min(c.k, n);
-    if (kept < n || c.p < 1.0) {
+    auto weigh = [&](int id, const auto &x) {
+        constexpr int N = sizeof(x) / sizeof(float);
+        uint64_t sum = 0;
+        int bin;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const uint64_t w = rule.weight(x[e], bin);
+            sum += rule.counts(x[e], id + e) ? w : 0;
+        }
+        return sum;
+    };
+    auto weigh_bare = [&](int id, const auto &x) {
+        constexpr int N = sizeof(x) / sizeof(float);
+        uint64_t sum = 0;
+        int bin;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const uint64_t w = rule.bare_weight(x[e], bin);
+            sum += rule.counts(x[e], id + e) ? w : 0;
+        }
+        return sum;
+    };
+    if (Row::kMemory && rule.bare) row.cells(s.cells, vocab, weigh_bare);
+    else row.cells(s.cells, vocab, weigh);
+    __syncthreads();
+    const BinSums<T, 1> sums(s, s.cells, 0);
+    const uint64_t target = share(u, sums.total);
+    sums.find(s, target);
+    const Ids ids = row.cell_ids(static_cast<int>(s.bin), vocab);
+    const int id = ids.from + 2 * static_cast<int>(threadIdx.x);
+    uint64_t w[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const float x[1] = {id + e < ids.to ? logit_at(logits, id + e) : -__builtin_inff()};
+        w[e] = weigh(id + e, x);
+    }
+    uint64_t all;
+    const uint64_t before = s.above + block_before<T>(w[0] + w[1], s.part, all);
+    if (before < target && target <= before + w[0] + w[1]) s.id = target <= before + w[0] ? id : id + 1;
+    __syncthreads();
+    return s.id;
+}
+
+// The token of a row whose kept logits are all in the list, n <= MinPSizes<T>::kSorted, and, where top-k keeps the whole list, none but
+// them (for thread 0).
+template <int T, typename InT>
+__device__ __forceinline__ int draw_from_list(MinPShared<T> &s, int n, const InT *logits, Rule<T> &rule, const RowCuts &c,
+                                              int vocab) {
+    if (n <= kWave) return threadIdx.x < kWave ? draw_from_few<T>(s, n, rule, c) : 0;
+    const HeldList<T, (MinPSizes<T>::kSorted > T ? MinPSizes<T>::kSorted : T)> listed(s, n);
+    if ((c.k < vocab && c.k <= n) || c.p < 1.0) {
+        const int k = min(c.k, n);
+        if (static_cast<int>(threadIdx.x) < n) s.list[threadIdx.x] = listed.e[0];
+        __syncthreads();
         sort_list<T>(s, n);
         if (c.p < 1.0) {
             const ListSums<T> sums(s, n, 0, rule);
-            sums.find_rank(s, kept - 1);
+            sums.find_rank(s, k - 1);
             const uint64_t mass = s.found_mass;
             __syncthreads();
             sums.find_mass(s, share(c.p, mass));
-            kept = static_cast<int>(s.bin) + 1;
+            rule.end_at(s.found);
+        } else {
+            rule.end_at(s.list[k - 1]);
         }
     }
-    for (int i = threadIdx.x; i < kept; i += T) s.list[i] = exchanged(s.list[i]);
-    __syncthreads();
-    sort_list<T>(s, kept);
-    const ListSums<T, true> sums(s, kept, 0, rule);
-    sums.find_mass(s, share(c.u, sums.total));
-    return entry_id(exchanged(s.found));
+    return draw_by_ids<T>(s, listed, logits, rule, c.u, vocab);
 }
 
 // The row's histogram: of counts (kMass false) or of masses.  The list's counter is cleared besides.
@@ -919,36 +996,6 @@ __device__ __forceinline__ void row_histogram(MinPShared<T> &s, const Row &row, 
     __syncthreads();
 }
 
-// A histogram's sums: thread t has the bins t E .. t E + E - 1.
-template <int T, int kEach = MinPSizes<T>::kEach>
-struct BinSums {
-    uint64_t h[kEach], before, total;
-    __device__ __forceinline__ BinSums(MinPShared<T> &s, const uint64_t *hist, uint64_t above) {
-        uint64_t own = 0;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int bin = kEach * threadIdx.x + i;
-            h[i] = hist[bin];
-            own += h[i];
-        }
-        before = above + block_before<T>(own, s.part, total);
-    }
-    // The first bin at which the sum reaches the target (the last does): s.bin, s.above before it, s.found_mass through it.
-    __device__ __forceinline__ void find(MinPShared<T> &s, uint64_t target) const {
-        uint64_t at = before;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            if (at < target && target <= at + h[i]) {
-                s.bin = kEach * threadIdx.x + i;
-                s.above = at;
-                s.found_mass = at + h[i];
-            }
-            at += h[i];
-        }
-        __syncthreads();
-    }
-};
-
 // Of the listed logits those in question, in order, and the first at which the sum of counts or masses reaches the target
 // (the last does): s.found, and the mass through it, s.found_mass.
 template <int T, typename Q>
@@ -1033,56 +1080,6 @@ __device__ __forceinline__ void locate(MinPShared<T> &s, const Row &row, const R
     pick<T>(s, HeldList<T>(s, static_cast<int>(s.n)), rule, above, target, mass, in_question);
 }
 
-// The token of a row by what is kept of it: the first id at which the sum of the masses reaches u of the whole.  The cells'
-// masses say in which one, and its logits are read again, two a thread.
-template <int T, typename Row, typename InT>
-__device__ __forceinline__ int draw_by_ids(MinPShared<T> &s, const Row &row, const InT *logits, const Rule<T> &rule,
-                                           double u, int vocab) {
-    for (int i = threadIdx.x; i < MinPSizes<T>::kBins; i += T) s.hist[i] = 0;
-    __syncthreads();
-    auto weigh = [&](int id, const auto &x) {
-        constexpr int N = sizeof(x) / sizeof(float);
-        uint64_t sum = 0;
-        int bin;
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const uint64_t w = rule.weight(x[e], bin);
-            sum += rule.counts(x[e], id + e) ? w : 0;
-        }
-        return sum;
-    };
-    auto weigh_bare = [&](int id, const auto &x) {
-        constexpr int N = sizeof(x) / sizeof(float);
-        uint64_t sum = 0;
-        int bin;
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const uint64_t w = rule.bare_weight(x[e], bin);
-            sum += rule.counts(x[e], id + e) ? w : 0;
-        }
-        return sum;
-    };
-    if (Row::kMemory && rule.bare) row.cells(s.hist, vocab, weigh_bare);
-    else row.cells(s.hist, vocab, weigh);
-    __syncthreads();
-    const BinSums<T> sums(s, s.hist, 0);
-    const uint64_t target = share(u, sums.total);
-    sums.find(s, target);
-    const Ids ids = row.cell_ids(static_cast<int>(s.bin), vocab);
-    const int id = ids.from + 2 * static_cast<int>(threadIdx.x);
-    uint64_t w[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const float x[1] = {id + e < ids.to ? logit_at(logits, id + e) : -__builtin_inff()};
-        w[e] = weigh(id + e, x);
-    }
-    uint64_t all;
-    const uint64_t before = s.above + block_before<T>(w[0] + w[1], s.part, all);
-    if (before < target && target <= before + w[0] + w[1]) s.id = target <= before + w[0] ? id : id + 1;
-    __syncthreads();
-    return s.id;
-}
-
 // The token of a row by its histograms.
 template <int T, typename Row, typename InT>
 __device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, const InT *logits, Rule<T> &rule,
@@ -1100,7 +1097,7 @@ __device__ __forceinline__ int draw_by_bins(MinPShared<T> &s, const Row &row, co
                         if (rule.counts(v, id) && rule.bin(v) <= bin) append<T>(s, id, v);
                     });  // at most MinPSizes<T>::kSorted
                     __syncthreads();
-                    return draw_from_list<T>(s, static_cast<int>(s.n), rule, c);
+                    return draw_from_list<T>(s, static_cast<int>(s.n), logits, rule, c, vocab);
                 }
                 __syncthreads();
             }
@@ -1222,7 +1219,7 @@ min_p_kernel(MinPArgs a) {
     const int n = static_cast<int>(s.n);
     int token;
     if (n > 0 && n <= MinPSizes<T>::kSorted) {
-        token = draw_from_list<T>(s, n, rule, cuts);
+        token = draw_from_list<T>(s, n, logits, rule, cuts, a.vocab);
     } else {
         __syncthreads();
         if constexpr (kHeld) {
