@@ -16,9 +16,10 @@
 // logits alone are collected and sorted; a bin too full for the list (equal logits) is cut by the digits of its entries.
 // The draw sums what is kept over cells of consecutive ids, and looks at the logits of the one cell that it falls into.
 //
-// Bound by the slowest row's passes.  64 x 65537 bf16 (us, replayed): the first rank 7, min-p .05 17, top-k 50 16, no cut 24,
-// top-p .95 30; 256 x 131072 fp32, whose reading takes 26: 28, 38, 54, 84, 94.  Of a row without a cut the maximum takes a pass (2.4 and
-// 17 us), the weights another (7 and 31: its atomics in LDS and its doubles), the drawn bin's logits a third (4 and 18).
+// Bound by the slowest row's passes.  64 x 65537 bf16 (us, replayed): the first rank 7, min-p .05 15, top-k 50 17, no cut 25,
+// top-p .95 41; 256 x 131072 fp32, whose reading takes 26: 29, 34, 51, 63, 115.  The maximum takes a pass (2.4 and 17 us), the cells'
+// masses another (15 and 34: some 27 vector instructions a logit where most are kept, in double), top-p before it a third for
+// the bins' masses (8 and 32) and a fourth for the cut bin's logits (6 and 17).  A top-p row that keeps few: 28 and 93.
 #include <type_traits>
 
 #include "nq_common.h"
@@ -949,9 +950,8 @@ __device__ __forceinline__ void row_histogram(MinPShared<T> &s, const Row &row, 
         row.several(weigh_bare);
     } else {
         // A bf16 row repeats its values: they are counted where the list will be, 32 binades of either sign down from the
-        // largest that counts, and each is weighed once, 5 instructions a logit instead of 21 (64 x 65537 without a cut 24 us, 28 with a
-        // test and a branch for each logit).  Counter 0 of a sign has what is smaller and zero, the last one what is larger
-        // (NaN, and what is too far below the maximum to count).
+        // largest that counts, and each is weighed once, 5 instructions a logit instead of 21 (65537 logits 8 us).  Counter 0 of a
+        // sign has what is smaller and zero, the last one what is larger (NaN, and what is too far below the maximum to count).
         constexpr int kHalf = MinPSizes<T>::kList;  // 32-bit counters of a sign
         static_assert(kHalf == 4096, "the sign's bit, moved by three, and the numbers share 16 bits");
         uint32_t *const count = reinterpret_cast<uint32_t *>(s.list);
